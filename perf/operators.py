@@ -2,7 +2,7 @@
 
 * ``norm``   -- residual addition + RMS norm, with a float or an 8-bit output (``add_rmsnorm``).
 * ``w4``     -- products with 4-bit weights and group scales (``W4Weights``).
-* ``verify`` -- drafted tokens checked against the target's probabilities (``DraftVerifier``).
+* ``verify`` -- drafted tokens checked against the target's probabilities (``verify_drafts``).
 
 ``own`` false: the operators' plain forms in elementary torch operations. True: the framework's calls.
 """
@@ -163,15 +163,12 @@ def prepare(case, seed):
                  out=torch.empty(case["tokens"], case["n_out"], dtype=_TYPES[case["y"]], device="cuda"))
         if own:  # the weights' handle that a program keeps
             import bebelm_b200 as bb
-            s["w"] = bb.W4Weights(codes, scales, zeros, group=case["group"], max_tokens=case["tokens"])
+            s["w"] = bb.W4Weights(codes, scales, zeros, group=case["group"])
     else:
         names = ("target", "draft", "tokens", "n_drafts", "u", "u_sample")
         s.update(zip(names, _verify_inputs(case, seed)))
         s["out"] = torch.empty(case["seqs"], case["drafts"] + 1, dtype=torch.int32, device="cuda")
         s["accepted"] = torch.empty(case["seqs"], dtype=torch.int32, device="cuda")
-        if own:  # the workspace that a program keeps
-            import bebelm_b200 as bb
-            s["v"] = bb.DraftVerifier(case["vocab"], max_seqs=case["seqs"], max_drafts=case["drafts"])
     return s
 
 
@@ -193,9 +190,11 @@ def _own_w4(s):
 
 
 def _own_verify(s):
+    import bebelm_b200 as bb
     case = s["case"]
-    tokens, accepted = s["v"].verify(s["target"], s["tokens"], s["u"], s["u_sample"], draft=s["draft"], n_drafts=s["n_drafts"],
-                                     temperature=case["temperature"], probs=case["probs"], out=s["out"], accepted=s["accepted"])
+    tokens, accepted = bb.verify_drafts(s["target"], s["tokens"], s["u"], s["u_sample"], draft=s["draft"],
+                                        n_drafts=s["n_drafts"], temperature=case["temperature"], probs=case["probs"],
+                                        out=s["out"], accepted=s["accepted"])
     return dict(tokens=tokens, accepted=accepted)
 
 
