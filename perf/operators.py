@@ -177,12 +177,12 @@ def _own_norm(s):
     import bebelm_b200 as bb
     case = s["case"]
     if case["out"] == "int8":
-        q, scales, h = bb.add_rmsnorm(s["x"], s["gain"], s["res"], EPS, out_dtype=bb.INT8, group=case["group"], out=s["out"],
+        q, scales, _ = bb.add_rmsnorm(s["x"], s["gain"], s["res"], EPS, out_dtype=bb.INT8, group=case["group"], out=s["out"],
                                       scales=s["scales"], sum_out=s["sum"])
         rows, ng = scales.shape  # what the 8 bits stand for
-        return dict(y=torch.mul(q.view(rows, ng, -1), scales.view(rows, ng, 1)).view(rows, -1), scales=scales, h=h)
-    y, h = bb.add_rmsnorm(s["x"], s["gain"], s["res"], EPS, out=s["out"], sum_out=s["sum"])
-    return dict(y=y, h=h)
+        return dict(y=torch.mul(q.view(rows, ng, -1), scales.view(rows, ng, 1)).view(rows, -1), scales=scales, h=s["sum"])
+    y, _ = bb.add_rmsnorm(s["x"], s["gain"], s["res"], EPS, out=s["out"], sum_out=s["sum"])
+    return dict(y=y, h=s["sum"])
 
 
 def _own_w4(s):
