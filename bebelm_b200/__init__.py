@@ -30,6 +30,7 @@ MEM_HOST, MEM_DEVICE = 0, 1
 F32, BF16 = 0, 1
 F32_TENSOR = 2  # prefill in_dtype: fp32 inputs, tensor-core attention
 FP8 = 3  # cache dtype: K/V as fp8 e4m3
+INT8, F16 = 4, 5  # 8-bit activations with scales; f16 weight scales
 
 # reference constants (src/config.rs:14-32)
 N_HEADS, N_KV_HEADS, HEAD_DIM, KV_DIM, HIDDEN = 32, 8, 64, 512, 2048
@@ -52,6 +53,8 @@ EXPORTS = [
     "bebelm_gguf_get_u32", "bebelm_gguf_get_f32", "bebelm_gguf_get_str", "bebelm_gguf_get_u32_array",
     "bebelm_gguf_array_len", "bebelm_gguf_get_str_at", "bebelm_gguf_validate", "bebelm_attn_weights_from_gguf",
     "bebelm_head_from_gguf", "bebelm_step_plan_launch_allgather", "bebelm_attn_prefill_allgather",
+    "bebelm_add_rmsnorm", "bebelm_w4_create", "bebelm_w4_destroy", "bebelm_w4_workspace", "bebelm_w4_matmul",
+    "bebelm_verify_workspace", "bebelm_verify_drafts",
 ]
 GGML_F32, GGML_F16, GGML_Q4_K, GGML_Q6_K = 0, 1, 12, 14
 IPC_HANDLE_BYTES = 64
@@ -151,6 +154,13 @@ def load_library(path: str = LIB_PATH):
         "bebelm_gguf_validate": ([vp], i),
         "bebelm_attn_weights_from_gguf": ([vp, i, i, C.POINTER(vp)], i),
         "bebelm_head_from_gguf": ([vp, i, C.POINTER(vp)], i),
+        "bebelm_add_rmsnorm": ([vp, sz, vp, sz, i, sz, sz, vp, f, vp, sz, vp, i, vp, sz, i, vp], i),
+        "bebelm_w4_create": ([i, sz, sz, sz, vp, vp, i, vp, i, C.POINTER(vp)], i),
+        "bebelm_w4_destroy": ([vp], i),
+        "bebelm_w4_workspace": ([vp, vp, i, sz, sz, C.POINTER(sz)], i),
+        "bebelm_w4_matmul": ([vp, vp, i, sz, vp, sz, sz, vp, i, vp, sz, i, vp], i),
+        "bebelm_verify_workspace": ([sz, sz, sz, i, i, f, C.POINTER(sz)], i),
+        "bebelm_verify_drafts": ([vp, sz, vp, sz, sz, sz, sz, i, f, vp, vp, vp, vp, vp, vp, vp, sz, i, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -747,6 +757,352 @@ def attn_decode_batched(caches, layer: int, q, k, v, q_gain, k_gain, pos, theta:
     _check(load_library().bebelm_attn_decode_batched(arr, n, layer, n_heads, qb[0], kb[0], vb[0], qg[0], kg[0], theta,
                                                      eps, posa, ob, mem, _stream_ptr(stream, mem)))
     return out
+
+
+# ------------------------------------------- operators around the attention --
+def _cuda_torch():
+    global _torch
+    if not _torch:
+        import torch
+        _torch = torch
+    return _torch
+
+
+def _dtype_of(t, what: str) -> int:
+    """F32 / BF16 / INT8 / F16 of a tensor or array."""
+    name = str(t.dtype).replace("torch.", "")
+    try:
+        return {"float32": F32, "bfloat16": BF16, "int8": INT8, "float16": F16}[name]
+    except KeyError:
+        raise ValueError(f"{what}: dtype {t.dtype} is not supported") from None
+
+
+def _rows_of(t, what: str):
+    """(rows, n, row stride) of a tensor whose last dimension is contiguous and whose rows are
+    evenly spaced."""
+    n = t.shape[-1]
+    if t.dim() <= 2 or t.is_contiguous():
+        if t.dim() > 1 and n > 1 and t.stride(-1) != 1 or t.dim() == 1 and n > 1 and t.stride(0) != 1:
+            raise ValueError(f"{what}: the last dimension must be contiguous")
+        if t.dim() == 1:
+            return 1, n, n
+        if t.dim() == 2:
+            return t.shape[0], n, max(t.stride(0), n) if t.shape[0] <= 1 else t.stride(0)
+        return (t.numel() // n if n else 0), n, n
+    raise ValueError(f"{what}: more than two dimensions must be contiguous")
+
+
+def _out_tensor(out, shape, dtype, device, what: str):
+    """`out`, checked, or a new tensor."""
+    torch = _cuda_torch()
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if out.dtype != dtype or out.device != device or not out.is_contiguous() or out.numel() != _numel(shape):
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {tuple(shape)} on {device}")
+    return out
+
+
+def _numel(shape) -> int:
+    n = 1
+    for d in shape:
+        n *= d
+    return n
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and (not _is_torch(t) or t.device != device):
+            raise ValueError(f"{name} must be a tensor on {device}")
+
+
+def _stream_on(stream, device) -> int:
+    """The cudaStream_t of a device-memory call: the given stream, or torch's current one there."""
+    if stream is None:
+        return _cuda_torch().cuda.current_stream(device).cuda_stream
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _workspace(workspace, need: int, device, stream):
+    """(tensor, pointer, bytes): the caller's scratch, or one from torch's allocator, which keeps
+    it from reuse on other streams until the work of ``stream`` that uses it is done."""
+    if not need:
+        return None, None, 0
+    torch = _cuda_torch()
+    if workspace is None:
+        if stream is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        else:
+            ext = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=device)
+            with torch.cuda.stream(ext):
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _on_device(device, call):
+    """Runs ``call`` with ``device`` current (the calls without a handle go to the current device)."""
+    cuda = _cuda_torch().cuda
+    if cuda.current_device() == device.index:
+        return call()
+    with cuda.device(device):
+        return call()
+
+
+def add_rmsnorm(x, gain, residual=None, eps: float = RMS_EPS, out_dtype: int | None = None, group: int = 0, sum_out=None,
+                out=None, scales=None, stream=None):
+    """The norm before a layer's products: ``rmsnorm`` (src/kernels/rmsnorm.rs:10-21) of x + residual.
+
+    x, residual [rows, n] (or [n]), float32 or bfloat16 CUDA tensors (rows may be strided), or float32
+    arrays; gain float32 [n]. Returns ``(y, h)``: h = x + residual in the type of x (x itself without a
+    residual), y in ``out_dtype`` (F32, BF16; default: the type of x). With ``out_dtype=INT8`` returns
+    ``(codes, scales, h)``: y = codes * scales, one scale per ``group`` values (32, 64, 128, 256; 0: the
+    row), rounded as the K-quant products round their activations. ``sum_out`` (for h; may be x or
+    residual), ``out`` and ``scales`` are optional result buffers."""
+    L = load_library()
+    if not _is_torch(x) or not x.is_cuda:
+        x = np.ascontiguousarray(x.numpy() if _is_torch(x) else x, np.float32)
+        rows, n = (1, x.size) if x.ndim <= 1 else (x.size // x.shape[-1] if x.shape[-1] else 0, x.shape[-1])
+        res = None if residual is None else np.ascontiguousarray(residual, np.float32)
+        g = np.ascontiguousarray(gain, np.float32)
+        if g.size != n or (res is not None and res.shape != x.shape):
+            raise ValueError("add_rmsnorm: gain is [n], residual has the shape of x")
+        od = F32 if out_dtype is None else out_dtype
+        if od not in (F32, INT8):
+            raise ValueError("host outputs are F32 or INT8")
+        if sum_out is not None or out is not None or scales is not None:
+            raise ValueError("result buffers are for device calls")
+        y = np.empty(x.shape, np.float32 if od == F32 else np.int8)
+        sc = np.empty((rows, n // (group or n or 1)), np.float32) if od == INT8 else None
+        h = x if res is None else np.empty_like(x)
+        _check(L.bebelm_add_rmsnorm(x.ctypes.data, n, None if res is None else res.ctypes.data, n, F32, rows, n, g.ctypes.data,
+                                    eps, None if res is None else h.ctypes.data, n, y.ctypes.data, od,
+                                    None if sc is None else sc.ctypes.data, group, MEM_HOST, None))
+        return (y, h) if sc is None else (y, sc, h)
+    torch = _cuda_torch()
+    dev = x.device
+    _same_device(dev, gain=gain, residual=residual, sum_out=sum_out, out=out, scales=scales)
+    dt = _dtype_of(x, "x")
+    rows, n, xs = _rows_of(x, "x")
+    if gain.dtype != torch.float32 or gain.numel() != n or not gain.is_contiguous():
+        raise ValueError("gain must be a contiguous float32 tensor of n elements")
+    rs = n
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise ValueError("residual must have the type and shape of x")
+        rs = _rows_of(residual, "residual")[2]
+    od = dt if out_dtype is None else out_dtype
+    if od == F32:
+        y = _out_tensor(out, x.shape, torch.float32, dev, "out")
+    elif od == BF16:
+        y = _out_tensor(out, x.shape, torch.bfloat16, dev, "out")
+    elif od == INT8:
+        y = _out_tensor(out, x.shape, torch.int8, dev, "out")
+        scales = _out_tensor(scales, (rows, n // (group or n or 1)), torch.float32, dev, "scales")
+    else:
+        raise ValueError("out_dtype must be F32, BF16 or INT8")
+    hs = n
+    if residual is None:
+        if sum_out is not None:
+            raise ValueError("sum_out needs a residual")
+        h = x
+    elif sum_out is None:
+        sum_out = h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    else:
+        if sum_out.dtype != x.dtype or sum_out.shape != x.shape:
+            raise ValueError("sum_out must have the type and shape of x")
+        h, hs = sum_out, _rows_of(sum_out, "sum_out")[2]
+    args = (x.data_ptr(), xs, None if residual is None else residual.data_ptr(), rs, dt, rows, n, gain.data_ptr(), eps,
+            None if sum_out is None else sum_out.data_ptr(), hs, y.data_ptr(), od,
+            scales.data_ptr() if od == INT8 else None, group, MEM_DEVICE, _stream_on(stream, dev))
+    _check(_on_device(dev, lambda: L.bebelm_add_rmsnorm(*args)))
+    return (y, scales, h) if od == INT8 else (y, h)
+
+
+class W4Weights:
+    """4-bit weights with group scales on the device, and their products.
+
+    codes uint8 [n_out, n_in / 2] (the input with the lower index in the low four bits), scales float16
+    or bfloat16 [n_out, n_in / group], zeros uint8 [n_out, n_in / group] (0..127) or None (8 everywhere):
+    w = (code - zero) * scale. numpy arrays, CPU tensors or CUDA tensors. The weights are laid out once; products of
+    one object may run on several streams."""
+
+    def __init__(self, codes, scales, zeros=None, group: int = 128, device: int | None = None):
+        dev_in = _is_torch(codes) and codes.is_cuda
+        if len(codes.shape) != 2 or len(scales.shape) != 2:
+            raise ValueError("codes are [n_out, n_in / 2], scales [n_out, n_in / group]")
+        self.n_out, self.n_in, self.group = codes.shape[0], 2 * codes.shape[1], group
+        want = (self.n_out, self.n_in // group if group > 0 else 0)
+        sd = _dtype_of(scales, "scales")
+        if str(codes.dtype).replace("torch.", "") != "uint8" or tuple(scales.shape) != want or sd not in (F16, BF16) or (
+                zeros is not None and (str(zeros.dtype).replace("torch.", "") != "uint8" or tuple(zeros.shape) != want)):
+            raise ValueError(f"codes and zeros are uint8, scales float16 or bfloat16, scales and zeros {want}")
+        keep = []
+        for t in (codes, scales, zeros):
+            if t is None:
+                keep.append(None)
+            elif _is_torch(t):
+                if t.is_cuda != dev_in or (dev_in and t.device != codes.device):
+                    raise ValueError("codes, scales and zeros must be in one place")
+                keep.append(t.contiguous())
+            elif dev_in:
+                raise ValueError("codes, scales and zeros must be in one place")
+            else:
+                keep.append(np.ascontiguousarray(t))
+        if device is None:
+            device = codes.device.index if dev_in else 0
+        elif dev_in and codes.device.index != device:
+            raise ValueError("device weights stay on their device")
+        self.device = device
+        ptr = [None if t is None else t.data_ptr() if _is_torch(t) else t.ctypes.data for t in keep]
+        self._h = C.c_void_p()
+        if dev_in:  # the layout kernel runs on its own: whatever makes the inputs is done first
+            _cuda_torch().cuda.current_stream(codes.device).synchronize()
+        _check(load_library().bebelm_w4_create(device, self.n_in, self.n_out, group, ptr[0], ptr[1], sd, ptr[2],
+                                               MEM_DEVICE if dev_in else MEM_HOST, C.byref(self._h)))
+
+    def matmul(self, x, x_scales=None, out_dtype: int | None = None, out=None, workspace=None, stream=None):
+        """y [n_tokens, n_out] = x W^T. x [n_tokens, n_in] (or [n_in]): float32, bfloat16, or int8 with
+        x_scales float32 [n_tokens, n_in / x_group] as :func:`add_rmsnorm` gives them. out_dtype F32 (the default,
+        except for bfloat16 x) or BF16. CUDA tensors (x may have strided rows), or float32 / int8 arrays."""
+        L = load_library()
+        if not _is_torch(x) or not x.is_cuda:
+            x = np.ascontiguousarray(x.numpy() if _is_torch(x) else x)
+            if x.dtype != np.int8:
+                x = x.astype(np.float32, copy=False)
+            if x.shape[-1] != self.n_in:
+                raise ValueError(f"x has {x.shape[-1]} columns, the weights {self.n_in}")
+            t = x.size // self.n_in
+            sc, xg = None, 0
+            if x.dtype == np.int8:
+                sc = np.ascontiguousarray(x_scales, np.float32).reshape(t, -1)
+                xg = self._x_group(sc.shape[1] if t else 1)
+            if out_dtype not in (None, F32) or out is not None or workspace is not None:
+                raise ValueError("host products are float32, without buffers")
+            y = np.empty((t, self.n_out), np.float32)
+            _check(L.bebelm_w4_matmul(self._h, x.ctypes.data, INT8 if sc is not None else F32, self.n_in,
+                                      None if sc is None else sc.ctypes.data, xg, t, y.ctypes.data, F32, None, 0, MEM_HOST,
+                                      None))
+            return y.reshape(*x.shape[:-1], self.n_out)
+        torch = _cuda_torch()
+        dev = x.device
+        if dev.index != self.device:
+            raise ValueError(f"x is on {dev}, the weights on cuda:{self.device}")
+        dt = _dtype_of(x, "x")
+        t, n, xs = _rows_of(x, "x")
+        if n != self.n_in:
+            raise ValueError(f"x has {n} columns, the weights {self.n_in}")
+        sp, xg = None, 0
+        if dt == INT8:
+            _same_device(dev, x_scales=x_scales)
+            if x_scales is None or x_scales.dtype != torch.float32 or not x_scales.is_contiguous() or (
+                    t and x_scales.numel() % t):
+                raise ValueError("int8 activations need contiguous float32 x_scales [n_tokens, n_in / x_group]")
+            xg = self._x_group(x_scales.numel() // t if t else 1)
+            sp = x_scales.data_ptr()
+        elif x_scales is not None:
+            raise ValueError("x_scales are for int8 activations")
+        od = (BF16 if dt == BF16 else F32) if out_dtype is None else out_dtype
+        if out is not None and out_dtype is None:
+            od = _dtype_of(out, "out")
+        if od not in (F32, BF16):
+            raise ValueError("products are F32 or BF16")
+        shape = (*x.shape[:-1], self.n_out)
+        y = _out_tensor(out, shape, torch.float32 if od == F32 else torch.bfloat16, dev, "out")
+        xp = x.data_ptr()
+        need = C.c_size_t()
+        _check(L.bebelm_w4_workspace(self._h, xp, dt, xs, t, C.byref(need)))
+        ws, wp, wb = _workspace(workspace, need.value, dev, stream)
+        _check(L.bebelm_w4_matmul(self._h, xp, dt, xs, sp, xg, t, y.data_ptr(), od, wp, wb, MEM_DEVICE,
+                                  _stream_on(stream, dev)))
+        return y
+
+    def _x_group(self, n_groups: int) -> int:
+        if n_groups == 1 or n_groups == 0:
+            return 0
+        if self.n_in % n_groups:
+            raise ValueError(f"{n_groups} scales a token do not divide {self.n_in} inputs")
+        return self.n_in // n_groups
+
+    def close(self):
+        if self._h:
+            load_library().bebelm_w4_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def verify_drafts(target, tokens, u, u_sample, draft=None, n_drafts=None, temperature: float = 1.0, probs: bool = False,
+                  out=None, accepted=None, workspace=None, stream=None):
+    """Checks drafted tokens against the target model's rows (see ``bebelm_verify_drafts``).
+
+    target float32 [n_seqs, d + 1, vocab] (logits, or probabilities with ``probs``), tokens int32 [n_seqs, d],
+    draft float32 [n_seqs, d, vocab] (the rows the drafts were sampled from) or None (certain drafts),
+    n_drafts int32 [n_seqs] or None (d each), u float32 [n_seqs, d] and u_sample [n_seqs] uniform in [0, 1)
+    (None with temperature 0: greedy). Rows of CUDA tensors may be padded (a stride above vocab). Returns
+    ``(tokens, accepted)``, int32 [n_seqs, d + 1] (the accepted drafts, the next token, then -1) and [n_seqs]."""
+    L = load_library()
+    if not _is_torch(target) or not target.is_cuda:
+        target = np.ascontiguousarray(target, np.float32)
+        b, d1, v = target.shape
+        d = d1 - 1
+        arr = [None if a is None else np.ascontiguousarray(a, t) for a, t in (
+            (draft, np.float32), (tokens, np.int32), (n_drafts, np.int32), (u, np.float32), (u_sample, np.float32))]
+        shapes = ((b, d, v), (b, d), (b,), (b, d), (b,))
+        if d < 0 or arr[1] is None or any(a is not None and a.shape != s for a, s in zip(arr, shapes)):
+            raise ValueError("verify_drafts: buffer shapes do not match target [n_seqs, d + 1, vocab]")
+        if out is not None or accepted is not None or workspace is not None:
+            raise ValueError("result buffers are for device calls")
+        o, acc = np.empty((b, d1), np.int32), np.empty(b, np.int32)
+        p = [None if a is None else a.ctypes.data for a in arr]
+        _check(L.bebelm_verify_drafts(target.ctypes.data, v, p[0], v, b, d, v, int(probs), temperature, p[1], p[2], p[3], p[4],
+                                      o.ctypes.data, acc.ctypes.data, None, 0, MEM_HOST, None))
+        return o, acc
+    torch = _cuda_torch()
+    dev = target.device
+    _same_device(dev, tokens=tokens, u=u, u_sample=u_sample, draft=draft, n_drafts=n_drafts, out=out, accepted=accepted)
+
+    def stride_of(t, rows, what):
+        if t.dtype != torch.float32 or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{what} must be float32 [n_seqs, rows, vocab] with contiguous rows")
+        st = t.stride(1) if rows > 1 else t.stride(0) if t.shape[0] > 1 else t.shape[2]
+        if t.shape[0] > 1 and rows > 1 and t.stride(0) != rows * st:
+            raise ValueError(f"{what}: its rows must be evenly spaced")
+        return st
+
+    b, d1, v = target.shape
+    d = d1 - 1
+    if d < 0:
+        raise ValueError("target needs a row behind the drafts")
+    ts, ds = stride_of(target, d1, "target"), v
+    if draft is not None:
+        if tuple(draft.shape) != (b, d, v):
+            raise ValueError(f"draft must be {(b, d, v)}")
+        if draft.numel():
+            ds = stride_of(draft, d, "draft")
+    for name, t, shape, dt in (("tokens", tokens, (b, d), torch.int32), ("u", u, (b, d), torch.float32),
+                               ("n_drafts", n_drafts, (b,), torch.int32), ("u_sample", u_sample, (b,), torch.float32)):
+        if t is not None and (t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {dt} tensor of {shape}")
+    o = _out_tensor(out, (b, d1), torch.int32, dev, "out")
+    acc = _out_tensor(accepted, (b,), torch.int32, dev, "accepted")
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+
+    def call():
+        need = C.c_size_t()
+        _check(L.bebelm_verify_workspace(b, d, v, int(draft is not None and d > 0 and temperature != 0.0), int(probs), temperature,
+                                         C.byref(need)))
+        ws, wp, wb = _workspace(workspace, need.value, dev, stream)
+        return L.bebelm_verify_drafts(target.data_ptr(), ts, ptr(draft), ds, b, d, v, int(probs), temperature, ptr(tokens),
+                                      ptr(n_drafts), ptr(u), ptr(u_sample), o.data_ptr(), acc.data_ptr(), wp, wb, MEM_DEVICE,
+                                      _stream_on(stream, dev))
+
+    _check(_on_device(dev, call))
+    return o, acc
 
 
 # ------------------------------------------------------------------ GGUF --

@@ -10,6 +10,7 @@
 #include <cstring>
 #include <condition_variable>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <unordered_map>
@@ -2562,6 +2563,368 @@ int bebelm_sample_greedy(float* logits, size_t n, const uint32_t* history, size_
     TRY(stage_out(P, o, token, 4, s));
     // the penalty rewrites the seen tokens' logits in place, as the reference's sampler does
     if (pen) CUDA_TRY(cudaMemcpy(logits, a0, 4 * n, cudaMemcpyDeviceToHost));
+    return 0;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// The operators around the attention: residual RMS norm, 4-bit products, draft verification.
+// ---------------------------------------------------------------------------
+namespace {
+
+size_t elem_size(int dtype) { return dtype == BEBELM_F32 ? 4 : dtype == BEBELM_INT8 ? 1 : 2; }
+size_t pad256(size_t n) { return (n + 255) & ~size_t(255); }
+
+int num_sms_of(int dev) {
+    static std::atomic<int> sms[64];
+    if (dev < 0 || dev >= 64) return 148;
+    int n = sms[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        sms[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// The current device, checked (once a device) to be one this library is built for.
+int current_device_cached(int* dev) {
+    static std::atomic<bool> known[64];
+    CUDA_TRY(cudaGetDevice(dev));
+    if (*dev >= 0 && *dev < 64 && known[*dev].load(std::memory_order_relaxed)) return 0;
+    TRY(check_device(*dev));
+    if (*dev < 64) known[*dev].store(true, std::memory_order_relaxed);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bebelm_add_rmsnorm(const void* x, size_t x_stride, const void* residual, size_t residual_stride, int dtype,
+                       size_t rows, size_t n, const float* gain, float eps, void* sum_out, size_t sum_stride, void* y,
+                       int y_dtype, float* y_scales, size_t group, int mem, void* stream) {
+    TRY(check_mem(mem));
+    if (dtype != BEBELM_F32 && dtype != BEBELM_BF16)
+        return fail(BEBELM_ERR_UNSUPPORTED, "dtype %d is not BEBELM_F32 or BEBELM_BF16", dtype);
+    if (y_dtype != BEBELM_F32 && y_dtype != BEBELM_BF16 && y_dtype != BEBELM_INT8)
+        return fail(BEBELM_ERR_UNSUPPORTED, "y_dtype %d is not BEBELM_F32, BEBELM_BF16 or BEBELM_INT8", y_dtype);
+    if (n == 0 || n > kAddNormMaxN) return fail(BEBELM_ERR_UNSUPPORTED, "n (%zu) must be 1..%zu", n, kAddNormMaxN);
+    if (rows >= (1ull << 31)) return fail(BEBELM_ERR_INVALID, "rows (%zu) must be below 2^31", rows);
+    if (y_dtype == BEBELM_INT8) {
+        if (group != 0 && group != 32 && group != 64 && group != 128 && group != 256)
+            return fail(BEBELM_ERR_UNSUPPORTED, "group (%zu) must be 0 (the row), 32, 64, 128 or 256", group);
+        if (group && n % group) return fail(BEBELM_ERR_INVALID, "n (%zu) must be a multiple of the group (%zu)", n, group);
+    } else if (group) {
+        return fail(BEBELM_ERR_INVALID, "group (%zu) is for BEBELM_INT8 outputs", group);
+    }
+    if (rows == 0) return 0;
+    if (!x || !gain || !y || (y_dtype == BEBELM_INT8 && !y_scales)) return fail(BEBELM_ERR_INVALID, "null buffer");
+    if (rows > 1 && (x_stride < n || (residual && residual_stride < n) || (sum_out && sum_stride < n)))
+        return fail(BEBELM_ERR_INVALID, "a row stride is below n (%zu)", n);
+    if (sum_out && sum_out == y) return fail(BEBELM_ERR_INVALID, "sum_out and y are the same buffer");
+    if (mem == BEBELM_MEM_HOST && rows > 1 &&
+        (x_stride != n || (residual && residual_stride != n) || (sum_out && sum_stride != n)))
+        return fail(BEBELM_ERR_INVALID, "host rows must be contiguous");
+    int dev;
+    TRY(current_device_cached(&dev));
+    cudaStream_t s = as_stream(stream);
+    AddNormArgs a{};
+    a.x = x, a.residual = residual, a.gain = gain, a.sum_out = sum_out, a.y = y, a.y_scales = y_scales;
+    a.x_stride = x_stride, a.residual_stride = residual_stride, a.sum_stride = sum_stride;
+    a.rows = rows, a.n = n, a.group = (unsigned)group, a.eps = eps;
+    a.bf16 = dtype == BEBELM_BF16;
+    a.out = y_dtype == BEBELM_F32 ? kNormOutF32 : y_dtype == BEBELM_BF16 ? kNormOutBf16 : kNormOutInt8;
+    if (mem == BEBELM_MEM_DEVICE) {
+        CUDA_TRY(launch_add_rmsnorm(a, s));
+        return 0;
+    }
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    bebelm_kv_pool* P = nullptr;
+    TRY(scratch_pool(dev, &P));
+    const size_t xb = rows * n * elem_size(dtype), yb = rows * n * elem_size(y_dtype);
+    const size_t hb = sum_out ? xb : 0, sb = y_dtype == BEBELM_INT8 ? 4 * rows * (group ? n / group : 1) : 0;
+    const size_t out_bytes = pad256(yb) + pad256(hb) + pad256(sb);
+    void *dx, *dr, *dg, *o;
+    Stage st[3] = {{x, xb, &dx}, {residual, residual ? xb : 0, &dr}, {gain, 4 * n, &dg}};
+    TRY(stage_in(P, st, 3, out_bytes, &o, s));
+    char* d = static_cast<char*>(o);
+    a.x = dx, a.residual = dr, a.gain = static_cast<const float*>(dg);
+    a.x_stride = a.residual_stride = a.sum_stride = n;
+    a.y = d;
+    a.sum_out = sum_out ? d + pad256(yb) : nullptr;
+    a.y_scales = reinterpret_cast<float*>(d + pad256(yb) + pad256(hb));
+    CUDA_TRY(launch_add_rmsnorm(a, s));
+    std::vector<char> back(out_bytes);
+    TRY(stage_out(P, o, back.data(), out_bytes, s));
+    std::memcpy(y, back.data(), yb);
+    if (hb) std::memcpy(sum_out, back.data() + pad256(yb), hb);
+    if (sb) std::memcpy(y_scales, back.data() + pad256(yb) + pad256(hb), sb);
+    return 0;
+}
+
+}  // extern "C"
+
+struct bebelm_w4 {
+    int device = 0;
+    W4View v{};
+    DevBuf codes, scales, zeros;
+    ErrWord err;  // a bounded wait of the many-token kernel that gave up
+    void release() {
+        codes.release();
+        scales.release();
+        zeros.release();
+        err.release();
+    }
+};
+
+namespace {
+
+int w4_fill(bebelm_w4* W, const uint8_t* codes, const void* scales, const uint8_t* zeros, int mem) {
+    W4View& v = W->v;
+    const size_t cb = v.n_out * (v.n_in / 2), ng = v.n_out * (v.n_in / v.group);
+    const size_t tiles = v.tile_rows * v.chunks, ns = tiles * v.per_chunk * 16;
+    DevBuf tmp;
+    struct Free {
+        DevBuf& b;
+        ~Free() { b.release(); }
+    } free_tmp{tmp};
+    const bool host = mem == BEBELM_MEM_HOST;
+    TRY(W->codes.ensure(tiles * 1024));
+    TRY(W->scales.ensure(ns * 2));
+    if (zeros) TRY(W->zeros.ensure(ns));
+    TRY(W->err.ensure());
+    TRY(tmp.ensure(256 + (host ? pad256(cb) + pad256(2 * ng) + pad256(ng) : 0)));
+    CUDA_TRY(cudaMemset(tmp.p, 0, 256));
+    const void *dc = codes, *ds = scales, *dz = zeros;
+    if (host) {
+        char* p = tmp.as<char>() + 256;
+        CUDA_TRY(cudaMemcpy(p, codes, cb, cudaMemcpyHostToDevice));
+        CUDA_TRY(cudaMemcpy(p + pad256(cb), scales, 2 * ng, cudaMemcpyHostToDevice));
+        if (zeros) CUDA_TRY(cudaMemcpy(p + pad256(cb) + pad256(2 * ng), zeros, ng, cudaMemcpyHostToDevice));
+        dc = p, ds = p + pad256(cb), dz = zeros ? p + pad256(cb) + pad256(2 * ng) : nullptr;
+    }
+    CUDA_TRY(cudaDeviceSynchronize());  // device inputs may come from any stream
+    CUDA_TRY(launch_w4_pack(static_cast<const uint8_t*>(dc), static_cast<const unsigned short*>(ds),
+                            static_cast<const uint8_t*>(dz), v, W->codes.as<uint32_t>(), W->scales.as<unsigned short>(),
+                            zeros ? W->zeros.as<uint8_t>() : nullptr, tmp.as<int>(), 0));
+    int bad = 0;
+    CUDA_TRY(cudaMemcpy(&bad, tmp.p, sizeof bad, cudaMemcpyDeviceToHost));
+    if (bad) return fail(BEBELM_ERR_INVALID, "a zero point is above 127");
+    v.codes = W->codes.as<uint4>();
+    v.scales = W->scales.as<uint32_t>();
+    v.zeros = zeros ? W->zeros.as<unsigned short>() : nullptr;
+    return 0;
+}
+
+int w4_x(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, const float* x_scales, size_t x_group,
+         size_t n_tokens, W4X* out) {
+    if (x_dtype != BEBELM_F32 && x_dtype != BEBELM_BF16 && x_dtype != BEBELM_INT8)
+        return fail(BEBELM_ERR_UNSUPPORTED, "x_dtype %d is not BEBELM_F32, BEBELM_BF16 or BEBELM_INT8", x_dtype);
+    if (x_dtype == BEBELM_INT8) {
+        if (x_group != 0 && x_group != 32 && x_group != 64 && x_group != 128 && x_group != 256)
+            return fail(BEBELM_ERR_UNSUPPORTED, "x_group (%zu) must be 0 (the row), 32, 64, 128 or 256", x_group);
+        if (x_group && W->v.n_in % x_group)
+            return fail(BEBELM_ERR_INVALID, "n_in (%zu) must be a multiple of x_group (%zu)", W->v.n_in, x_group);
+    } else if (x_group || x_scales) {
+        return fail(BEBELM_ERR_INVALID, "x_scales and x_group are for BEBELM_INT8 activations");
+    }
+    if (n_tokens >= (1ull << 31)) return fail(BEBELM_ERR_INVALID, "n_tokens (%zu) must be below 2^31", n_tokens);
+    *out = W4X{};
+    out->x = x;
+    out->scales = x_scales;
+    out->stride = x_stride;
+    out->tokens = n_tokens;
+    out->n_in = W->v.n_in;
+    out->kind = x_dtype == BEBELM_F32 ? kW4XF32 : x_dtype == BEBELM_BF16 ? kW4XBf16 : kW4XInt8;
+    out->group = (int)x_group;
+    for (size_t g = x_group; g > 1; g >>= 1) ++out->group_shift;
+    out->n_groups = x_group ? W->v.n_in / x_group : 1;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bebelm_w4_create(int device, size_t n_in, size_t n_out, size_t group, const uint8_t* codes, const void* scales,
+                     int scale_dtype, const uint8_t* zeros, int mem, bebelm_w4** out) {
+    if (!out) return fail(BEBELM_ERR_INVALID, "out is null");
+    *out = nullptr;
+    TRY(check_mem(mem));
+    if (!codes || !scales) return fail(BEBELM_ERR_INVALID, "null buffer");
+    if (scale_dtype != BEBELM_F16 && scale_dtype != BEBELM_BF16)
+        return fail(BEBELM_ERR_UNSUPPORTED, "scale_dtype %d is not BEBELM_F16 or BEBELM_BF16", scale_dtype);
+    if (group != 32 && group != 64 && (group == 0 || group % 128))
+        return fail(BEBELM_ERR_UNSUPPORTED, "group (%zu) must be 32, 64 or a multiple of 128", group);
+    if (n_in == 0 || n_in % group)
+        return fail(BEBELM_ERR_INVALID, "n_in (%zu) must be a positive multiple of the group (%zu)", n_in, group);
+    if (n_out == 0 || n_out >= (1ull << 31) || n_in >= (1ull << 31))
+        return fail(BEBELM_ERR_INVALID, "n_out (%zu) and n_in (%zu) must be 1..2^31-1", n_out, n_in);
+    TRY(check_device(device));
+    DeviceGuard g(device);
+    auto* W = new (std::nothrow) bebelm_w4();
+    if (!W) return fail(BEBELM_ERR_OOM, "out of host memory");
+    W->device = device;
+    W4View& v = W->v;
+    v.n_in = n_in, v.n_out = n_out, v.group = group;
+    v.chunks = (n_in + 127) / 128;
+    v.tile_rows = (n_out + 127) / 128 * 8;
+    v.per_chunk = group >= 128 ? 1 : (int)(128 / group);
+    v.scale_bf16 = scale_dtype == BEBELM_BF16;
+    const int rc = w4_fill(W, codes, scales, zeros, mem);
+    if (rc) {
+        W->release();
+        delete W;
+        return rc;
+    }
+    *out = W;
+    return 0;
+}
+
+int bebelm_w4_destroy(bebelm_w4* W) {
+    if (!W) return 0;
+    DeviceGuard g(W->device);
+    cudaDeviceSynchronize();
+    W->release();
+    delete W;
+    return 0;
+}
+
+int bebelm_w4_workspace(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, size_t n_tokens, size_t* bytes) {
+    if (!W || !bytes) return fail(BEBELM_ERR_INVALID, "null argument");
+    W4X xv;
+    TRY(w4_x(W, x, x_dtype, x_stride, nullptr, 0, n_tokens, &xv));
+    *bytes = w4_workspace(W->v, xv);
+    return 0;
+}
+
+int bebelm_w4_matmul(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, const float* x_scales, size_t x_group,
+                     size_t n_tokens, void* y, int y_dtype, void* workspace, size_t workspace_bytes, int mem, void* stream) {
+    if (!W) return fail(BEBELM_ERR_INVALID, "null weights");
+    TRY(check_mem(mem));
+    W4X xv;
+    TRY(w4_x(W, x, x_dtype, x_stride, x_scales, x_group, n_tokens, &xv));
+    if (y_dtype != BEBELM_F32 && y_dtype != BEBELM_BF16)
+        return fail(BEBELM_ERR_UNSUPPORTED, "y_dtype %d is not BEBELM_F32 or BEBELM_BF16", y_dtype);
+    if (n_tokens == 0) return 0;
+    const W4View& v = W->v;
+    if (!x || !y || (x_dtype == BEBELM_INT8 && !x_scales)) return fail(BEBELM_ERR_INVALID, "null buffer");
+    if (n_tokens > 1 && x_stride < v.n_in) return fail(BEBELM_ERR_INVALID, "x_stride is below n_in (%zu)", v.n_in);
+    if (mem == BEBELM_MEM_HOST && n_tokens > 1 && x_stride != v.n_in)
+        return fail(BEBELM_ERR_INVALID, "host rows must be contiguous");
+    DeviceGuard g(W->device);
+    cudaStream_t s = as_stream(stream);
+    const int sms = num_sms_of(W->device);
+    if (mem == BEBELM_MEM_DEVICE) {
+        const size_t need = w4_workspace(v, xv);
+        if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+            return fail(BEBELM_ERR_INVALID, "the product needs %zu bytes of workspace, 256-byte aligned (got %zu)", need,
+                        workspace ? workspace_bytes : 0);
+        CUDA_TRY(launch_w4_stream(v, xv, y, y_dtype == BEBELM_BF16, workspace, sms, s));
+        return 0;
+    }
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    bebelm_kv_pool* P = nullptr;
+    TRY(scratch_pool(W->device, &P));
+    const size_t xb = n_tokens * v.n_in * elem_size(x_dtype), yb = n_tokens * v.n_out * elem_size(y_dtype);
+    void *dx, *dsc, *o;
+    Stage st[2] = {{x, xb, &dx}, {x_scales, x_scales ? 4 * n_tokens * xv.n_groups : 0, &dsc}};
+    TRY(stage_in(P, st, 2, yb, &o, s));
+    xv.x = dx;
+    xv.scales = static_cast<const float*>(dsc);
+    xv.stride = v.n_in;
+    TRY(P->q8.ensure(std::max<size_t>(w4_workspace(v, xv), 256), false, s));
+    CUDA_TRY(launch_w4_stream(v, xv, o, y_dtype == BEBELM_BF16, P->q8.p, sms, s));
+    return stage_out(P, o, y, yb, s);
+}
+
+int bebelm_verify_workspace(size_t n_seqs, size_t n_drafts, size_t vocab, int draft_rows, int probs, float temperature,
+                            size_t* bytes) {
+    if (!bytes) return fail(BEBELM_ERR_INVALID, "bytes is null");
+    if (n_seqs >= (1u << 20) || n_drafts >= (1u << 10) || vocab == 0 || vocab >= (1ull << 31))
+        return fail(BEBELM_ERR_INVALID, "n_seqs (%zu) must be below 2^20, n_drafts (%zu) below 2^10, vocab (%zu) 1..2^31-1",
+                    n_seqs, n_drafts, vocab);
+    int dev;
+    TRY(current_device_cached(&dev));
+    VerifyArgs a{};
+    a.seqs = (int)n_seqs, a.drafts = (int)n_drafts, a.vocab = vocab, a.probs = probs, a.temperature = temperature;
+    static const float some = 0.f;
+    a.draft = draft_rows ? &some : nullptr;
+    *bytes = n_seqs ? verify_workspace(a, num_sms_of(dev)) : 0;
+    return 0;
+}
+
+int bebelm_verify_drafts(const float* target, size_t target_stride, const float* draft, size_t draft_stride, size_t n_seqs,
+                         size_t n_drafts, size_t vocab, int probs, float temperature, const int32_t* tokens,
+                         const int32_t* n_per_seq, const float* u, const float* u_sample, int32_t* out_tokens,
+                         int32_t* accepted, void* workspace, size_t workspace_bytes, int mem, void* stream) {
+    TRY(check_mem(mem));
+    if (n_seqs >= (1u << 20) || n_drafts >= (1u << 10) || vocab == 0 || vocab >= (1ull << 31))
+        return fail(BEBELM_ERR_INVALID, "n_seqs (%zu) must be below 2^20, n_drafts (%zu) below 2^10, vocab (%zu) 1..2^31-1",
+                    n_seqs, n_drafts, vocab);
+    if (!(temperature == 0.f || (temperature >= 1e-6f && temperature <= 1e6f)))
+        return fail(BEBELM_ERR_INVALID, "temperature (%g) must be 0 or 1e-6..1e6", (double)temperature);
+    if (probs && temperature != 1.f && temperature != 0.f)
+        return fail(BEBELM_ERR_INVALID, "probabilities take temperature 1, or 0 for the most likely token");
+    if (n_seqs == 0) return 0;
+    const bool greedy = temperature == 0.f;
+    if (!target || !out_tokens || !accepted || (n_drafts && !tokens) || (!greedy && (!u_sample || (n_drafts && !u))))
+        return fail(BEBELM_ERR_INVALID, "null buffer");
+    if (target_stride < vocab || (draft && draft_stride < vocab))
+        return fail(BEBELM_ERR_INVALID, "a row stride is below vocab (%zu)", vocab);
+    if (mem == BEBELM_MEM_HOST) {
+        if (target_stride != vocab || (draft && draft_stride != vocab))
+            return fail(BEBELM_ERR_INVALID, "host rows must be contiguous");
+        for (size_t i = 0; i < n_seqs * n_drafts; ++i)
+            if (tokens[i] < 0 || (size_t)tokens[i] >= vocab) {
+                if (n_per_seq && (int32_t)(i % n_drafts) >= n_per_seq[i / n_drafts]) continue;
+                return fail(BEBELM_ERR_INVALID, "drafted token %d out of range", tokens[i]);
+            }
+        for (size_t b = 0; n_per_seq && b < n_seqs; ++b)
+            if (n_per_seq[b] < 0 || (size_t)n_per_seq[b] > n_drafts)
+                return fail(BEBELM_ERR_INVALID, "sequence %zu has %d of at most %zu drafts", b, n_per_seq[b], n_drafts);
+    }
+    int dev;
+    TRY(current_device_cached(&dev));
+    cudaStream_t s = as_stream(stream);
+    const int sms = num_sms_of(dev);
+    VerifyArgs a{};
+    a.target = target, a.draft = greedy || !n_drafts ? nullptr : draft;
+    a.target_stride = target_stride, a.draft_stride = draft_stride, a.vocab = vocab;
+    a.seqs = (int)n_seqs, a.drafts = (int)n_drafts;
+    a.tokens = tokens, a.n_drafts = n_per_seq, a.u = u, a.u_sample = u_sample;
+    a.probs = probs ? 1 : 0, a.temperature = temperature;
+    a.out = out_tokens, a.accepted = accepted, a.workspace = workspace;
+    const size_t need = verify_workspace(a, sms);
+    if (mem == BEBELM_MEM_DEVICE) {
+        if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+            return fail(BEBELM_ERR_INVALID, "verification needs %zu bytes of workspace, 256-byte aligned (got %zu)", need,
+                        workspace ? workspace_bytes : 0);
+        CUDA_TRY(launch_verify(a, sms, s));
+        return 0;
+    }
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    bebelm_kv_pool* P = nullptr;
+    TRY(scratch_pool(dev, &P));
+    const size_t nd = n_seqs * n_drafts, tb = 4 * nd, ob = 4 * (nd + n_seqs);
+    void *d0, *d1, *d2, *d3, *d4, *d5, *o;
+    Stage st[6] = {{target, 4 * vocab * (nd + n_seqs), &d0}, {a.draft, a.draft ? 4 * vocab * nd : 0, &d1},
+                   {tokens, tb, &d2}, {n_per_seq, n_per_seq ? 4 * n_seqs : 0, &d3},
+                   {greedy ? nullptr : u, greedy ? 0 : tb, &d4}, {greedy ? nullptr : u_sample, greedy ? 0 : 4 * n_seqs, &d5}};
+    TRY(stage_in(P, st, 6, pad256(ob) + 4 * n_seqs, &o, s));
+    TRY(P->q8.ensure(std::max<size_t>(need, 256), false, s));
+    a.target = static_cast<const float*>(d0), a.draft = static_cast<const float*>(d1);
+    a.tokens = static_cast<const int*>(d2), a.n_drafts = static_cast<const int*>(d3);
+    a.u = static_cast<const float*>(d4), a.u_sample = static_cast<const float*>(d5);
+    a.out = static_cast<int*>(o);
+    a.accepted = reinterpret_cast<int*>(static_cast<char*>(o) + pad256(ob));
+    a.workspace = P->q8.p;
+    CUDA_TRY(launch_verify(a, sms, s));
+    std::vector<char> back(pad256(ob) + 4 * n_seqs);
+    TRY(stage_out(P, o, back.data(), back.size(), s));
+    std::memcpy(out_tokens, back.data(), ob);
+    std::memcpy(accepted, back.data() + pad256(ob), 4 * n_seqs);
     return 0;
 }
 

@@ -321,5 +321,67 @@ cudaError_t launch_rmsnorm_row(const float* x, const float* gain, int n, float e
 cudaError_t launch_greedy(float* logits, size_t n, const uint32_t* history, size_t n_history, float penalty,
                           uint32_t* bitmap, uint32_t* token, cudaStream_t s);
 
+// ---- residual addition + RMS norm (addnorm.cu) ----
+constexpr int kNormOutF32 = 0, kNormOutBf16 = 1, kNormOutInt8 = 2;
+constexpr size_t kAddNormMaxN = 32768;  // a row's values stay in one CTA's registers
+struct AddNormArgs {
+    const void* x;         // [rows][n], rows x_stride elements apart; f32 or bf16 (bf16 != 0)
+    const void* residual;  // same type, or null
+    const float* gain;     // [n]
+    void* sum_out;         // x + residual in the type of x, or null; may be x or residual
+    void* y;               // [rows][n] contiguous, in `out`'s type
+    float* y_scales;       // kNormOutInt8: [rows][n / group], group 0: [rows]
+    size_t x_stride, residual_stride, sum_stride, rows, n;
+    unsigned group;        // 0 (the row), 32, 64, 128 or 256
+    float eps;
+    int bf16, out;
+};
+cudaError_t launch_add_rmsnorm(const AddNormArgs& a, cudaStream_t s);
+
+// ---- products with 4-bit weights and group scales (w4.cu, w4_tc.cu) ----
+constexpr int kW4XF32 = 0, kW4XBf16 = 1, kW4XInt8 = 2;
+// The weights in the layout of w4.cu.
+struct W4View {
+    const uint4* codes;
+    const uint32_t* scales;        // two 16-bit scales a word (rows g and g + 8 of a tile)
+    const unsigned short* zeros;   // two bytes, or null: every zero point is 8
+    size_t n_in, n_out, group;
+    size_t chunks, tile_rows;      // tiles of 128 inputs; of 16 rows (a multiple of 8)
+    int per_chunk;                 // scales of a row in a tile: 1, 2 or 4
+    int scale_bf16;                // scales are bf16, not f16
+};
+// The activations: [tokens][n_in], rows `stride` elements apart; int8 with scales [tokens][n_groups].
+struct W4X {
+    const void* x;
+    const float* scales;
+    size_t stride, tokens, n_in, n_groups;
+    int kind, group, group_shift;  // group 0: one scale a token
+};
+// *bad is set where a zero point is above 127
+cudaError_t launch_w4_pack(const uint8_t* codes, const unsigned short* scales, const uint8_t* zeros, const W4View& w,
+                           uint32_t* out_c, unsigned short* out_s, uint8_t* out_z, int* bad, cudaStream_t s);
+cudaError_t launch_w4_planes(const W4X& x, size_t kp, __nv_bfloat16* out, cudaStream_t s);
+size_t w4_workspace(const W4View& w, const W4X& x);  // bytes of device scratch a product needs
+cudaError_t launch_w4_stream(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms,
+                             cudaStream_t s);
+
+// ---- drafted tokens against the target's rows (verify.cu) ----
+struct VerifyArgs {
+    const float* target;   // [seqs][drafts + 1] rows of `vocab`, target_stride elements apart
+    const float* draft;    // [seqs][drafts] rows, draft_stride apart, or null: each draft was certain
+    size_t target_stride, draft_stride, vocab;
+    int seqs, drafts;
+    const int* tokens;     // [seqs][drafts]
+    const int* n_drafts;   // [seqs], or null: drafts each
+    const float* u;        // [seqs][drafts]
+    const float* u_sample; // [seqs]
+    int probs;             // rows are probabilities, not logits
+    float temperature;     // 0: greedy
+    int* out;              // [seqs][drafts + 1]
+    int* accepted;         // [seqs]
+    void* workspace;
+};
+size_t verify_workspace(const VerifyArgs& a, int num_sms);
+cudaError_t launch_verify(const VerifyArgs& a, int num_sms, cudaStream_t s);
 
 }  // namespace bebelm

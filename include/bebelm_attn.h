@@ -60,6 +60,8 @@ enum { BEBELM_MEM_HOST = 0, BEBELM_MEM_DEVICE = 1 };
 enum { BEBELM_F32 = 0, BEBELM_BF16 = 1 };
 /* cache dtype only: K and V stored as fp8 e4m3 (one byte each) */
 enum { BEBELM_FP8_E4M3 = 3 };
+/* the operators around the attention: 8-bit activations with scales, and f16 weight scales */
+enum { BEBELM_INT8 = 4, BEBELM_F16 = 5 };
 /* bebelm_attn_prefill only: fp32 inputs (as the reference's attn_batch passes them), attention
  * on the tensor cores. */
 enum { BEBELM_F32_TENSOR = 2 };
@@ -377,6 +379,75 @@ BEBELM_API int bebelm_head_logits(bebelm_head* head, const float* h, float eps, 
  * history ids >= n are ignored. */
 BEBELM_API int bebelm_sample_greedy(float* logits, size_t n, const uint32_t* history, size_t n_history,
                                     float repeat_penalty, uint32_t* token, int mem, void* stream);
+
+/* --------------------------------------- residual addition + RMS norm ---
+ * The norm before a layer's products: rmsnorm (src/kernels/rmsnorm.rs:10-21) of x + residual, over
+ * rows of n values (1..32768). x and residual (nullable) are [rows][n] in `dtype` (BEBELM_F32 or
+ * BEBELM_BF16), their rows x_stride / residual_stride elements apart; gain is f32 [n].
+ *  - h = x + residual rounded to `dtype`; written to sum_out (nullable, rows sum_stride apart),
+ *    which may be x or residual itself (same stride).
+ *  - y [rows][n] (contiguous) in y_dtype: BEBELM_F32, BEBELM_BF16, or BEBELM_INT8 with y_scales
+ *    [rows][n / group]: the values stand for y * y_scales of their group of `group` (32, 64, 128 or
+ *    256, dividing n; 0: the row) neighbours, in the rule of the K-quant products' activations
+ *    (scale = max|t| / 127, codes rounded half away from zero; a group of zeros has scale 0).
+ *    y may be x or residual when their type and rows are the same; y and sum_out are distinct.
+ * The steps and their f32 roundings are the reference's (each one IEEE operation, the sum of
+ * squares in f64), so codes do not depend on the launch. Values are expected finite; a NaN or
+ * an infinity stays in its row. Host buffers are contiguous. Device buffers lie on the current device. */
+BEBELM_API int bebelm_add_rmsnorm(const void* x, size_t x_stride, const void* residual, size_t residual_stride,
+                                  int dtype, size_t rows, size_t n, const float* gain, float eps, void* sum_out,
+                                  size_t sum_stride, void* y, int y_dtype, float* y_scales, size_t group, int mem,
+                                  void* stream);
+
+/* ----------------------------- products with 4-bit weights, group scales ---
+ * Beside the GGML types of bebelm_matmul: y[t][n] = sum over k of (code[n][k] - zero[n][k / group]) *
+ * scale[n][k / group] * x[t][k]. codes [n_out][n_in / 2] bytes, the input with the lower index in
+ * the low four bits; scales [n_out][n_in / group] in scale_dtype (BEBELM_F16 or BEBELM_BF16); zeros
+ * [n_out][n_in / group] bytes (0..127), or NULL: 8 everywhere. group 32, 64 or a multiple of 128;
+ * n_in a multiple of it. create lays the weights out once on `device` (pointers as `mem` says); the handle
+ * is not changed afterwards, so products of one handle may run on several streams and threads. */
+typedef struct bebelm_w4 bebelm_w4;
+BEBELM_API int bebelm_w4_create(int device, size_t n_in, size_t n_out, size_t group, const uint8_t* codes,
+                                const void* scales, int scale_dtype, const uint8_t* zeros, int mem, bebelm_w4** out);
+BEBELM_API int bebelm_w4_destroy(bebelm_w4* w);
+/* Device scratch of a product of these activations (x only for its alignment: BEBELM_BF16 rows that
+ * are 16-byte aligned need none). */
+BEBELM_API int bebelm_w4_workspace(const bebelm_w4* w, const void* x, int x_dtype, size_t x_stride, size_t n_tokens,
+                                   size_t* bytes);
+/* x [n_tokens][n_in] in x_dtype, rows x_stride elements apart: BEBELM_F32, BEBELM_BF16, or BEBELM_INT8
+ * with x_scales [n_tokens][n_in / x_group] (x_group 32, 64, 128 or 256, or 0: one scale a token), as
+ * bebelm_add_rmsnorm writes them. y [n_tokens][n_out] in y_dtype (BEBELM_F32 or BEBELM_BF16). Activations are
+ * taken exactly, sums are f32; a group is summed before its scale is applied, so the sum of |code - zero| |x| over
+ * a group has to stay below 3.4e38. Infinities and NaN stay in their token's row. Device memory: `workspace` (256-byte aligned, of bebelm_w4_workspace
+ * bytes) is used until the call's work is done; calls that may overlap need one each. Host memory: none. */
+BEBELM_API int bebelm_w4_matmul(const bebelm_w4* w, const void* x, int x_dtype, size_t x_stride, const float* x_scales,
+                                size_t x_group, size_t n_tokens, void* y, int y_dtype, void* workspace,
+                                size_t workspace_bytes, int mem, void* stream);
+
+/* ------------------------------------------ drafted tokens, verified ---
+ * No counterpart in the reference. Tokens that a smaller model (or a lookup) drafted, checked
+ * against the target model's rows so that what comes out is distributed as the target's own
+ * samples. target [n_seqs][n_drafts + 1] rows of `vocab` (row i: after i drafts), draft
+ * [n_seqs][n_drafts] rows the drafts were sampled from, or NULL when they were not sampled
+ * (each then counts as certain); rows target_stride / draft_stride elements apart. Rows hold
+ * logits (probs 0; probabilities are softmax(row / temperature)) or probabilities (probs 1).
+ * tokens [n_seqs][n_drafts]; n_per_seq [n_seqs] drafts of each sequence (nullable: n_drafts); u
+ * [n_seqs][n_drafts] and u_sample [n_seqs] uniform random numbers in [0, 1).
+ *  - Draft i is accepted iff all before it were and u_i * q_i(token) < p_i(token). A token outside the
+ *    vocabulary is refused (host memory: BEBELM_ERR_INVALID).
+ *  - The next token: after a refusal at i from max(p_i - q_i, 0) (p_i if that is zero everywhere), after all
+ *    drafts from the row behind them: the lowest index whose running sum exceeds u_sample times the total.
+ *  - temperature 0: accepted iff equal to the row's first maximum, which is also the next token
+ *    (u, u_sample and draft are not read). NaN never wins; a row with nothing above -inf gives 0.
+ * out_tokens [n_seqs][n_drafts + 1]: the accepted drafts, the next token, then -1; accepted [n_seqs]
+ * their counts. Rows behind a sequence's drafts are not read. workspace as for bebelm_w4_matmul. */
+BEBELM_API int bebelm_verify_workspace(size_t n_seqs, size_t n_drafts, size_t vocab, int draft_rows, int probs,
+                                       float temperature, size_t* bytes);
+BEBELM_API int bebelm_verify_drafts(const float* target, size_t target_stride, const float* draft, size_t draft_stride,
+                                    size_t n_seqs, size_t n_drafts, size_t vocab, int probs, float temperature,
+                                    const int32_t* tokens, const int32_t* n_per_seq, const float* u,
+                                    const float* u_sample, int32_t* out_tokens, int32_t* accepted, void* workspace,
+                                    size_t workspace_bytes, int mem, void* stream);
 
 /* ------------------------------------------------------------- GGUF weights ---
  * The reference's GGUF reader (src/gguf.rs): GgufFile::open memory-maps a file and

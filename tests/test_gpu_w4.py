@@ -1,0 +1,220 @@
+"""Products with 4-bit weights and group scales against the formula in 64 bits.
+
+Two kinds of inputs. Whole-numbered activations with scales that are powers of two: every product,
+group sum and total is a whole multiple of one power of two below 2^24 of them, so any order of f32 additions
+gives the exact result and the outputs must be equal. Normal activations: the products c - z times a
+bf16 term are exact; the tensor cores add 16 of them and the running sum per step, each addition within
+one f32 step (2^-23) of the sum of absolute terms A_g of the group; with s steps a group (group / 16 per
+bf16 term of an activation, 3 terms for f32) and 17 additions a step that is 17 s 2^-23 A_g. The groups
+are then scaled and added in f32: one rounding each for the scale product, the activations' scale and the
+addition, (groups + 2) 2^-24 A. A bf16 output adds half a step, 2^-8 of the value.
+"""
+import numpy as np
+import pytest
+import torch
+
+import bebelm_b200 as bb
+
+pytestmark = pytest.mark.gpu
+
+KINDS = {"f32": torch.float32, "bf16": torch.bfloat16, "int8": torch.int8}
+
+
+def weights(n_out, n_in, group, seed, zeros=True, scales=torch.float16, exact=False):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 256, (n_out, n_in // 2), device="cuda", generator=g, dtype=torch.uint8)
+    ng = n_in // group
+    if exact:
+        sc = torch.exp2(-torch.randint(0, 3, (n_out, ng), device="cuda", generator=g).float()).to(scales)
+    else:
+        sc = (0.02 * torch.randn(n_out, ng, device="cuda", generator=g)).to(scales)
+    z = torch.randint(0, 16, (n_out, ng), device="cuda", generator=g, dtype=torch.uint8) if zeros else None
+    return codes, sc, z
+
+
+def activations(t, n_in, kind, x_group, seed, exact=False):
+    g = torch.Generator(device="cuda").manual_seed(seed + 77)
+    if kind == "int8":
+        hi = 4 if exact else 128
+        x = torch.randint(-hi + 1, hi, (t, n_in), device="cuda", generator=g).to(torch.int8)
+        ng = n_in // x_group if x_group else 1
+        if exact:
+            xs = torch.exp2(-torch.randint(0, 3, (t, ng), device="cuda", generator=g).float())
+        else:
+            xs = 0.01 + torch.rand(t, ng, device="cuda", generator=g)
+        return x, xs
+    if exact:
+        return torch.randint(-3, 4, (t, n_in), device="cuda", generator=g).to(KINDS[kind]), None
+    return torch.randn(t, n_in, device="cuda", generator=g).to(KINDS[kind]), None
+
+
+def dense(codes, sc, z, group):
+    n_out, half = codes.shape
+    w = torch.empty(n_out, 2 * half, dtype=torch.float64, device=codes.device)
+    w[:, 0::2], w[:, 1::2] = (codes & 15).double(), (codes >> 4).double()
+    w -= 8 if z is None else z.double().repeat_interleave(group, 1)
+    return w * sc.double().repeat_interleave(group, 1)
+
+
+def floats(x, xs):
+    x = x.double()
+    return x if xs is None else x * xs.double().repeat_interleave(x.shape[1] // xs.shape[1], 1)
+
+
+def check(case, exact):
+    t, n_in, n_out, group, kind, x_group, zeros, sdt, ydt = case
+    codes, sc, z = weights(n_out, n_in, group, hash(case[:4]) & 0xffff, zeros, sdt, exact)
+    x, xs = activations(t, n_in, kind, x_group, n_in + t, exact)
+    w = bb.W4Weights(codes, sc, z, group=group)
+    y = w.matmul(x, xs, out_dtype=ydt)
+    assert y.shape == (t, n_out)
+    assert torch.equal(y, w.matmul(x, xs, out_dtype=ydt))  # the same bits again
+    wd, xd = dense(codes, sc, z, group), floats(x, xs)
+    want = xd @ wd.t()
+    if exact and ydt == bb.F32:
+        assert torch.equal(y.double(), want)
+    else:
+        a = xd.abs() @ wd.abs().t()
+        steps = max(1, group // 16) * (3 if kind == "f32" else 1)
+        tol = (17 * steps * 2.0 ** -23 + (n_in / min(group, x_group or group) + 2) * 2.0 ** -24) * a
+        if ydt == bb.BF16:
+            tol = tol * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs()
+        bad = (y.double() - want).abs() > tol
+        assert not bad.any(), (int(bad.sum()), float(((y.double() - want).abs() / a.clamp(min=1e-30)).max()))
+    w.close()
+
+
+CASES = [
+    # tokens, n_in, n_out, group, kind, x_group, zeros, scales, out
+    (1, 32, 1, 32, "f32", 0, False, torch.float16, bb.F32),
+    (1, 2048, 2048, 128, "f32", 0, True, torch.float16, bb.F32),
+    (1, 2048, 512, 32, "bf16", 0, True, torch.bfloat16, bb.F32),
+    (3, 96, 17, 32, "bf16", 0, True, torch.float16, bb.BF16),
+    (2, 192, 130, 64, "int8", 0, True, torch.float16, bb.F32),
+    (5, 2080, 515, 32, "f32", 0, True, torch.bfloat16, bb.F32),
+    (7, 1024, 100, 64, "int8", 32, False, torch.float16, bb.F32),
+    (8, 512, 333, 128, "int8", 256, True, torch.bfloat16, bb.F32),
+    (9, 768, 48, 256, "int8", 64, True, torch.float16, bb.BF16),
+    (16, 640, 1000, 640, "f32", 0, True, torch.float16, bb.F32),
+    (17, 2048, 129, 128, "bf16", 0, False, torch.float16, bb.BF16),
+    (31, 320, 64, 64, "f32", 0, True, torch.float16, bb.F32),
+    (32, 8192, 40, 128, "bf16", 0, True, torch.float16, bb.F32),
+    (33, 256, 200, 32, "f32", 0, True, torch.float16, bb.F32),
+    (64, 2048, 300, 128, "int8", 128, True, torch.float16, bb.F32),
+    (65, 416, 257, 32, "int8", 0, False, torch.bfloat16, bb.F32),
+    (100, 1024, 128, 256, "bf16", 0, True, torch.float16, bb.BF16),
+    (129, 160, 385, 32, "bf16", 0, True, torch.float16, bb.F32),
+    (200, 2048, 2048, 64, "f32", 0, True, torch.bfloat16, bb.F32),
+    (257, 512, 640, 128, "int8", 32, True, torch.float16, bb.BF16),
+    (513, 1280, 1000, 128, "bf16", 0, True, torch.float16, bb.F32),
+]
+IDS = ["-".join(str(v).replace("torch.", "") for v in c) for c in CASES]
+
+
+@pytest.mark.parametrize("case", CASES, ids=IDS)
+def test_exact_in_whole_numbers(case):
+    check(case, True)
+
+
+@pytest.mark.parametrize("case", CASES, ids=IDS)
+def test_normal_activations(case):
+    check(case, False)
+
+
+def test_many_rows_stream():
+    """A vocabulary-sized matrix: every persistent CTA takes several tiles."""
+    check((5, 2048, 60001, 128, "int8", 256, False, torch.float16, bb.F32), False)
+    check((1, 1024, 70000, 64, "bf16", 0, True, torch.float16, bb.F32), True)
+
+
+def test_host_buffers_and_numpy_weights():
+    codes, sc, z = weights(300, 512, 64, 5)
+    x, _ = activations(6, 512, "f32", 0, 1)
+    xi, xs = activations(6, 512, "int8", 128, 1)
+    wd = bb.W4Weights(codes, sc, z, group=64)
+    wh = bb.W4Weights(codes.cpu().numpy(), sc.cpu().numpy(), z.cpu().numpy(), group=64)
+    wc = bb.W4Weights(codes.cpu(), sc.cpu(), z.cpu(), group=64)
+    want = wd.matmul(x).cpu().numpy()
+    for w in (wh, wc):
+        np.testing.assert_array_equal(w.matmul(x).cpu().numpy(), want)
+        np.testing.assert_array_equal(w.matmul(x.cpu().numpy()), want)
+        np.testing.assert_array_equal(w.matmul(xi.cpu().numpy(), xs.cpu().numpy()), wd.matmul(xi, xs).cpu().numpy())
+    np.testing.assert_array_equal(wh.matmul(x[0].cpu().numpy()), want[0])
+    assert torch.equal(wd.matmul(x[2]), wd.matmul(x[2:3])[0])
+
+
+@pytest.mark.parametrize("t", [1, 6, 40, 150])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "int8"])
+def test_strided_and_unaligned_rows(kind, t):
+    codes, sc, z = weights(260, 416, 32, 9)
+    w = bb.W4Weights(codes, sc, z, group=32)
+    big, xs = activations(t, 433, kind, 0, 3)
+    for off in (0, 1, 5, 16):
+        view = big[:, off:off + 416]
+        assert torch.equal(w.matmul(view, xs), w.matmul(view.contiguous(), xs)), off
+    wide, _ = activations(t, 480, kind, 0, 3)  # aligned rows with a gap
+    assert torch.equal(w.matmul(wide[:, :416], xs), w.matmul(wide[:, :416].contiguous(), xs))
+
+
+@pytest.mark.parametrize("t", [3, 70])
+def test_infinities_and_nan_stay_in_their_token(t):
+    codes, sc, z = weights(64, 256, 64, 2)
+    w = bb.W4Weights(codes, sc, z, group=64)
+    for kind in ("f32", "bf16"):
+        x, _ = activations(t, 256, kind, 0, 8)
+        clean = w.matmul(x, out_dtype=bb.F32)
+        x[1, 5] = float("inf")
+        x[2, 7] = float("nan")
+        y = w.matmul(x, out_dtype=bb.F32)
+        assert not torch.isfinite(y[1]).any() and torch.isnan(y[2]).all()
+        assert torch.equal(y[0], clean[0]) and torch.equal(y[3:], clean[3:])
+
+
+def test_the_largest_sums():
+    """A group's sum is formed in f32 before its scale: finite up to the documented limit, where the
+    sum of |code - zero| |x| reaches the largest float. (The split of an activation does not overflow.)"""
+    codes, sc, z = weights(64, 256, 64, 2)
+    w = bb.W4Weights(codes, sc, z, group=64)
+    for t in (1, 50):
+        x = torch.zeros((t, 256), device="cuda")
+        x[:, 0] = 2.2e37  # 15 times that is below 3.4e38
+        want = x.double() @ dense(codes, sc, z, 64).t()
+        y = w.matmul(x).double()
+        assert ((y - want).abs() <= 2.0 ** -20 * want.abs()).all()
+
+
+def test_no_tokens_and_output_neighbours():
+    codes, sc, z = weights(100, 256, 128, 6)
+    w = bb.W4Weights(codes, sc, z, group=128)
+    assert w.matmul(torch.empty(0, 256, device="cuda")).shape == (0, 100)
+    for t in (1, 9, 40, 129):
+        buf = torch.full((t + 2, 100), 5.0, device="cuda")
+        x, _ = activations(t, 256, "f32", 0, 1)
+        w.matmul(x, out=buf[1:t + 1])
+        assert (buf[0] == 5).all() and (buf[t + 1] == 5).all()
+        assert torch.equal(buf[1:t + 1], w.matmul(x))
+
+
+@pytest.mark.parametrize("t", [1, 8, 48, 200])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "int8"])
+def test_two_streams_and_a_graph(kind, t):
+    """Products of one handle on two streams at once, and replayed from a graph with new activations."""
+    codes, sc, z = weights(512, 1024, 128, 3)
+    w = bb.W4Weights(codes, sc, z, group=128)
+    a, xs = activations(t, 1024, kind, 128 if kind == "int8" else 0, 1)
+    b, _ = activations(t, 1024, kind, 128 if kind == "int8" else 0, 2)
+    wa, wb = w.matmul(a, xs), w.matmul(b, xs)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        got += [(w.matmul(a, xs, stream=s1), wa), (w.matmul(b, xs, stream=s2), wb)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in got)
+    static, out = a.clone(), torch.empty_like(wa)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.matmul(static, xs, out=out)
+    static.copy_(b)
+    graph.replay()
+    assert torch.equal(out, wb)
