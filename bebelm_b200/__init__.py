@@ -157,7 +157,7 @@ def load_library(path: str = LIB_PATH):
         "bebelm_add_rmsnorm": ([vp, sz, vp, sz, i, sz, sz, vp, f, vp, sz, vp, i, vp, sz, i, vp], i),
         "bebelm_w4_create": ([i, sz, sz, sz, vp, vp, i, vp, i, C.POINTER(vp)], i),
         "bebelm_w4_destroy": ([vp], i),
-        "bebelm_w4_workspace": ([vp, vp, i, sz, sz, C.POINTER(sz)], i),
+        "bebelm_w4_workspace": ([vp, vp, i, sz, sz, sz, C.POINTER(sz)], i),
         "bebelm_w4_matmul": ([vp, vp, i, sz, vp, sz, sz, vp, i, vp, sz, i, vp], i),
         "bebelm_verify_workspace": ([sz, sz, sz, i, i, f, C.POINTER(sz)], i),
         "bebelm_verify_drafts": ([vp, sz, vp, sz, sz, sz, sz, i, f, vp, vp, vp, vp, vp, vp, vp, sz, i, vp], i),
@@ -1011,7 +1011,7 @@ class W4Weights:
         y = _out_tensor(out, shape, torch.float32 if od == F32 else torch.bfloat16, dev, "out")
         xp = x.data_ptr()
         need = C.c_size_t()
-        _check(L.bebelm_w4_workspace(self._h, xp, dt, xs, t, C.byref(need)))
+        _check(L.bebelm_w4_workspace(self._h, xp, dt, xs, xg, t, C.byref(need)))
         ws, wp, wb = _workspace(workspace, need.value, dev, stream)
         _check(L.bebelm_w4_matmul(self._h, xp, dt, xs, sp, xg, t, y.data_ptr(), od, wp, wb, MEM_DEVICE,
                                   _stream_on(stream, dev)))

@@ -2692,7 +2692,7 @@ int w4_fill(bebelm_w4* W, const uint8_t* codes, const void* scales, const uint8_
     const bool host = mem == BEBELM_MEM_HOST;
     TRY(W->codes.ensure(tiles * 1024));
     TRY(W->scales.ensure(ns * 2));
-    if (zeros) TRY(W->zeros.ensure(ns));
+    if (zeros) TRY(W->zeros.ensure(tiles * 8 * (v.per_chunk == 4 ? 8 : 4)));
     TRY(W->err.ensure());
     TRY(tmp.ensure(256 + (host ? pad256(cb) + pad256(2 * ng) + pad256(ng) : 0)));
     CUDA_TRY(cudaMemset(tmp.p, 0, 256));
@@ -2715,6 +2715,24 @@ int w4_fill(bebelm_w4* W, const uint8_t* codes, const void* scales, const uint8_
     v.scales = W->scales.as<uint32_t>();
     v.zeros = zeros ? W->zeros.as<unsigned short>() : nullptr;
     return 0;
+}
+
+// Few tokens are bound by the weights' bytes, many by the products: the streaming kernel up to 16
+// tokens, the tensor cores' tiles above.
+constexpr size_t kW4StreamTokens = 16;
+size_t w4_scratch(const W4View& w, const W4X& x) {
+    return x.tokens <= kW4StreamTokens ? w4_stream_workspace(w, x) : w4_tc_workspace(w, x);
+}
+cudaError_t w4_run(const bebelm_w4* W, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms, cudaStream_t s) {
+    if (x.tokens <= kW4StreamTokens) return launch_w4_stream(W->v, x, y, y_bf16, workspace, num_sms, s);
+    return launch_w4_tc(W->v, x, y, y_bf16, workspace, W->err.d, s);
+}
+
+int w4_timeout(const bebelm_w4* W) {
+    const int e = W->err.read();
+    if (!e) return 0;
+    *reinterpret_cast<volatile int*>(W->err.h) = 0;
+    return fail(BEBELM_ERR_TIMEOUT, "a device-side wait of a 4-bit product timed out (code %d)", e);
 }
 
 int w4_x(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, const float* x_scales, size_t x_group,
@@ -2791,11 +2809,12 @@ int bebelm_w4_destroy(bebelm_w4* W) {
     return 0;
 }
 
-int bebelm_w4_workspace(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, size_t n_tokens, size_t* bytes) {
+int bebelm_w4_workspace(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, size_t x_group, size_t n_tokens,
+                        size_t* bytes) {
     if (!W || !bytes) return fail(BEBELM_ERR_INVALID, "null argument");
     W4X xv;
-    TRY(w4_x(W, x, x_dtype, x_stride, nullptr, 0, n_tokens, &xv));
-    *bytes = w4_workspace(W->v, xv);
+    TRY(w4_x(W, x, x_dtype, x_stride, nullptr, x_group, n_tokens, &xv));
+    *bytes = w4_scratch(W->v, xv);
     return 0;
 }
 
@@ -2816,12 +2835,13 @@ int bebelm_w4_matmul(const bebelm_w4* W, const void* x, int x_dtype, size_t x_st
     DeviceGuard g(W->device);
     cudaStream_t s = as_stream(stream);
     const int sms = num_sms_of(W->device);
+    TRY(w4_timeout(W));  // of an earlier device-memory call
     if (mem == BEBELM_MEM_DEVICE) {
-        const size_t need = w4_workspace(v, xv);
+        const size_t need = w4_scratch(v, xv);
         if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
             return fail(BEBELM_ERR_INVALID, "the product needs %zu bytes of workspace, 256-byte aligned (got %zu)", need,
                         workspace ? workspace_bytes : 0);
-        CUDA_TRY(launch_w4_stream(v, xv, y, y_dtype == BEBELM_BF16, workspace, sms, s));
+        CUDA_TRY(w4_run(W, xv, y, y_dtype == BEBELM_BF16, workspace, sms, s));
         return 0;
     }
     std::lock_guard<std::mutex> lk(g_scratch_mu);
@@ -2834,9 +2854,10 @@ int bebelm_w4_matmul(const bebelm_w4* W, const void* x, int x_dtype, size_t x_st
     xv.x = dx;
     xv.scales = static_cast<const float*>(dsc);
     xv.stride = v.n_in;
-    TRY(P->q8.ensure(std::max<size_t>(w4_workspace(v, xv), 256), false, s));
-    CUDA_TRY(launch_w4_stream(v, xv, o, y_dtype == BEBELM_BF16, P->q8.p, sms, s));
-    return stage_out(P, o, y, yb, s);
+    TRY(P->q8.ensure(std::max<size_t>(w4_scratch(v, xv), 256), false, s));
+    CUDA_TRY(w4_run(W, xv, o, y_dtype == BEBELM_BF16, P->q8.p, sms, s));
+    TRY(stage_out(P, o, y, yb, s));
+    return w4_timeout(W);
 }
 
 int bebelm_verify_workspace(size_t n_seqs, size_t n_drafts, size_t vocab, int draft_rows, int probs, float temperature,

@@ -360,10 +360,14 @@ struct W4X {
 // *bad is set where a zero point is above 127
 cudaError_t launch_w4_pack(const uint8_t* codes, const unsigned short* scales, const uint8_t* zeros, const W4View& w,
                            uint32_t* out_c, unsigned short* out_s, uint8_t* out_z, int* bad, cudaStream_t s);
-cudaError_t launch_w4_planes(const W4X& x, size_t kp, __nv_bfloat16* out, cudaStream_t s);
-size_t w4_workspace(const W4View& w, const W4X& x);  // bytes of device scratch a product needs
+// Few tokens (w4.cu) and many (w4_tc.cu): device scratch in bytes, and the product.
+size_t w4_stream_workspace(const W4View& w, const W4X& x);
+size_t w4_tc_workspace(const W4View& w, const W4X& x);
 cudaError_t launch_w4_stream(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms,
                              cudaStream_t s);
+// cudaErrorNotSupported (nothing launched) where the activations cannot be described to TMA. A bounded wait
+// that gives up stores kErrWaitTimeout to *err.
+cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int* err, cudaStream_t s);
 
 // ---- drafted tokens against the target's rows (verify.cu) ----
 struct VerifyArgs {

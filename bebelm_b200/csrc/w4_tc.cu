@@ -1,0 +1,543 @@
+// Products with 4-bit weights and group scales for many tokens, on the 5th-generation tensor cores.
+//
+//     y[t][n] = Σ_g s[n][g] · sx[t][g'] · Σ_{k in g} (c[n][k] - z[n][g]) · x[t][k]
+//
+// A = c - z (128 rows of weights, 16-bit floats, exact), B = activations (N tokens), D = the inner sum in f32
+// (`tcgen05.mma kind::f16`, M 128). The scales stay out of the operands: a group's sum is read from TMEM and
+// added, times its scale, to running f32 sums in registers, so nothing is rounded to 16 bits. Activations:
+//   bf16: as they are (bf16 MMA), straight from the caller's rows by TMA.
+//   int8: as f16 (exact).
+//   f32: the sum of two f16 terms of x · 2^e, with e a token's, chosen so that its largest magnitude comes to
+//        [2^14, 2^15). The terms hold x to 2^-24 of its value, half a step of f32 (and to 2^-39 of the token's
+//        largest where the second term runs out of exponent). 2^-e is applied with the output.
+// w4_terms_kernel writes the last two as [terms][tokens][kp].
+//
+// One CTA per 128 rows x N tokens, one CTA an SM, 16 warps:
+//   warp 0       TMA: per 128 inputs the weights' codes, scales and zero points (three bulk copies: they lie together,
+//                see w4.cu) and the activations' 128-byte-swizzled tiles, through a ring.
+//   warp 1       issues the MMAs, A from TMEM, B from shared memory.
+//   warps 4-7    unpack codes to A in TMEM, two buffers of 128 inputs: a warp's lanes hold (row g and g + 8,
+//                pairs 4 i + q), the fragment of `tcgen05.st.16x128b`. A never passes through shared memory,
+//                whose bandwidth the MMA needs for B.
+//   warps 8-15   read each group's sums (two buffers), scale and add them; a thread has a row and N / 2 tokens.
+// Bound: the tensor pipe for many tokens (a group of 128: 8 MMAs of N / 2 cycles each against ~N cycles of TMEM reads
+// and N / 2 FMAs a thread). All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
+// MMAs in flight, reports kErrWaitTimeout and stores nothing.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "internal.h"
+
+namespace bebelm {
+namespace {
+
+constexpr int kM = 128, kK = 128, kThreads = 512;
+constexpr int kConvert0 = 4, kEpi0 = 8;  // first converter and first epilogue warp
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColA = 256;          // two A buffers of 64 columns behind the accumulators (2 x N columns)
+constexpr long long kWaitLimit = 1ll << 22;
+constexpr size_t kRing = 200 * 1024;     // shared memory for the ring
+
+struct TcArgs {
+    W4View w;
+    void* y;
+    size_t tokens;
+    const float* col_scale;   // [tokens]: one factor a token, or null
+    const float* x_scales;    // [n_groups][tokens padded to 128]: a factor per group of inputs, or null
+    size_t x_pitch;
+    int x_shift;              // log2 of that group
+    int fb;                   // blocks of 32 inputs whose sum is scaled together: 1, 2 or 4
+    int y_bf16, stages, plane_rows;  // plane_rows: rows of B between the terms
+    int* err;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {  // 128B swizzle, K-major, SBO 1024, version 1
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(16 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// kind::f16, f32 accumulator, A and B both bf16 or both f16, K-major, M = 128
+__host__ __device__ constexpr uint32_t instr_desc(int n, bool bf16) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity) {
+    for (long long it = 0; it < kWaitLimit; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// 16 lanes x 64 columns: registers 2 i and 2 i + 1 of lane (g, q) go to column 4 i + q of lanes g and g + 8
+__device__ __forceinline__ void tmem_st_tile(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// 32 lanes x 16 columns; tmem_ld_wait() before the registers are used
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// word of 8 codes to 4 pairs of c - z: 128 + c less 128 + z in bf16, 1024 + c less 1024 + z in f16
+template <bool BF16>
+__device__ __forceinline__ void pairs(uint32_t w, uint32_t zz, uint32_t* o) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t u = ((w >> (4 * j)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
+        if constexpr (BF16) {
+            const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&zz));
+            o[j] = *reinterpret_cast<const uint32_t*>(&a);
+        } else {
+            const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&zz));
+            o[j] = *reinterpret_cast<const uint32_t*>(&a);
+        }
+    }
+}
+
+__device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
+    if (bf16) return __uint_as_float(h << 16);
+    __half_raw r;
+    r.x = (unsigned short)h;
+    return __half2float(__half(r));
+}
+
+template <int N, int TERMS>
+struct Lay {
+    static constexpr int kAtom = N * 128;             // N tokens x 64 inputs
+    static constexpr int kB = 2 * TERMS * kAtom;      // [term][half]
+    static constexpr int kCodes = kB, kScales = kCodes + 8192, kZeros = kScales + 1024;
+    static constexpr int kStage = kZeros + 512 + (1024 - 512) % 1024;  // scales <= 1024 B, zero points <= 512 B
+    static constexpr int kStages = (int)(kRing / kStage) < 6 ? (int)(kRing / kStage) : 6;
+    static constexpr int kSmem = kStages * kStage + 1024;
+};
+
+template <int N, int TERMS, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, TcArgs a) {
+    using L = Lay<N, TERMS>;
+    constexpr int S = L::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sb = smem_u32(sm);
+    __shared__ uint64_t s_bar[2 * S + 9];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_fail;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rb = blockIdx.x, t0 = (int)blockIdx.y * N, chunks = (int)a.w.chunks, pc = a.w.per_chunk;
+    const uint32_t bars = smem_u32(s_bar);
+    auto full = [&](int i) { return bars + 8 * i; };
+    auto empty = [&](int i) { return bars + 8 * (S + i); };
+    auto a_full = [&](int i) { return bars + 8 * (2 * S + i); };
+    auto a_empty = [&](int i) { return bars + 8 * (2 * S + 2 + i); };
+    auto d_full = [&](int i) { return bars + 8 * (2 * S + 4 + i); };
+    auto d_empty = [&](int i) { return bars + 8 * (2 * S + 6 + i); };
+    const uint32_t drained = bars + 8 * (2 * S + 8);
+
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 32) {
+        auto init = [&](uint32_t b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n)); };
+        for (int i = 0; i < S; ++i) {
+            init(full(i), 1);
+            init(empty(i), 5);  // the stage's MMAs, and the four converter warps that read its codes
+        }
+        for (int i = 0; i < 2; ++i) init(a_full(i), 4), init(a_empty(i), 1), init(d_full(i), 1), init(d_empty(i), 8);
+        init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        s_fail = 0;
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = s_tmem;
+    const int per_flush = a.fb, flushes = 4 / per_flush;  // sums a chunk
+    // scales and activations' terms may come from the kernel before
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t zb = a.w.zeros ? 64u * (pc == 4 ? 8 : 4) : 0u, scb = 256u * (uint32_t)pc;
+            const unsigned char* code = reinterpret_cast<const unsigned char*>(a.w.codes) + (size_t)rb * chunks * 8192;
+            const unsigned char* scale = reinterpret_cast<const unsigned char*>(a.w.scales) + (size_t)rb * chunks * scb;
+            const unsigned char* zero = reinterpret_cast<const unsigned char*>(a.w.zeros) + (size_t)rb * chunks * zb;
+            int issued = 0;
+            for (int c = 0; c < chunks; ++c) {
+                const int st = c % S;
+                if (c >= S && !mbar_wait(empty(st), ((c / S) - 1) & 1)) {
+                    s_fail = 1;
+                    break;
+                }
+                const uint32_t base = sb + st * L::kStage;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(st)), "r"((uint32_t)L::kB + 8192u + scb + zb)
+                             : "memory");
+                bulk(base + L::kCodes, code + (size_t)c * 8192, 8192, full(st));
+                bulk(base + L::kScales, scale + (size_t)c * scb, scb, full(st));
+                if (zb) bulk(base + L::kZeros, zero + (size_t)c * zb, zb, full(st));
+#pragma unroll
+                for (int p = 0; p < TERMS; ++p)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        tma_2d(base + (2 * p + h) * L::kAtom, &tm_x, c * kK + 64 * h, t0 + p * a.plane_rows, full(st));
+                issued = c + 1;
+            }
+            // nothing may be in flight when the CTA exits
+            for (int c = issued > S ? issued - S : 0; c < issued; ++c) mbar_wait(full(c % S), (c / S) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = instr_desc(N, BF16);
+            int u = 0;  // sums so far
+            bool ok = true;
+            for (int c = 0; ok && c < chunks; ++c) {
+                const int st = c % S, ab = c & 1;
+                ok = mbar_wait(full(st), (c / S) & 1) && mbar_wait(a_full(ab), (c >> 1) & 1);
+                for (int f = 0; ok && f < flushes; ++f, ++u) {
+                    const int db = u & 1;
+                    if (u >= 2 && !mbar_wait(d_empty(db), ((u >> 1) - 1) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_after();
+                    for (int k = 2 * per_flush * f; k < 2 * per_flush * (f + 1); ++k) {  // 16 inputs: 8 columns of A, 32 bytes of B
+#pragma unroll
+                        for (int p = 0; p < TERMS; ++p)
+                            mma_ts(tmem + db * N, tmem + kColA + 64 * ab + 8 * k,
+                                   smem_desc(sb + st * L::kStage + (2 * p + (k >> 2)) * L::kAtom + (k & 3) * 32), idesc,
+                                   k > 2 * per_flush * f || p > 0);
+                    }
+                    commit(d_full(db));
+                }
+                if (ok) {
+                    commit(empty(st));
+                    commit(a_empty(ab));
+                }
+            }
+            if (!ok) s_fail = 1;
+            commit(drained);  // every MMA of this CTA done, also after a failed wait
+            mbar_wait(drained, 0);
+        }
+    } else if (warp >= kConvert0 && warp < kEpi0) {
+        const int w = warp - kConvert0, g = lane >> 2;
+        bool ok = true;
+        for (int c = 0; c < chunks; ++c) {
+            const int st = c % S, ab = c & 1;
+            ok = mbar_wait(full(st), (c / S) & 1) && (c < 2 || mbar_wait(a_empty(ab), ((c >> 1) - 1) & 1));
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_after();
+            const unsigned char* base = sm + st * L::kStage;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {  // tiles of 16 rows
+                const int tile = 2 * w + m;
+                const uint4 va = *reinterpret_cast<const uint4*>(base + L::kCodes + tile * 1024 + lane * 16);
+                const uint4 vb = *reinterpret_cast<const uint4*>(base + L::kCodes + tile * 1024 + 512 + lane * 16);
+                const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+                uint32_t r[32];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t z0 = 8, z1 = 8;
+                    if (a.w.zeros) {
+                        const unsigned char* z = base + L::kZeros + (tile * 8 + g) * (pc == 4 ? 8 : 4) + 2 * (b * pc / 4);
+                        z0 = z[0], z1 = z[1];
+                    }
+                    const uint32_t one = BF16 ? 0x43004300u : 0x64006400u;
+                    uint32_t pa[4], pb[4];
+                    pairs<BF16>(wa[b], one + z0 * 0x10001u, pa);
+                    pairs<BF16>(wb[b], one + z1 * 0x10001u, pb);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r[2 * (4 * b + j)] = pa[j], r[2 * (4 * b + j) + 1] = pb[j];
+                }
+                tmem_st_tile(tmem + ((uint32_t)(32 * w + 16 * m) << 16) + kColA + 64 * ab, r);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(a_full(ab)), mbar_arrive(empty(st));
+        }
+        if (!ok && lane == 0) s_fail = 1;
+    } else if (warp >= kEpi0) {
+        constexpr int C = N / 2;  // columns of a thread
+        const int w = warp - kEpi0, half = w >> 2, row = 32 * (w & 3) + lane;
+        const uint32_t t_d = tmem + ((uint32_t)(32 * (w & 3)) << 16) + half * C;
+        // this row's scales: [tile][row % 8][block][row / 8]
+        const int tile = row >> 4, g = row & 7, h = (row >> 3) & 1;
+        const unsigned short* sp = reinterpret_cast<const unsigned short*>(a.w.scales) + ((size_t)rb * chunks * 64 + tile * 8 + g) * pc * 2 + h;
+        const int total = chunks * flushes;
+        float acc[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) acc[i] = 0.f;
+        auto scale_at = [&](int u) -> float {
+            const int c = u / flushes, blk = (u % flushes) * per_flush * pc / 4;
+            return scale_of(sp[((size_t)c * 64 * pc + blk) * 2], a.w.scale_bf16);
+        };
+        float s_next = scale_at(0);
+        bool ok = true;
+        for (int u = 0; u < total; ++u) {
+            const float s = s_next;
+            if (u + 1 < total) s_next = scale_at(u + 1);
+            ok = __all_sync(0xffffffffu, mbar_wait(d_full(u & 1), (u >> 1) & 1));
+            if (!ok) break;
+            tc_after();
+            const size_t k = (size_t)(u / flushes) * kK + (size_t)(u % flushes) * per_flush * 32;
+            const float* xs = a.x_scales ? a.x_scales + (k >> a.x_shift) * a.x_pitch + t0 + half * C : nullptr;
+            constexpr int B = C < 32 ? C : 32;  // columns in registers at a time
+#pragma unroll
+            for (int c = 0; c < C; c += B) {
+                uint32_t d[B];
+#pragma unroll
+                for (int i = 0; i < B; i += 16) tmem_ld16(t_d + (u & 1) * N + c + i, d + i);
+                tmem_ld_wait();
+                if (c + B == C) {
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(d_empty(u & 1));
+                }
+                if (xs) {
+                    if (k < a.w.n_in) {  // padded inputs have no scale: their sum is zero
+#pragma unroll
+                        for (int i = 0; i < B; i += 4) {
+                            const float4 f = __ldg(reinterpret_cast<const float4*>(xs + c + i));
+                            acc[c + i] = fmaf(__uint_as_float(d[i]) * f.x, s, acc[c + i]);
+                            acc[c + i + 1] = fmaf(__uint_as_float(d[i + 1]) * f.y, s, acc[c + i + 1]);
+                            acc[c + i + 2] = fmaf(__uint_as_float(d[i + 2]) * f.z, s, acc[c + i + 2]);
+                            acc[c + i + 3] = fmaf(__uint_as_float(d[i + 3]) * f.w, s, acc[c + i + 3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < B; ++i) acc[c + i] = fmaf(__uint_as_float(d[i]), s, acc[c + i]);
+                }
+            }
+        }
+        if (!ok) {
+            if (lane == 0) s_fail = 1;
+        } else {
+            const size_t r = (size_t)rb * kM + row;
+            if (r < a.w.n_out) {
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    const size_t t = (size_t)t0 + half * C + i;
+                    if (t >= a.tokens) break;
+                    const float v = a.col_scale ? acc[i] * __ldg(a.col_scale + t) : acc[i];
+                    if (a.y_bf16)
+                        static_cast<__nv_bfloat16*>(a.y)[t * a.w.n_out + r] = __float2bfloat16_rn(v);
+                    else
+                        static_cast<float*>(a.y)[t * a.w.n_out + r] = v;
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_before();
+    __syncthreads();
+    if (tid == 0 && *reinterpret_cast<volatile int*>(&s_fail)) *reinterpret_cast<volatile int*>(a.err) = kErrWaitTimeout;
+    if (warp == 0) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
+}
+
+// A token's row as 16-bit terms with zeros up to kp, and its factor. f32: two f16 terms of x · 2^e, factor 2^-e;
+// int8: f16, factor its scale (when it has one for the row); bf16: copied. Grouped scales are transposed.
+__global__ void __launch_bounds__(256) w4_terms_kernel(W4X x, size_t kp, uint16_t* out, float* col_scale, float* x_scales,
+                                                       size_t x_pitch) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    __shared__ float s_max[8];
+    const size_t plane = x.tokens * kp;
+    for (size_t t = blockIdx.x; t < x.tokens; t += gridDim.x) {
+        uint16_t* o = out + t * kp;
+        if (x.kind == kW4XF32) {
+            const float* p = static_cast<const float*>(x.x) + t * x.stride;
+            float m = 0.f;
+            for (size_t k = threadIdx.x; k < x.n_in; k += 256) m = fmaxf(m, fabsf(p[k]));
+#pragma unroll
+            for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, s_max[i]);
+            // 2^e with m 2^e in [2^14, 2^15); an infinity or only zeros: e = 0. Two factors, since 2^e may
+            // itself be out of f32's range.
+            const int em = (int)(__float_as_uint(m) >> 23);
+            const int e = m > 0.f && em < 255 ? 14 - (max(em, 1) - 127) : 0, e1 = e / 2, e2 = e - e1;
+            const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23), f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+            if (threadIdx.x == 0) col_scale[t] = ldexpf(1.f, -e);
+            for (size_t k = 2 * threadIdx.x; k < kp; k += 512) {
+                uint32_t hi = 0, lo = 0;
+                if (k < x.n_in) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float v = p[k + j] * f1 * f2;
+                        const __half a = __float2half_rn(v);
+                        const float rest = v - __half2float(a);
+                        const __half b = __float2half_rn(fabsf(rest) <= 65504.f ? rest : 0.f);  // v not finite: no second term
+                        hi |= (uint32_t)__half_as_ushort(a) << (16 * j), lo |= (uint32_t)__half_as_ushort(b) << (16 * j);
+                    }
+                }
+                *reinterpret_cast<uint32_t*>(o + k) = hi;
+                *reinterpret_cast<uint32_t*>(o + plane + k) = lo;
+            }
+        } else {
+            for (size_t k = 2 * threadIdx.x; k < kp; k += 512) {
+                uint32_t v = 0;
+                if (k < x.n_in) {
+                    if (x.kind == kW4XInt8) {
+                        const signed char* p = static_cast<const signed char*>(x.x) + t * x.stride + k;
+                        v = (uint32_t)__half_as_ushort(__short2half_rn(p[0])) | (uint32_t)__half_as_ushort(__short2half_rn(p[1])) << 16;
+                    } else {
+                        const unsigned short* p = static_cast<const unsigned short*>(x.x) + t * x.stride + k;
+                        v = (uint32_t)p[0] | (uint32_t)p[1] << 16;
+                    }
+                }
+                *reinterpret_cast<uint32_t*>(o + k) = v;
+            }
+            if (x_scales)
+                for (size_t j = threadIdx.x; j < x.n_groups; j += 256) x_scales[j * x_pitch + t] = x.scales[t * x.n_groups + j];
+        }
+    }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+
+// bf16 rows that TMA can read as they are
+bool direct_rows(const W4X& x) {
+    return x.kind == kW4XBf16 && (reinterpret_cast<uintptr_t>(x.x) & 15) == 0 && x.stride % 8 == 0;
+}
+size_t pad(size_t n, size_t to) { return (n + to - 1) / to * to; }
+size_t terms_bytes(const W4View& w, const W4X& x) {
+    return pad((x.kind == kW4XF32 ? 2 : 1) * x.tokens * w.chunks * kK * 2, 256);
+}
+
+template <int N, int TERMS, bool BF16>
+cudaError_t run(const CUtensorMap& tm, TcArgs& a, bool pdl, cudaStream_t s) {
+    using L = Lay<N, TERMS>;
+    auto kernel = w4_tc_kernel<N, TERMS, BF16>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.w.tile_rows / 8), (unsigned)((a.tokens + N - 1) / N));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = L::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, tm, a);
+}
+template <int N>
+cudaError_t run_kind(const CUtensorMap& tm, TcArgs& a, int kind, bool pdl, cudaStream_t s) {
+    return kind == kW4XBf16  ? run<N, 1, true>(tm, a, pdl, s)
+           : kind == kW4XF32 ? run<N, 2, false>(tm, a, pdl, s)
+                             : run<N, 1, false>(tm, a, pdl, s);
+}
+
+}  // namespace
+
+size_t w4_tc_workspace(const W4View& w, const W4X& x) {
+    if (direct_rows(x)) return 0;
+    size_t n = terms_bytes(w, x) + pad(4 * x.tokens, 256);
+    if (x.group) n += 4 * x.n_groups * pad(x.tokens, 128);
+    return n;
+}
+
+cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int* err, cudaStream_t s) {
+    const auto enc = map_encoder();
+    const size_t kp = w.chunks * kK, terms = x.kind == kW4XF32 ? 2 : 1;
+    if (!enc || x.tokens * terms >= (1ull << 31) || x.tokens > 65535 * size_t(32)) return cudaErrorNotSupported;
+    TcArgs a{};
+    a.w = w;
+    a.y = y, a.y_bf16 = y_bf16, a.tokens = x.tokens, a.err = err;
+    a.fb = 4 / w.per_chunk;
+    if (x.group) a.fb = std::min(a.fb, x.group / 32);
+    const bool direct = direct_rows(x);
+    const void* rows = x.x;
+    size_t stride = x.stride, n_in = x.n_in;
+    const int n_tile = x.tokens <= 32 ? 32 : x.tokens <= 64 ? 64 : 128;
+    if (!direct) {
+        uint16_t* t = static_cast<uint16_t*>(workspace);
+        float* col = reinterpret_cast<float*>(static_cast<char*>(workspace) + terms_bytes(w, x));
+        float* xs = reinterpret_cast<float*>(reinterpret_cast<char*>(col) + pad(4 * x.tokens, 256));
+        a.x_pitch = pad(x.tokens, 128);
+        a.x_scales = x.group ? xs : nullptr;
+        a.x_shift = x.group_shift;
+        a.col_scale = x.kind == kW4XF32 ? col : x.kind == kW4XInt8 && !x.group ? x.scales : nullptr;
+        w4_terms_kernel<<<(unsigned)std::min<size_t>(x.tokens, 1 << 20), 256, 0, s>>>(x, kp, t, col, x.group ? xs : nullptr, a.x_pitch);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        rows = t;
+        stride = n_in = kp;
+        a.plane_rows = (int)x.tokens;
+    }
+    CUtensorMap tm;
+    const cuuint64_t dims[2] = {(cuuint64_t)n_in, (cuuint64_t)(x.tokens * terms)};
+    const cuuint64_t strides[1] = {(cuuint64_t)(stride * 2)};
+    const cuuint32_t box[2] = {64, (cuuint32_t)n_tile}, es[2] = {1, 1};
+    if (enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(rows), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    return n_tile == 32   ? run_kind<32>(tm, a, x.kind, !direct, s)
+           : n_tile == 64 ? run_kind<64>(tm, a, x.kind, !direct, s)
+                          : run_kind<128>(tm, a, x.kind, !direct, s);
+}
+
+}  // namespace bebelm

@@ -410,10 +410,9 @@ typedef struct bebelm_w4 bebelm_w4;
 BEBELM_API int bebelm_w4_create(int device, size_t n_in, size_t n_out, size_t group, const uint8_t* codes,
                                 const void* scales, int scale_dtype, const uint8_t* zeros, int mem, bebelm_w4** out);
 BEBELM_API int bebelm_w4_destroy(bebelm_w4* w);
-/* Device scratch of a product of these activations (x only for its alignment: BEBELM_BF16 rows that
- * are 16-byte aligned need none). */
-BEBELM_API int bebelm_w4_workspace(const bebelm_w4* w, const void* x, int x_dtype, size_t x_stride, size_t n_tokens,
-                                   size_t* bytes);
+/* Device scratch that a product of these activations needs (0 for many; x only for its alignment). */
+BEBELM_API int bebelm_w4_workspace(const bebelm_w4* w, const void* x, int x_dtype, size_t x_stride, size_t x_group,
+                                   size_t n_tokens, size_t* bytes);
 /* x [n_tokens][n_in] in x_dtype, rows x_stride elements apart: BEBELM_F32, BEBELM_BF16, or BEBELM_INT8
  * with x_scales [n_tokens][n_in / x_group] (x_group 32, 64, 128 or 256, or 0: one scale a token), as
  * bebelm_add_rmsnorm writes them. y [n_tokens][n_out] in y_dtype (BEBELM_F32 or BEBELM_BF16). Activations are

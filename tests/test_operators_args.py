@@ -48,7 +48,7 @@ def test_w4_create_refuses(kw, code):
 def test_w4_needs_a_handle():
     L, n = bb.load_library(), C.c_size_t()
     assert L.bebelm_w4_matmul(None, P, bb.F32, 128, None, 0, 1, P, bb.F32, None, 0, bb.MEM_HOST, None) == bb.ERR_INVALID
-    assert L.bebelm_w4_workspace(None, P, bb.F32, 128, 1, C.byref(n)) == bb.ERR_INVALID
+    assert L.bebelm_w4_workspace(None, P, bb.F32, 128, 0, 1, C.byref(n)) == bb.ERR_INVALID
     assert L.bebelm_w4_destroy(None) == bb.OK
 
 
