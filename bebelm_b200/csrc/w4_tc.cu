@@ -12,14 +12,15 @@
 //        largest where the second term runs out of exponent). 2^-e is applied with the output.
 // w4_terms_kernel writes the last two as [terms][tokens][kp].
 //
-// One CTA per 128 rows x N tokens, one CTA an SM, 16 warps:
+// One CTA per 128 rows x N tokens, one CTA an SM, 20 warps:
 //   warp 0       TMA: per 128 inputs the weights' codes, scales and zero points (three bulk copies: they lie together,
 //                see w4.cu) and the activations' 128-byte-swizzled tiles, through a ring.
 //   warp 1       issues the MMAs, A from TMEM, B from shared memory.
-//   warps 4-7    unpack codes to A in TMEM, two buffers of 128 inputs: a warp's lanes hold (row g and g + 8,
-//                pairs 4 i + q), the fragment of `tcgen05.st.16x128b`. A never passes through shared memory,
-//                whose bandwidth the MMA needs for B.
-//   warps 8-15   read each group's sums (two buffers), scale and add them; a thread has a row and N / 2 tokens.
+//   warps 4-11   unpack codes to A in TMEM, four buffers of 128 inputs, warps 4-7 the even and 8-11 the odd
+//                ones (one set took longer than the MMAs): a warp's lanes hold (row g and g + 8, pairs 4 i + q), the
+//                fragment of `tcgen05.st.16x128b`. A never passes through shared memory, whose bandwidth the
+//                MMA needs for B.
+//   warps 12-19  read each group's sums (two buffers), scale and add them; a thread has a row and N / 2 tokens.
 // Bound: the tensor pipe for many tokens (a group of 128: 8 MMAs of N / 2 cycles each against ~N cycles of TMEM reads
 // and N / 2 FMAs a thread). All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
 // MMAs in flight, reports kErrWaitTimeout and stores nothing.
@@ -34,10 +35,10 @@
 namespace bebelm {
 namespace {
 
-constexpr int kM = 128, kK = 128, kThreads = 512;
-constexpr int kConvert0 = 4, kEpi0 = 8;  // first converter and first epilogue warp
+constexpr int kM = 128, kK = 128, kThreads = 640;
+constexpr int kConvert0 = 4, kEpi0 = 12;  // first converter and first epilogue warp
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColA = 256;          // two A buffers of 64 columns behind the accumulators (2 x N columns)
+constexpr uint32_t kColA = 256;          // four A buffers of 64 columns behind the accumulators (2 x N columns)
 constexpr long long kWaitLimit = 1ll << 22;
 constexpr size_t kRing = 200 * 1024;     // shared memory for the ring
 
@@ -47,10 +48,9 @@ struct TcArgs {
     size_t tokens;
     const float* col_scale;   // [tokens]: one factor a token, or null
     const float* x_scales;    // [n_groups][tokens padded to 128]: a factor per group of inputs, or null
-    size_t x_pitch;
-    int x_shift;              // log2 of that group
-    int fb;                   // blocks of 32 inputs whose sum is scaled together: 1, 2 or 4
-    int y_bf16, stages, plane_rows;  // plane_rows: rows of B between the terms
+    size_t x_pitch, x_groups;
+    int x_group;              // inputs of a group
+    int y_bf16, plane_rows;  // plane_rows: rows of B between the terms
     int* err;
 };
 
@@ -124,19 +124,37 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// word of 8 codes to 4 pairs of c - z: 128 + c less 128 + z in bf16, 1024 + c less 1024 + z in f16
+// Word of 8 codes to 4 pairs of c - z, exactly (see w4.cu): 128 + c less 128 + z in bf16; in f16 1024 + c less
+// 1024 + z, and 1/16 of 1024 + 16 c less 64 + z.
 template <bool BF16>
-__device__ __forceinline__ void pairs(uint32_t w, uint32_t zz, uint32_t* o) {
+__device__ __forceinline__ void pairs(uint32_t w, uint32_t za, uint32_t zb, uint32_t* o) {
+    if constexpr (BF16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t u = ((w >> (4 * j)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
-        if constexpr (BF16) {
-            const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&zz));
-            o[j] = *reinterpret_cast<const uint32_t*>(&a);
-        } else {
-            const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&zz));
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t u = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+            const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&za));
             o[j] = *reinterpret_cast<const uint32_t*>(&a);
         }
+    } else {
+        const __half2 s16 = __float2half2_rn(0.0625f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t v = i ? w >> 8 : w;
+            const uint32_t lo = (v & 0x000f000fu) | 0x64006400u, hi = (v & 0x00f000f0u) | 0x64006400u;
+            const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&za));
+            const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), s16, __hneg2(*reinterpret_cast<const __half2*>(&zb)));
+            o[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+            o[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+    }
+}
+// the pairs to take off for zero point z
+template <bool BF16>
+__device__ __forceinline__ void zero_pairs(uint32_t z, uint32_t& za, uint32_t& zb) {
+    za = (BF16 ? 0x43004300u : 0x64006400u) + z * 0x10001u;
+    if constexpr (!BF16) {
+        const __half2 h = __half2half2(__ushort2half_rn((unsigned short)(64 + z)));
+        zb = *reinterpret_cast<const uint32_t*>(&h);
     }
 }
 
@@ -152,19 +170,21 @@ struct Lay {
     static constexpr int kAtom = N * 128;             // N tokens x 64 inputs
     static constexpr int kB = 2 * TERMS * kAtom;      // [term][half]
     static constexpr int kCodes = kB, kScales = kCodes + 8192, kZeros = kScales + 1024;
-    static constexpr int kStage = kZeros + 512 + (1024 - 512) % 1024;  // scales <= 1024 B, zero points <= 512 B
+    static constexpr int kXs = kZeros + 512;          // scales <= 1024 B, zero points <= 512 B
+    static constexpr int kStage = (kXs + 4 * N * 4 + 1023) / 1024 * 1024;  // activations' scales: up to 4 x N
     static constexpr int kStages = (int)(kRing / kStage) < 6 ? (int)(kRing / kStage) : 6;
     static constexpr int kSmem = kStages * kStage + 1024;
 };
 
-template <int N, int TERMS, bool BF16>
+// FB: blocks of 32 inputs whose sum is scaled together
+template <int N, int TERMS, bool BF16, int FB>
 __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, TcArgs a) {
     using L = Lay<N, TERMS>;
-    constexpr int S = L::kStages;
+    constexpr int S = L::kStages, F = 4 / FB;  // ring stages, sums a chunk
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sb = smem_u32(sm);
-    __shared__ uint64_t s_bar[2 * S + 9];
+    __shared__ uint64_t s_bar[2 * S + 13];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -173,10 +193,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
     auto full = [&](int i) { return bars + 8 * i; };
     auto empty = [&](int i) { return bars + 8 * (S + i); };
     auto a_full = [&](int i) { return bars + 8 * (2 * S + i); };
-    auto a_empty = [&](int i) { return bars + 8 * (2 * S + 2 + i); };
-    auto d_full = [&](int i) { return bars + 8 * (2 * S + 4 + i); };
-    auto d_empty = [&](int i) { return bars + 8 * (2 * S + 6 + i); };
-    const uint32_t drained = bars + 8 * (2 * S + 8);
+    auto a_empty = [&](int i) { return bars + 8 * (2 * S + 4 + i); };
+    auto d_full = [&](int i) { return bars + 8 * (2 * S + 8 + i); };
+    auto d_empty = [&](int i) { return bars + 8 * (2 * S + 10 + i); };
+    const uint32_t drained = bars + 8 * (2 * S + 12);
 
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(kTmemCols));
@@ -186,9 +206,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         auto init = [&](uint32_t b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n)); };
         for (int i = 0; i < S; ++i) {
             init(full(i), 1);
-            init(empty(i), 5);  // the stage's MMAs, and the four converter warps that read its codes
+            init(empty(i), 13);  // the stage's MMAs, the four converter warps of its codes, the epilogue's eight (its scales)
         }
-        for (int i = 0; i < 2; ++i) init(a_full(i), 4), init(a_empty(i), 1), init(d_full(i), 1), init(d_empty(i), 8);
+        for (int i = 0; i < 4; ++i) init(a_full(i), 4), init(a_empty(i), 1);
+        for (int i = 0; i < 2; ++i) init(d_full(i), 1), init(d_empty(i), 8);
         init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_fail = 0;
@@ -197,13 +218,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
     __syncthreads();
     tc_after();
     const uint32_t tmem = s_tmem;
-    const int per_flush = a.fb, flushes = 4 / per_flush;  // sums a chunk
     // scales and activations' terms may come from the kernel before
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp == 0) {
         if (lane == 0) {
             const uint32_t zb = a.w.zeros ? 64u * (pc == 4 ? 8 : 4) : 0u, scb = 256u * (uint32_t)pc;
+            const int xs_rows = a.x_scales ? (a.x_group < kK ? kK / a.x_group : 1) : 0;  // groups that meet 128 inputs
+            const uint32_t xsb = xs_rows * N * 4u;
             const unsigned char* code = reinterpret_cast<const unsigned char*>(a.w.codes) + (size_t)rb * chunks * 8192;
             const unsigned char* scale = reinterpret_cast<const unsigned char*>(a.w.scales) + (size_t)rb * chunks * scb;
             const unsigned char* zero = reinterpret_cast<const unsigned char*>(a.w.zeros) + (size_t)rb * chunks * zb;
@@ -215,11 +237,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
                     break;
                 }
                 const uint32_t base = sb + st * L::kStage;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(st)), "r"((uint32_t)L::kB + 8192u + scb + zb)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(st)), "r"((uint32_t)L::kB + 8192u + scb + zb + xsb)
                              : "memory");
                 bulk(base + L::kCodes, code + (size_t)c * 8192, 8192, full(st));
                 bulk(base + L::kScales, scale + (size_t)c * scb, scb, full(st));
                 if (zb) bulk(base + L::kZeros, zero + (size_t)c * zb, zb, full(st));
+                for (int j = 0; j < xs_rows; ++j) {  // behind the last group (padded inputs) the last one again
+                    const size_t gr = min((size_t)c * kK / a.x_group + j, a.x_groups - 1);
+                    bulk(base + L::kXs + j * N * 4, a.x_scales + gr * a.x_pitch + t0, N * 4, full(st));
+                }
 #pragma unroll
                 for (int p = 0; p < TERMS; ++p)
 #pragma unroll
@@ -232,31 +258,45 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         }
     } else if (warp == 1) {
         if (lane == 0) {
+            // One thread's issue is on the critical path: every offset below is a constant of the unrolled
+            // loops, ring positions and phases are carried along (with run-time loops and divisions an
+            // MMA took 130 cycles to issue and a passed wait 250).
             constexpr uint32_t idesc = instr_desc(N, BF16);
-            int u = 0;  // sums so far
+            const uint64_t b0 = smem_desc(sb);
+            uint64_t bd = b0;
+            uint32_t f_bar = full(0), e_bar = empty(0), ab = 0;
+            unsigned ph = 0, a_ph = 0, d_ph = 1;  // d_ph: of the buffers' last reads; the first round passes
             bool ok = true;
-            for (int c = 0; ok && c < chunks; ++c) {
-                const int st = c % S, ab = c & 1;
-                ok = mbar_wait(full(st), (c / S) & 1) && mbar_wait(a_full(ab), (c >> 1) & 1);
-                for (int f = 0; ok && f < flushes; ++f, ++u) {
-                    const int db = u & 1;
-                    if (u >= 2 && !mbar_wait(d_empty(db), ((u >> 1) - 1) & 1)) {
+            for (int c = 0, st = 0; c < chunks; ++c) {
+                ok = mbar_wait(f_bar, ph) && mbar_wait(a_full(0) + 8 * ab, a_ph);
+                if (!ok) break;
+                const uint32_t ta = tmem + kColA + 64 * ab;
+#pragma unroll
+                for (int f = 0; f < F; ++f) {
+                    const uint32_t db = F == 1 ? (uint32_t)(c & 1) : (uint32_t)(f & 1);
+                    if (!mbar_wait(d_empty(0) + 8 * db, d_ph)) {
                         ok = false;
                         break;
                     }
                     tc_after();
-                    for (int k = 2 * per_flush * f; k < 2 * per_flush * (f + 1); ++k) {  // 16 inputs: 8 columns of A, 32 bytes of B
+                    const uint32_t td = tmem + db * N;
+#pragma unroll
+                    for (int k = 2 * FB * f; k < 2 * FB * (f + 1); ++k)  // 16 inputs: 8 columns of A, 32 bytes of B
 #pragma unroll
                         for (int p = 0; p < TERMS; ++p)
-                            mma_ts(tmem + db * N, tmem + kColA + 64 * ab + 8 * k,
-                                   smem_desc(sb + st * L::kStage + (2 * p + (k >> 2)) * L::kAtom + (k & 3) * 32), idesc,
-                                   k > 2 * per_flush * f || p > 0);
-                    }
-                    commit(d_full(db));
+                            mma_ts(td, ta + 8 * k, bd + (uint64_t)(((2 * p + (k >> 2)) * L::kAtom + (k & 3) * 32) >> 4), idesc,
+                                   k > 2 * FB * f || p > 0);
+                    commit(d_full(0) + 8 * db);
+                    if (F == 1 ? (c & 1) : (f & 1)) d_ph ^= 1;
                 }
-                if (ok) {
-                    commit(empty(st));
-                    commit(a_empty(ab));
+                if (!ok) break;
+                commit(e_bar);
+                commit(a_empty(0) + 8 * ab);
+                if (++ab == 4) ab = 0, a_ph ^= 1;
+                if (++st == S) {
+                    st = 0, ph ^= 1, bd = b0, f_bar = full(0), e_bar = empty(0);
+                } else {
+                    bd += L::kStage >> 4, f_bar += 8, e_bar += 8;
                 }
             }
             if (!ok) s_fail = 1;
@@ -264,33 +304,36 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
             mbar_wait(drained, 0);
         }
     } else if (warp >= kConvert0 && warp < kEpi0) {
-        const int w = warp - kConvert0, g = lane >> 2;
+        const int w = warp & 3, g = lane >> 2, rec = pc == 4 ? 8 : 4;
         bool ok = true;
-        for (int c = 0; c < chunks; ++c) {
-            const int st = c % S, ab = c & 1;
-            ok = mbar_wait(full(st), (c / S) & 1) && (c < 2 || mbar_wait(a_empty(ab), ((c >> 1) - 1) & 1));
+        for (int c = (warp - kConvert0) >> 2; c < chunks; c += 2) {
+            const int st = c % S, ab = c & 3;
+            ok = mbar_wait(full(st), (c / S) & 1) && (c < 4 || mbar_wait(a_empty(ab), ((c >> 2) - 1) & 1));
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_after();
             const unsigned char* base = sm + st * L::kStage;
+            uint4 v[2][2];
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                v[m >> 1][m & 1] = *reinterpret_cast<const uint4*>(base + L::kCodes + w * 2048 + m * 512 + lane * 16);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {  // tiles of 16 rows
                 const int tile = 2 * w + m;
-                const uint4 va = *reinterpret_cast<const uint4*>(base + L::kCodes + tile * 1024 + lane * 16);
-                const uint4 vb = *reinterpret_cast<const uint4*>(base + L::kCodes + tile * 1024 + 512 + lane * 16);
-                const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+                const uint32_t wa[4] = {v[m][0].x, v[m][0].y, v[m][0].z, v[m][0].w}, wb[4] = {v[m][1].x, v[m][1].y, v[m][1].z, v[m][1].w};
+                const unsigned char* z = base + L::kZeros + (tile * 8 + g) * rec;
+                uint32_t za = 0, za2 = 0, zb = 0, zb2 = 0;
                 uint32_t r[32];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    uint32_t z0 = 8, z1 = 8;
-                    if (a.w.zeros) {
-                        const unsigned char* z = base + L::kZeros + (tile * 8 + g) * (pc == 4 ? 8 : 4) + 2 * (b * pc / 4);
-                        z0 = z[0], z1 = z[1];
+                    if (b * pc % 4 == 0) {
+                        const uint32_t zz = a.w.zeros ? *reinterpret_cast<const unsigned short*>(z + 2 * (b * pc / 4)) : 0x0808u;
+                        zero_pairs<BF16>(zz & 0xffu, za, za2);
+                        zero_pairs<BF16>(zz >> 8, zb, zb2);
                     }
-                    const uint32_t one = BF16 ? 0x43004300u : 0x64006400u;
                     uint32_t pa[4], pb[4];
-                    pairs<BF16>(wa[b], one + z0 * 0x10001u, pa);
-                    pairs<BF16>(wb[b], one + z1 * 0x10001u, pb);
+                    pairs<BF16>(wa[b], za, za2, pa);
+                    pairs<BF16>(wb[b], zb, zb2, pb);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) r[2 * (4 * b + j)] = pa[j], r[2 * (4 * b + j) + 1] = pb[j];
                 }
@@ -306,55 +349,52 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         constexpr int C = N / 2;  // columns of a thread
         const int w = warp - kEpi0, half = w >> 2, row = 32 * (w & 3) + lane;
         const uint32_t t_d = tmem + ((uint32_t)(32 * (w & 3)) << 16) + half * C;
-        // this row's scales: [tile][row % 8][block][row / 8]
-        const int tile = row >> 4, g = row & 7, h = (row >> 3) & 1;
-        const unsigned short* sp = reinterpret_cast<const unsigned short*>(a.w.scales) + ((size_t)rb * chunks * 64 + tile * 8 + g) * pc * 2 + h;
-        const int total = chunks * flushes;
+        // this row's scales in a stage: [tile][row % 8][block][row / 8]
+        const int sc_at = L::kScales + (((row >> 4) * 8 + (row & 7)) * pc * 2 + ((row >> 3) & 1)) * 2;
+        const int xs_step = a.x_scales && a.x_group < kK ? N * 4 * 32 * FB / a.x_group : 0;  // bytes a sum
         float acc[C];
 #pragma unroll
         for (int i = 0; i < C; ++i) acc[i] = 0.f;
-        auto scale_at = [&](int u) -> float {
-            const int c = u / flushes, blk = (u % flushes) * per_flush * pc / 4;
-            return scale_of(sp[((size_t)c * 64 * pc + blk) * 2], a.w.scale_bf16);
-        };
-        float s_next = scale_at(0);
         bool ok = true;
-        for (int u = 0; u < total; ++u) {
-            const float s = s_next;
-            if (u + 1 < total) s_next = scale_at(u + 1);
-            ok = __all_sync(0xffffffffu, mbar_wait(d_full(u & 1), (u >> 1) & 1));
-            if (!ok) break;
-            tc_after();
-            const size_t k = (size_t)(u / flushes) * kK + (size_t)(u % flushes) * per_flush * 32;
-            const float* xs = a.x_scales ? a.x_scales + (k >> a.x_shift) * a.x_pitch + t0 + half * C : nullptr;
-            constexpr int B = C < 32 ? C : 32;  // columns in registers at a time
+        int u = 0;
+        for (int c = 0; ok && c < chunks; ++c) {
+            const int st = c % S;
+            const unsigned char* base = sm + st * L::kStage;
+            ok = __all_sync(0xffffffffu, mbar_wait(full(st), (c / S) & 1));
+            for (int f = 0; ok && f < F; ++f, ++u) {
+                const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (f * FB * pc / 4) * 4), a.w.scale_bf16);
+                const unsigned char* xs = base + L::kXs + half * C * 4 + f * xs_step;
+                ok = __all_sync(0xffffffffu, mbar_wait(d_full(u & 1), (u >> 1) & 1));
+                if (!ok) break;
+                tc_after();
+                constexpr int B = 16;  // columns in registers at a time
 #pragma unroll
-            for (int c = 0; c < C; c += B) {
-                uint32_t d[B];
-#pragma unroll
-                for (int i = 0; i < B; i += 16) tmem_ld16(t_d + (u & 1) * N + c + i, d + i);
-                tmem_ld_wait();
-                if (c + B == C) {
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(d_empty(u & 1));
-                }
-                if (xs) {
-                    if (k < a.w.n_in) {  // padded inputs have no scale: their sum is zero
+                for (int i0 = 0; i0 < C; i0 += B) {
+                    uint32_t d[B];
+                    tmem_ld16(t_d + (u & 1) * N + i0, d);
+                    tmem_ld_wait();
+                    if (i0 + B == C) {
+                        tc_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(d_empty(u & 1));
+                    }
+                    if (a.x_scales) {
 #pragma unroll
                         for (int i = 0; i < B; i += 4) {
-                            const float4 f = __ldg(reinterpret_cast<const float4*>(xs + c + i));
-                            acc[c + i] = fmaf(__uint_as_float(d[i]) * f.x, s, acc[c + i]);
-                            acc[c + i + 1] = fmaf(__uint_as_float(d[i + 1]) * f.y, s, acc[c + i + 1]);
-                            acc[c + i + 2] = fmaf(__uint_as_float(d[i + 2]) * f.z, s, acc[c + i + 2]);
-                            acc[c + i + 3] = fmaf(__uint_as_float(d[i + 3]) * f.w, s, acc[c + i + 3]);
+                            const float4 x4 = *reinterpret_cast<const float4*>(xs + (i0 + i) * 4);
+                            acc[i0 + i] = fmaf(__uint_as_float(d[i]) * x4.x, s, acc[i0 + i]);
+                            acc[i0 + i + 1] = fmaf(__uint_as_float(d[i + 1]) * x4.y, s, acc[i0 + i + 1]);
+                            acc[i0 + i + 2] = fmaf(__uint_as_float(d[i + 2]) * x4.z, s, acc[i0 + i + 2]);
+                            acc[i0 + i + 3] = fmaf(__uint_as_float(d[i + 3]) * x4.w, s, acc[i0 + i + 3]);
                         }
-                    }
-                } else {
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < B; ++i) acc[c + i] = fmaf(__uint_as_float(d[i]), s, acc[c + i]);
+                        for (int i = 0; i < B; ++i) acc[i0 + i] = fmaf(__uint_as_float(d[i]), s, acc[i0 + i]);
+                    }
                 }
             }
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(empty(st));
         }
         if (!ok) {
             if (lane == 0) s_fail = 1;
@@ -466,10 +506,10 @@ size_t terms_bytes(const W4View& w, const W4X& x) {
     return pad((x.kind == kW4XF32 ? 2 : 1) * x.tokens * w.chunks * kK * 2, 256);
 }
 
-template <int N, int TERMS, bool BF16>
+template <int N, int TERMS, bool BF16, int FB>
 cudaError_t run(const CUtensorMap& tm, TcArgs& a, bool pdl, cudaStream_t s) {
     using L = Lay<N, TERMS>;
-    auto kernel = w4_tc_kernel<N, TERMS, BF16>;
+    auto kernel = w4_tc_kernel<N, TERMS, BF16, FB>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -484,11 +524,17 @@ cudaError_t run(const CUtensorMap& tm, TcArgs& a, bool pdl, cudaStream_t s) {
     cfg.numAttrs = pdl ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, tm, a);
 }
+template <int N, int TERMS, bool BF16>
+cudaError_t run_fb(const CUtensorMap& tm, TcArgs& a, int fb, bool pdl, cudaStream_t s) {
+    return fb == 4   ? run<N, TERMS, BF16, 4>(tm, a, pdl, s)
+           : fb == 2 ? run<N, TERMS, BF16, 2>(tm, a, pdl, s)
+                     : run<N, TERMS, BF16, 1>(tm, a, pdl, s);
+}
 template <int N>
-cudaError_t run_kind(const CUtensorMap& tm, TcArgs& a, int kind, bool pdl, cudaStream_t s) {
-    return kind == kW4XBf16  ? run<N, 1, true>(tm, a, pdl, s)
-           : kind == kW4XF32 ? run<N, 2, false>(tm, a, pdl, s)
-                             : run<N, 1, false>(tm, a, pdl, s);
+cudaError_t run_kind(const CUtensorMap& tm, TcArgs& a, int kind, int fb, bool pdl, cudaStream_t s) {
+    return kind == kW4XBf16  ? run_fb<N, 1, true>(tm, a, fb, pdl, s)
+           : kind == kW4XF32 ? run_fb<N, 2, false>(tm, a, fb, pdl, s)
+                             : run_fb<N, 1, false>(tm, a, fb, pdl, s);
 }
 
 }  // namespace
@@ -507,8 +553,8 @@ cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, voi
     TcArgs a{};
     a.w = w;
     a.y = y, a.y_bf16 = y_bf16, a.tokens = x.tokens, a.err = err;
-    a.fb = 4 / w.per_chunk;
-    if (x.group) a.fb = std::min(a.fb, x.group / 32);
+    int fb = 4 / w.per_chunk;
+    if (x.group) fb = std::min(fb, x.group / 32);
     const bool direct = direct_rows(x);
     const void* rows = x.x;
     size_t stride = x.stride, n_in = x.n_in;
@@ -519,7 +565,8 @@ cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, voi
         float* xs = reinterpret_cast<float*>(reinterpret_cast<char*>(col) + pad(4 * x.tokens, 256));
         a.x_pitch = pad(x.tokens, 128);
         a.x_scales = x.group ? xs : nullptr;
-        a.x_shift = x.group_shift;
+        a.x_group = x.group;
+        a.x_groups = x.n_groups;
         a.col_scale = x.kind == kW4XF32 ? col : x.kind == kW4XInt8 && !x.group ? x.scales : nullptr;
         w4_terms_kernel<<<(unsigned)std::min<size_t>(x.tokens, 1 << 20), 256, 0, s>>>(x, kp, t, col, x.group ? xs : nullptr, a.x_pitch);
         const cudaError_t e = cudaGetLastError();
@@ -535,9 +582,9 @@ cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, voi
     if (enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(rows), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    return n_tile == 32   ? run_kind<32>(tm, a, x.kind, !direct, s)
-           : n_tile == 64 ? run_kind<64>(tm, a, x.kind, !direct, s)
-                          : run_kind<128>(tm, a, x.kind, !direct, s);
+    return n_tile == 32   ? run_kind<32>(tm, a, x.kind, fb, !direct, s)
+           : n_tile == 64 ? run_kind<64>(tm, a, x.kind, fb, !direct, s)
+                          : run_kind<128>(tm, a, x.kind, fb, !direct, s);
 }
 
 }  // namespace bebelm
