@@ -39,8 +39,8 @@ constexpr int kM = 128, kK = 128, kThreads = 640;
 constexpr int kConvert0 = 4, kEpi0 = 12;  // first converter and first epilogue warp
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColA = 256;          // four A buffers of 64 columns behind the accumulators (2 x N columns)
-constexpr long long kWaitLimit = 1ll << 22;
-constexpr size_t kRing = 200 * 1024;     // shared memory for the ring
+constexpr int kWaitLimit = 1 << 22;
+constexpr size_t kRing = 225 * 1024;     // shared memory for the ring
 
 struct TcArgs {
     W4View w;
@@ -64,7 +64,7 @@ __host__ __device__ constexpr uint32_t instr_desc(int n, bool bf16) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity) {
-    for (long long it = 0; it < kWaitLimit; ++it) {
+    for (int it = 0; it < kWaitLimit; ++it) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -74,6 +74,20 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity) {
         if (ok) return true;
     }
     return false;
+}
+// The MMA issuer's waits are mostly for what is already there: a try_wait takes about 280 cycles even then, a
+// test_wait 80. (Polling with test_wait in the other warps slows everyone down: they sleep in try_wait.)
+__device__ __forceinline__ bool mbar_ready_or_wait(uint32_t bar, unsigned parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok || mbar_wait(bar, parity);
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, unsigned parity) {
+    return __all_sync(0xffffffffu, mbar_ready_or_wait(bar, parity));
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -171,7 +185,7 @@ struct Lay {
     static constexpr int kB = 2 * TERMS * kAtom;      // [term][half]
     static constexpr int kCodes = kB, kScales = kCodes + 8192, kZeros = kScales + 1024;
     static constexpr int kXs = kZeros + 512;          // scales <= 1024 B, zero points <= 512 B
-    static constexpr int kStage = (kXs + 4 * N * 4 + 1023) / 1024 * 1024;  // activations' scales: up to 4 x N
+    static constexpr int kStage = (kXs + (TERMS == 1 ? 4 * N * 4 : 0) + 1023) / 1024 * 1024;  // activations' scales: up to 4 x N
     static constexpr int kStages = (int)(kRing / kStage) < 6 ? (int)(kRing / kStage) : 6;
     static constexpr int kSmem = kStages * kStage + 1024;
 };
@@ -264,17 +278,18 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
             constexpr uint32_t idesc = instr_desc(N, BF16);
             const uint64_t b0 = smem_desc(sb);
             uint64_t bd = b0;
-            uint32_t f_bar = full(0), e_bar = empty(0), ab = 0;
-            unsigned ph = 0, a_ph = 0, d_ph = 1;  // d_ph: of the buffers' last reads; the first round passes
+            uint32_t e_bar = empty(0), ab = 0;
+            unsigned a_ph = 0, d_ph = 1;  // d_ph: of the buffers' last reads; the first round passes
             bool ok = true;
             for (int c = 0, st = 0; c < chunks; ++c) {
-                ok = mbar_wait(f_bar, ph) && mbar_wait(a_full(0) + 8 * ab, a_ph);
+                // the converters have seen the stage's copies land before they hand A over
+                ok = mbar_ready_or_wait(a_full(0) + 8 * ab, a_ph);
                 if (!ok) break;
                 const uint32_t ta = tmem + kColA + 64 * ab;
 #pragma unroll
                 for (int f = 0; f < F; ++f) {
                     const uint32_t db = F == 1 ? (uint32_t)(c & 1) : (uint32_t)(f & 1);
-                    if (!mbar_wait(d_empty(0) + 8 * db, d_ph)) {
+                    if (!mbar_ready_or_wait(d_empty(0) + 8 * db, d_ph)) {
                         ok = false;
                         break;
                     }
@@ -294,9 +309,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
                 commit(a_empty(0) + 8 * ab);
                 if (++ab == 4) ab = 0, a_ph ^= 1;
                 if (++st == S) {
-                    st = 0, ph ^= 1, bd = b0, f_bar = full(0), e_bar = empty(0);
+                    st = 0, bd = b0, e_bar = empty(0);
                 } else {
-                    bd += L::kStage >> 4, f_bar += 8, e_bar += 8;
+                    bd += L::kStage >> 4, e_bar += 8;
                 }
             }
             if (!ok) s_fail = 1;
@@ -308,8 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         bool ok = true;
         for (int c = (warp - kConvert0) >> 2; c < chunks; c += 2) {
             const int st = c % S, ab = c & 3;
-            ok = mbar_wait(full(st), (c / S) & 1) && (c < 4 || mbar_wait(a_empty(ab), ((c >> 2) - 1) & 1));
-            ok = __all_sync(0xffffffffu, ok);
+            ok = mbar_wait_warp(full(st), (c / S) & 1) && (c < 4 || mbar_wait_warp(a_empty(ab), ((c >> 2) - 1) & 1));
             if (!ok) break;
             tc_after();
             const unsigned char* base = sm + st * L::kStage;
@@ -360,11 +374,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         for (int c = 0; ok && c < chunks; ++c) {
             const int st = c % S;
             const unsigned char* base = sm + st * L::kStage;
-            ok = __all_sync(0xffffffffu, mbar_wait(full(st), (c / S) & 1));
+            ok = mbar_wait_warp(full(st), (c / S) & 1);
             for (int f = 0; ok && f < F; ++f, ++u) {
                 const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (f * FB * pc / 4) * 4), a.w.scale_bf16);
                 const unsigned char* xs = base + L::kXs + half * C * 4 + f * xs_step;
-                ok = __all_sync(0xffffffffu, mbar_wait(d_full(u & 1), (u >> 1) & 1));
+                ok = mbar_wait_warp(d_full(u & 1), (u >> 1) & 1);
                 if (!ok) break;
                 tc_after();
                 constexpr int B = 16;  // columns in registers at a time
