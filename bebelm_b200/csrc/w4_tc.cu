@@ -13,8 +13,10 @@
 // w4_terms_kernel writes the last two as [terms][tokens][kp].
 //
 // One CTA per 128 rows x N tokens, one CTA an SM, 20 warps:
-//   warp 0       TMA: per 128 inputs the weights' codes, scales and zero points (three bulk copies: they lie together,
-//                see w4.cu) and the activations' 128-byte-swizzled tiles, through a ring.
+//   warps 0, 2, 3  copies, a ring each, since they are held for different times: the activations' 128-byte-swizzled
+//                tiles of 64 inputs (TMA, until their MMAs are done), the codes and zero points of 128 inputs (bulk copies:
+//                they lie together, see w4.cu; until they are unpacked) and the scales (until they are applied).
+//                With one ring for the three its depth bound everything: 5 stages against a stage's 6000 cycles.
 //   warp 1       issues the MMAs, A from TMEM, B from shared memory.
 //   warps 4-11   unpack codes to A in TMEM, four buffers of 128 inputs, warps 4-7 the even and 8-11 the odd
 //                ones (one set took longer than the MMAs): a warp's lanes hold (row g and g + 8, pairs 4 i + q), the
@@ -40,7 +42,7 @@ constexpr int kConvert0 = 4, kEpi0 = 12;  // first converter and first epilogue 
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColA = 256;          // four A buffers of 64 columns behind the accumulators (2 x N columns)
 constexpr int kWaitLimit = 1 << 22;
-constexpr size_t kRing = 225 * 1024;     // shared memory for the ring
+constexpr int kRings = 225 * 1024;       // shared memory for the rings
 
 struct TcArgs {
     W4View w;
@@ -75,8 +77,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity) {
     }
     return false;
 }
-// The MMA issuer's waits are mostly for what is already there: a try_wait takes about 280 cycles even then, a
-// test_wait 80. (Polling with test_wait in the other warps slows everyone down: they sleep in try_wait.)
+// A try_wait takes about 280 cycles even for a phase that is complete, a test_wait 80; but polling with it slows the
+// other warps down. So one test, then try_wait, which sleeps.
 __device__ __forceinline__ bool mbar_ready_or_wait(uint32_t bar, unsigned parity) {
     uint32_t ok;
     asm volatile(
@@ -92,27 +94,42 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, unsigned parity) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// One elected lane of a converged warp issues: with the whole warp in step, addresses and descriptors stay in
+// uniform registers. (Issued by a lane in its own branch, an MMA took 130 cycles and a loop's end 250:
+// 132 us against 102 for 2048 tokens x 8192 x 2048.)
 __device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
+        : "memory");
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
         "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
 __device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(dst), "l"(src),
+        "r"(bytes), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
@@ -179,38 +196,46 @@ __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
     return __half2float(__half(r));
 }
 
-template <int N, int TERMS>
+template <int N, int TERMS, bool BF16>
 struct Lay {
-    static constexpr int kAtom = N * 128;             // N tokens x 64 inputs
-    static constexpr int kB = 2 * TERMS * kAtom;      // [term][half]
-    static constexpr int kCodes = kB, kScales = kCodes + 8192, kZeros = kScales + 1024;
-    static constexpr int kXs = kZeros + 512;          // scales <= 1024 B, zero points <= 512 B
-    static constexpr int kStage = (kXs + (TERMS == 1 ? 4 * N * 4 : 0) + 1023) / 1024 * 1024;  // activations' scales: up to 4 x N
-    static constexpr int kStages = (int)(kRing / kStage) < 6 ? (int)(kRing / kStage) : 6;
-    static constexpr int kSmem = kStages * kStage + 1024;
+    static constexpr int kAtom = N * 128;                  // N tokens x 64 inputs
+    static constexpr int kB = TERMS * kAtom;               // a stage: 64 inputs
+    static constexpr int kW = 8192 + 512, kSW = 6;         // codes and zero points (<= 512 bytes) of 128 inputs
+    static constexpr int kXs = 1024;                       // scales <= 1024 bytes, then the activations' (up to 4 x N)
+    static constexpr int kS = kXs + (TERMS == 1 && !BF16 ? 4 * N * 4 : 0), kSS = 8;
+    static constexpr int kOffW = 0, kOffS = kSW * kW, kOffB = (kOffS + kSS * kS + 1023) / 1024 * 1024;
+    static constexpr int kSB = (kRings - kOffB) / kB < 12 ? (kRings - kOffB) / kB : 12;
+    static constexpr int kSmem = kOffB + kSB * kB + 1024;
+    static constexpr int kBars = 2 * (kSB + kSW + kSS) + 13;
+    static_assert(kSB >= 4, "ring");
 };
 
 // FB: blocks of 32 inputs whose sum is scaled together
 template <int N, int TERMS, bool BF16, int FB>
 __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, TcArgs a) {
-    using L = Lay<N, TERMS>;
-    constexpr int S = L::kStages, F = 4 / FB;  // ring stages, sums a chunk
+    using L = Lay<N, TERMS, BF16>;
+    constexpr int SB = L::kSB, SW = L::kSW, SS = L::kSS, F = 4 / FB;  // ring stages, sums a chunk of 128 inputs
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sb = smem_u32(sm);
-    __shared__ uint64_t s_bar[2 * S + 13];
+    __shared__ uint64_t s_bar[L::kBars];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int rb = blockIdx.x, t0 = (int)blockIdx.y * N, chunks = (int)a.w.chunks, pc = a.w.per_chunk;
     const uint32_t bars = smem_u32(s_bar);
-    auto full = [&](int i) { return bars + 8 * i; };
-    auto empty = [&](int i) { return bars + 8 * (S + i); };
-    auto a_full = [&](int i) { return bars + 8 * (2 * S + i); };
-    auto a_empty = [&](int i) { return bars + 8 * (2 * S + 4 + i); };
-    auto d_full = [&](int i) { return bars + 8 * (2 * S + 8 + i); };
-    auto d_empty = [&](int i) { return bars + 8 * (2 * S + 10 + i); };
-    const uint32_t drained = bars + 8 * (2 * S + 12);
+    auto b_full = [&](int i) { return bars + 8 * i; };
+    auto b_empty = [&](int i) { return bars + 8 * (SB + i); };
+    auto w_full = [&](int i) { return bars + 8 * (2 * SB + i); };
+    auto w_empty = [&](int i) { return bars + 8 * (2 * SB + SW + i); };
+    auto s_full = [&](int i) { return bars + 8 * (2 * (SB + SW) + i); };
+    auto s_empty = [&](int i) { return bars + 8 * (2 * (SB + SW) + SS + i); };
+    constexpr int R = 2 * (SB + SW + SS);
+    auto a_full = [&](int i) { return bars + 8 * (R + i); };
+    auto a_empty = [&](int i) { return bars + 8 * (R + 4 + i); };
+    auto d_full = [&](int i) { return bars + 8 * (R + 8 + i); };
+    auto d_empty = [&](int i) { return bars + 8 * (R + 10 + i); };
+    const uint32_t drained = bars + 8 * (R + 12);
 
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(kTmemCols));
@@ -218,10 +243,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
     }
     if (tid == 32) {
         auto init = [&](uint32_t b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n)); };
-        for (int i = 0; i < S; ++i) {
-            init(full(i), 1);
-            init(empty(i), 13);  // the stage's MMAs, the four converter warps of its codes, the epilogue's eight (its scales)
-        }
+        for (int i = 0; i < SB; ++i) init(b_full(i), 1), init(b_empty(i), 1);
+        for (int i = 0; i < SW; ++i) init(w_full(i), 1), init(w_empty(i), 4);
+        for (int i = 0; i < SS; ++i) init(s_full(i), 1), init(s_empty(i), 8);
         for (int i = 0; i < 4; ++i) init(a_full(i), 4), init(a_empty(i), 1);
         for (int i = 0; i < 2; ++i) init(d_full(i), 1), init(d_empty(i), 8);
         init(drained, 1);
@@ -231,111 +255,121 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     // scales and activations' terms may come from the kernel before
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
+    // A copying warp: n stages through a ring, each issued by `load(stage, i)`.
+    auto feed = [&](int n, int stages, uint32_t full0, uint32_t empty0, uint32_t bytes, auto load) {
+        int i = 0;
+        for (int st = 0, ph = 1; i < n; ++i) {
+            if (!mbar_wait_warp(empty0 + 8 * st, ph)) {  // the first round passes
+                if (lane == 0) s_fail = 1;
+                break;
+            }
+            expect_tx(full0 + 8 * st, bytes);
+            load(st, i);
+            if (++st == stages) st = 0, ph ^= 1;
+        }
+        // nothing may be in flight when the CTA exits
+        for (int j = i > stages ? i - stages : 0; j < i; ++j) mbar_wait_warp(full0 + 8 * (j % stages), (j / stages) & 1);
+    };
     if (warp == 0) {
-        if (lane == 0) {
-            const uint32_t zb = a.w.zeros ? 64u * (pc == 4 ? 8 : 4) : 0u, scb = 256u * (uint32_t)pc;
-            const int xs_rows = a.x_scales ? (a.x_group < kK ? kK / a.x_group : 1) : 0;  // groups that meet 128 inputs
-            const uint32_t xsb = xs_rows * N * 4u;
-            const unsigned char* code = reinterpret_cast<const unsigned char*>(a.w.codes) + (size_t)rb * chunks * 8192;
-            const unsigned char* scale = reinterpret_cast<const unsigned char*>(a.w.scales) + (size_t)rb * chunks * scb;
-            const unsigned char* zero = reinterpret_cast<const unsigned char*>(a.w.zeros) + (size_t)rb * chunks * zb;
-            int issued = 0;
-            for (int c = 0; c < chunks; ++c) {
-                const int st = c % S;
-                if (c >= S && !mbar_wait(empty(st), ((c / S) - 1) & 1)) {
-                    s_fail = 1;
-                    break;
-                }
-                const uint32_t base = sb + st * L::kStage;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(st)), "r"((uint32_t)L::kB + 8192u + scb + zb + xsb)
-                             : "memory");
-                bulk(base + L::kCodes, code + (size_t)c * 8192, 8192, full(st));
-                bulk(base + L::kScales, scale + (size_t)c * scb, scb, full(st));
-                if (zb) bulk(base + L::kZeros, zero + (size_t)c * zb, zb, full(st));
-                for (int j = 0; j < xs_rows; ++j) {  // behind the last group (padded inputs) the last one again
-                    const size_t gr = min((size_t)c * kK / a.x_group + j, a.x_groups - 1);
-                    bulk(base + L::kXs + j * N * 4, a.x_scales + gr * a.x_pitch + t0, N * 4, full(st));
-                }
+        feed(2 * chunks, SB, b_full(0), b_empty(0), L::kB, [&](int st, int i) {
 #pragma unroll
                 for (int p = 0; p < TERMS; ++p)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        tma_2d(base + (2 * p + h) * L::kAtom, &tm_x, c * kK + 64 * h, t0 + p * a.plane_rows, full(st));
-                issued = c + 1;
-            }
-            // nothing may be in flight when the CTA exits
-            for (int c = issued > S ? issued - S : 0; c < issued; ++c) mbar_wait(full(c % S), (c / S) & 1);
+                    tma_2d(sb + L::kOffB + st * L::kB + p * L::kAtom, &tm_x, i * 64, t0 + p * a.plane_rows, b_full(st));
+            });
+    } else if (warp == 2) {
+        {
+            const uint32_t zb = a.w.zeros ? 64u * (pc == 4 ? 8 : 4) : 0u;
+            const unsigned char* code = reinterpret_cast<const unsigned char*>(a.w.codes) + (size_t)rb * chunks * 8192;
+            const unsigned char* zero = reinterpret_cast<const unsigned char*>(a.w.zeros) + (size_t)rb * chunks * zb;
+            feed(chunks, SW, w_full(0), w_empty(0), 8192u + zb, [&](int st, int c) {
+                bulk(sb + L::kOffW + st * L::kW, code + (size_t)c * 8192, 8192, w_full(st));
+                if (zb) bulk(sb + L::kOffW + st * L::kW + 8192, zero + (size_t)c * zb, zb, w_full(st));
+            });
+        }
+    } else if (warp == 3) {
+        {
+            const uint32_t scb = 256u * (uint32_t)pc;
+            const int xs_rows = a.x_scales ? (a.x_group < kK ? kK / a.x_group : 1) : 0;  // groups that meet 128 inputs
+            const unsigned char* scale = reinterpret_cast<const unsigned char*>(a.w.scales) + (size_t)rb * chunks * scb;
+            feed(chunks, SS, s_full(0), s_empty(0), scb + xs_rows * N * 4u, [&](int st, int c) {
+                bulk(sb + L::kOffS + st * L::kS, scale + (size_t)c * scb, scb, s_full(st));
+                for (int j = 0; j < xs_rows; ++j) {  // behind the last group (padded inputs) the last one again
+                    const size_t gr = min((size_t)c * kK / a.x_group + j, a.x_groups - 1);
+                    bulk(sb + L::kOffS + st * L::kS + L::kXs + j * N * 4, a.x_scales + gr * a.x_pitch + t0, N * 4, s_full(st));
+                }
+            });
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // One thread's issue is on the critical path: every offset below is a constant of the unrolled
-            // loops, ring positions and phases are carried along (with run-time loops and divisions an
-            // MMA took 130 cycles to issue and a passed wait 250).
+        {
+            // Issue is on the critical path: every offset below is a constant of the unrolled loop, ring
+            // positions and phases are carried along.
             constexpr uint32_t idesc = instr_desc(N, BF16);
-            const uint64_t b0 = smem_desc(sb);
+            const uint64_t b0 = smem_desc(sb + L::kOffB);
             uint64_t bd = b0;
-            uint32_t e_bar = empty(0), ab = 0;
-            unsigned a_ph = 0, d_ph = 1;  // d_ph: of the buffers' last reads; the first round passes
+            uint32_t st8 = 0, ab = 0;  // byte offset of the stage's barriers, A buffer
+            unsigned b_ph = 0, a_ph = 0, d_ph = 1;  // d_ph: of the buffers' last reads; the first round passes
             bool ok = true;
-            for (int c = 0, st = 0; c < chunks; ++c) {
-                // the converters have seen the stage's copies land before they hand A over
-                ok = mbar_ready_or_wait(a_full(0) + 8 * ab, a_ph);
+            for (int c = 0; ok && c < chunks; ++c) {
+                ok = mbar_wait_warp(a_full(0) + 8 * ab, a_ph);
                 if (!ok) break;
                 const uint32_t ta = tmem + kColA + 64 * ab;
 #pragma unroll
-                for (int f = 0; f < F; ++f) {
-                    const uint32_t db = F == 1 ? (uint32_t)(c & 1) : (uint32_t)(f & 1);
-                    if (!mbar_ready_or_wait(d_empty(0) + 8 * db, d_ph)) {
+                for (int i = 0; i < 8; ++i) {  // 16 inputs: 8 columns of A, 32 bytes of B
+                    if (i % 4 == 0 && !mbar_wait_warp(b_full(0) + st8, b_ph)) {
                         ok = false;
                         break;
                     }
-                    tc_after();
-                    const uint32_t td = tmem + db * N;
+                    const int f = i / (2 * FB);
+                    const uint32_t db = F == 1 ? (uint32_t)(c & 1) : (uint32_t)(f & 1);
+                    if (i % (2 * FB) == 0 && !mbar_wait_warp(d_empty(0) + 8 * db, d_ph)) {
+                        ok = false;
+                        break;
+                    }
+                    if (i % 4 == 0 || i % (2 * FB) == 0) tc_after();
 #pragma unroll
-                    for (int k = 2 * FB * f; k < 2 * FB * (f + 1); ++k)  // 16 inputs: 8 columns of A, 32 bytes of B
-#pragma unroll
-                        for (int p = 0; p < TERMS; ++p)
-                            mma_ts(td, ta + 8 * k, bd + (uint64_t)(((2 * p + (k >> 2)) * L::kAtom + (k & 3) * 32) >> 4), idesc,
-                                   k > 2 * FB * f || p > 0);
-                    commit(d_full(0) + 8 * db);
-                    if (F == 1 ? (c & 1) : (f & 1)) d_ph ^= 1;
+                    for (int p = 0; p < TERMS; ++p)
+                        mma_ts(tmem + db * N, ta + 8 * i, bd + (uint64_t)((p * L::kAtom + (i & 3) * 32) >> 4), idesc,
+                               i % (2 * FB) > 0 || p > 0);
+                    if ((i + 1) % (2 * FB) == 0) {
+                        commit(d_full(0) + 8 * db);
+                        if (F == 1 ? (c & 1) : (f & 1)) d_ph ^= 1;
+                    }
+                    if (i % 4 == 3) {
+                        commit(b_empty(0) + st8);
+                        st8 += 8, bd += L::kB >> 4;
+                        if (st8 == 8 * SB) st8 = 0, bd = b0, b_ph ^= 1;
+                    }
                 }
                 if (!ok) break;
-                commit(e_bar);
                 commit(a_empty(0) + 8 * ab);
                 if (++ab == 4) ab = 0, a_ph ^= 1;
-                if (++st == S) {
-                    st = 0, bd = b0, e_bar = empty(0);
-                } else {
-                    bd += L::kStage >> 4, e_bar += 8;
-                }
             }
-            if (!ok) s_fail = 1;
+            if (!ok && lane == 0) s_fail = 1;
             commit(drained);  // every MMA of this CTA done, also after a failed wait
-            mbar_wait(drained, 0);
+            mbar_wait_warp(drained, 0);
         }
     } else if (warp >= kConvert0 && warp < kEpi0) {
         const int w = warp & 3, g = lane >> 2, rec = pc == 4 ? 8 : 4;
         bool ok = true;
         for (int c = (warp - kConvert0) >> 2; c < chunks; c += 2) {
-            const int st = c % S, ab = c & 3;
-            ok = mbar_wait_warp(full(st), (c / S) & 1) && (c < 4 || mbar_wait_warp(a_empty(ab), ((c >> 2) - 1) & 1));
+            const int st = c % SW, ab = c & 3;
+            ok = mbar_wait_warp(w_full(st), (c / SW) & 1) && (c < 4 || mbar_wait_warp(a_empty(ab), ((c >> 2) - 1) & 1));
             if (!ok) break;
             tc_after();
-            const unsigned char* base = sm + st * L::kStage;
+            const unsigned char* base = sm + L::kOffW + st * L::kW;
             uint4 v[2][2];
 #pragma unroll
             for (int m = 0; m < 4; ++m)
-                v[m >> 1][m & 1] = *reinterpret_cast<const uint4*>(base + L::kCodes + w * 2048 + m * 512 + lane * 16);
+                v[m >> 1][m & 1] = *reinterpret_cast<const uint4*>(base + w * 2048 + m * 512 + lane * 16);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {  // tiles of 16 rows
                 const int tile = 2 * w + m;
                 const uint32_t wa[4] = {v[m][0].x, v[m][0].y, v[m][0].z, v[m][0].w}, wb[4] = {v[m][1].x, v[m][1].y, v[m][1].z, v[m][1].w};
-                const unsigned char* z = base + L::kZeros + (tile * 8 + g) * rec;
+                const unsigned char* z = base + 8192 + (tile * 8 + g) * rec;
                 uint32_t za = 0, za2 = 0, zb = 0, zb2 = 0;
                 uint32_t r[32];
 #pragma unroll
@@ -356,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(a_full(ab)), mbar_arrive(empty(st));
+            if (lane == 0) mbar_arrive(a_full(ab)), mbar_arrive(w_empty(st));
         }
         if (!ok && lane == 0) s_fail = 1;
     } else if (warp >= kEpi0) {
@@ -364,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         const int w = warp - kEpi0, half = w >> 2, row = 32 * (w & 3) + lane;
         const uint32_t t_d = tmem + ((uint32_t)(32 * (w & 3)) << 16) + half * C;
         // this row's scales in a stage: [tile][row % 8][block][row / 8]
-        const int sc_at = L::kScales + (((row >> 4) * 8 + (row & 7)) * pc * 2 + ((row >> 3) & 1)) * 2;
+        const int sc_at = (((row >> 4) * 8 + (row & 7)) * pc * 2 + ((row >> 3) & 1)) * 2;
         const int xs_step = a.x_scales && a.x_group < kK ? N * 4 * 32 * FB / a.x_group : 0;  // bytes a sum
         float acc[C];
 #pragma unroll
@@ -372,9 +406,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         bool ok = true;
         int u = 0;
         for (int c = 0; ok && c < chunks; ++c) {
-            const int st = c % S;
-            const unsigned char* base = sm + st * L::kStage;
-            ok = mbar_wait_warp(full(st), (c / S) & 1);
+            const int st = c % SS;
+            const unsigned char* base = sm + L::kOffS + st * L::kS;
+            ok = mbar_wait_warp(s_full(st), (c / SS) & 1);
             for (int f = 0; ok && f < F; ++f, ++u) {
                 const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (f * FB * pc / 4) * 4), a.w.scale_bf16);
                 const unsigned char* xs = base + L::kXs + half * C * 4 + f * xs_step;
@@ -408,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
                 }
             }
             __syncwarp();
-            if (ok && lane == 0) mbar_arrive(empty(st));
+            if (ok && lane == 0) mbar_arrive(s_empty(st));
         }
         if (!ok) {
             if (lane == 0) s_fail = 1;
@@ -522,7 +556,7 @@ size_t terms_bytes(const W4View& w, const W4X& x) {
 
 template <int N, int TERMS, bool BF16, int FB>
 cudaError_t run(const CUtensorMap& tm, TcArgs& a, bool pdl, cudaStream_t s) {
-    using L = Lay<N, TERMS>;
+    using L = Lay<N, TERMS, BF16>;
     auto kernel = w4_tc_kernel<N, TERMS, BF16, FB>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
