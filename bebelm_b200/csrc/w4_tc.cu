@@ -12,7 +12,7 @@
 //        largest where the second term runs out of exponent). 2^-e is applied with the output.
 // w4_terms_kernel writes the last two as [terms][tokens][kp].
 //
-// One CTA per 128 rows x N tokens, one CTA an SM, 20 warps:
+// One CTA per 128 rows x N tokens, one CTA an SM, 20 or 28 warps:
 //   warps 0, 2, 3  copies, a ring each, since they are held for different times: the activations' 128-byte-swizzled
 //                tiles of 64 inputs (TMA, until their MMAs are done), the codes and zero points of 128 inputs (bulk copies:
 //                they lie together, see w4.cu; until they are unpacked) and the scales (until they are applied).
@@ -22,7 +22,9 @@
 //                ones (one set took longer than the MMAs): a warp's lanes hold (row g and g + 8, pairs 4 i + q), the
 //                fragment of `tcgen05.st.16x128b`. A never passes through shared memory, whose bandwidth the
 //                MMA needs for B.
-//   warps 12-19  read each group's sums (two buffers), scale and add them; a thread has a row and N / 2 tokens.
+//   warps 12-    read each group's sums, scale and add them; a thread has a row and 32 tokens (16 of 32). Sums go
+//                over in two buffers of up to 128 columns: of few tokens' groups several at once, since a handing
+//                over costs each side some 300 cycles.
 // Bound: the tensor pipe for many tokens (a group of 128: 8 MMAs of N / 2 cycles each against ~N cycles of TMEM reads
 // and N / 2 FMAs a thread). All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
 // MMAs in flight, reports kErrWaitTimeout and stores nothing.
@@ -37,10 +39,10 @@
 namespace bebelm {
 namespace {
 
-constexpr int kM = 128, kK = 128, kThreads = 640;
-constexpr int kConvert0 = 4, kEpi0 = 12;  // first converter and first epilogue warp
+constexpr int kM = 128, kK = 128, kFixedWarps = 12;
+constexpr int kConvert0 = 4, kEpi0 = kFixedWarps;  // first converter and first epilogue warp
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColA = 256;          // four A buffers of 64 columns behind the accumulators (2 x N columns)
+constexpr uint32_t kColA = 256;          // four A buffers of 64 columns behind the accumulators (2 x 128 columns)
 constexpr int kWaitLimit = 1 << 22;
 constexpr int kRings = 225 * 1024;       // shared memory for the rings
 
@@ -144,14 +146,24 @@ __device__ __forceinline__ void tmem_st_tile(uint32_t taddr, const uint32_t* r) 
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-// 32 lanes x 16 columns; tmem_ld_wait() before the registers are used
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+// 32 lanes x C columns (16 or 32); tmem_ld_wait() before the registers are used
+template <int C>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
+    if constexpr (C == 8) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(taddr));
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i += 16)
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                "%15}, [%16];"
+                : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]),
+                  "=r"(r[i + 7]), "=r"(r[i + 8]), "=r"(r[i + 9]), "=r"(r[i + 10]), "=r"(r[i + 11]), "=r"(r[i + 12]),
+                  "=r"(r[i + 13]), "=r"(r[i + 14]), "=r"(r[i + 15])
+                : "r"(taddr + i));
+    }
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -198,6 +210,7 @@ __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
 
 template <int N, int TERMS, bool BF16>
 struct Lay {
+    static constexpr int kEpiWarps = N == 128 ? 16 : 8, kThreads = 32 * (kFixedWarps + kEpiWarps);
     static constexpr int kAtom = N * 128;                  // N tokens x 64 inputs
     static constexpr int kB = TERMS * kAtom;               // a stage: 64 inputs
     static constexpr int kW = 8192 + 512, kSW = 6;         // codes and zero points (<= 512 bytes) of 128 inputs
@@ -212,9 +225,11 @@ struct Lay {
 
 // FB: blocks of 32 inputs whose sum is scaled together
 template <int N, int TERMS, bool BF16, int FB>
-__global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, TcArgs a) {
+__global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, TcArgs a) {
     using L = Lay<N, TERMS, BF16>;
-    constexpr int SB = L::kSB, SW = L::kSW, SS = L::kSS, F = 4 / FB;  // ring stages, sums a chunk of 128 inputs
+    constexpr int SB = L::kSB, SW = L::kSW, SS = L::kSS;  // ring stages
+    // sums a chunk of 128 inputs, sums handed over at once, times a chunk that this happens
+    constexpr int F = 4 / FB, U = F < 128 / N ? F : 128 / N, H = F / U;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sb = smem_u32(sm);
@@ -245,9 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         auto init = [&](uint32_t b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n)); };
         for (int i = 0; i < SB; ++i) init(b_full(i), 1), init(b_empty(i), 1);
         for (int i = 0; i < SW; ++i) init(w_full(i), 1), init(w_empty(i), 4);
-        for (int i = 0; i < SS; ++i) init(s_full(i), 1), init(s_empty(i), 8);
+        for (int i = 0; i < SS; ++i) init(s_full(i), 1), init(s_empty(i), L::kEpiWarps);
         for (int i = 0; i < 4; ++i) init(a_full(i), 4), init(a_empty(i), 1);
-        for (int i = 0; i < 2; ++i) init(d_full(i), 1), init(d_empty(i), 8);
+        for (int i = 0; i < 2; ++i) init(d_full(i), 1), init(d_empty(i), L::kEpiWarps);
         init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_fail = 0;
@@ -323,20 +338,20 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
                         ok = false;
                         break;
                     }
-                    const int f = i / (2 * FB);
-                    const uint32_t db = F == 1 ? (uint32_t)(c & 1) : (uint32_t)(f & 1);
-                    if (i % (2 * FB) == 0 && !mbar_wait_warp(d_empty(0) + 8 * db, d_ph)) {
+                    constexpr int kUnit = 2 * FB * U;  // steps of 16 inputs between two handings over
+                    const uint32_t db = H == 1 ? (uint32_t)(c & 1) : (uint32_t)(i / kUnit & 1);
+                    if (i % kUnit == 0 && !mbar_wait_warp(d_empty(0) + 8 * db, d_ph)) {
                         ok = false;
                         break;
                     }
-                    if (i % 4 == 0 || i % (2 * FB) == 0) tc_after();
+                    if (i % 4 == 0 || i % kUnit == 0) tc_after();
 #pragma unroll
                     for (int p = 0; p < TERMS; ++p)
-                        mma_ts(tmem + db * N, ta + 8 * i, bd + (uint64_t)((p * L::kAtom + (i & 3) * 32) >> 4), idesc,
-                               i % (2 * FB) > 0 || p > 0);
-                    if ((i + 1) % (2 * FB) == 0) {
+                        mma_ts(tmem + db * 128 + i % kUnit / (2 * FB) * N, ta + 8 * i,
+                               bd + (uint64_t)((p * L::kAtom + (i & 3) * 32) >> 4), idesc, i % (2 * FB) > 0 || p > 0);
+                    if ((i + 1) % kUnit == 0) {
                         commit(d_full(0) + 8 * db);
-                        if (F == 1 ? (c & 1) : (f & 1)) d_ph ^= 1;
+                        if (db) d_ph ^= 1;
                     }
                     if (i % 4 == 3) {
                         commit(b_empty(0) + st8);
@@ -361,14 +376,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
             if (!ok) break;
             tc_after();
             const unsigned char* base = sm + L::kOffW + st * L::kW;
-            uint4 v[2][2];
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-                v[m >> 1][m & 1] = *reinterpret_cast<const uint4*>(base + w * 2048 + m * 512 + lane * 16);
-#pragma unroll
+#pragma unroll 1
             for (int m = 0; m < 2; ++m) {  // tiles of 16 rows
                 const int tile = 2 * w + m;
-                const uint32_t wa[4] = {v[m][0].x, v[m][0].y, v[m][0].z, v[m][0].w}, wb[4] = {v[m][1].x, v[m][1].y, v[m][1].z, v[m][1].w};
+                const uint4 va = *reinterpret_cast<const uint4*>(base + tile * 1024 + lane * 16);
+                const uint4 vb = *reinterpret_cast<const uint4*>(base + tile * 1024 + 512 + lane * 16);
+                const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
                 const unsigned char* z = base + 8192 + (tile * 8 + g) * rec;
                 uint32_t za = 0, za2 = 0, zb = 0, zb2 = 0;
                 uint32_t r[32];
@@ -394,9 +407,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
         }
         if (!ok && lane == 0) s_fail = 1;
     } else if (warp >= kEpi0) {
-        constexpr int C = N / 2;  // columns of a thread
-        const int w = warp - kEpi0, half = w >> 2, row = 32 * (w & 3) + lane;
-        const uint32_t t_d = tmem + ((uint32_t)(32 * (w & 3)) << 16) + half * C;
+        constexpr int C = N * 4 / L::kEpiWarps;  // columns of a thread
+        const int w = warp - kEpi0, part = w >> 2, row = 32 * (w & 3) + lane;
+        const uint32_t t_d = tmem + ((uint32_t)(32 * (w & 3)) << 16) + part * C;
         // this row's scales in a stage: [tile][row % 8][block][row / 8]
         const int sc_at = (((row >> 4) * 8 + (row & 7)) * pc * 2 + ((row >> 3) & 1)) * 2;
         const int xs_step = a.x_scales && a.x_group < kK ? N * 4 * 32 * FB / a.x_group : 0;  // bytes a sum
@@ -404,45 +417,54 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
 #pragma unroll
         for (int i = 0; i < C; ++i) acc[i] = 0.f;
         bool ok = true;
-        int u = 0;
-        for (int c = 0; ok && c < chunks; ++c) {
-            const int st = c % SS;
+        unsigned d_ph = 0;
+        for (int c = 0, st = 0, s_ph = 0; ok && c < chunks; ++c) {
             const unsigned char* base = sm + L::kOffS + st * L::kS;
-            ok = mbar_wait_warp(s_full(st), (c / SS) & 1);
-            for (int f = 0; ok && f < F; ++f, ++u) {
-                const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (f * FB * pc / 4) * 4), a.w.scale_bf16);
-                const unsigned char* xs = base + L::kXs + half * C * 4 + f * xs_step;
-                ok = mbar_wait_warp(d_full(u & 1), (u >> 1) & 1);
-                if (!ok) break;
+            ok = mbar_wait_warp(s_full(st), s_ph);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int db = H == 1 ? c & 1 : h & 1;
+                if (!ok || !mbar_wait_warp(d_full(db), d_ph)) {
+                    ok = false;
+                    break;
+                }
+                if (db) d_ph ^= 1;
                 tc_after();
-                constexpr int B = 16;  // columns in registers at a time
 #pragma unroll
-                for (int i0 = 0; i0 < C; i0 += B) {
-                    uint32_t d[B];
-                    tmem_ld16(t_d + (u & 1) * N + i0, d);
-                    tmem_ld_wait();
-                    if (i0 + B == C) {
-                        tc_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(d_empty(u & 1));
-                    }
-                    if (a.x_scales) {
+                for (int f = 0; f < U; ++f) {
+                    const int sum = h * U + f;
+                    const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (sum * FB * pc / 4) * 4), a.w.scale_bf16);
+                    const unsigned char* xs = base + L::kXs + part * C * 4 + sum * xs_step;
+                    constexpr int B = C < 16 ? C : 16;  // columns in registers at a time
 #pragma unroll
-                        for (int i = 0; i < B; i += 4) {
-                            const float4 x4 = *reinterpret_cast<const float4*>(xs + (i0 + i) * 4);
-                            acc[i0 + i] = fmaf(__uint_as_float(d[i]) * x4.x, s, acc[i0 + i]);
-                            acc[i0 + i + 1] = fmaf(__uint_as_float(d[i + 1]) * x4.y, s, acc[i0 + i + 1]);
-                            acc[i0 + i + 2] = fmaf(__uint_as_float(d[i + 2]) * x4.z, s, acc[i0 + i + 2]);
-                            acc[i0 + i + 3] = fmaf(__uint_as_float(d[i + 3]) * x4.w, s, acc[i0 + i + 3]);
+                    for (int j = 0; j < C; j += B) {
+                        uint32_t d[B];
+                        tmem_ld<B>(t_d + db * 128 + f * N + j, d);
+                        tmem_ld_wait();
+                        if (f == U - 1 && j + B == C) {
+                            tc_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(d_empty(db));
                         }
-                    } else {
+                        if (a.x_scales) {
 #pragma unroll
-                        for (int i = 0; i < B; ++i) acc[i0 + i] = fmaf(__uint_as_float(d[i]), s, acc[i0 + i]);
+                            for (int i = 0; i < B; i += 4) {
+                                const float4 x4 = *reinterpret_cast<const float4*>(xs + (j + i) * 4);
+                                acc[j + i] = fmaf(__uint_as_float(d[i]) * x4.x, s, acc[j + i]);
+                                acc[j + i + 1] = fmaf(__uint_as_float(d[i + 1]) * x4.y, s, acc[j + i + 1]);
+                                acc[j + i + 2] = fmaf(__uint_as_float(d[i + 2]) * x4.z, s, acc[j + i + 2]);
+                                acc[j + i + 3] = fmaf(__uint_as_float(d[i + 3]) * x4.w, s, acc[j + i + 3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < B; ++i) acc[j + i] = fmaf(__uint_as_float(d[i]), s, acc[j + i]);
+                        }
                     }
                 }
             }
             __syncwarp();
             if (ok && lane == 0) mbar_arrive(s_empty(st));
+            if (++st == SS) st = 0, s_ph ^= 1;
         }
         if (!ok) {
             if (lane == 0) s_fail = 1;
@@ -451,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_tc_kernel(const __grid_constan
             if (r < a.w.n_out) {
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
-                    const size_t t = (size_t)t0 + half * C + i;
+                    const size_t t = (size_t)t0 + part * C + i;
                     if (t >= a.tokens) break;
                     const float v = a.col_scale ? acc[i] * __ldg(a.col_scale + t) : acc[i];
                     if (a.y_bf16)
@@ -562,7 +584,7 @@ cudaError_t run(const CUtensorMap& tm, TcArgs& a, bool pdl, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.w.tile_rows / 8), (unsigned)((a.tokens + N - 1) / N));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(L::kThreads);
     cfg.dynamicSmemBytes = L::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute at{};
