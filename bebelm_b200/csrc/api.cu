@@ -2725,7 +2725,7 @@ size_t w4_scratch(const W4View& w, const W4X& x) {
 }
 cudaError_t w4_run(const bebelm_w4* W, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms, cudaStream_t s) {
     if (x.tokens <= kW4StreamTokens) return launch_w4_stream(W->v, x, y, y_bf16, workspace, num_sms, s);
-    return launch_w4_tc(W->v, x, y, y_bf16, workspace, W->err.d, s);
+    return launch_w4_tc(W->v, x, y, y_bf16, workspace, num_sms, W->err.d, s);
 }
 
 int w4_timeout(const bebelm_w4* W) {

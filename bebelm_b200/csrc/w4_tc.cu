@@ -12,12 +12,12 @@
 //        largest where the second term runs out of exponent). 2^-e is applied with the output.
 // w4_terms_kernel writes the last two as [terms][tokens][kp].
 //
-// One CTA per 128 rows x N tokens, one CTA an SM, 20 or 28 warps:
-//   warps 0, 2, 3  copies, a ring each, since they are held for different times: the activations' 128-byte-swizzled
+// Tiles of 128 rows x N tokens, one CTA an SM that takes one tile after the other, 20 or 28 warps:
+//   warps 0, 2   copies, a ring each, since they are held for different times: the activations' 128-byte-swizzled
 //                tiles of 64 inputs (TMA, until their MMAs are done), the codes and zero points of 128 inputs (bulk copies:
 //                they lie together, see w4.cu; until they are unpacked) and the scales (until they are applied).
 //                With one ring for the three its depth bound everything: 5 stages against a stage's 6000 cycles.
-//   warp 1       issues the MMAs, A from TMEM, B from shared memory.
+//   warps 1, 3   issue the MMAs, A from TMEM, B from shared memory.
 //   warps 4-11   unpack codes to A in TMEM, four buffers of 128 inputs, warps 4-7 the even and 8-11 the odd
 //                ones (one set took longer than the MMAs): a warp's lanes hold (row g and g + 8, pairs 4 i + q), the
 //                fragment of `tcgen05.st.16x128b`. A never passes through shared memory, whose bandwidth the
@@ -54,7 +54,7 @@ struct TcArgs {
     const float* x_scales;    // [n_groups][tokens padded to 128]: a factor per group of inputs, or null
     size_t x_pitch, x_groups;
     int x_group;              // inputs of a group
-    int y_bf16, plane_rows;  // plane_rows: rows of B between the terms
+    int y_bf16, tiles, plane_rows;  // plane_rows: rows of B between the terms
     int* err;
 };
 
@@ -219,7 +219,7 @@ struct Lay {
     static constexpr int kOffW = 0, kOffS = kSW * kW, kOffB = (kOffS + kSS * kS + 1023) / 1024 * 1024;
     static constexpr int kSB = (kRings - kOffB) / kB < 12 ? (kRings - kOffB) / kB : 12;
     static constexpr int kSmem = kOffB + kSB * kB + 1024;
-    static constexpr int kBars = 2 * (kSB + kSW + kSS) + 13;
+    static constexpr int kBars = 2 * (kSB + kSW + kSS) + 14;
     static_assert(kSB >= 4, "ring");
 };
 
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
     using L = Lay<N, TERMS, BF16>;
     constexpr int SB = L::kSB, SW = L::kSW, SS = L::kSS;  // ring stages
     // sums a chunk of 128 inputs, sums handed over at once, times a chunk that this happens
-    constexpr int F = 4 / FB, U = F < 128 / N ? F : 128 / N, H = F / U;
+    constexpr int F = 4 / FB, U = F < 128 / N ? F : 128 / N, H = F / U, kIssuers = H == 1 ? 2 : 1;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sb = smem_u32(sm);
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int rb = blockIdx.x, t0 = (int)blockIdx.y * N, chunks = (int)a.w.chunks, pc = a.w.per_chunk;
+    const int chunks = (int)a.w.chunks, pc = a.w.per_chunk, row_blocks = (int)(a.w.tile_rows / 8);
     const uint32_t bars = smem_u32(s_bar);
     auto b_full = [&](int i) { return bars + 8 * i; };
     auto b_empty = [&](int i) { return bars + 8 * (SB + i); };
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         for (int i = 0; i < SS; ++i) init(s_full(i), 1), init(s_empty(i), L::kEpiWarps);
         for (int i = 0; i < 4; ++i) init(a_full(i), 4), init(a_empty(i), 1);
         for (int i = 0; i < 2; ++i) init(d_full(i), 1), init(d_empty(i), L::kEpiWarps);
-        init(drained, 1);
+        init(drained, 1), init(drained + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_fail = 0;
     }
@@ -274,105 +274,140 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
     // scales and activations' terms may come from the kernel before
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // A copying warp: n stages through a ring, each issued by `load(stage, i)`.
-    auto feed = [&](int n, int stages, uint32_t full0, uint32_t empty0, uint32_t bytes, auto load) {
-        int i = 0;
-        for (int st = 0, ph = 1; i < n; ++i) {
-            if (!mbar_wait_warp(empty0 + 8 * st, ph)) {  // the first round passes
-                if (lane == 0) s_fail = 1;
-                break;
-            }
-            expect_tx(full0 + 8 * st, bytes);
-            load(st, i);
-            if (++st == stages) st = 0, ph ^= 1;
+    // A ring's position at the side that fills it: a stage is waited for, filled, and the next one is up.
+    struct Fill {
+        int st = 0, done = 0;
+        unsigned ph = 1;  // the first round passes
+    };
+    auto fill = [&](Fill& r, int stages, uint32_t full0, uint32_t empty0, uint32_t bytes) -> bool {
+        if (!mbar_wait_warp(empty0 + 8 * r.st, r.ph)) {
+            if (lane == 0) s_fail = 1;
+            return false;
         }
-        // nothing may be in flight when the CTA exits
-        for (int j = i > stages ? i - stages : 0; j < i; ++j) mbar_wait_warp(full0 + 8 * (j % stages), (j / stages) & 1);
+        expect_tx(full0 + 8 * r.st, bytes);
+        r.done = min(r.done + 1, stages);
+        return true;
+    };
+    auto next = [](Fill& r, int stages) {
+        if (++r.st == stages) r.st = 0, r.ph ^= 1;
+    };
+    // Nothing may be in flight when the CTA exits: the last filling of each stage has to land.
+    auto landed = [&](Fill& r, int stages, uint32_t full0) {
+        for (; r.done > 0; --r.done) {
+            if (--r.st < 0) r.st = stages - 1, r.ph ^= 1;
+            mbar_wait_warp(full0 + 8 * r.st, r.ph ^ 1);
+        }
     };
     if (warp == 0) {
-        feed(2 * chunks, SB, b_full(0), b_empty(0), L::kB, [&](int st, int i) {
+        Fill r;
+        for (int tile = blockIdx.x, ok = 1; ok && tile < a.tiles; tile += gridDim.x) {
+            const int t0 = tile / row_blocks * N;
+            for (int i = 0; i < 2 * chunks; ++i) {
+                ok = fill(r, SB, b_full(0), b_empty(0), L::kB);
+                if (!ok) break;
 #pragma unroll
                 for (int p = 0; p < TERMS; ++p)
-                    tma_2d(sb + L::kOffB + st * L::kB + p * L::kAtom, &tm_x, i * 64, t0 + p * a.plane_rows, b_full(st));
-            });
-    } else if (warp == 2) {
-        {
-            const uint32_t zb = a.w.zeros ? 64u * (pc == 4 ? 8 : 4) : 0u;
-            const unsigned char* code = reinterpret_cast<const unsigned char*>(a.w.codes) + (size_t)rb * chunks * 8192;
-            const unsigned char* zero = reinterpret_cast<const unsigned char*>(a.w.zeros) + (size_t)rb * chunks * zb;
-            feed(chunks, SW, w_full(0), w_empty(0), 8192u + zb, [&](int st, int c) {
-                bulk(sb + L::kOffW + st * L::kW, code + (size_t)c * 8192, 8192, w_full(st));
-                if (zb) bulk(sb + L::kOffW + st * L::kW + 8192, zero + (size_t)c * zb, zb, w_full(st));
-            });
+                    tma_2d(sb + L::kOffB + r.st * L::kB + p * L::kAtom, &tm_x, i * 64, t0 + p * a.plane_rows, b_full(r.st));
+                next(r, SB);
+            }
         }
-    } else if (warp == 3) {
-        {
-            const uint32_t scb = 256u * (uint32_t)pc;
-            const int xs_rows = a.x_scales ? (a.x_group < kK ? kK / a.x_group : 1) : 0;  // groups that meet 128 inputs
-            const unsigned char* scale = reinterpret_cast<const unsigned char*>(a.w.scales) + (size_t)rb * chunks * scb;
-            feed(chunks, SS, s_full(0), s_empty(0), scb + xs_rows * N * 4u, [&](int st, int c) {
-                bulk(sb + L::kOffS + st * L::kS, scale + (size_t)c * scb, scb, s_full(st));
+        landed(r, SB, b_full(0));
+    } else if (warp == 2) {
+        const uint32_t zb = a.w.zeros ? 64u * (pc == 4 ? 8 : 4) : 0u, scb = 256u * (uint32_t)pc;
+        const int xs_rows = a.x_scales ? (a.x_group < kK ? kK / a.x_group : 1) : 0;  // groups that meet 128 inputs
+        Fill r, q;
+        for (int tile = blockIdx.x, ok = 1; ok && tile < a.tiles; tile += gridDim.x) {
+            const int rb = tile % row_blocks, t0 = tile / row_blocks * N;
+            for (int c = 0; c < chunks; ++c) {
+                const size_t at = (size_t)rb * chunks + c;
+                ok = fill(r, SW, w_full(0), w_empty(0), 8192u + zb);
+                if (!ok) break;
+                bulk(sb + L::kOffW + r.st * L::kW, reinterpret_cast<const unsigned char*>(a.w.codes) + at * 8192, 8192, w_full(r.st));
+                if (zb)
+                    bulk(sb + L::kOffW + r.st * L::kW + 8192, reinterpret_cast<const unsigned char*>(a.w.zeros) + at * zb, zb, w_full(r.st));
+                next(r, SW);
+                ok = fill(q, SS, s_full(0), s_empty(0), scb + xs_rows * N * 4u);
+                if (!ok) break;
+                bulk(sb + L::kOffS + q.st * L::kS, reinterpret_cast<const unsigned char*>(a.w.scales) + at * scb, scb, s_full(q.st));
                 for (int j = 0; j < xs_rows; ++j) {  // behind the last group (padded inputs) the last one again
                     const size_t gr = min((size_t)c * kK / a.x_group + j, a.x_groups - 1);
-                    bulk(sb + L::kOffS + st * L::kS + L::kXs + j * N * 4, a.x_scales + gr * a.x_pitch + t0, N * 4, s_full(st));
+                    bulk(sb + L::kOffS + q.st * L::kS + L::kXs + j * N * 4, a.x_scales + gr * a.x_pitch + t0, N * 4, s_full(q.st));
                 }
-            });
-        }
-    } else if (warp == 1) {
-        {
-            // Issue is on the critical path: every offset below is a constant of the unrolled loop, ring
-            // positions and phases are carried along.
-            constexpr uint32_t idesc = instr_desc(N, BF16);
-            const uint64_t b0 = smem_desc(sb + L::kOffB);
-            uint64_t bd = b0;
-            uint32_t st8 = 0, ab = 0;  // byte offset of the stage's barriers, A buffer
-            unsigned b_ph = 0, a_ph = 0, d_ph = 1;  // d_ph: of the buffers' last reads; the first round passes
-            bool ok = true;
-            for (int c = 0; ok && c < chunks; ++c) {
-                ok = mbar_wait_warp(a_full(0) + 8 * ab, a_ph);
-                if (!ok) break;
-                const uint32_t ta = tmem + kColA + 64 * ab;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {  // 16 inputs: 8 columns of A, 32 bytes of B
-                    if (i % 4 == 0 && !mbar_wait_warp(b_full(0) + st8, b_ph)) {
-                        ok = false;
-                        break;
-                    }
-                    constexpr int kUnit = 2 * FB * U;  // steps of 16 inputs between two handings over
-                    const uint32_t db = H == 1 ? (uint32_t)(c & 1) : (uint32_t)(i / kUnit & 1);
-                    if (i % kUnit == 0 && !mbar_wait_warp(d_empty(0) + 8 * db, d_ph)) {
-                        ok = false;
-                        break;
-                    }
-                    if (i % 4 == 0 || i % kUnit == 0) tc_after();
-#pragma unroll
-                    for (int p = 0; p < TERMS; ++p)
-                        mma_ts(tmem + db * 128 + i % kUnit / (2 * FB) * N, ta + 8 * i,
-                               bd + (uint64_t)((p * L::kAtom + (i & 3) * 32) >> 4), idesc, i % (2 * FB) > 0 || p > 0);
-                    if ((i + 1) % kUnit == 0) {
-                        commit(d_full(0) + 8 * db);
-                        if (db) d_ph ^= 1;
-                    }
-                    if (i % 4 == 3) {
-                        commit(b_empty(0) + st8);
-                        st8 += 8, bd += L::kB >> 4;
-                        if (st8 == 8 * SB) st8 = 0, bd = b0, b_ph ^= 1;
-                    }
-                }
-                if (!ok) break;
-                commit(a_empty(0) + 8 * ab);
-                if (++ab == 4) ab = 0, a_ph ^= 1;
+                next(q, SS);
             }
-            if (!ok && lane == 0) s_fail = 1;
-            commit(drained);  // every MMA of this CTA done, also after a failed wait
-            mbar_wait_warp(drained, 0);
         }
-    } else if (warp >= kConvert0 && warp < kEpi0) {
-        const int w = warp & 3, g = lane >> 2, rec = pc == 4 ? 8 : 4;
+        landed(r, SW, w_full(0));
+        landed(q, SS, s_full(0));
+    } else if (warp == 1 || (warp == 3 && kIssuers == 2)) {
+        // Issue is on the critical path: every offset below is a constant of the unrolled loop, ring
+        // positions and phases are carried along. Four waits, four commits and eight MMAs a chunk take a warp some
+        // 900 cycles, more than 128 tokens' MMAs do: where a chunk is one handing over, two warps take
+        // turns, each with an accumulator and two A buffers of its own.
+        constexpr uint32_t idesc = instr_desc(N, BF16);
+        const int first = warp == 3, total = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * chunks;
+        const uint64_t b0 = smem_desc(sb + L::kOffB);
+        int st = 2 * first;  // ring stage
+        uint32_t ab = first, db = first;
+        unsigned b_ph = 0, a_ph = 0, d_ph = 1;  // d_ph: of the accumulators' last reads; the first round passes
         bool ok = true;
-        for (int c = (warp - kConvert0) >> 2; c < chunks; c += 2) {
-            const int st = c % SW, ab = c & 3;
-            ok = mbar_wait_warp(w_full(st), (c / SW) & 1) && (c < 4 || mbar_wait_warp(a_empty(ab), ((c >> 2) - 1) & 1));
+        for (int c = first; ok && c < total; c += kIssuers) {
+            ok = mbar_wait_warp(a_full(0) + 8 * ab, a_ph);
+            if (!ok) break;
+            const uint32_t ta = tmem + kColA + 64 * ab;
+            uint64_t bd = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {  // 16 inputs: 8 columns of A, 32 bytes of B
+                constexpr int kUnit = 2 * FB * U;  // steps of 16 inputs between two handings over
+                // The accumulator first: once it is free, every chunk before the last two is done, so the
+                // stage's phase before the one waited for is over whichever warp used it.
+                if (i % kUnit == 0) {
+                    ok = mbar_wait_warp(d_empty(0) + 8 * db, d_ph);
+                    if (!ok) break;
+                }
+                if (i % 4 == 0) {
+                    ok = mbar_wait_warp(b_full(0) + 8 * st, b_ph);
+                    if (!ok) break;
+                    bd = b0 + (uint64_t)(st * (L::kB >> 4));
+                }
+                if (i % 4 == 0 || i % kUnit == 0) tc_after();
+#pragma unroll
+                for (int p = 0; p < TERMS; ++p)
+                    mma_ts(tmem + db * 128 + i % kUnit / (2 * FB) * N, ta + 8 * i,
+                           bd + (uint64_t)((p * L::kAtom + (i & 3) * 32) >> 4), idesc, i % (2 * FB) > 0 || p > 0);
+                if ((i + 1) % kUnit == 0) {
+                    commit(d_full(0) + 8 * db);
+                    if (kIssuers == 2) {
+                        d_ph ^= 1;
+                    } else {
+                        db ^= 1;
+                        if (db == 0) d_ph ^= 1;
+                    }
+                }
+                if (i % 4 == 3) {
+                    commit(b_empty(0) + 8 * st);
+                    if (++st == SB) st = 0, b_ph ^= 1;
+                }
+            }
+            if (!ok) break;
+            commit(a_empty(0) + 8 * ab);
+            ab += kIssuers;
+            if (ab >= 4) ab -= 4, a_ph ^= 1;
+            if (kIssuers == 2) {  // the other warp's two stages
+                st += 2;
+                if (st >= SB) st -= SB, b_ph ^= 1;
+            }
+        }
+        if (!ok && lane == 0) s_fail = 1;
+        commit(drained + 8 * first);  // every MMA of this warp done, also after a failed wait
+        mbar_wait_warp(drained + 8 * first, 0);
+    } else if (warp >= kConvert0 && warp < kEpi0) {
+        const int w = warp & 3, g = lane >> 2, rec = pc == 4 ? 8 : 4, set = (warp - kConvert0) >> 2;
+        const int total = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * chunks;
+        bool ok = true;
+        int st = set, ab = set;
+        unsigned w_ph = 0, a_ph = 1;  // the first round of A buffers passes
+        for (int c = set; c < total; c += 2) {
+            ok = mbar_wait_warp(w_full(st), w_ph) && mbar_wait_warp(a_empty(ab), a_ph);
             if (!ok) break;
             tc_after();
             const unsigned char* base = sm + L::kOffW + st * L::kW;
@@ -404,6 +439,9 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
             tc_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(a_full(ab)), mbar_arrive(w_empty(st));
+            st += 2, ab += 2;
+            if (st >= SW) st -= SW, w_ph ^= 1;
+            if (ab >= 4) ab -= 4, a_ph ^= 1;
         }
         if (!ok && lane == 0) s_fail = 1;
     } else if (warp >= kEpi0) {
@@ -413,64 +451,62 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         // this row's scales in a stage: [tile][row % 8][block][row / 8]
         const int sc_at = (((row >> 4) * 8 + (row & 7)) * pc * 2 + ((row >> 3) & 1)) * 2;
         const int xs_step = a.x_scales && a.x_group < kK ? N * 4 * 32 * FB / a.x_group : 0;  // bytes a sum
-        float acc[C];
-#pragma unroll
-        for (int i = 0; i < C; ++i) acc[i] = 0.f;
         bool ok = true;
-        unsigned d_ph = 0;
-        for (int c = 0, st = 0, s_ph = 0; ok && c < chunks; ++c) {
-            const unsigned char* base = sm + L::kOffS + st * L::kS;
-            ok = mbar_wait_warp(s_full(st), s_ph);
+        int st = 0, db = 0;
+        unsigned d_ph = 0, s_ph = 0;
+        for (int tile = blockIdx.x; ok && tile < a.tiles; tile += gridDim.x) {
+            const int rb = tile % row_blocks, t0 = tile / row_blocks * N;
+            float acc[C];
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                const int db = H == 1 ? c & 1 : h & 1;
-                if (!ok || !mbar_wait_warp(d_full(db), d_ph)) {
-                    ok = false;
-                    break;
-                }
-                if (db) d_ph ^= 1;
-                tc_after();
+            for (int i = 0; i < C; ++i) acc[i] = 0.f;
+            for (int c = 0; ok && c < chunks; ++c) {
+                const unsigned char* base = sm + L::kOffS + st * L::kS;
+                ok = mbar_wait_warp(s_full(st), s_ph);
 #pragma unroll
-                for (int f = 0; f < U; ++f) {
-                    const int sum = h * U + f;
-                    const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (sum * FB * pc / 4) * 4), a.w.scale_bf16);
-                    const unsigned char* xs = base + L::kXs + part * C * 4 + sum * xs_step;
-                    constexpr int B = C < 16 ? C : 16;  // columns in registers at a time
+                for (int h = 0; h < H; ++h) {
+                    ok = ok && mbar_wait_warp(d_full(db), d_ph);
+                    if (!ok) break;
+                    tc_after();
 #pragma unroll
-                    for (int j = 0; j < C; j += B) {
-                        uint32_t d[B];
-                        tmem_ld<B>(t_d + db * 128 + f * N + j, d);
-                        tmem_ld_wait();
-                        if (f == U - 1 && j + B == C) {
-                            tc_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(d_empty(db));
-                        }
-                        if (a.x_scales) {
+                    for (int f = 0; f < U; ++f) {
+                        const int sum = h * U + f;
+                        const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (sum * FB * pc / 4) * 4), a.w.scale_bf16);
+                        const unsigned char* xs = base + L::kXs + part * C * 4 + sum * xs_step;
+                        constexpr int B = C < 16 ? C : 16;  // columns in registers at a time
 #pragma unroll
-                            for (int i = 0; i < B; i += 4) {
-                                const float4 x4 = *reinterpret_cast<const float4*>(xs + (j + i) * 4);
-                                acc[j + i] = fmaf(__uint_as_float(d[i]) * x4.x, s, acc[j + i]);
-                                acc[j + i + 1] = fmaf(__uint_as_float(d[i + 1]) * x4.y, s, acc[j + i + 1]);
-                                acc[j + i + 2] = fmaf(__uint_as_float(d[i + 2]) * x4.z, s, acc[j + i + 2]);
-                                acc[j + i + 3] = fmaf(__uint_as_float(d[i + 3]) * x4.w, s, acc[j + i + 3]);
+                        for (int j = 0; j < C; j += B) {
+                            uint32_t d[B];
+                            tmem_ld<B>(t_d + db * 128 + f * N + j, d);
+                            tmem_ld_wait();
+                            if (f == U - 1 && j + B == C) {
+                                tc_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(d_empty(db));
                             }
-                        } else {
+                            if (a.x_scales) {
 #pragma unroll
-                            for (int i = 0; i < B; ++i) acc[j + i] = fmaf(__uint_as_float(d[i]), s, acc[j + i]);
+                                for (int i = 0; i < B; i += 4) {
+                                    const float4 x4 = *reinterpret_cast<const float4*>(xs + (j + i) * 4);
+                                    acc[j + i] = fmaf(__uint_as_float(d[i]) * x4.x, s, acc[j + i]);
+                                    acc[j + i + 1] = fmaf(__uint_as_float(d[i + 1]) * x4.y, s, acc[j + i + 1]);
+                                    acc[j + i + 2] = fmaf(__uint_as_float(d[i + 2]) * x4.z, s, acc[j + i + 2]);
+                                    acc[j + i + 3] = fmaf(__uint_as_float(d[i + 3]) * x4.w, s, acc[j + i + 3]);
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < B; ++i) acc[j + i] = fmaf(__uint_as_float(d[i]), s, acc[j + i]);
+                            }
                         }
                     }
+                    db ^= 1;
+                    if (db == 0) d_ph ^= 1;
                 }
+                __syncwarp();
+                if (ok && lane == 0) mbar_arrive(s_empty(st));
+                if (++st == SS) st = 0, s_ph ^= 1;
             }
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(s_empty(st));
-            if (++st == SS) st = 0, s_ph ^= 1;
-        }
-        if (!ok) {
-            if (lane == 0) s_fail = 1;
-        } else {
             const size_t r = (size_t)rb * kM + row;
-            if (r < a.w.n_out) {
+            if (ok && r < a.w.n_out) {
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const size_t t = (size_t)t0 + part * C + i;
@@ -483,6 +519,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
                 }
             }
         }
+        if (!ok && lane == 0) s_fail = 1;
     }
     __syncwarp();
     tc_before();
@@ -577,13 +614,14 @@ size_t terms_bytes(const W4View& w, const W4X& x) {
 }
 
 template <int N, int TERMS, bool BF16, int FB>
-cudaError_t run(const CUtensorMap& tm, TcArgs& a, bool pdl, cudaStream_t s) {
+cudaError_t run(const CUtensorMap& tm, TcArgs& a, int num_sms, bool pdl, cudaStream_t s) {
     using L = Lay<N, TERMS, BF16>;
     auto kernel = w4_tc_kernel<N, TERMS, BF16, FB>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(a.w.tile_rows / 8), (unsigned)((a.tokens + N - 1) / N));
+    a.tiles = (int)(a.w.tile_rows / 8 * ((a.tokens + N - 1) / N));
+    cfg.gridDim = dim3((unsigned)std::min(a.tiles, num_sms));
     cfg.blockDim = dim3(L::kThreads);
     cfg.dynamicSmemBytes = L::kSmem;
     cfg.stream = s;
@@ -595,16 +633,16 @@ cudaError_t run(const CUtensorMap& tm, TcArgs& a, bool pdl, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, kernel, tm, a);
 }
 template <int N, int TERMS, bool BF16>
-cudaError_t run_fb(const CUtensorMap& tm, TcArgs& a, int fb, bool pdl, cudaStream_t s) {
-    return fb == 4   ? run<N, TERMS, BF16, 4>(tm, a, pdl, s)
-           : fb == 2 ? run<N, TERMS, BF16, 2>(tm, a, pdl, s)
-                     : run<N, TERMS, BF16, 1>(tm, a, pdl, s);
+cudaError_t run_fb(const CUtensorMap& tm, TcArgs& a, int fb, int num_sms, bool pdl, cudaStream_t s) {
+    return fb == 4   ? run<N, TERMS, BF16, 4>(tm, a, num_sms, pdl, s)
+           : fb == 2 ? run<N, TERMS, BF16, 2>(tm, a, num_sms, pdl, s)
+                     : run<N, TERMS, BF16, 1>(tm, a, num_sms, pdl, s);
 }
 template <int N>
-cudaError_t run_kind(const CUtensorMap& tm, TcArgs& a, int kind, int fb, bool pdl, cudaStream_t s) {
-    return kind == kW4XBf16  ? run_fb<N, 1, true>(tm, a, fb, pdl, s)
-           : kind == kW4XF32 ? run_fb<N, 2, false>(tm, a, fb, pdl, s)
-                             : run_fb<N, 1, false>(tm, a, fb, pdl, s);
+cudaError_t run_kind(const CUtensorMap& tm, TcArgs& a, int kind, int fb, int num_sms, bool pdl, cudaStream_t s) {
+    return kind == kW4XBf16  ? run_fb<N, 1, true>(tm, a, fb, num_sms, pdl, s)
+           : kind == kW4XF32 ? run_fb<N, 2, false>(tm, a, fb, num_sms, pdl, s)
+                             : run_fb<N, 1, false>(tm, a, fb, num_sms, pdl, s);
 }
 
 }  // namespace
@@ -616,10 +654,10 @@ size_t w4_tc_workspace(const W4View& w, const W4X& x) {
     return n;
 }
 
-cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int* err, cudaStream_t s) {
+cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms, int* err, cudaStream_t s) {
     const auto enc = map_encoder();
     const size_t kp = w.chunks * kK, terms = x.kind == kW4XF32 ? 2 : 1;
-    if (!enc || x.tokens * terms >= (1ull << 31) || x.tokens > 65535 * size_t(32)) return cudaErrorNotSupported;
+    if (!enc || x.tokens * terms >= (1ull << 31) || w.tile_rows / 8 * (x.tokens / 32 + 1) >= (1ull << 31)) return cudaErrorNotSupported;
     TcArgs a{};
     a.w = w;
     a.y = y, a.y_bf16 = y_bf16, a.tokens = x.tokens, a.err = err;
@@ -652,9 +690,9 @@ cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, voi
     if (enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(rows), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    return n_tile == 32   ? run_kind<32>(tm, a, x.kind, fb, !direct, s)
-           : n_tile == 64 ? run_kind<64>(tm, a, x.kind, fb, !direct, s)
-                          : run_kind<128>(tm, a, x.kind, fb, !direct, s);
+    return n_tile == 32   ? run_kind<32>(tm, a, x.kind, fb, num_sms, !direct, s)
+           : n_tile == 64 ? run_kind<64>(tm, a, x.kind, fb, num_sms, !direct, s)
+                          : run_kind<128>(tm, a, x.kind, fb, num_sms, !direct, s);
 }
 
 }  // namespace bebelm
