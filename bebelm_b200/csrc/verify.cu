@@ -34,7 +34,7 @@ namespace cg = cooperative_groups;
 namespace bebelm {
 namespace {
 
-constexpr int kRowThreads = 256, kPickThreads = 512, kMaxSlices = 64;
+constexpr int kRowThreads = 256, kMaxSlices = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct RowPart {  // of one slice of a row
@@ -62,6 +62,7 @@ __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int b) {
 // grid (target rows then draft rows, slices)
 template <bool GREEDY, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(VerifyArgs a, RowPart* parts, int slices) {
+    asm volatile("griddepcontrol.launch_dependents;");
     const int row = blockIdx.x, target_rows = a.seqs * (a.drafts + 1);
     const float* p;
     if (row < target_rows) {
@@ -153,8 +154,28 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(VerifyArgs a, 
     }
 }
 
-// the slices of one row joined by a warp (every lane gets the answer)
-__device__ __forceinline__ RowPart join_row(const RowPart* parts, int slices, double inv_t, bool greedy) {
+// 2^y for y <= 0 to 2e-14: y = k + f with f in [-1/2, 1/2] (k from the rounding of 1.5 * 2^52 + y), 2^f a polynomial of
+// degree 9 through 2^f at the 10 Chebyshev nodes of the interval, 2^k added to the exponent. 0 below 2^-1000.
+// (exp() of the same arguments took the pass over a row half as long again.)
+__device__ __forceinline__ double exp2_neg(double y) {
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52
+    const double t = fmax(y, -1001.0) + magic, f = fmax(y, -1001.0) - (t - magic);
+    double p = 1.0205905413765595e-07;
+    p = fma(p, f, 1.325964524488711e-06);
+    p = fma(p, f, 1.5252672924850737e-05);
+    p = fma(p, f, 0.0001540343375125101);
+    p = fma(p, f, 0.0013333558200794592);
+    p = fma(p, f, 0.009618129193934313);
+    p = fma(p, f, 0.05550410866465167);
+    p = fma(p, f, 0.2402265069564034);
+    p = fma(p, f, 0.6931471805599462);
+    p = fma(p, f, 1.0000000000000135);
+    const double r = __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+    return y < -1000.0 ? 0.0 : r;
+}
+
+// the slices of one row joined by a warp (every lane gets the answer); scale = log2(e) / temperature
+__device__ __forceinline__ RowPart join_row(const RowPart* parts, int slices, double scale, bool greedy) {
     const int lane = threadIdx.x & 31;
     RowPart r{-CUDART_INF_F, 0xffffffffu, 0.0};
     for (int i = lane; i < slices; i += 32) r.m = fmaxf(r.m, parts[i].m);
@@ -165,7 +186,7 @@ __device__ __forceinline__ RowPart join_row(const RowPart* parts, int slices, do
         if (greedy) {
             if (p.m == r.m) r.i = min(r.i, p.i);
         } else if (p.s > 0.0) {
-            r.s += p.s * exp(((double)p.m - (double)r.m) * inv_t);
+            r.s += p.s * exp2_neg(((double)p.m - (double)r.m) * scale);
         }
     }
     if (greedy) {
@@ -196,151 +217,170 @@ __global__ void __launch_bounds__(32) verify_greedy_kernel(VerifyArgs a, const R
     }
 }
 
-__device__ __forceinline__ double block_sum(double v, double* s_part) {  // every thread gets the sum
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double t = 0.0;
-    for (int w = 0; w < kPickThreads / 32; ++w) t += s_part[w];
-    return t;
-}
-
-// One row of probabilities, of logits with a known maximum and sum, or a certain draft, as f64.
+// One row of probabilities, or of logits with a known maximum, as f64 weights: f · 2^((l - m) c) or f · p.
 struct Row {
     const float* p;
-    double m, inv_t, inv_s;
+    double m, c, f;
     int probs;
-    __device__ __forceinline__ double raw(size_t j) const {  // before the division by the sum
-        const float l = p[j];
-        if (probs) return clean_p(l);
-        const double d = (double)clean(l) - m;
-        return exp(d * inv_t);
+    __device__ __forceinline__ double weigh(float l) const {
+        return probs ? clean_p(l) * f : exp2_neg(((double)clean(l) - m) * c) * f;
     }
-    __device__ __forceinline__ double at(size_t j) const { return raw(j) * inv_s; }
 };
+// 4 entries from j (a multiple of 4); those at and past `end` count as nothing
+template <bool VEC>
+__device__ __forceinline__ void entries4(const Row& r, size_t j, size_t end, float* v) {
+    if (VEC && j + 4 <= end) {
+        const float4 t = __ldg(reinterpret_cast<const float4*>(r.p + j));
+        v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = j + i < end ? __ldg(r.p + j + i) : -CUDART_INF_F;
+    }
+}
 
-__global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(VerifyArgs a, const RowPart* parts, int slices) {
+// PT threads; 64 registers each, so that an SM holds 1024 of them however they are split
+template <int PT, bool VEC>
+__global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a, const RowPart* parts, int slices) {
     cg::cluster_group cl = cg::this_cluster();
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), b = blockIdx.x / ctas;
-    __shared__ double s_part[kPickThreads / 32], s_sum[3], s_m[2];
-    __shared__ double s_prob[2][64];  // p_i(x_i), q_i(x_i)
-    __shared__ int s_acc;
-    const int n = drafts_of(a, b), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kPickThreads / 32;
+    __shared__ double s_part[4][PT / 32], s_sum[4];
+    __shared__ double s_prob[2][33], s_m[2][33];  // p_i(x_i), q_i(x_i) and the rows' maxima
+    const int n = drafts_of(a, b), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = PT / 32;
     const int* tok = a.tokens + (size_t)b * a.drafts;
-    const double inv_t = 1.0 / (double)a.temperature;
+    const double scale = 1.4426950408889634074 / (double)a.temperature;
     const RowPart* tp = parts + (size_t)b * (a.drafts + 1) * slices;
     const RowPart* dp = parts + ((size_t)a.seqs * (a.drafts + 1) + (size_t)b * a.drafts) * slices;
     const float* trow = a.target + (size_t)b * (a.drafts + 1) * a.target_stride;
     const float* drow = a.draft ? a.draft + (size_t)b * a.drafts * a.draft_stride : nullptr;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- the decisions, in groups of 64 drafts (every CTA makes them for itself) ----
-    int n_acc = 0;
-    for (int base = 0; base < n && n_acc == base; base += 64) {
-        const int cnt = min(64, n - base);
-        for (int k = warp; k < 2 * cnt; k += warps) {  // a warp per value
-            const int i = base + (k >> 1), side = k & 1, x = tok[i];
+    // ---- the decisions, in groups of 32 drafts (every CTA makes them for itself) ----
+    int n_acc = 0, base = 0;
+    for (;;) {
+        const int cnt = min(32, n - base);
+        // a warp per value: p and q of each draft, and the maximum of the row behind the group
+        for (int k = warp; k <= 2 * cnt; k += warps) {
+            const int at = k >> 1, i = base + at, side = k & 1, x = at < cnt ? tok[i] : -1;
             double v = side ? 1.0 : 0.0;
-            if (x >= 0 && (size_t)x < a.vocab && (side == 0 || drow)) {
+            if (side == 0 || drow) {
                 const float* p = side ? drow + (size_t)i * a.draft_stride : trow + (size_t)i * a.target_stride;
+                const bool in = x >= 0 && (size_t)x < a.vocab;
+                const float l = in ? __ldg(p + x) : 0.f;
                 if (a.probs) {
-                    v = clean_p(p[x]);
+                    if (in) v = clean_p(l);
                 } else {
-                    const RowPart r = join_row((side ? dp : tp) + (size_t)i * slices, slices, inv_t, false);
-                    v = r.s > 0.0 ? exp(((double)clean(p[x]) - (double)r.m) * inv_t) / r.s : 0.0;
+                    const RowPart r = join_row((side ? dp : tp) + (size_t)i * slices, slices, scale, false);
+                    if (in) v = r.s > 0.0 ? exp2_neg(((double)clean(l) - (double)r.m) * scale) / r.s : 0.0;
+                    if (lane == 0) s_m[side][at] = r.m;
                 }
             }
-            if (lane == 0) s_prob[side][k >> 1] = v;
+            if (lane == 0) s_prob[side][at] = v;
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int i = 0;
-            while (i < cnt && (double)a.u[(size_t)b * a.drafts + base + i] * s_prob[1][i] < s_prob[0][i]) ++i;
-            s_acc = base + i;
-        }
+        const bool yes = lane < cnt && (double)a.u[(size_t)b * a.drafts + base + lane] * s_prob[1][lane] < s_prob[0][lane];
+        const int run = __ffs((int)~__ballot_sync(0xffffffffu, yes)) - 1;  // drafts accepted; -1: all 32
+        const int got = run < 0 ? 32 : run;
+        n_acc = base + got;
+        if (got < cnt || base + cnt == n) break;
+        base += 32;
         __syncthreads();
-        n_acc = s_acc;
     }
 
     // ---- the rows the next token is drawn from ----
     const bool refused = n_acc < n;
     const bool with_q = refused && drow;
     const int skip = refused && !drow ? tok[n_acc] : -1;  // a certain draft takes its own place away
-    Row P{trow + (size_t)n_acc * a.target_stride, 0.0, inv_t, 1.0, a.probs};
-    Row Q{with_q ? drow + (size_t)n_acc * a.draft_stride : nullptr, 0.0, inv_t, 1.0, a.probs};
+    Row P{trow + (size_t)n_acc * a.target_stride, 0.0, scale, 1.0, a.probs};
+    Row Q{with_q ? drow + (size_t)n_acc * a.draft_stride : P.p, 0.0, scale, 1.0, a.probs};
     if (!a.probs) {
-        if (warp == 0) {
-            const RowPart r = join_row(tp + (size_t)n_acc * slices, slices, inv_t, false);
-            if (lane == 0) s_m[0] = r.m;
-        } else if (warp == 1 && with_q) {
-            const RowPart r = join_row(dp + (size_t)n_acc * slices, slices, inv_t, false);
-            if (lane == 0) s_m[1] = r.m;
-        }
-        __syncthreads();
-        P.m = s_m[0];
-        if (with_q) Q.m = s_m[1];
+        P.m = s_m[0][n_acc - base];
+        if (with_q) Q.m = s_m[1][n_acc - base];
     }
-    const size_t j0 = a.vocab * me / ctas, j1 = a.vocab * (me + 1) / ctas;
-    const bool p_empty = !a.probs && P.m == -(double)CUDART_INF_F, q_empty = with_q && !a.probs && Q.m == -(double)CUDART_INF_F;
+    // this CTA's part of the row, whole groups of 4; a thread takes 4 and the next 4 after all others'
+    const size_t quads = (a.vocab + 3) / 4, j0 = 4 * (quads * me / ctas), j1 = min(a.vocab, 4 * (quads * (me + 1) / ctas));
+    if (!a.probs) {  // a row with nothing above -inf weighs nothing
+        if (P.m == -(double)CUDART_INF_F) P.m = 0.0, P.f = 0.0;
+        if (Q.m == -(double)CUDART_INF_F) Q.m = 0.0, Q.f = 0.0;
+    }
+    constexpr size_t kStep = 4 * PT;
 
-    // part sums of this CTA, exchanged: [0] of p, [1] of q, [2] of the weights
-    auto exchange = [&](int k, double v, double* before, double* total) {
-        v = block_sum(v, s_part);
-        if (threadIdx.x == 0) s_sum[k] = v;
-        cl.sync();
-        double bf = 0.0, t = 0.0;
-        for (int c = 0; c < ctas; ++c) {
-            const double o = *cl.map_shared_rank(&s_sum[k], c);
-            if (c < me) bf += o;
-            t += o;
-        }
-        *before = bf;
-        *total = t;
+    // The threads' values summed over the CTA (slot k), and the CTAs' sums exchanged: lane c gets the sum of
+    // the CTAs up to c. One barrier of the CTA and one of the cluster for up to two values; a slot is used once.
+    auto cta_sum = [&](int k, double v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) s_part[k][warp] = v;
     };
-    double before, total;
-    if (with_q && !a.probs) {  // normalise both rows in f64 before they are compared
-        double sp = 0.0, sq = 0.0, t;
-        for (size_t j = j0 + threadIdx.x; j < j1; j += kPickThreads) {
-            if (!p_empty) sp += P.raw(j);
-            if (!q_empty) sq += Q.raw(j);
+    auto cta_join = [&](int k) {
+        double v = lane < warps ? s_part[k][lane] : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (threadIdx.x == 0) s_sum[k] = v;
+    };
+    auto running = [&](int k, double* own) -> double {
+        double v = lane < ctas ? *cl.map_shared_rank(&s_sum[k], lane) : 0.0;
+        *own = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
         }
-        exchange(0, sp, &before, &t);
-        P.inv_s = t > 0.0 ? 1.0 / t : 0.0;
-        exchange(1, sq, &before, &t);
-        Q.inv_s = t > 0.0 ? 1.0 / t : 0.0;
+        return v;
+    };
+    if (with_q && !a.probs) {  // normalise both rows in f64 before they are compared
+        double sp = 0.0, sq = 0.0, own;
+        for (size_t j = j0 + 4 * threadIdx.x; j < j1; j += kStep) {
+            float x[4], y[4];
+            entries4<VEC>(P, j, j1, x), entries4<VEC>(Q, j, j1, y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sp += P.weigh(x[i]), sq += Q.weigh(y[i]);
+        }
+        cta_sum(0, sp), cta_sum(1, sq);
+        __syncthreads();
+        if (warp == 0) cta_join(0), cta_join(1);
+        cl.sync();
+        const double p = __shfl_sync(0xffffffffu, running(0, &own), 31), q = __shfl_sync(0xffffffffu, running(1, &own), 31);
+        P.f = p > 0.0 ? 1.0 / p : 0.0;
+        Q.f = q > 0.0 ? 1.0 / q : 0.0;
     }
-    auto weight = [&](size_t j, bool plain) -> double {
-        if (p_empty) return 0.0;
-        const double p = P.at(j);
-        if (plain) return p;
-        if ((long long)j == skip) return 0.0;
-        if (!with_q || q_empty) return p;
-        const double w = p - Q.at(j);
-        return w > 0.0 ? w : 0.0;
+    // the weights of entries j .. j + 3
+    auto weights4 = [&](size_t j, bool plain, double* w) {
+        float x[4], y[4];
+        entries4<VEC>(P, j, j1, x);
+        if (with_q && !plain) entries4<VEC>(Q, j, j1, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = P.weigh(x[i]);
+            if (with_q && !plain) w[i] = fmax(w[i] - Q.weigh(y[i]), 0.0);
+            if (!plain && (long long)(j + i) == skip) w[i] = 0.0;
+        }
     };
     bool plain = !refused;
-    for (int pass = 0; pass < 2; ++pass) {  // the second pass only where p - q is zero everywhere
-        double w = 0.0;
-        for (size_t j = j0 + threadIdx.x; j < j1; j += kPickThreads) w += weight(j, plain);
-        if (pass) cl.sync();  // everyone has read the first pass's sums
-        exchange(2, w, &before, &total);
-        if (total > 0.0 || plain) break;
-        plain = true;
-    }
-    // ---- the place: this CTA's, if the border lies in its part ----
-    const double border = (double)a.u_sample[b] * total;
-    // The first CTA whose sums pass the border; if rounding leaves none, the last one with any weight.
-    int owner = -1, last = -1;
-    {
-        double run = 0.0;
-        for (int c = 0; c < ctas; ++c) {
-            const double o = *cl.map_shared_rank(&s_sum[2], c);
-            run += o;
-            if (o > 0.0) last = c;
-            if (owner < 0 && o > 0.0 && run > border) owner = c;
+    double before, border;
+    int owner;
+    for (int slot = 2;; ++slot) {  // a second time only where p - q is zero everywhere
+        double w = 0.0, own;
+        for (size_t j = j0 + 4 * threadIdx.x; j < j1; j += kStep) {
+            double v[4];
+            weights4(j, plain, v);
+            w += (v[0] + v[1]) + (v[2] + v[3]);
         }
-        if (owner < 0) owner = last;
+        cta_sum(slot, w);
+        __syncthreads();
+        if (warp == 0) cta_join(slot);
+        cl.sync();
+        const double run = running(slot, &own), total = __shfl_sync(0xffffffffu, run, 31);
+        if (!(total > 0.0) && !plain) {
+            plain = true;
+            continue;
+        }
+        // The first CTA whose sum passes the border, or, if rounding leaves none, the last with any weight.
+        border = (double)a.u_sample[b] * total;
+        const unsigned any = __ballot_sync(0xffffffffu, own > 0.0), over = __ballot_sync(0xffffffffu, own > 0.0 && run > border);
+        owner = over ? __ffs((int)over) - 1 : any ? 31 - __clz((int)any) : -1;
+        const double b4 = __shfl_up_sync(0xffffffffu, run, 1);
+        before = me ? __shfl_sync(0xffffffffu, b4, me) : 0.0;
+        break;
     }
     cl.sync();  // nobody reads another CTA's memory after this
     if (owner < 0) {  // a row without any weight
@@ -348,23 +388,21 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(VerifyArgs a,
         return;
     }
     if (me != owner) return;
-    // tiles of 8 values a thread in order: the tile, the thread, the value
-    constexpr int kPer = 8;
-    __shared__ double s_scan[kPickThreads / 32];
+    // tiles of 4 values a thread in order: the tile, the thread, the value
+    __shared__ double s_scan[PT / 32];
     __shared__ int s_place, s_last;
     if (threadIdx.x == 0) s_place = INT_MAX, s_last = -1;
     __syncthreads();
     double run = before;
-    for (size_t t0 = j0; t0 < j1; t0 += kPickThreads * kPer) {
-        const size_t f = t0 + (size_t)threadIdx.x * kPer;
-        double v[kPer], sum = 0.0;
+    for (size_t t0 = j0; t0 < j1; t0 += kStep) {
+        const size_t f = t0 + 4 * threadIdx.x;
+        double v[4] = {0.0, 0.0, 0.0, 0.0};
+        if (f < j1) weights4(f, plain, v);
         int lastw = -1;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            v[i] = f + i < j1 ? weight(f + i, plain) : 0.0;
+        for (int i = 0; i < 4; ++i)
             if (v[i] > 0.0) lastw = (int)(f + i);
-            sum += v[i];
-        }
+        const double sum = (v[0] + v[1]) + (v[2] + v[3]);
         double inc = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -374,12 +412,12 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(VerifyArgs a,
         if (lane == 31) s_scan[warp] = inc;
         __syncthreads();
         double at = run, all = 0.0;
-        for (int w = 0; w < kPickThreads / 32; ++w) {
+        for (int w = 0; w < PT / 32; ++w) {
             if (w < warp) at += s_scan[w];
             all += s_scan[w];
         }
         at += inc - sum;
-        for (int i = 0; i < kPer; ++i) {
+        for (int i = 0; i < 4; ++i) {
             at += v[i];
             if (v[i] > 0.0 && at > border) {
                 atomicMin(&s_place, (int)(f + i));
@@ -393,6 +431,33 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(VerifyArgs a,
         __syncthreads();
     }
     if (warp == 0) write_out(a, b, n_acc, s_place != INT_MAX ? s_place : max(s_last, 0));
+}
+
+template <int PT, bool VEC>
+cudaError_t launch_pick(const VerifyArgs& a, const RowPart* parts, int slices, cudaStream_t s) {
+    // CTAs a sequence: parts of 4096 entries, up to the portable cluster of 8; 16 (which has to be asked for)
+    // while that fills no more than the SMs
+    auto kernel = verify_pick_kernel<PT, VEC>;
+    int ctas = 1;
+    while (ctas < 8 && a.vocab >= (size_t)ctas * 8192) ctas *= 2;
+    if (ctas == 8 && PT == 1024 && a.vocab >= 65536) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        ctas = 16;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.seqs * ctas));
+    cfg.blockDim = dim3(PT);
+    cfg.stream = s;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)ctas;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // behind the rows' kernel
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = a.probs ? 1 : 2;
+    return cudaLaunchKernelEx(&cfg, kernel, a, parts, slices);
 }
 
 int slices_of(const VerifyArgs& a, int num_sms) {
@@ -436,19 +501,10 @@ cudaError_t launch_verify(const VerifyArgs& a, int num_sms, cudaStream_t s) {
         verify_greedy_kernel<<<a.seqs, 32, 0, s>>>(a, parts, slices);
         return cudaGetLastError();
     }
-    // CTAs a sequence: 8 (the portable cluster) from 16384 entries on
-    const int ctas = a.vocab >= 16384 ? 8 : a.vocab >= 4096 ? 2 : 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(a.seqs * ctas));
-    cfg.blockDim = dim3(kPickThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)ctas;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, verify_pick_kernel, a, (const RowPart*)parts, slices);
+    // few sequences: a CTA's part of a row should be few steps; many: four CTAs an SM share its latencies
+    if (a.seqs * 16 <= num_sms)
+        return vec ? launch_pick<1024, true>(a, parts, slices, s) : launch_pick<1024, false>(a, parts, slices, s);
+    return vec ? launch_pick<256, true>(a, parts, slices, s) : launch_pick<256, false>(a, parts, slices, s);
 }
 
 }  // namespace bebelm
