@@ -198,6 +198,15 @@ __device__ __forceinline__ RowPart join_row(const RowPart* parts, int slices, do
     return r;
 }
 
+// the same by one thread
+__device__ __forceinline__ RowPart join_row_alone(const RowPart* parts, int slices, double scale) {
+    RowPart r{-CUDART_INF_F, 0xffffffffu, 0.0};
+    for (int i = 0; i < slices; ++i) r.m = fmaxf(r.m, parts[i].m);
+    for (int i = 0; i < slices; ++i)
+        if (parts[i].s > 0.0) r.s += parts[i].s * exp2_neg(((double)parts[i].m - (double)r.m) * scale);
+    return r;
+}
+
 // the accepted drafts, the next token and -1 behind it
 __device__ __forceinline__ void write_out(const VerifyArgs& a, int b, int n_acc, int next) {
     int* out = a.out + (size_t)b * (a.drafts + 1);
@@ -243,8 +252,9 @@ template <int PT, bool VEC>
 __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a, const RowPart* parts, int slices) {
     cg::cluster_group cl = cg::this_cluster();
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), b = blockIdx.x / ctas;
-    __shared__ double s_part[4][PT / 32], s_sum[4];
-    __shared__ double s_prob[2][33], s_m[2][33];  // p_i(x_i), q_i(x_i) and the rows' maxima
+    constexpr int kBlocks = 64;  // a part's steps whose sums are kept, so that the border's block is gone through alone
+    __shared__ double s_part[PT / 32][4], s_sum[2][4], s_all[16][4], s_block[kBlocks][PT / 32][2];
+    __shared__ double s_prob[2][33], s_m[2][33], s_s[2][33];  // p_i(x_i), q_i(x_i); the rows' maxima and sums
     const int n = drafts_of(a, b), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = PT / 32;
     const int* tok = a.tokens + (size_t)b * a.drafts;
     const double scale = 1.4426950408889634074 / (double)a.temperature;
@@ -258,8 +268,11 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     int n_acc = 0, base = 0;
     for (;;) {
         const int cnt = min(32, n - base);
-        // a warp per value: p and q of each draft, and the maximum of the row behind the group
-        for (int k = warp; k <= 2 * cnt; k += warps) {
+        // p and q of each draft, and the maximum and sum of the row behind the group: a warp each, or a
+        // thread each where rows were cut into few slices
+        const bool alone = slices <= 4;
+        const int per = alone ? PT : warps;
+        for (int k = alone ? (int)threadIdx.x : warp; k <= 2 * cnt; k += per) {
             const int at = k >> 1, i = base + at, side = k & 1, x = at < cnt ? tok[i] : -1;
             double v = side ? 1.0 : 0.0;
             if (side == 0 || drow) {
@@ -269,12 +282,13 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
                 if (a.probs) {
                     if (in) v = clean_p(l);
                 } else {
-                    const RowPart r = join_row((side ? dp : tp) + (size_t)i * slices, slices, scale, false);
+                    const RowPart* rp = (side ? dp : tp) + (size_t)i * slices;
+                    const RowPart r = alone ? join_row_alone(rp, slices, scale) : join_row(rp, slices, scale, false);
                     if (in) v = r.s > 0.0 ? exp2_neg(((double)clean(l) - (double)r.m) * scale) / r.s : 0.0;
-                    if (lane == 0) s_m[side][at] = r.m;
+                    if (alone || lane == 0) s_m[side][at] = r.m, s_s[side][at] = r.s;
                 }
             }
-            if (lane == 0) s_prob[side][at] = v;
+            if (alone || lane == 0) s_prob[side][at] = v;
         }
         __syncthreads();
         const bool yes = lane < cnt && (double)a.u[(size_t)b * a.drafts + base + lane] * s_prob[1][lane] < s_prob[0][lane];
@@ -293,8 +307,9 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     Row P{trow + (size_t)n_acc * a.target_stride, 0.0, scale, 1.0, a.probs};
     Row Q{with_q ? drow + (size_t)n_acc * a.draft_stride : P.p, 0.0, scale, 1.0, a.probs};
     if (!a.probs) {
-        P.m = s_m[0][n_acc - base];
-        if (with_q) Q.m = s_m[1][n_acc - base];
+        // Weights relative to the rows' maxima, made comparable by the sums of the first pass.
+        P.m = s_m[0][n_acc - base], P.f = s_s[0][n_acc - base] > 0.0 ? 1.0 / s_s[0][n_acc - base] : 0.0;
+        if (with_q) Q.m = s_m[1][n_acc - base], Q.f = s_s[1][n_acc - base] > 0.0 ? 1.0 / s_s[1][n_acc - base] : 0.0;
     }
     // this CTA's part of the row, whole groups of 4; a thread takes 4 and the next 4 after all others'
     const size_t quads = (a.vocab + 3) / 4, j0 = 4 * (quads * me / ctas), j1 = min(a.vocab, 4 * (quads * (me + 1) / ctas));
@@ -304,72 +319,81 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     }
     constexpr size_t kStep = 4 * PT;
 
-    // The threads' values summed over the CTA (slot k), and the CTAs' sums exchanged: lane c gets the sum of
-    // the CTAs up to c. One barrier of the CTA and one of the cluster for up to two values; a slot is used once.
-    auto cta_sum = [&](int k, double v) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) s_part[k][warp] = v;
-    };
-    auto cta_join = [&](int k) {
-        double v = lane < warps ? s_part[k][lane] : 0.0;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (threadIdx.x == 0) s_sum[k] = v;
-    };
-    auto running = [&](int k, double* own) -> double {
-        double v = lane < ctas ? *cl.map_shared_rank(&s_sum[k], lane) : 0.0;
-        *own = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
-        }
-        return v;
-    };
-    if (with_q && !a.probs) {  // normalise both rows in f64 before they are compared
-        double sp = 0.0, sq = 0.0, own;
-        for (size_t j = j0 + 4 * threadIdx.x; j < j1; j += kStep) {
-            float x[4], y[4];
-            entries4<VEC>(P, j, j1, x), entries4<VEC>(Q, j, j1, y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sp += P.weigh(x[i]), sq += Q.weigh(y[i]);
-        }
-        cta_sum(0, sp), cta_sum(1, sq);
-        __syncthreads();
-        if (warp == 0) cta_join(0), cta_join(1);
-        cl.sync();
-        const double p = __shfl_sync(0xffffffffu, running(0, &own), 31), q = __shfl_sync(0xffffffffu, running(1, &own), 31);
-        P.f = p > 0.0 ? 1.0 / p : 0.0;
-        Q.f = q > 0.0 ? 1.0 / q : 0.0;
-    }
-    // the weights of entries j .. j + 3
-    auto weights4 = [&](size_t j, bool plain, double* w) {
+    // The row is gone through once for all sums. With P and Q relative to the first pass's f32-grade sums,
+    // p / Sp > q / Sq is decided as well by P > Q (it differs only where p - q is 1e-7 of p, and weighs as little);
+    // with the sums of P, Q, and of P and Q where P > Q, the weights' total is A / Sp - B / Sq. Probabilities
+    // are differences at once: A.
+    const bool ratio = with_q && !a.probs;
+    auto weights4 = [&](size_t j, bool plain, double fp, double fq, double* sums, double* w) {
         float x[4], y[4];
         entries4<VEC>(P, j, j1, x);
         if (with_q && !plain) entries4<VEC>(Q, j, j1, y);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = P.weigh(x[i]);
-            if (with_q && !plain) w[i] = fmax(w[i] - Q.weigh(y[i]), 0.0);
-            if (!plain && (long long)(j + i) == skip) w[i] = 0.0;
+            const double p = P.weigh(x[i]), q = with_q && !plain ? Q.weigh(y[i]) : 0.0;
+            const bool in = p > q && (plain || (long long)(j + i) != skip);
+            if (sums) {
+                sums[0] += p, sums[1] += q;
+                if (in) sums[2] += ratio ? p : p - q, sums[3] += q;
+            } else {
+                w[i] = in ? fmax(fma(p, fp, -(q * fq)), 0.0) : 0.0;
+            }
         }
     };
+    const int steps = (int)((j1 - j0 + kStep - 1) / kStep);
+    int shift = 0;  // steps of a block
+    while (steps >> shift >= kBlocks) ++shift;
     bool plain = !refused;
-    double before, border;
+    double before = 0.0, border, fp = 1.0, fq = 1.0;
     int owner;
-    for (int slot = 2;; ++slot) {  // a second time only where p - q is zero everywhere
-        double w = 0.0, own;
-        for (size_t j = j0 + 4 * threadIdx.x; j < j1; j += kStep) {
-            double v[4];
-            weights4(j, plain, v);
-            w += (v[0] + v[1]) + (v[2] + v[3]);
+    for (int slot = 0;; ++slot) {  // a second time only where p - q is zero everywhere
+        double sums[4] = {0.0, 0.0, 0.0, 0.0}, seen[2] = {0.0, 0.0};
+        for (int t = 0; t < steps; ++t) {
+            const size_t j = j0 + t * kStep + 4 * threadIdx.x;
+            if (j < j1) weights4(j, plain, 1.0, 1.0, sums, nullptr);
+            if ((t + 1) >> shift != t >> shift || t + 1 == steps) {  // the block's end
+                double u = sums[2] - seen[0], v = sums[3] - seen[1];
+                seen[0] = sums[2], seen[1] = sums[3];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    u += __shfl_xor_sync(0xffffffffu, u, o);
+                    if (ratio) v += __shfl_xor_sync(0xffffffffu, v, o);
+                }
+                if (lane == 0) s_block[t >> shift][warp][0] = u, s_block[t >> shift][warp][1] = v;
+            }
         }
-        cta_sum(slot, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            double v = sums[k];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == 0) s_part[warp][k] = v;
+        }
         __syncthreads();
-        if (warp == 0) cta_join(slot);
+        if (threadIdx.x < 4) {
+            double v = 0.0;
+            for (int w = 0; w < warps; ++w) v += s_part[w][threadIdx.x];
+            s_sum[slot][threadIdx.x] = v;
+        }
         cl.sync();
-        const double run = running(slot, &own), total = __shfl_sync(0xffffffffu, run, 31);
+        // a warp per sum reads the other CTAs' (every warp reading them took 8000 cycles)
+        if (warp < 4 && lane < ctas) s_all[lane][warp] = *cl.map_shared_rank(&s_sum[slot][warp], lane);
+        __syncthreads();
+        if (ratio && !plain) {
+            double sp = 0.0, sq = 0.0;
+            for (int c = 0; c < ctas; ++c) sp += s_all[c][0], sq += s_all[c][1];
+            fp = sp > 0.0 ? 1.0 / sp : 0.0, fq = sq > 0.0 ? 1.0 / sq : 0.0;
+        } else {
+            fp = fq = 1.0;
+        }
+        const double own = lane >= ctas ? 0.0 : ratio && !plain ? fmax(fma(s_all[lane][2], fp, -(s_all[lane][3] * fq)), 0.0) : s_all[lane][2];
+        double run = own;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            const double u = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += u;
+        }
+        const double total = __shfl_sync(0xffffffffu, run, 15);
         if (!(total > 0.0) && !plain) {
             plain = true;
             continue;
@@ -378,8 +402,7 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
         border = (double)a.u_sample[b] * total;
         const unsigned any = __ballot_sync(0xffffffffu, own > 0.0), over = __ballot_sync(0xffffffffu, own > 0.0 && run > border);
         owner = over ? __ffs((int)over) - 1 : any ? 31 - __clz((int)any) : -1;
-        const double b4 = __shfl_up_sync(0xffffffffu, run, 1);
-        before = me ? __shfl_sync(0xffffffffu, b4, me) : 0.0;
+        if (me) before = __shfl_sync(0xffffffffu, run, me - 1);
         break;
     }
     cl.sync();  // nobody reads another CTA's memory after this
@@ -388,16 +411,26 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
         return;
     }
     if (me != owner) return;
-    // tiles of 4 values a thread in order: the tile, the thread, the value
+    // The first block whose running sum passes the border; from it on, steps of 4 values a thread in order: the
+    // step, the thread, the value.
+    const int blocks = (steps + (1 << shift) - 1) >> shift;
+    double run = before;
+    int block = 0;
+    for (; block + 1 < blocks; ++block) {
+        double u = 0.0, v = 0.0;
+        for (int w = 0; w < warps; ++w) u += s_block[block][w][0], v += s_block[block][w][1];
+        const double w = ratio && !plain ? fmax(fma(u, fp, -(v * fq)), 0.0) : u;
+        if (w > 0.0 && run + w > border) break;
+        run += w;
+    }
     __shared__ double s_scan[PT / 32];
     __shared__ int s_place, s_last;
     if (threadIdx.x == 0) s_place = INT_MAX, s_last = -1;
     __syncthreads();
-    double run = before;
-    for (size_t t0 = j0; t0 < j1; t0 += kStep) {
+    for (size_t t0 = j0 + ((size_t)block << shift) * kStep; t0 < j1; t0 += kStep) {
         const size_t f = t0 + 4 * threadIdx.x;
         double v[4] = {0.0, 0.0, 0.0, 0.0};
-        if (f < j1) weights4(f, plain, v);
+        if (f < j1) weights4(f, plain, fp, fq, nullptr, v);
         int lastw = -1;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
