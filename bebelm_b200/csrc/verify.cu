@@ -154,25 +154,26 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(VerifyArgs a, 
     }
 }
 
-// 2^y for y <= 0 to 2e-14: y = k + f with f in [-1/2, 1/2] (k from the rounding of 1.5 * 2^52 + y), 2^f a polynomial of
-// degree 9 through 2^f at the 10 Chebyshev nodes of the interval, 2^k added to the exponent. 0 below 2^-1000.
-// (exp() of the same arguments took the pass over a row half as long again.)
-__device__ __forceinline__ double exp2_neg(double y) {
+// 2^y for -1001 <= y <= 1 to 1.1e-12: y = k + f with f in [-1/2, 1/2] (k from the rounding of 1.5 * 2^52 + y), 2^f a
+// polynomial of degree 8 through 2^f at the 9 Chebyshev nodes of the interval, 2^k added to the exponent. 13 f64
+// operations with the product before it: the pass over a row is bound by the f64 pipe (64 a cycle and SM), and with
+// exp() and its argument formed in two steps it took 2.5 times as long.
+__device__ __forceinline__ double exp2_bounded(double y) {
     const double magic = 6755399441055744.0;  // 1.5 * 2^52
-    const double t = fmax(y, -1001.0) + magic, f = fmax(y, -1001.0) - (t - magic);
-    double p = 1.0205905413765595e-07;
-    p = fma(p, f, 1.325964524488711e-06);
-    p = fma(p, f, 1.5252672924850737e-05);
-    p = fma(p, f, 0.0001540343375125101);
-    p = fma(p, f, 0.0013333558200794592);
-    p = fma(p, f, 0.009618129193934313);
-    p = fma(p, f, 0.05550410866465167);
-    p = fma(p, f, 0.2402265069564034);
-    p = fma(p, f, 0.6931471805599462);
-    p = fma(p, f, 1.0000000000000135);
-    const double r = __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
-    return y < -1000.0 ? 0.0 : r;
+    const double t = y + magic, f = y - (t - magic);
+    double p = 1.3255224878668817e-06;
+    p = fma(p, f, 1.5310079402249296e-05);
+    p = fma(p, f, 0.00015403455852453838);
+    p = fma(p, f, 0.0013333450568000645);
+    p = fma(p, f, 0.009618129159402558);
+    p = fma(p, f, 0.05550410941205933);
+    p = fma(p, f, 0.2402265069581299);
+    p = fma(p, f, 0.6931471805459335);
+    p = fma(p, f, 1.0);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
+// the same for any y <= 1: 0 below 2^-1000
+__device__ __forceinline__ double exp2_neg(double y) { return y < -1000.0 ? 0.0 : exp2_bounded(y); }
 
 // the slices of one row joined by a warp (every lane gets the answer); scale = log2(e) / temperature
 __device__ __forceinline__ RowPart join_row(const RowPart* parts, int slices, double scale, bool greedy) {
@@ -226,13 +227,23 @@ __global__ void __launch_bounds__(32) verify_greedy_kernel(VerifyArgs a, const R
     }
 }
 
-// One row of probabilities, or of logits with a known maximum, as f64 weights: f · 2^((l - m) c) or f · p.
+// One row of probabilities, or of logits whose probabilities are 2^(c l + k), as f64 weights.
 struct Row {
     const float* p;
-    double m, c, f;
+    double c, k;
+    float lim;  // logits at and below it weigh nothing (2^-1000), NaN neither
     int probs;
+    // maximum m and sum s of exp((l - m) / temperature), scale = log2(e) / temperature
+    __device__ __forceinline__ void logits(double m, double s, double scale) {
+        const bool any = s > 0.0;  // else nothing is above -inf
+        c = any ? scale : 0.0;
+        k = any ? -(m * scale) - log2(s) : 0.0;
+        lim = any ? (float)((-1000.0 - k) / scale) : CUDART_INF_F;
+    }
     __device__ __forceinline__ double weigh(float l) const {
-        return probs ? clean_p(l) * f : exp2_neg(((double)clean(l) - m) * c) * f;
+        if (probs) return clean_p(l);
+        const double w = exp2_bounded(fma((double)fminf(l, 3.402823466e38f), c, k));
+        return l > lim ? w : 0.0;
     }
 };
 // 4 entries from j (a multiple of 4); those at and past `end` count as nothing
@@ -304,25 +315,20 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     const bool refused = n_acc < n;
     const bool with_q = refused && drow;
     const int skip = refused && !drow ? tok[n_acc] : -1;  // a certain draft takes its own place away
-    Row P{trow + (size_t)n_acc * a.target_stride, 0.0, scale, 1.0, a.probs};
-    Row Q{with_q ? drow + (size_t)n_acc * a.draft_stride : P.p, 0.0, scale, 1.0, a.probs};
-    if (!a.probs) {
-        // Weights relative to the rows' maxima, made comparable by the sums of the first pass.
-        P.m = s_m[0][n_acc - base], P.f = s_s[0][n_acc - base] > 0.0 ? 1.0 / s_s[0][n_acc - base] : 0.0;
-        if (with_q) Q.m = s_m[1][n_acc - base], Q.f = s_s[1][n_acc - base] > 0.0 ? 1.0 / s_s[1][n_acc - base] : 0.0;
+    Row P{trow + (size_t)n_acc * a.target_stride, 0.0, 0.0, 0.f, a.probs};
+    Row Q{with_q ? drow + (size_t)n_acc * a.draft_stride : P.p, 0.0, 0.0, 0.f, a.probs};
+    if (!a.probs) {  // normalised by the sums of the first pass
+        P.logits(s_m[0][n_acc - base], s_s[0][n_acc - base], scale);
+        if (with_q) Q.logits(s_m[1][n_acc - base], s_s[1][n_acc - base], scale);
     }
     // this CTA's part of the row, whole groups of 4; a thread takes 4 and the next 4 after all others'
     const size_t quads = (a.vocab + 3) / 4, j0 = 4 * (quads * me / ctas), j1 = min(a.vocab, 4 * (quads * (me + 1) / ctas));
-    if (!a.probs) {  // a row with nothing above -inf weighs nothing
-        if (P.m == -(double)CUDART_INF_F) P.m = 0.0, P.f = 0.0;
-        if (Q.m == -(double)CUDART_INF_F) Q.m = 0.0, Q.f = 0.0;
-    }
     constexpr size_t kStep = 4 * PT;
 
-    // The row is gone through once for all sums. With P and Q relative to the first pass's f32-grade sums,
-    // p / Sp > q / Sq is decided as well by P > Q (it differs only where p - q is 1e-7 of p, and weighs as little);
-    // with the sums of P, Q, and of P and Q where P > Q, the weights' total is A / Sp - B / Sq. Probabilities
-    // are differences at once: A.
+    // The row is gone through once for all sums. p and q are normalised by the first pass's f32-grade sums, which
+    // decides p > q as well as exact ones (it differs only where p - q is 1e-7 of p, and weighs as little); with the
+    // sums Sp, Sq of p and q, and A, B of p and q where p > q, the weights' total is A / Sp - B / Sq.
+    // Probabilities in hand are differences at once: A.
     const bool ratio = with_q && !a.probs;
     auto weights4 = [&](size_t j, bool plain, double fp, double fq, double* sums, double* w) {
         float x[4], y[4];
@@ -466,14 +472,18 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     if (warp == 0) write_out(a, b, n_acc, s_place != INT_MAX ? s_place : max(s_last, 0));
 }
 
-template <int PT, bool VEC>
-cudaError_t launch_pick(const VerifyArgs& a, const RowPart* parts, int slices, cudaStream_t s) {
-    // CTAs a sequence: parts of 4096 entries, up to the portable cluster of 8; 16 (which has to be asked for)
-    // while that fills no more than the SMs
-    auto kernel = verify_pick_kernel<PT, VEC>;
+// CTAs a sequence: parts of 4096 entries at least, up to the portable cluster of 8
+int pick_ctas(const VerifyArgs& a) {
     int ctas = 1;
     while (ctas < 8 && a.vocab >= (size_t)ctas * 8192) ctas *= 2;
-    if (ctas == 8 && PT == 1024 && a.vocab >= 65536) {
+    return ctas;
+}
+
+template <int PT, bool VEC>
+cudaError_t launch_pick(const VerifyArgs& a, const RowPart* parts, int slices, int num_sms, cudaStream_t s) {
+    auto kernel = verify_pick_kernel<PT, VEC>;
+    int ctas = pick_ctas(a);
+    if (PT == 1024 && a.vocab >= 65536 && a.seqs * 16 <= num_sms) {  // 16 have to be asked for
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         ctas = 16;
@@ -535,9 +545,9 @@ cudaError_t launch_verify(const VerifyArgs& a, int num_sms, cudaStream_t s) {
         return cudaGetLastError();
     }
     // few sequences: a CTA's part of a row should be few steps; many: four CTAs an SM share its latencies
-    if (a.seqs * 16 <= num_sms)
-        return vec ? launch_pick<1024, true>(a, parts, slices, s) : launch_pick<1024, false>(a, parts, slices, s);
-    return vec ? launch_pick<256, true>(a, parts, slices, s) : launch_pick<256, false>(a, parts, slices, s);
+    if (a.seqs * 16 <= num_sms || a.seqs * pick_ctas(a) <= num_sms)
+        return vec ? launch_pick<1024, true>(a, parts, slices, num_sms, s) : launch_pick<1024, false>(a, parts, slices, num_sms, s);
+    return vec ? launch_pick<256, true>(a, parts, slices, num_sms, s) : launch_pick<256, false>(a, parts, slices, num_sms, s);
 }
 
 }  // namespace bebelm
