@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "internal.h"
 
@@ -228,11 +229,11 @@ __global__ void __launch_bounds__(32) verify_greedy_kernel(VerifyArgs a, const R
 }
 
 // One row of probabilities, or of logits whose probabilities are 2^(c l + k), as f64 weights.
+template <bool PROBS>
 struct Row {
     const float* p;
     double c, k;
     float lim;  // logits at and below it weigh nothing (2^-1000), NaN neither
-    int probs;
     // maximum m and sum s of exp((l - m) / temperature), scale = log2(e) / temperature
     __device__ __forceinline__ void logits(double m, double s, double scale) {
         const bool any = s > 0.0;  // else nothing is above -inf
@@ -241,14 +242,14 @@ struct Row {
         lim = any ? (float)((-1000.0 - k) / scale) : CUDART_INF_F;
     }
     __device__ __forceinline__ double weigh(float l) const {
-        if (probs) return clean_p(l);
+        if constexpr (PROBS) return clean_p(l);
         const double w = exp2_bounded(fma((double)fminf(l, 3.402823466e38f), c, k));
         return l > lim ? w : 0.0;
     }
 };
 // 4 entries from j (a multiple of 4); those at and past `end` count as nothing
-template <bool VEC>
-__device__ __forceinline__ void entries4(const Row& r, size_t j, size_t end, float* v) {
+template <bool VEC, bool PROBS>
+__device__ __forceinline__ void entries4(const Row<PROBS>& r, size_t j, size_t end, float* v) {
     if (VEC && j + 4 <= end) {
         const float4 t = __ldg(reinterpret_cast<const float4*>(r.p + j));
         v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
@@ -259,7 +260,7 @@ __device__ __forceinline__ void entries4(const Row& r, size_t j, size_t end, flo
 }
 
 // PT threads; 64 registers each, so that an SM holds 1024 of them however they are split
-template <int PT, bool VEC>
+template <int PT, bool VEC, bool PROBS>
 __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a, const RowPart* parts, int slices) {
     cg::cluster_group cl = cg::this_cluster();
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), b = blockIdx.x / ctas;
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
                 const float* p = side ? drow + (size_t)i * a.draft_stride : trow + (size_t)i * a.target_stride;
                 const bool in = x >= 0 && (size_t)x < a.vocab;
                 const float l = in ? __ldg(p + x) : 0.f;
-                if (a.probs) {
+                if constexpr (PROBS) {
                     if (in) v = clean_p(l);
                 } else {
                     const RowPart* rp = (side ? dp : tp) + (size_t)i * slices;
@@ -315,9 +316,9 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     const bool refused = n_acc < n;
     const bool with_q = refused && drow;
     const int skip = refused && !drow ? tok[n_acc] : -1;  // a certain draft takes its own place away
-    Row P{trow + (size_t)n_acc * a.target_stride, 0.0, 0.0, 0.f, a.probs};
-    Row Q{with_q ? drow + (size_t)n_acc * a.draft_stride : P.p, 0.0, 0.0, 0.f, a.probs};
-    if (!a.probs) {  // normalised by the sums of the first pass
+    Row<PROBS> P{trow + (size_t)n_acc * a.target_stride, 0.0, 0.0, 0.f};
+    Row<PROBS> Q{with_q ? drow + (size_t)n_acc * a.draft_stride : P.p, 0.0, 0.0, 0.f};
+    if constexpr (!PROBS) {  // normalised by the sums of the first pass
         P.logits(s_m[0][n_acc - base], s_s[0][n_acc - base], scale);
         if (with_q) Q.logits(s_m[1][n_acc - base], s_s[1][n_acc - base], scale);
     }
@@ -329,21 +330,45 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     // decides p > q as well as exact ones (it differs only where p - q is 1e-7 of p, and weighs as little); with the
     // sums Sp, Sq of p and q, and A, B of p and q where p > q, the weights' total is A / Sp - B / Sq.
     // Probabilities in hand are differences at once: A.
-    const bool ratio = with_q && !a.probs;
-    auto weights4 = [&](size_t j, bool plain, double fp, double fq, double* sums, double* w) {
+    const bool ratio = with_q && !PROBS;
+    // of the entries j .. j + 3: their shares of Sp, Sq, A, B
+    auto add4 = [&](auto use_q, size_t j, bool plain, double* sums) {
+        constexpr bool kQ = decltype(use_q)::value;
         float x[4], y[4];
         entries4<VEC>(P, j, j1, x);
-        if (with_q && !plain) entries4<VEC>(Q, j, j1, y);
+        if constexpr (kQ) entries4<VEC>(Q, j, j1, y);
+        const int sk = !plain && skip >= 0 && (size_t)skip - j < 4 ? skip - (int)j : -1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const double p = P.weigh(x[i]), q = with_q && !plain ? Q.weigh(y[i]) : 0.0;
-            const bool in = p > q && (plain || (long long)(j + i) != skip);
-            if (sums) {
-                sums[0] += p, sums[1] += q;
-                if (in) sums[2] += ratio ? p : p - q, sums[3] += q;
+            const double p = P.weigh(x[i]);
+            if constexpr (kQ) {
+                const double q = Q.weigh(y[i]);
+                if constexpr (PROBS) {
+                    sums[2] += fmax(p - q, 0.0);
+                } else {
+                    sums[0] += p, sums[1] += q;
+                    if (p > q) sums[2] += p, sums[3] += q;
+                }
             } else {
-                w[i] = in ? fmax(fma(p, fp, -(q * fq)), 0.0) : 0.0;
+                if (i != sk) sums[2] += p;
             }
+        }
+    };
+    // their weights, normalised by fp = 1 / Sp and fq = 1 / Sq
+    auto weights4 = [&](size_t j, bool plain, double fp, double fq, double* w) {
+        float x[4], y[4];
+        const bool q = with_q && !plain;
+        entries4<VEC>(P, j, j1, x);
+        if (q) entries4<VEC>(Q, j, j1, y);
+        const int sk = !plain && skip >= 0 && (size_t)skip - j < 4 ? skip - (int)j : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = P.weigh(x[i]);
+            if (q) {
+                const double v = Q.weigh(y[i]);
+                w[i] = w[i] > v ? fmax(fma(w[i], fp, -(v * fq)), 0.0) : 0.0;
+            }
+            if (i == sk) w[i] = 0.0;
         }
     };
     const int steps = (int)((j1 - j0 + kStep - 1) / kStep);
@@ -354,20 +379,25 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     int owner;
     for (int slot = 0;; ++slot) {  // a second time only where p - q is zero everywhere
         double sums[4] = {0.0, 0.0, 0.0, 0.0}, seen[2] = {0.0, 0.0};
-        for (int t = 0; t < steps; ++t) {
-            const size_t j = j0 + t * kStep + 4 * threadIdx.x;
-            if (j < j1) weights4(j, plain, 1.0, 1.0, sums, nullptr);
-            if ((t + 1) >> shift != t >> shift || t + 1 == steps) {  // the block's end
-                double u = sums[2] - seen[0], v = sums[3] - seen[1];
+        auto go = [&](auto use_q) {
+            for (int t = 0; t < steps; ++t) {
+                const size_t j = j0 + t * kStep + 4 * threadIdx.x;
+                if (j < j1) add4(use_q, j, plain, sums);
+                if ((t + 1) >> shift == t >> shift && t + 1 < steps) continue;
+                double u = sums[2] - seen[0], v = sums[3] - seen[1];  // the block's end
                 seen[0] = sums[2], seen[1] = sums[3];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) {
                     u += __shfl_xor_sync(0xffffffffu, u, o);
-                    if (ratio) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    if (use_q.value && !PROBS) v += __shfl_xor_sync(0xffffffffu, v, o);
                 }
                 if (lane == 0) s_block[t >> shift][warp][0] = u, s_block[t >> shift][warp][1] = v;
             }
-        }
+        };
+        if (with_q && !plain)
+            go(std::true_type{});
+        else
+            go(std::false_type{});
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             double v = sums[k];
@@ -436,7 +466,7 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     for (size_t t0 = j0 + ((size_t)block << shift) * kStep; t0 < j1; t0 += kStep) {
         const size_t f = t0 + 4 * threadIdx.x;
         double v[4] = {0.0, 0.0, 0.0, 0.0};
-        if (f < j1) weights4(f, plain, fp, fq, nullptr, v);
+        if (f < j1) weights4(f, plain, fp, fq, v);
         int lastw = -1;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -479,9 +509,9 @@ int pick_ctas(const VerifyArgs& a) {
     return ctas;
 }
 
-template <int PT, bool VEC>
+template <int PT, bool VEC, bool PROBS>
 cudaError_t launch_pick(const VerifyArgs& a, const RowPart* parts, int slices, int num_sms, cudaStream_t s) {
-    auto kernel = verify_pick_kernel<PT, VEC>;
+    auto kernel = verify_pick_kernel<PT, VEC, PROBS>;
     int ctas = pick_ctas(a);
     if (PT == 1024 && a.vocab >= 65536 && a.seqs * 16 <= num_sms) {  // 16 have to be asked for
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -499,8 +529,18 @@ cudaError_t launch_pick(const VerifyArgs& a, const RowPart* parts, int slices, i
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // behind the rows' kernel
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = a.probs ? 1 : 2;
+    cfg.numAttrs = PROBS ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, kernel, a, parts, slices);
+}
+
+template <bool PROBS>
+cudaError_t pick_probs(const VerifyArgs& a, const RowPart* parts, int slices, bool vec, int num_sms, cudaStream_t s) {
+    // few sequences: a CTA's part of a row should be few steps; many: four CTAs an SM share its latencies
+    if (a.seqs * pick_ctas(a) <= num_sms)
+        return vec ? launch_pick<1024, true, PROBS>(a, parts, slices, num_sms, s)
+                   : launch_pick<1024, false, PROBS>(a, parts, slices, num_sms, s);
+    return vec ? launch_pick<256, true, PROBS>(a, parts, slices, num_sms, s)
+               : launch_pick<256, false, PROBS>(a, parts, slices, num_sms, s);
 }
 
 int slices_of(const VerifyArgs& a, int num_sms) {
@@ -544,10 +584,7 @@ cudaError_t launch_verify(const VerifyArgs& a, int num_sms, cudaStream_t s) {
         verify_greedy_kernel<<<a.seqs, 32, 0, s>>>(a, parts, slices);
         return cudaGetLastError();
     }
-    // few sequences: a CTA's part of a row should be few steps; many: four CTAs an SM share its latencies
-    if (a.seqs * 16 <= num_sms || a.seqs * pick_ctas(a) <= num_sms)
-        return vec ? launch_pick<1024, true>(a, parts, slices, num_sms, s) : launch_pick<1024, false>(a, parts, slices, num_sms, s);
-    return vec ? launch_pick<256, true>(a, parts, slices, num_sms, s) : launch_pick<256, false>(a, parts, slices, num_sms, s);
+    return a.probs ? pick_probs<true>(a, parts, slices, vec, num_sms, s) : pick_probs<false>(a, parts, slices, vec, num_sms, s);
 }
 
 }  // namespace bebelm
