@@ -760,93 +760,91 @@ def attn_decode_batched(caches, layer: int, q, k, v, q_gain, k_gain, pos, theta:
 
 
 # ------------------------------------------- operators around the attention --
+# These are called once per layer and token, on small tensors: a call's checks are kept to what an
+# attribute read costs, since the kernels behind them take a few microseconds.
+_TORCH_DTYPES = None  # torch dtype -> F32 / BF16 / INT8 / F16
+
+
 def _cuda_torch():
-    global _torch
-    if not _torch:
+    global _torch, _TORCH_DTYPES
+    if _TORCH_DTYPES is None:
         import torch
         _torch = torch
+        _TORCH_DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: INT8, torch.float16: F16}
     return _torch
 
 
 def _dtype_of(t, what: str) -> int:
     """F32 / BF16 / INT8 / F16 of a tensor or array."""
-    name = str(t.dtype).replace("torch.", "")
-    try:
-        return {"float32": F32, "bfloat16": BF16, "int8": INT8, "float16": F16}[name]
-    except KeyError:
-        raise ValueError(f"{what}: dtype {t.dtype} is not supported") from None
+    if _is_torch(t):
+        _cuda_torch()
+        dt = _TORCH_DTYPES.get(t.dtype)
+    else:
+        dt = {"float32": F32, "int8": INT8, "float16": F16}.get(str(t.dtype))
+    if dt is None:
+        raise ValueError(f"{what}: dtype {t.dtype} is not supported")
+    return dt
 
 
 def _rows_of(t, what: str):
     """(rows, n, row stride) of a tensor whose last dimension is contiguous and whose rows are
     evenly spaced."""
-    n = t.shape[-1]
-    if t.dim() <= 2 or t.is_contiguous():
-        if t.dim() > 1 and n > 1 and t.stride(-1) != 1 or t.dim() == 1 and n > 1 and t.stride(0) != 1:
+    if t.dim() == 2:
+        rows, n = t.shape
+        step, inner = t.stride()
+        if n > 1 and inner != 1:
             raise ValueError(f"{what}: the last dimension must be contiguous")
-        if t.dim() == 1:
-            return 1, n, n
-        if t.dim() == 2:
-            return t.shape[0], n, max(t.stride(0), n) if t.shape[0] <= 1 else t.stride(0)
-        return (t.numel() // n if n else 0), n, n
-    raise ValueError(f"{what}: more than two dimensions must be contiguous")
+        if rows > 1 and step < n:
+            raise ValueError(f"{what}: rows must not overlap")
+        return rows, n, step if rows > 1 else n
+    if not t.is_contiguous() or t.dim() == 0:
+        raise ValueError(f"{what}: one, three and more dimensions must be contiguous")
+    n = t.shape[-1]
+    return t.numel() // n if n else 0, n, n
 
 
-def _out_tensor(out, shape, dtype, device, what: str):
-    """`out`, checked, or a new tensor."""
-    torch = _cuda_torch()
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if out.dtype != dtype or out.device != device or not out.is_contiguous() or out.numel() != _numel(shape):
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {tuple(shape)} on {device}")
-    return out
+def _check_out(t, numel: int, dtype, dev: int, what: str):
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() != numel:
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {numel} elements on cuda:{dev}")
 
 
-def _numel(shape) -> int:
-    n = 1
-    for d in shape:
-        n *= d
-    return n
+def _check_in(t, shape, dtype, dev: int, what: str):
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.shape != shape:
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {tuple(shape)} on cuda:{dev}")
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (not _is_torch(t) or t.device != device):
-            raise ValueError(f"{name} must be a tensor on {device}")
-
-
-def _stream_on(stream, device) -> int:
+def _stream_on(stream, dev: int) -> int:
     """The cudaStream_t of a device-memory call: the given stream, or torch's current one there."""
     if stream is None:
-        return _cuda_torch().cuda.current_stream(device).cuda_stream
+        return _torch._C._cuda_getCurrentRawStream(dev)
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _workspace(workspace, need: int, device, stream):
+def _workspace(workspace, need: int, dev: int, stream):
     """(tensor, pointer, bytes): the caller's scratch, or one from torch's allocator, which keeps
     it from reuse on other streams until the work of ``stream`` that uses it is done."""
     if not need:
         return None, None, 0
-    torch = _cuda_torch()
+    torch = _torch
     if workspace is None:
         if stream is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
-            ext = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=device)
+            ext = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=dev)
             with torch.cuda.stream(ext):
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.device != device or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _on_device(device, call):
-    """Runs ``call`` with ``device`` current (the calls without a handle go to the current device)."""
-    cuda = _cuda_torch().cuda
-    if cuda.current_device() == device.index:
-        return call()
-    with cuda.device(device):
-        return call()
+def _on_device(dev: int, fn, *args):
+    """fn(*args) with device ``dev`` current (calls without a handle go to the current device)."""
+    if _torch._C._cuda_getDevice() == dev:
+        _check(fn(*args))
+    else:
+        with _torch.cuda.device(dev):
+            _check(fn(*args))
 
 
 def add_rmsnorm(x, gain, residual=None, eps: float = RMS_EPS, out_dtype: int | None = None, group: int = 0, sum_out=None,
@@ -880,43 +878,48 @@ def add_rmsnorm(x, gain, residual=None, eps: float = RMS_EPS, out_dtype: int | N
                                     None if sc is None else sc.ctypes.data, group, MEM_HOST, None))
         return (y, h) if sc is None else (y, sc, h)
     torch = _cuda_torch()
-    dev = x.device
-    _same_device(dev, gain=gain, residual=residual, sum_out=sum_out, out=out, scales=scales)
+    dev = x.get_device()
     dt = _dtype_of(x, "x")
+    if dt > BF16:
+        raise ValueError("x must be float32 or bfloat16")
     rows, n, xs = _rows_of(x, "x")
-    if gain.dtype != torch.float32 or gain.numel() != n or not gain.is_contiguous():
-        raise ValueError("gain must be a contiguous float32 tensor of n elements")
-    rs = n
-    if residual is not None:
-        if residual.dtype != x.dtype or residual.shape != x.shape:
-            raise ValueError("residual must have the type and shape of x")
-        rs = _rows_of(residual, "residual")[2]
+    _check_out(gain, n, torch.float32, dev, "gain")
     od = dt if out_dtype is None else out_dtype
-    if od == F32:
-        y = _out_tensor(out, x.shape, torch.float32, dev, "out")
-    elif od == BF16:
-        y = _out_tensor(out, x.shape, torch.bfloat16, dev, "out")
-    elif od == INT8:
-        y = _out_tensor(out, x.shape, torch.int8, dev, "out")
-        scales = _out_tensor(scales, (rows, n // (group or n or 1)), torch.float32, dev, "scales")
-    else:
+    od_torch = torch.float32 if od == F32 else torch.bfloat16 if od == BF16 else torch.int8 if od == INT8 else None
+    if od_torch is None:
         raise ValueError("out_dtype must be F32, BF16 or INT8")
-    hs = n
+    if out is None:
+        out = torch.empty(x.shape, dtype=od_torch, device=dev)
+    else:
+        _check_out(out, rows * n, od_torch, dev, "out")
+    sp = None
+    if od == INT8:
+        ng = n // (group or n or 1)
+        if scales is None:
+            scales = torch.empty((rows, ng), dtype=torch.float32, device=dev)
+        else:
+            _check_out(scales, rows * ng, torch.float32, dev, "scales")
+        sp = scales.data_ptr()
+    rp = hp = None
+    rs = hs = n
     if residual is None:
         if sum_out is not None:
             raise ValueError("sum_out needs a residual")
         h = x
-    elif sum_out is None:
-        sum_out = h = torch.empty(x.shape, dtype=x.dtype, device=dev)
     else:
-        if sum_out.dtype != x.dtype or sum_out.shape != x.shape:
-            raise ValueError("sum_out must have the type and shape of x")
-        h, hs = sum_out, _rows_of(sum_out, "sum_out")[2]
-    args = (x.data_ptr(), xs, None if residual is None else residual.data_ptr(), rs, dt, rows, n, gain.data_ptr(), eps,
-            None if sum_out is None else sum_out.data_ptr(), hs, y.data_ptr(), od,
-            scales.data_ptr() if od == INT8 else None, group, MEM_DEVICE, _stream_on(stream, dev))
-    _check(_on_device(dev, lambda: L.bebelm_add_rmsnorm(*args)))
-    return (y, scales, h) if od == INT8 else (y, h)
+        if residual.dtype is not x.dtype or residual.shape != x.shape or residual.get_device() != dev:
+            raise ValueError("residual must have the type, shape and device of x")
+        rs, rp = _rows_of(residual, "residual")[2], residual.data_ptr()
+        if sum_out is None:
+            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        else:
+            if sum_out.dtype is not x.dtype or sum_out.shape != x.shape or sum_out.get_device() != dev:
+                raise ValueError("sum_out must have the type, shape and device of x")
+            h, hs = sum_out, _rows_of(sum_out, "sum_out")[2]
+        hp = h.data_ptr()
+    _on_device(dev, L.bebelm_add_rmsnorm, x.data_ptr(), xs, rp, rs, dt, rows, n, gain.data_ptr(), eps, hp, hs, out.data_ptr(), od,
+               sp, group, MEM_DEVICE, _stream_on(stream, dev))
+    return (out, scales, h) if od == INT8 else (out, h)
 
 
 class W4Weights:
@@ -924,8 +927,8 @@ class W4Weights:
 
     codes uint8 [n_out, n_in / 2] (the input with the lower index in the low four bits), scales float16
     or bfloat16 [n_out, n_in / group], zeros uint8 [n_out, n_in / group] (0..127) or None (8 everywhere):
-    w = (code - zero) * scale. numpy arrays, CPU tensors or CUDA tensors. The weights are laid out once; products of
-    one object may run on several streams."""
+    w = (code - zero) * scale. numpy arrays (float16 scales), CPU tensors or CUDA tensors. The weights are laid
+    out once; products of one object may run on several streams."""
 
     def __init__(self, codes, scales, zeros=None, group: int = 128, device: int | None = None):
         dev_in = _is_torch(codes) and codes.is_cuda
@@ -939,16 +942,9 @@ class W4Weights:
             raise ValueError(f"codes and zeros are uint8, scales float16 or bfloat16, scales and zeros {want}")
         keep = []
         for t in (codes, scales, zeros):
-            if t is None:
-                keep.append(None)
-            elif _is_torch(t):
-                if t.is_cuda != dev_in or (dev_in and t.device != codes.device):
-                    raise ValueError("codes, scales and zeros must be in one place")
-                keep.append(t.contiguous())
-            elif dev_in:
+            if t is not None and (_is_torch(t) and t.is_cuda) != dev_in or dev_in and t is not None and t.device != codes.device:
                 raise ValueError("codes, scales and zeros must be in one place")
-            else:
-                keep.append(np.ascontiguousarray(t))
+            keep.append(None if t is None else t.contiguous() if _is_torch(t) else np.ascontiguousarray(t))
         if device is None:
             device = codes.device.index if dev_in else 0
         elif dev_in and codes.device.index != device:
@@ -985,40 +981,42 @@ class W4Weights:
                                       None))
             return y.reshape(*x.shape[:-1], self.n_out)
         torch = _cuda_torch()
-        dev = x.device
-        if dev.index != self.device:
-            raise ValueError(f"x is on {dev}, the weights on cuda:{self.device}")
+        dev = x.get_device()
+        if dev != self.device:
+            raise ValueError(f"x is on cuda:{dev}, the weights on cuda:{self.device}")
         dt = _dtype_of(x, "x")
         t, n, xs = _rows_of(x, "x")
         if n != self.n_in:
             raise ValueError(f"x has {n} columns, the weights {self.n_in}")
         sp, xg = None, 0
         if dt == INT8:
-            _same_device(dev, x_scales=x_scales)
-            if x_scales is None or x_scales.dtype != torch.float32 or not x_scales.is_contiguous() or (
-                    t and x_scales.numel() % t):
+            ns = x_scales.numel() if x_scales is not None else -1
+            if ns < t or x_scales.dtype is not torch.float32 or not x_scales.is_contiguous() or x_scales.get_device() != dev or (
+                    t and ns % t):
                 raise ValueError("int8 activations need contiguous float32 x_scales [n_tokens, n_in / x_group]")
-            xg = self._x_group(x_scales.numel() // t if t else 1)
+            xg = self._x_group(ns // t if t else 1)
             sp = x_scales.data_ptr()
         elif x_scales is not None:
             raise ValueError("x_scales are for int8 activations")
-        od = (BF16 if dt == BF16 else F32) if out_dtype is None else out_dtype
-        if out is not None and out_dtype is None:
-            od = _dtype_of(out, "out")
+        od = out_dtype
+        if od is None:
+            od = _dtype_of(out, "out") if out is not None else BF16 if dt == BF16 else F32
         if od not in (F32, BF16):
             raise ValueError("products are F32 or BF16")
-        shape = (*x.shape[:-1], self.n_out)
-        y = _out_tensor(out, shape, torch.float32 if od == F32 else torch.bfloat16, dev, "out")
+        od_torch = torch.float32 if od == F32 else torch.bfloat16
+        if out is None:
+            out = torch.empty((*x.shape[:-1], self.n_out), dtype=od_torch, device=dev)
+        else:
+            _check_out(out, t * self.n_out, od_torch, dev, "out")
         xp = x.data_ptr()
         need = C.c_size_t()
         _check(L.bebelm_w4_workspace(self._h, xp, dt, xs, xg, t, C.byref(need)))
         ws, wp, wb = _workspace(workspace, need.value, dev, stream)
-        _check(L.bebelm_w4_matmul(self._h, xp, dt, xs, sp, xg, t, y.data_ptr(), od, wp, wb, MEM_DEVICE,
-                                  _stream_on(stream, dev)))
-        return y
+        _check(L.bebelm_w4_matmul(self._h, xp, dt, xs, sp, xg, t, out.data_ptr(), od, wp, wb, MEM_DEVICE, _stream_on(stream, dev)))
+        return out
 
     def _x_group(self, n_groups: int) -> int:
-        if n_groups == 1 or n_groups == 0:
+        if n_groups <= 1:
             return 0
         if self.n_in % n_groups:
             raise ValueError(f"{n_groups} scales a token do not divide {self.n_in} inputs")
@@ -1034,6 +1032,19 @@ class W4Weights:
             self.close()
         except Exception:
             pass
+
+
+def _spaced_rows(t, rows: int, v: int, dev: int, what: str) -> int:
+    """The stride of [n_seqs, rows, v] rows that are evenly spaced, each contiguous."""
+    if t.dtype is not _torch.float32 or t.get_device() != dev:
+        raise ValueError(f"{what} must be float32 on cuda:{dev}")
+    s0, s1, s2 = t.stride()
+    if v > 1 and s2 != 1:
+        raise ValueError(f"{what} must have contiguous rows")
+    st = s1 if rows > 1 else s0 if t.shape[0] > 1 else v
+    if t.shape[0] > 1 and rows > 1 and s0 != rows * st or st < v:
+        raise ValueError(f"{what}: its rows must be evenly spaced")
+    return st
 
 
 def verify_drafts(target, tokens, u, u_sample, draft=None, n_drafts=None, temperature: float = 1.0, probs: bool = False,
@@ -1063,46 +1074,43 @@ def verify_drafts(target, tokens, u, u_sample, draft=None, n_drafts=None, temper
                                       o.ctypes.data, acc.ctypes.data, None, 0, MEM_HOST, None))
         return o, acc
     torch = _cuda_torch()
-    dev = target.device
-    _same_device(dev, tokens=tokens, u=u, u_sample=u_sample, draft=draft, n_drafts=n_drafts, out=out, accepted=accepted)
-
-    def stride_of(t, rows, what):
-        if t.dtype != torch.float32 or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-            raise ValueError(f"{what} must be float32 [n_seqs, rows, vocab] with contiguous rows")
-        st = t.stride(1) if rows > 1 else t.stride(0) if t.shape[0] > 1 else t.shape[2]
-        if t.shape[0] > 1 and rows > 1 and t.stride(0) != rows * st:
-            raise ValueError(f"{what}: its rows must be evenly spaced")
-        return st
-
+    dev = target.get_device()
+    if target.dim() != 3 or target.shape[1] < 1:
+        raise ValueError("target must be [n_seqs, d + 1, vocab]")
     b, d1, v = target.shape
     d = d1 - 1
-    if d < 0:
-        raise ValueError("target needs a row behind the drafts")
-    ts, ds = stride_of(target, d1, "target"), v
-    if draft is not None:
-        if tuple(draft.shape) != (b, d, v):
+    ts = _spaced_rows(target, d1, v, dev, "target")
+    i32, f32 = torch.int32, torch.float32
+    _check_in(tokens, (b, d), i32, dev, "tokens")
+    dp, ds = None, v
+    if draft is not None and temperature != 0.0 and b and d:
+        if draft.shape != (b, d, v):
             raise ValueError(f"draft must be {(b, d, v)}")
-        if draft.numel():
-            ds = stride_of(draft, d, "draft")
-    for name, t, shape, dt in (("tokens", tokens, (b, d), torch.int32), ("u", u, (b, d), torch.float32),
-                               ("n_drafts", n_drafts, (b,), torch.int32), ("u_sample", u_sample, (b,), torch.float32)):
-        if t is not None and (t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous {dt} tensor of {shape}")
-    o = _out_tensor(out, (b, d1), torch.int32, dev, "out")
-    acc = _out_tensor(accepted, (b,), torch.int32, dev, "accepted")
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-
-    def call():
-        need = C.c_size_t()
-        _check(L.bebelm_verify_workspace(b, d, v, int(draft is not None and d > 0 and temperature != 0.0), int(probs), temperature,
-                                         C.byref(need)))
-        ws, wp, wb = _workspace(workspace, need.value, dev, stream)
-        return L.bebelm_verify_drafts(target.data_ptr(), ts, ptr(draft), ds, b, d, v, int(probs), temperature, ptr(tokens),
-                                      ptr(n_drafts), ptr(u), ptr(u_sample), o.data_ptr(), acc.data_ptr(), wp, wb, MEM_DEVICE,
-                                      _stream_on(stream, dev))
-
-    _check(_on_device(dev, call))
-    return o, acc
+        dp, ds = draft.data_ptr(), _spaced_rows(draft, d, v, dev, "draft")
+    np_ = up = sp = None
+    if n_drafts is not None:
+        _check_in(n_drafts, (b,), i32, dev, "n_drafts")
+        np_ = n_drafts.data_ptr()
+    if u is not None:
+        _check_in(u, (b, d), f32, dev, "u")
+        up = u.data_ptr()
+    if u_sample is not None:
+        _check_in(u_sample, (b,), f32, dev, "u_sample")
+        sp = u_sample.data_ptr()
+    if out is None:
+        out = torch.empty((b, d1), dtype=i32, device=dev)
+    else:
+        _check_out(out, b * d1, i32, dev, "out")
+    if accepted is None:
+        accepted = torch.empty((b,), dtype=i32, device=dev)
+    else:
+        _check_out(accepted, b, i32, dev, "accepted")
+    need = C.c_size_t()
+    _on_device(dev, L.bebelm_verify_workspace, b, d, v, dp is not None, probs, temperature, C.byref(need))
+    ws, wp, wb = _workspace(workspace, need.value, dev, stream)
+    _on_device(dev, L.bebelm_verify_drafts, target.data_ptr(), ts, dp, ds, b, d, v, probs, temperature, tokens.data_ptr(), np_, up,
+               sp, out.data_ptr(), accepted.data_ptr(), wp, wb, MEM_DEVICE, _stream_on(stream, dev))
+    return out, accepted
 
 
 # ------------------------------------------------------------------ GGUF --

@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 #include <stddef.h>
 #include <stdint.h>
+#include <atomic>
 
 namespace bebelm {
 
@@ -337,6 +338,21 @@ struct AddNormArgs {
     int bf16, out;
 };
 cudaError_t launch_add_rmsnorm(const AddNormArgs& a, cudaStream_t s);
+
+// A kernel's dynamic shared memory limit, set once per device (the call costs about a microsecond). Two
+// threads may both set it, to the same value.
+struct SmemOnce {
+    std::atomic<bool> done[64] = {};
+    cudaError_t set(const void* kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+        return e;
+    }
+};
 
 // ---- products with 4-bit weights and group scales (w4.cu, w4_tc.cu) ----
 constexpr int kW4XF32 = 0, kW4XBf16 = 1, kW4XInt8 = 2;

@@ -444,7 +444,8 @@ cudaError_t run_stream(StreamArgs& a, const StreamPlan& pl, cudaStream_t s) {
     a.tiles = (int)((rows + kWarps / ks - 1) / (kWarps / ks));
     a.sums_at = (int)((ring + pl.plane_bytes) / sizeof(float));
     const size_t smem = ring + pl.plane_bytes + (ks > 1 ? sums : 0);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemOnce once;  // the most this kernel is ever given
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), (int)(ring + kPlaneSmem + sums));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)std::min(a.tiles, pl.num_sms * resident));

@@ -617,7 +617,8 @@ template <int N, int TERMS, bool BF16, int FB>
 cudaError_t run(const CUtensorMap& tm, TcArgs& a, int num_sms, bool pdl, cudaStream_t s) {
     using L = Lay<N, TERMS, BF16>;
     auto kernel = w4_tc_kernel<N, TERMS, BF16, FB>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    static SmemOnce once;
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), L::kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     a.tiles = (int)(a.w.tile_rows / 8 * ((a.tokens + N - 1) / N));
