@@ -1,29 +1,34 @@
 // Products with 4-bit weights and group scales, few tokens (w4_stream_kernel), and the weights'
-// layout (w4_pack_kernel) and the activations' (w4_planes_kernel) that the many-token kernel
-// (w4_tc.cu) shares.
+// layout (w4_pack_kernel) that the many-token kernel (w4_tc.cu) shares.
 //
 //     y[t][n] = Σ_g s[n][g] · sx[t][g'] · Σ_{k in g} (c[n][k] - z[n][g]) · x[t][k]
 //
 // with 4-bit codes c, a zero point z (8 when the weights have none), a scale s per group of one
 // row's weights, and for int8 activations a scale sx per row or per x_group values of a token.
 //
-// The inner sum runs on the tensor cores in bf16 with f32 accumulation, and loses nothing there:
-// c - z is an integer in [-127, 15] (zero points above 127 are refused), so a bf16; a bf16 or int8
-// activation is a bf16 too; an f32 activation is the sum of three bf16 (8 + 8 + 8 significant bits, split
-// by truncation, so exactly), one MMA each. Scales
-// are applied in f32 to the f32 sum of each group, as the formula has it.
+// The inner sum runs on the tensor cores in whole numbers (m16n8k32, u8 x s8 -> s32), exactly. int8 activations are
+// one such product. bf16 and f32 activations are made whole per token and 128 inputs: X = round(x · 2^e), e chosen
+// so that the largest |X| is in (2^21.99, 2^22.99), and X = 65536 d1 + 256 d2 + d3 with d in [-128, 127]: three
+// products. That keeps an activation to 2^-23 of the largest of its 128 (half a step of X; a sum's error is that
+// of f32 sums), and bf16 ones down to 2^-16 of the largest exactly. A chunk with an infinity or a NaN is a NaN.
+// z is taken off as z · Σ X, also whole: the accumulators start at -z Σ d, plus the bits of 1.5 · 2^23, so that they
+// are read as floats without a conversion (|Σ (c - z) d| <= 127 · 128 · 128 < 2^22). A flush per group makes a float of
+// the digits and applies the scales in f32.
 //
-// Bound: a weight is read once, for at most 32 tokens, so HBM. What a weight costs on the way: one
-// half of a logic operation and a shift to move two codes into a bf16 pair (0x4300 | c is 128 + c), one
-// packed subtraction of 128 + z per pair, 1/256 of an MMA per 8 tokens and bf16 term.
+// Bound: a weight is read once, for at most 16 tokens, so HBM. On the way a weight costs 3/8 of a logic operation (two
+// masks and a shift for a word of 8 codes); unpacked to 16-bit floats it cost 11/8 and the logic unit bound the
+// kernel (8192 x 8192, one bf16 token: 16 us; 128000 x 2048, 5 int8 tokens: 44 us).
 //
 // Layout: rows padded to 128, inputs to 128 (scale 0). A tile of 16 rows x 128 inputs is 1024 bytes,
 // [row / 8][row % 8][q = 0..3][b = 0..3] words of 8 codes; the 8 tiles of 128 rows lie together, then the next 128
-// inputs. Word (q, b) of a row holds inputs 32 b + 8 j + 2 q + e (j = 0..3, e = 0, 1) in nibble j + 4 e: what lane
-// (g, q) of a warp gives to the A fragments of two m16n8k16 MMAs, and (w >> 4 j) & 0x000f000f is a pair of neighbours.
-// A lane reads 16 bytes of its rows g and g + 8. The activations of 32 inputs are laid out alike ([q][j][e], 16 bytes a
-// lane). Blocks of 32 inputs stay whole, so a group of 32 ends with an MMA. Scales [tile][row % 8][block of
-// min(group, 128) inputs][row / 8], zero points the same in bytes: a lane's scales of a tile are one load.
+// inputs. Word (q, b) of a row holds inputs 32 b + 8 j + 2 q + e (j = 0..3, e = 0, 1) in nibble j + 4 e. Here its low
+// and high nibbles are the two words that lane (g, q) of a warp gives to an MMA for rows g (and g + 8) and 32 inputs, in
+// some order of these inputs; the activations are laid out in the same order, 8 bytes a lane and 32 inputs. (w >> 4 j) &
+// 0x000f000f is a pair of neighbours, which the other kernel uses.) Blocks of 32 inputs stay whole, so a
+// group of 32 ends with an MMA. Scales [tile][row % 8][block of min(group, 128) inputs][row / 8], zero points the
+// same in bytes: a lane's scales of a tile are one load.
+#include <math_constants.h>
+
 #include <algorithm>
 #include <cstdint>
 
@@ -32,69 +37,17 @@
 namespace bebelm {
 namespace {
 
-constexpr int kWarps = 8;    // of a CTA
-constexpr int kChunk = 128;  // inputs of a tile
+constexpr int kWarps = 8;               // of a CTA
+constexpr int kChunk = 128;             // inputs of a tile
+constexpr size_t kTokens = 16;          // the most of a call
+constexpr int kMagicBits = 0x4B400000;  // 1.5 · 2^23: a float whose last bits are a whole number
+constexpr float kMagic = 12582912.0f;
 
-// How a kernel takes its activations: as they are (bf16), as three bf16 terms (f32), or as f16 (int8 with a
-// scale a token, or a scale a group).
-constexpr int kBf16 = 0, kF32x3 = 1, kI8Row = 2, kI8Group = 3;
-
-// The zero points of a row as a pair to subtract: 128 + z in bf16, or, packed for f16, 1024 + z and 64 + z.
-template <bool F16>
-struct Zero {
-    uint32_t a, b;
-    __device__ __forceinline__ void set(uint32_t z) {  // z: one byte
-        if constexpr (F16) {
-            a = 0x64006400u + z * 0x10001u;
-            // f16 of 64 + z: 10 mantissa bits below 2^6 up to 127, below 2^7 from 128 on
-            const __half2 h = __half2half2(__ushort2half_rn((unsigned short)(64 + z)));
-            b = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-            a = 0x43004300u + z * 0x10001u;
-        }
-    }
-};
-
-// 8 codes of a word to 4 pairs of c - z, exactly.
-// bf16: 0x4300 | c is 128 + c; 128 + z is taken off. f16: two fields of a half word fit the mantissa: 0x6400 | c is
-// 1024 + c, and 0x6400 | 16 c is 1024 + 16 c, 1/16 of which less 64 + z is c - z: one shift a word instead of three.
-template <bool F16>
-__device__ __forceinline__ void code_pairs(uint32_t w, const Zero<F16>& z, uint32_t* o) {
-    if constexpr (F16) {
-        const __half2 za = *reinterpret_cast<const __half2*>(&z.a), zb = *reinterpret_cast<const __half2*>(&z.b);
-        const __half2 s16 = __float2half2_rn(0.0625f);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t v = i ? w >> 8 : w;
-            const uint32_t lo = (v & 0x000f000fu) | 0x64006400u, hi = (v & 0x00f000f0u) | 0x64006400u;
-            const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), za);
-            const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), s16, __hneg2(zb));
-            o[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
-            o[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-    } else {
-        const __nv_bfloat162 zz = *reinterpret_cast<const __nv_bfloat162*>(&z.a);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-            const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), zz);
-            o[i] = *reinterpret_cast<const uint32_t*>(&a);
-        }
-    }
-}
-
-template <bool F16>
-__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    if constexpr (F16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_u8s8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
@@ -104,57 +57,101 @@ __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
     return __half2float(__half(r));
 }
 
-// x = p0 + p1 + p2 exactly: 8 significant bits each, cut off towards zero. A non-finite x stays in p0 alone.
-__device__ __forceinline__ void split3(float x, uint32_t* p) {
-    p[0] = __float_as_uint(x) & 0xffff0000u;
-    float r = x - __uint_as_float(p[0]);
-    if (!(fabsf(x) <= 3.4028234663852886e38f)) {  // inf or NaN (whose kept bits must not be all zero)
-        if (x != x) p[0] |= 0x00400000u;
-        r = 0.f;
-    }
-    p[1] = __float_as_uint(r) & 0xffff0000u;
-    p[2] = __float_as_uint(r - __uint_as_float(p[1]));  // at most 8 bits are left
+// The activations as digits, in shared memory or (where that is too small) the workspace: D planes of rows of
+// `row` bytes, the sums of the digits [token][flush][D], and for D = 3 a scale per token and 128 inputs.
+struct Digits {
+    unsigned char* d;
+    int* sums;
+    float* scales;
+    size_t row, plane;
+};
+__host__ __device__ inline size_t digit_row(size_t chunks) { return chunks * kChunk + 64; }  // 64 modulo 128: no bank twice
+__host__ __device__ inline size_t digit_bytes(int D, size_t tokens, size_t chunks, int fb) {
+    return D * tokens * digit_row(chunks) + tokens * chunks * (4 / fb) * D * 4 + (D == 3 ? tokens * chunks * 4 : 0);
+}
+__host__ __device__ inline Digits digits_at(unsigned char* p, int D, size_t tokens, size_t chunks, int fb) {
+    Digits o;
+    o.row = digit_row(chunks), o.plane = tokens * o.row;
+    o.d = p, o.sums = reinterpret_cast<int*>(p + D * o.plane);
+    o.scales = reinterpret_cast<float*>(o.sums + tokens * chunks * (4 / fb) * D);
+    return o;
 }
 
-// Four pairs of a token's activations as P x 4 words of two 16-bit values; zeros past n_in (a multiple of 32). The pairs
-// start at inputs k, k + d, k + 2 d, k + 3 d of one block of 32. f32: three bf16 terms; bf16: as they are; int8: f16.
-template <int P>
-__device__ __forceinline__ void x_pairs(const W4X& x, size_t t, size_t k, int d, uint32_t (*v)[4]) {
+__device__ __forceinline__ float x_at(const W4X& x, size_t o) {
+    if (x.kind == kW4XF32) return static_cast<const float*>(x.x)[o];
+    return __uint_as_float((uint32_t)static_cast<const unsigned short*>(x.x)[o] << 16);
+}
+
+// 128 inputs of a token by half a warp: lane (b, q) the 8 of block b that lane q of an MMA gets
+template <int D, int FB>
+__device__ __forceinline__ void make_digits(const W4X& x, const Digits& o, int chunks, int t, int c) {
+    const int l = threadIdx.x & 15, b = l >> 2, q = l & 3;
+    const int k = c * kChunk + 32 * b + 2 * q;
+    const bool in = (size_t)k < x.n_in;  // n_in is a multiple of 32
+    constexpr int kAt[8] = {0, 16, 1, 17, 8, 24, 9, 25};  // inputs of the bytes
+    const size_t base = (size_t)t * x.stride + k;
+    uint32_t w[D][2];
+    int sum[D];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t a[3] = {0, 0, 0}, b[3] = {0, 0, 0};
-        if (k < x.n_in) {
-            const size_t o = t * x.stride + k + j * d;
-            if (P == 3) {
-                const float* p = static_cast<const float*>(x.x) + o;
-                split3(p[0], a), split3(p[1], b);
-            } else if (x.kind == kW4XInt8) {
-                const signed char* p = static_cast<const signed char*>(x.x) + o;
-                a[0] = (uint32_t)__half_as_ushort(__short2half_rn(p[0])) << 16;
-                b[0] = (uint32_t)__half_as_ushort(__short2half_rn(p[1])) << 16;
-            } else {
-                const unsigned short* p = static_cast<const unsigned short*>(x.x) + o;
-                a[0] = (uint32_t)p[0] << 16, b[0] = (uint32_t)p[1] << 16;
+    for (int d = 0; d < D; ++d) sum[d] = 0, w[d][0] = w[d][1] = 0;
+    if constexpr (D == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int v = in ? static_cast<const signed char*>(x.x)[base + kAt[i]] : 0;
+            sum[0] += v;
+            w[0][i >> 2] |= (uint32_t)(v & 255) << (8 * (i & 3));
+        }
+    } else {
+        float v[8], m = 0.f;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] = in ? x_at(x, base + kAt[i]) : 0.f;
+            odd |= !(fabsf(v[i]) <= 3.4028234663852886e38f);
+            m = fmaxf(m, fabsf(v[i]));
+        }
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1) {
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+            odd |= __shfl_xor_sync(0xffffffffu, (int)odd, s) != 0;
+        }
+        // 2^e: the largest to 2^22 .. 2^23, or half of that where its digits would not fit; e <= 122
+        int e = 22 - max((int)(__float_as_uint(m) >> 23) - 127, -100);
+        if (odd) e = 0;
+        if (m * __uint_as_float((uint32_t)(127 + e) << 23) > 8355711.f) --e;  // 127 (65536 + 256 + 1)
+        const float f = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            int r = odd ? 0 : __float2int_rn(v[i] * f);
+#pragma unroll
+            for (int d = D - 1; d >= 0; --d) {
+                const int digit = d ? (int)(signed char)(r & 255) : r;
+                r = (r - digit) >> 8;
+                sum[d] += digit;
+                w[d][i >> 2] |= (uint32_t)(digit & 255) << (8 * (i & 3));
             }
         }
+        if (l == 0) o.scales[(size_t)t * chunks + c] = odd ? CUDART_NAN_F : __uint_as_float((uint32_t)(127 - e) << 23);
+    }
 #pragma unroll
-        for (int i = 0; i < P; ++i) v[i][j] = __byte_perm(a[i], b[i], 0x7632);
+    for (int d = 0; d < D; ++d) {
+        *reinterpret_cast<uint2*>(o.d + d * o.plane + t * o.row + c * kChunk + (b >> 1) * 64 + q * 16 + (b & 1) * 8) = make_uint2(w[d][0], w[d][1]);
+#pragma unroll
+        for (int s = 1; s < 4 * FB; s <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], s);
+        if (l % (4 * FB) == 0) o.sums[((size_t)t * chunks * (4 / FB) + c * (4 / FB) + b / FB) * D + d] = sum[d];
     }
 }
 
-// The activations in the lanes' order, [P][tokens][kp] with zeros past n_in.
-template <int P>
-__global__ void __launch_bounds__(256) w4_planes_kernel(W4X x, size_t kp, uint16_t* out) {
+template <int D, int FB>
+__global__ void __launch_bounds__(256) w4_digits_kernel(W4X x, int chunks, unsigned char* out) {
     asm volatile("griddepcontrol.launch_dependents;");
-    const size_t plane = x.tokens * kp;
-    for (size_t t = blockIdx.y; t < x.tokens; t += gridDim.y)
-        for (size_t k = 8 * ((size_t)blockIdx.x * blockDim.x + threadIdx.x); k < kp; k += 8 * (size_t)gridDim.x * blockDim.x) {
-            uint32_t v[P][4];
-            x_pairs<P>(x, t, (k & ~size_t(31)) + (k >> 2 & 6), 8, v);
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-                *reinterpret_cast<uint4*>(out + i * plane + t * kp + k) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
-        }
+    const Digits o = digits_at(out, D, x.tokens, chunks, FB);
+    // half a warp per 128 inputs of a token; whole warps stay in step
+    const int n = (int)x.tokens * chunks;
+    for (int i = (blockIdx.x * 256 + threadIdx.x) >> 4; (i & ~1) < n; i += gridDim.x * 16) {
+        const int j = min(i, n - 1);
+        make_digits<D, FB>(x, o, chunks, j / chunks, j % chunks);
+    }
 }
 
 // codes [n_out][n_in / 2], scales and zeros [n_out][n_in / group] into the layout above, a
@@ -191,11 +188,12 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* codes, cons
 struct StreamArgs {
     W4View w;
     W4X x;
-    const uint16_t* planes;  // [P][x.tokens][ldp], 16-byte aligned rows; null: made in shared memory
-    size_t ldp, plane;            // elements of a row and of a plane
+    unsigned char* digits;   // in the workspace; null: made in shared memory
+    const float* x_scales;   // a factor per token and 2^x_shift inputs, `x_pitch` a token (D = 3: the digits' own)
+    int x_pitch, x_shift;
     void* y;
-    int y_bf16, ks, tiles;        // ks warps share a row of tiles; `tiles` groups of kWarps / ks of them
-    int sums_at;                  // float offset of the warps' partial sums behind ring and planes in shared memory
+    int y_bf16, ks, tiles;   // ks warps share a row of tiles; `tiles` groups of kWarps / ks of them
+    int digits_at, sums_at;  // in shared memory, behind the ring: the digits (bytes), the warps' partial sums (floats)
 };
 
 // N bytes from global to shared memory, asynchronously; 16-byte copies pass L1 by
@@ -211,19 +209,17 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
 // what it reads itself, so a stage needs no barrier, only its own lane's copies to have landed.
 template <int MT, int PC>
 struct Stage4 {
-    static constexpr int kStages = MT == 1 ? 5 : 3;  // 4 KB in flight a warp while one stage is multiplied
+    static constexpr int kStages = MT == 1 ? 6 : 4;
     static constexpr int kZero = PC == 4 ? 8 : 4;  // bytes of zero points of a lane and tile (4 for PC 1: padded)
     static constexpr int kScaleAt = MT * 1024, kZeroAt = kScaleAt + MT * 32 * 4 * PC;
     static constexpr int kBytes = kZeroAt + MT * 32 * kZero;
 };
 
-// A warp: MT x 16 rows x NT x 8 tokens over its part of the inputs. PC scales of a row in 128 inputs; FB:
-// blocks of 32 inputs after which a sum meets its scales.
-template <int MT, int NT, int X, int PC, int FB>
+// A warp: MT x 16 rows x NT x 8 tokens over its part of the inputs. D digits an activation; PC scales of a row in
+// 128 inputs; FB: blocks of 32 inputs after which a sum meets its scales; XS: activations' scales at each flush.
+template <int MT, int NT, int D, int PC, int FB, bool XS>
 __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a) {
     using S = Stage4<MT, PC>;
-    constexpr bool F16 = X >= kI8Row;
-    constexpr int P = X == kF32x3 ? 3 : 1;
     extern __shared__ __align__(16) unsigned char s_mem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int per = kWarps / a.ks, sub = warp % a.ks;
@@ -266,42 +262,37 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
     // The weights do not depend on the kernel before, the activations may.
     for (int i = 0; i < S::kStages - 1; ++i) produce();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint16_t* planes = a.planes;
-    size_t ldp = a.ldp, plane = a.plane;
-    if (!planes) {  // rows 64 bytes apart modulo 128: the 8 rows of a fragment load meet no bank twice
-        uint16_t* sx = reinterpret_cast<uint16_t*>(s_mem + kWarps * S::kStages * S::kBytes);
-        const int kp = chunks * kChunk;
-        ldp = kp + 32;
-        plane = T * ldp;
-        for (int t = 0; t < T; ++t)
-            for (int k = 8 * threadIdx.x; k < kp; k += 8 * kWarps * 32) {
-                uint32_t v[P][4];
-                x_pairs<P>(a.x, t, (k & ~31) + (k >> 2 & 6), 8, v);
-#pragma unroll
-                for (int p = 0; p < P; ++p)
-                    *reinterpret_cast<uint4*>(sx + p * plane + t * ldp + k) = make_uint4(v[p][0], v[p][1], v[p][2], v[p][3]);
-            }
-        planes = sx;
+    const Digits x = digits_at(a.digits ? a.digits : s_mem + a.digits_at, D, T, chunks, FB);
+    if (!a.digits) {
+        const int n = T * chunks;
+        for (int i = threadIdx.x >> 4; (i & ~1) < n; i += kWarps * 2) {
+            const int j = min(i, n - 1);
+            make_digits<D, FB>(a.x, x, chunks, j / chunks, j % chunks);
+        }
         __syncthreads();
     }
-    const uint16_t* xr[NT][P];  // a lane without a token repeats the last one's row: its sums are not stored
+    constexpr int FL = 4 / FB;  // flushes of 128 inputs
+    const unsigned char* xr[NT];  // a lane without a token repeats the last one's row: its sums are not stored
+    const int* xq[NT][2];         // the digits' sums of tokens 8 n + 2 q, + 1, and their scales
+    const float* xs[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+        xr[n] = x.d + (size_t)min(8 * n + g, T - 1) * x.row + 16 * q;
 #pragma unroll
-        for (int p = 0; p < P; ++p) xr[n][p] = planes + (size_t)min(8 * n + g, T - 1) * ldp + p * plane + 8 * q;
-    const float* xs[NT][2];  // X == kI8Group: the scales of tokens 8 n + 2 q, + 1
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) xs[n][e] = a.x.scales + (size_t)min(8 * n + 2 * q + e, T - 1) * a.x.n_groups;
+        for (int e = 0; e < 2; ++e) {
+            const size_t t = min(8 * n + 2 * q + e, T - 1);
+            xq[n][e] = x.sums + t * chunks * FL * D;
+            xs[n][e] = D == 3 ? x.scales + t * chunks : a.x_scales + t * a.x_pitch;
+        }
+    }
 
     const unsigned char* st = ring;
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
         const int tr = tile * per + warp / a.ks;
         const bool has = tr < rows;
-        float acc[MT][NT][4], ga[MT][NT][4];
+        float acc[MT][NT][4];
 #pragma unroll
-        for (int i = 0; i < MT * NT * 4; ++i) acc[i / (4 * NT)][i / 4 % NT][i % 4] = ga[i / (4 * NT)][i / 4 % NT][i % 4] = 0.f;
+        for (int i = 0; i < MT * NT * 4; ++i) acc[i / (4 * NT)][i / 4 % NT][i % 4] = 0.f;
         for (int c = c0; has && c < c1; ++c) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
             produce();  // into the stage of the tile before this one
@@ -320,57 +311,61 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
                                      : 0x08080808u;
             }
             st = st == ring + (S::kStages - 1) * S::kBytes ? ring : st + S::kBytes;
-            Zero<F16> za[MT], zb[MT];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                constexpr int kPer = 4 / PC;  // blocks of a scale
-                const int blk = b / kPer;
-                uint32_t f[MT][2][4];
+            for (int f = 0; f < FL; ++f) {
+                const int blk = f * FB * PC / 4;  // scale block of the chunk
+                int d[MT][NT][D][4];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    if (b % kPer == 0) {
-                        const uint32_t z2 = zz[m][blk / 2] >> (16 * (blk & 1));
-                        za[m].set(z2 & 0xffu), zb[m].set((z2 >> 8) & 0xffu);
-                    }
-                    uint32_t pa[4], pb[4];
-                    code_pairs<F16>(b == 0 ? va[m].x : b == 1 ? va[m].y : b == 2 ? va[m].z : va[m].w, za[m], pa);
-                    code_pairs<F16>(b == 0 ? vb[m].x : b == 1 ? vb[m].y : b == 2 ? vb[m].z : vb[m].w, zb[m], pb);
+                    const uint32_t z2 = zz[m][blk / 2] >> (16 * (blk & 1));
+                    const int z0 = -(int)(z2 & 0xffu), z1 = -(int)((z2 >> 8) & 0xffu);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) f[m][i >> 1][2 * (i & 1)] = pa[i], f[m][i >> 1][2 * (i & 1) + 1] = pb[i];
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < D; ++i) {
+                            const int q0 = xq[n][0][(c * FL + f) * D + i], q1 = xq[n][1][(c * FL + f) * D + i];
+                            d[m][n][i][0] = z0 * q0 + kMagicBits, d[m][n][i][1] = z0 * q1 + kMagicBits;
+                            d[m][n][i][2] = z1 * q0 + kMagicBits, d[m][n][i][3] = z1 * q1 + kMagicBits;
+                        }
+                }
+#pragma unroll
+                for (int b = f * FB; b < (f + 1) * FB; ++b) {
+                    uint32_t fr[MT][4];
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const uint32_t wa = b == 0 ? va[m].x : b == 1 ? va[m].y : b == 2 ? va[m].z : va[m].w;
+                        const uint32_t wb = b == 0 ? vb[m].x : b == 1 ? vb[m].y : b == 2 ? vb[m].z : vb[m].w;
+                        fr[m][0] = wa & 0x0f0f0f0fu, fr[m][1] = wb & 0x0f0f0f0fu;
+                        fr[m][2] = (wa >> 4) & 0x0f0f0f0fu, fr[m][3] = (wb >> 4) & 0x0f0f0f0fu;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < D; ++i) {
+                            const uint2 xf = *reinterpret_cast<const uint2*>(xr[n] + i * x.plane + c * kChunk + (b >> 1) * 64 + (b & 1) * 8);
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) mma_u8s8(d[m][n][i], fr[m], xf.x, xf.y);
+                        }
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        const uint4 xf = *reinterpret_cast<const uint4*>(xr[n][p] + c * kChunk + 32 * b);
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            mma16816<F16>(ga[m][n], f[m][0], xf.x, xf.y);
-                            mma16816<F16>(ga[m][n], f[m][1], xf.z, xf.w);
-                        }
-                    }
-                }
-                if ((b + 1) % FB == 0) {
-                    float x0[NT], x1[NT];
-                    if constexpr (X == kI8Group) {
-                        const int xi = (c * kChunk + 32 * b) >> a.x.group_shift;
-                        const int at = min(xi, (int)a.x.n_groups - 1);  // padded inputs: the weights' scale is 0
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) x0[n] = __ldg(xs[n][0] + at), x1[n] = __ldg(xs[n][1] + at);
+                    float x0 = 1.f, x1 = 1.f;
+                    if constexpr (XS) {
+                        // padded inputs: the weights' scale is 0
+                        const int at = D == 3 ? c : min((c * kChunk + 32 * FB * f) >> a.x_shift, a.x_pitch - 1);
+                        x0 = xs[n][0][at], x1 = xs[n][1][at];
                     }
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         const float s0 = scale_of(sc[m][blk] & 0xffffu, a.w.scale_bf16), s1 = scale_of(sc[m][blk] >> 16, a.w.scale_bf16);
+                        float v[4];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            if constexpr (X == kI8Group)
-                                ga[m][n][0] *= x0[n], ga[m][n][1] *= x1[n], ga[m][n][2] *= x0[n], ga[m][n][3] *= x1[n];
-                            acc[m][n][0] = fmaf(ga[m][n][0], s0, acc[m][n][0]);
-                            acc[m][n][1] = fmaf(ga[m][n][1], s0, acc[m][n][1]);
-                            acc[m][n][2] = fmaf(ga[m][n][2], s1, acc[m][n][2]);
-                            acc[m][n][3] = fmaf(ga[m][n][3], s1, acc[m][n][3]);
+                        for (int e = 0; e < 4; ++e) {
+                            v[e] = __int_as_float(d[m][n][0][e]) - kMagic;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) ga[m][n][e] = 0.f;
+                            for (int i = 1; i < D; ++i) v[e] = fmaf(v[e], 256.f, __int_as_float(d[m][n][i][e]) - kMagic);
+                            if constexpr (XS) v[e] *= e & 1 ? x1 : x0;
+                            acc[m][n][e] = fmaf(v[e], e & 2 ? s1 : s0, acc[m][n][e]);
                         }
                     }
                 }
@@ -398,12 +393,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
                 for (int e = 0; e < 4; ++e) {
                     const size_t t = 8 * n + 2 * q + (e & 1);
                     if (t >= a.x.tokens) continue;
-                    const float xscale = X == kI8Row ? a.x.scales[t] : 1.f;
+                    const float factor = XS ? 1.f : a.x_scales[t];
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         const size_t r = ((size_t)tr * MT + m) * 16 + g + 8 * (e >> 1);
                         if (r >= a.w.n_out) continue;
-                        const float v = X == kI8Row ? acc[m][n][e] * xscale : acc[m][n][e];
+                        const float v = XS ? acc[m][n][e] : acc[m][n][e] * factor;
                         if (a.y_bf16)
                             static_cast<__nv_bfloat16*>(a.y)[t * a.w.n_out + r] = __float2bfloat16_rn(v);
                         else
@@ -415,24 +410,25 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Shared memory for the activations' planes, beside the ring.
-constexpr size_t kPlaneSmem = 48 * 1024;
+// Shared memory for the digits, beside the ring: two CTAs an SM.
+constexpr size_t kDigitSmem = 48 * 1024;
 
-struct StreamPlan {
-    int num_sms;
-    size_t plane_bytes;  // of the planes in shared memory
-    bool pdl;            // launched as a programmatic dependent of the planes' kernel
-};
+int flush_blocks(const W4View& w, const W4X& x) {
+    const int fb = 4 / w.per_chunk;
+    return x.group ? std::min(fb, x.group / 32) : fb;
+}
+int digits_of(const W4X& x) { return x.kind == kW4XInt8 ? 1 : 3; }
 
-template <int MT, int NT, int X, int PC, int FB>
-cudaError_t run_stream(StreamArgs& a, const StreamPlan& pl, cudaStream_t s) {
-    auto kernel = w4_stream_kernel<MT, NT, X, PC, FB>;
+template <int MT, int NT, int D, int PC, int FB, bool XS>
+cudaError_t run_stream(StreamArgs& a, int num_sms, cudaStream_t s) {
+    auto kernel = w4_stream_kernel<MT, NT, D, PC, FB, XS>;
     const size_t ring = (size_t)kWarps * Stage4<MT, PC>::kStages * Stage4<MT, PC>::kBytes;
     const size_t sums = kWarps * 32 * 4 * NT * MT * sizeof(float);
-    const int resident = ring + pl.plane_bytes + sums <= 112 * 1024 ? 2 : 1;
+    const size_t own = a.digits ? 0 : (digit_bytes(D, a.x.tokens, a.w.chunks, FB) + 15) & ~size_t(15);
+    const int resident = ring + own + sums <= 113 * 1024 ? 2 : 1;
     // Warps that share a row of tiles: the split with the shortest chain of tiles for a warp, where a round
     // costs about as much as 3 tiles (its first loads, its sums joined).
-    const size_t rows = a.w.tile_rows / MT, ctas = (size_t)pl.num_sms * resident;
+    const size_t rows = a.w.tile_rows / MT, ctas = (size_t)num_sms * resident;
     int ks = 1;
     size_t best = ~size_t(0);
     for (int k = 1; k <= kWarps && (size_t)k <= a.w.chunks; k *= 2) {
@@ -442,13 +438,14 @@ cudaError_t run_stream(StreamArgs& a, const StreamPlan& pl, cudaStream_t s) {
     }
     a.ks = ks;
     a.tiles = (int)((rows + kWarps / ks - 1) / (kWarps / ks));
-    a.sums_at = (int)((ring + pl.plane_bytes) / sizeof(float));
-    const size_t smem = ring + pl.plane_bytes + (ks > 1 ? sums : 0);
+    a.digits_at = (int)ring;
+    a.sums_at = (int)((ring + own) / sizeof(float));
+    const size_t smem = ring + own + (ks > 1 ? sums : 0);
     static SmemOnce once;  // the most this kernel is ever given
-    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), (int)(ring + kPlaneSmem + sums));
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), (int)(ring + kDigitSmem + 16 + sums));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)std::min(a.tiles, pl.num_sms * resident));
+    cfg.gridDim = dim3((unsigned)std::min(a.tiles, num_sms * resident));
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -456,32 +453,41 @@ cudaError_t run_stream(StreamArgs& a, const StreamPlan& pl, cudaStream_t s) {
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
-    cfg.numAttrs = pl.pdl ? 1 : 0;
+    cfg.numAttrs = a.digits ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
-template <int MT, int NT, int X>
-cudaError_t run_pc(StreamArgs& a, const StreamPlan& pl, cudaStream_t s) {
-    const int pc = a.w.per_chunk;
-    if constexpr (X == kI8Group)  // groups of activations smaller than the weights': scales every 32 inputs
-        if (a.x.group * pc < kChunk) return pc == 1 ? run_stream<MT, NT, X, 1, 1>(a, pl, s) : run_stream<MT, NT, X, 2, 1>(a, pl, s);
-    return pc == 1   ? run_stream<MT, NT, X, 1, 4>(a, pl, s)
-           : pc == 2 ? run_stream<MT, NT, X, 2, 2>(a, pl, s)
-                     : run_stream<MT, NT, X, 4, 1>(a, pl, s);
+template <int MT, int NT, int D, bool XS>
+cudaError_t run_pc(StreamArgs& a, int num_sms, cudaStream_t s) {
+    const int pc = a.w.per_chunk, fb = flush_blocks(a.w, a.x);
+    if constexpr (D == 1 && XS) {  // groups of activations smaller than the weights'
+        if (fb < 4 / pc)
+            return pc == 2   ? run_stream<MT, NT, D, 2, 1, XS>(a, num_sms, s)
+                   : fb == 2 ? run_stream<MT, NT, D, 1, 2, XS>(a, num_sms, s)
+                             : run_stream<MT, NT, D, 1, 1, XS>(a, num_sms, s);
+    }
+    return pc == 1   ? run_stream<MT, NT, D, 1, 4, XS>(a, num_sms, s)
+           : pc == 2 ? run_stream<MT, NT, D, 2, 2, XS>(a, num_sms, s)
+                     : run_stream<MT, NT, D, 4, 1, XS>(a, num_sms, s);
 }
-template <int X>
-cudaError_t run_nt(StreamArgs& a, const StreamPlan& pl, cudaStream_t s) {
+template <int D, bool XS>
+cudaError_t run_nt(StreamArgs& a, int num_sms, cudaStream_t s) {
     // Two row tiles a warp share the activations' fragments and the loop's overhead; one tile a warp where
-    // that would leave SMs without a full CTA.
-    if (a.x.tokens <= 8)
-        return a.w.tile_rows < (size_t)pl.num_sms * 2 * kWarps ? run_pc<1, 1, X>(a, pl, s) : run_pc<2, 1, X>(a, pl, s);
-    return a.x.tokens <= 16 ? run_pc<2, 2, X>(a, pl, s) : run_pc<1, 4, X>(a, pl, s);
+    // that would leave SMs without a full CTA, and where 16 tokens' accumulators fill the registers.
+    if (a.x.tokens > 8) return D == 1 ? run_pc<2, 2, D, XS>(a, num_sms, s) : run_pc<1, 2, D, XS>(a, num_sms, s);
+    return a.w.tile_rows < (size_t)num_sms * 2 * kWarps ? run_pc<1, 1, D, XS>(a, num_sms, s) : run_pc<2, 1, D, XS>(a, num_sms, s);
 }
 
-int terms_of(const W4X& x) { return x.kind == kW4XF32 ? 3 : 1; }
-size_t plane_smem(const W4View& w, const W4X& x, size_t tokens) {
-    return terms_of(x) * tokens * (w.chunks * kChunk + 32) * sizeof(uint16_t);
+template <int D>
+cudaError_t run_digits(const W4X& x, int chunks, int fb, unsigned char* out, cudaStream_t s) {
+    const unsigned grid = (unsigned)std::min<size_t>((x.tokens * chunks + 15) / 16, 1024);
+    if (fb == 4)
+        w4_digits_kernel<D, 4><<<grid, 256, 0, s>>>(x, chunks, out);
+    else if (fb == 2)
+        w4_digits_kernel<D, 2><<<grid, 256, 0, s>>>(x, chunks, out);
+    else
+        w4_digits_kernel<D, 1><<<grid, 256, 0, s>>>(x, chunks, out);
+    return cudaGetLastError();
 }
-constexpr size_t kStreamTokens = 32;  // of one launch
 
 }  // namespace
 
@@ -493,48 +499,25 @@ cudaError_t launch_w4_pack(const uint8_t* codes, const unsigned short* scales, c
 }
 
 size_t w4_stream_workspace(const W4View& w, const W4X& x) {
-    if (plane_smem(w, x, std::min(x.tokens, kStreamTokens)) <= kPlaneSmem) return 0;
-    return terms_of(x) * x.tokens * w.chunks * kChunk * sizeof(uint16_t);
+    const size_t n = digit_bytes(digits_of(x), x.tokens, w.chunks, flush_blocks(w, x));
+    return n <= kDigitSmem ? 0 : n;
 }
 
 cudaError_t launch_w4_stream(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms,
                              cudaStream_t s) {
+    if (x.tokens > kTokens) return cudaErrorInvalidValue;
     StreamArgs a{};
-    a.w = w;
-    a.y_bf16 = y_bf16;
-    const bool planes = w4_stream_workspace(w, x) > 0;
-    if (planes) {
-        const size_t kp = w.chunks * kChunk;
-        uint16_t* out = static_cast<uint16_t*>(workspace);
-        const dim3 grid((unsigned)std::min<size_t>((kp / 8 + 255) / 256, 64), (unsigned)std::min<size_t>(x.tokens, 65535));
-        if (x.kind == kW4XF32)
-            w4_planes_kernel<3><<<grid, 256, 0, s>>>(x, kp, out);
-        else
-            w4_planes_kernel<1><<<grid, 256, 0, s>>>(x, kp, out);
-        const cudaError_t e = cudaGetLastError();
-        if (e != cudaSuccess) return e;
-        a.planes = out;
-        a.ldp = kp;
-        a.plane = x.tokens * kp;
-    }
-    const size_t es = x.kind == kW4XF32 ? 4 : x.kind == kW4XBf16 ? 2 : 1;
-    for (size_t t = 0; t < x.tokens; t += kStreamTokens) {
-        StreamArgs b = a;
-        b.x = x;
-        b.x.x = static_cast<const char*>(x.x) + t * x.stride * es;
-        b.x.tokens = std::min(kStreamTokens, x.tokens - t);
-        b.x.scales = x.scales ? x.scales + t * x.n_groups : nullptr;
-        if (a.planes) b.planes = a.planes + t * a.ldp;
-        b.y = y_bf16 ? static_cast<void*>(static_cast<__nv_bfloat16*>(y) + t * w.n_out)
-                     : static_cast<void*>(static_cast<float*>(y) + t * w.n_out);
-        const StreamPlan pl{num_sms, a.planes ? 0 : plane_smem(w, x, b.x.tokens), planes && t == 0};
-        const cudaError_t e = x.kind == kW4XF32    ? run_nt<kF32x3>(b, pl, s)
-                              : x.kind == kW4XBf16 ? run_nt<kBf16>(b, pl, s)
-                              : x.group > 0        ? run_nt<kI8Group>(b, pl, s)
-                                                   : run_nt<kI8Row>(b, pl, s);
+    a.w = w, a.x = x, a.y = y, a.y_bf16 = y_bf16;
+    a.x_scales = x.scales, a.x_pitch = (int)x.n_groups, a.x_shift = x.group_shift;
+    if (w4_stream_workspace(w, x)) {
+        a.digits = static_cast<unsigned char*>(workspace);
+        const cudaError_t e = digits_of(x) == 3 ? run_digits<3>(x, (int)w.chunks, flush_blocks(w, x), a.digits, s)
+                                                : run_digits<1>(x, (int)w.chunks, flush_blocks(w, x), a.digits, s);
         if (e != cudaSuccess) return e;
     }
-    return cudaSuccess;
+    return digits_of(x) == 3 ? run_nt<3, true>(a, num_sms, s)
+           : x.group > 0     ? run_nt<1, true>(a, num_sms, s)
+                             : run_nt<1, false>(a, num_sms, s);
 }
 
 }  // namespace bebelm
