@@ -37,7 +37,7 @@
 namespace bebelm {
 namespace {
 
-constexpr int kWarps = 8;               // of a CTA
+constexpr int kWarps = 16;              // of a CTA, one an SM
 constexpr int kChunk = 128;             // inputs of a tile
 constexpr size_t kTokens = 16;          // the most of a call
 constexpr int kMagicBits = 0x4B400000;  // 1.5 · 2^23: a float whose last bits are a whole number
@@ -58,99 +58,120 @@ __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
 }
 
 // The activations as digits, in shared memory or (where that is too small) the workspace: D planes of rows of
-// `row` bytes, the sums of the digits [token][flush][D], and for D = 3 a scale per token and 128 inputs.
+// `row` bytes, and a record per flush and token: the digits' sums and the scale, {Σ d, scale} or {Σ d1, Σ d2, Σ d3, scale}.
 struct Digits {
     unsigned char* d;
-    int* sums;
-    float* scales;
+    unsigned char* records;
     size_t row, plane;
 };
 __host__ __device__ inline size_t digit_row(size_t chunks) { return chunks * kChunk + 64; }  // 64 modulo 128: no bank twice
+__host__ __device__ inline size_t even(size_t n) { return (n + 1) & ~size_t(1); }
 __host__ __device__ inline size_t digit_bytes(int D, size_t tokens, size_t chunks, int fb) {
-    return D * tokens * digit_row(chunks) + tokens * chunks * (4 / fb) * D * 4 + (D == 3 ? tokens * chunks * 4 : 0);
+    return D * tokens * digit_row(chunks) + even(tokens) * chunks * (4 / fb) * (D == 3 ? 16 : 8);
 }
-__host__ __device__ inline Digits digits_at(unsigned char* p, int D, size_t tokens, size_t chunks, int fb) {
+__host__ __device__ inline Digits digits_at(unsigned char* p, int D, size_t tokens, size_t chunks) {
     Digits o;
     o.row = digit_row(chunks), o.plane = tokens * o.row;
-    o.d = p, o.sums = reinterpret_cast<int*>(p + D * o.plane);
-    o.scales = reinterpret_cast<float*>(o.sums + tokens * chunks * (4 / fb) * D);
+    o.d = p, o.records = p + D * o.plane;
     return o;
 }
 
-__device__ __forceinline__ float x_at(const W4X& x, size_t o) {
-    if (x.kind == kW4XF32) return static_cast<const float*>(x.x)[o];
-    return __uint_as_float((uint32_t)static_cast<const unsigned short*>(x.x)[o] << 16);
+// two neighbours; `pairs`: they are aligned to their size
+__device__ __forceinline__ float2 x_pair(const W4X& x, size_t o, bool pairs) {
+    if (x.kind == kW4XF32) {
+        const float* p = static_cast<const float*>(x.x) + o;
+        return pairs ? *reinterpret_cast<const float2*>(p) : make_float2(p[0], p[1]);
+    }
+    const unsigned short* p = static_cast<const unsigned short*>(x.x) + o;
+    const uint32_t u = pairs ? *reinterpret_cast<const uint32_t*>(p) : (uint32_t)p[0] | (uint32_t)p[1] << 16;
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ bool x_pairs(const W4X& x) {
+    const size_t to = x.kind == kW4XF32 ? 8 : 4;
+    return x.stride % 2 == 0 && reinterpret_cast<uintptr_t>(x.x) % to == 0;
 }
 
 // 128 inputs of a token by half a warp: lane (b, q) the 8 of block b that lane q of an MMA gets
 template <int D, int FB>
-__device__ __forceinline__ void make_digits(const W4X& x, const Digits& o, int chunks, int t, int c) {
+__device__ __forceinline__ void make_digits(const W4X& x, const Digits& o, int t, int c) {
     const int l = threadIdx.x & 15, b = l >> 2, q = l & 3;
     const int k = c * kChunk + 32 * b + 2 * q;
     const bool in = (size_t)k < x.n_in;  // n_in is a multiple of 32
-    constexpr int kAt[8] = {0, 16, 1, 17, 8, 24, 9, 25};  // inputs of the bytes
     const size_t base = (size_t)t * x.stride + k;
-    uint32_t w[D][2];
+    uint32_t w[D][2];  // bytes: inputs 0, 16, 1, 17 and 8, 24, 9, 25 from k
     int sum[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) sum[d] = 0, w[d][0] = w[d][1] = 0;
+    float scale;
     if constexpr (D == 1) {
+        constexpr int kAt[8] = {0, 16, 1, 17, 8, 24, 9, 25};
+        w[0][0] = w[0][1] = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int v = in ? static_cast<const signed char*>(x.x)[base + kAt[i]] : 0;
-            sum[0] += v;
-            w[0][i >> 2] |= (uint32_t)(v & 255) << (8 * (i & 3));
+            const uint32_t v = in ? static_cast<const unsigned char*>(x.x)[base + kAt[i]] : 0u;
+            w[0][i >> 2] |= v << (8 * (i & 3));
         }
+        // padded inputs: any scale
+        const int at = x.group ? min(k >> x.group_shift, (int)x.n_groups - 1) : 0;
+        scale = x.scales[(size_t)t * x.n_groups + at];
+        sum[0] = __dp4a((int)w[0][0], 0x01010101, __dp4a((int)w[0][1], 0x01010101, 0));
     } else {
-        float v[8], m = 0.f;
-        bool odd = false;
+        float v[8];
+        const bool pairs = x_pairs(x);
+        constexpr int kAt[4] = {0, 16, 8, 24};
+        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[i] = in ? x_at(x, base + kAt[i]) : 0.f;
-            odd |= !(fabsf(v[i]) <= 3.4028234663852886e38f);
-            m = fmaxf(m, fabsf(v[i]));
+        for (int i = 0; i < 4; ++i) {
+            const float2 u = in ? x_pair(x, base + kAt[i], pairs) : make_float2(0.f, 0.f);
+            v[4 * (i >> 1) + (i & 1)] = u.x, v[4 * (i >> 1) + (i & 1) + 2] = u.y;
         }
 #pragma unroll
-        for (int s = 8; s > 0; s >>= 1) {
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-            odd |= __shfl_xor_sync(0xffffffffu, (int)odd, s) != 0;
-        }
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);  // an infinity or a NaN is the largest
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
+        const bool odd = m > 0x7f7fffffu;
         // 2^e: the largest to 2^22 .. 2^23, or half of that where its digits would not fit; e <= 122
-        int e = 22 - max((int)(__float_as_uint(m) >> 23) - 127, -100);
-        if (odd) e = 0;
-        if (m * __uint_as_float((uint32_t)(127 + e) << 23) > 8355711.f) --e;  // 127 (65536 + 256 + 1)
+        int e = odd ? 0 : 22 - max((int)(m >> 23) - 127, -100);
+        if (__uint_as_float(m) * __uint_as_float((uint32_t)(127 + e) << 23) > 8355711.f) --e;  // 127 (65536 + 256 + 1)
         const float f = __uint_as_float((uint32_t)(127 + e) << 23);
+        // X + 0x808080 has the digits + 128 as its bytes
+        uint32_t u[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            int r = odd ? 0 : __float2int_rn(v[i] * f);
+        for (int i = 0; i < 8; ++i) u[i] = odd ? 0x808080u : (uint32_t)(__float2int_rn(v[i] * f) + 0x808080);
 #pragma unroll
-            for (int d = D - 1; d >= 0; --d) {
-                const int digit = d ? (int)(signed char)(r & 255) : r;
-                r = (r - digit) >> 8;
-                sum[d] += digit;
-                w[d][i >> 2] |= (uint32_t)(digit & 255) << (8 * (i & 3));
-            }
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t *p = u + 4 * h, a0 = __byte_perm(p[0], p[1], 0x5140), a1 = __byte_perm(p[2], p[3], 0x5140),
+                           b0 = __byte_perm(p[0], p[1], 0x0062), b1 = __byte_perm(p[2], p[3], 0x0062);
+            w[D - 1][h] = __byte_perm(a0, a1, 0x5410) ^ 0x80808080u;
+            w[D - 2][h] = __byte_perm(a0, a1, 0x7632) ^ 0x80808080u;
+            w[0][h] = __byte_perm(b0, b1, 0x5410) ^ 0x80808080u;
         }
-        if (l == 0) o.scales[(size_t)t * chunks + c] = odd ? CUDART_NAN_F : __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+        for (int d = 0; d < D; ++d) sum[d] = __dp4a((int)w[d][0], 0x01010101, __dp4a((int)w[d][1], 0x01010101, 0));
+        scale = odd ? CUDART_NAN_F : __uint_as_float((uint32_t)(127 - e) << 23);
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) {
         *reinterpret_cast<uint2*>(o.d + d * o.plane + t * o.row + c * kChunk + (b >> 1) * 64 + q * 16 + (b & 1) * 8) = make_uint2(w[d][0], w[d][1]);
 #pragma unroll
         for (int s = 1; s < 4 * FB; s <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], s);
-        if (l % (4 * FB) == 0) o.sums[((size_t)t * chunks * (4 / FB) + c * (4 / FB) + b / FB) * D + d] = sum[d];
+    }
+    if (l % (4 * FB) == 0) {
+        unsigned char* r = o.records + ((size_t)(c * (4 / FB) + b / FB) * even(x.tokens) + t) * (D == 3 ? 16 : 8);
+        if constexpr (D == 3)
+            *reinterpret_cast<int4*>(r) = make_int4(sum[0], sum[1], sum[D - 1], __float_as_int(scale));
+        else
+            *reinterpret_cast<int2*>(r) = make_int2(sum[0], __float_as_int(scale));
     }
 }
 
 template <int D, int FB>
 __global__ void __launch_bounds__(256) w4_digits_kernel(W4X x, int chunks, unsigned char* out) {
     asm volatile("griddepcontrol.launch_dependents;");
-    const Digits o = digits_at(out, D, x.tokens, chunks, FB);
+    const Digits o = digits_at(out, D, x.tokens, chunks);
     // half a warp per 128 inputs of a token; whole warps stay in step
     const int n = (int)x.tokens * chunks;
     for (int i = (blockIdx.x * 256 + threadIdx.x) >> 4; (i & ~1) < n; i += gridDim.x * 16) {
         const int j = min(i, n - 1);
-        make_digits<D, FB>(x, o, chunks, j / chunks, j % chunks);
+        make_digits<D, FB>(x, o, j / chunks, j % chunks);
     }
 }
 
@@ -188,11 +209,9 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* codes, cons
 struct StreamArgs {
     W4View w;
     W4X x;
-    unsigned char* digits;   // in the workspace; null: made in shared memory
-    const float* x_scales;   // a factor per token and 2^x_shift inputs, `x_pitch` a token (D = 3: the digits' own)
-    int x_pitch, x_shift;
+    unsigned char* digits;   // in the workspace (WS), else made in shared memory
     void* y;
-    int y_bf16, ks, tiles;   // ks warps share a row of tiles; `tiles` groups of kWarps / ks of them
+    int y_bf16, ks, tiles;   // 2^ks warps share a row of tiles; `tiles` groups of kWarps / 2^ks of them
     int digits_at, sums_at;  // in shared memory, behind the ring: the digits (bytes), the warps' partial sums (floats)
 };
 
@@ -209,22 +228,22 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
 // what it reads itself, so a stage needs no barrier, only its own lane's copies to have landed.
 template <int MT, int PC>
 struct Stage4 {
-    static constexpr int kStages = MT == 1 ? 6 : 4;
+    static constexpr int kStages = MT == 1 ? (PC == 4 ? 4 : 5) : (PC == 4 ? 2 : 3);  // beside 60 KB of digits
     static constexpr int kZero = PC == 4 ? 8 : 4;  // bytes of zero points of a lane and tile (4 for PC 1: padded)
     static constexpr int kScaleAt = MT * 1024, kZeroAt = kScaleAt + MT * 32 * 4 * PC;
     static constexpr int kBytes = kZeroAt + MT * 32 * kZero;
 };
 
 // A warp: MT x 16 rows x NT x 8 tokens over its part of the inputs. D digits an activation; PC scales of a row in
-// 128 inputs; FB: blocks of 32 inputs after which a sum meets its scales; XS: activations' scales at each flush.
-template <int MT, int NT, int D, int PC, int FB, bool XS>
-__global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a) {
+// 128 inputs; FB: blocks of 32 inputs after which a sum meets its scales; WS: the digits are in the workspace.
+template <int MT, int NT, int D, int PC, int FB, bool WS>
+__global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a) {
     using S = Stage4<MT, PC>;
     extern __shared__ __align__(16) unsigned char s_mem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    const int per = kWarps / a.ks, sub = warp % a.ks;
+    const int per = kWarps >> a.ks, sub = warp & ((1 << a.ks) - 1);
     const int chunks = (int)a.w.chunks, T = (int)a.x.tokens, rows = (int)(a.w.tile_rows / MT);
-    const int c0 = (int)((long long)chunks * sub / a.ks), c1 = (int)((long long)chunks * (sub + 1) / a.ks);
+    const int c0 = chunks * sub >> a.ks, c1 = chunks * (sub + 1) >> a.ks;
     const bool zeros = a.w.zeros != nullptr;
     unsigned char* ring = s_mem + warp * S::kStages * S::kBytes;
 
@@ -232,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
     int p_tile = blockIdx.x, p_left = 0;
     const unsigned char *p_code = nullptr, *p_scale = nullptr, *p_zero = nullptr;
     auto p_start = [&]() {  // the pointers of the producer's next row of tiles, if there is one
-        const int tr = p_tile * per + warp / a.ks;
+        const int tr = p_tile * per + (warp >> a.ks);
         if (p_tile >= a.tiles || tr >= rows) return;
         const size_t at = ((size_t)(tr * MT >> 3) * chunks + c0) * 8 + (tr * MT & 7);
         p_code = reinterpret_cast<const unsigned char*>(a.w.codes) + at * 1024 + lane * 16;
@@ -262,33 +281,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
     // The weights do not depend on the kernel before, the activations may.
     for (int i = 0; i < S::kStages - 1; ++i) produce();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Digits x = digits_at(a.digits ? a.digits : s_mem + a.digits_at, D, T, chunks, FB);
-    if (!a.digits) {
+    const Digits x = digits_at(WS ? a.digits : s_mem + a.digits_at, D, T, chunks);
+    if constexpr (!WS) {
         const int n = T * chunks;
+#pragma unroll 2
         for (int i = threadIdx.x >> 4; (i & ~1) < n; i += kWarps * 2) {
-            const int j = min(i, n - 1);
-            make_digits<D, FB>(a.x, x, chunks, j / chunks, j % chunks);
+            const int j = min(i, n - 1), t = T == 1 ? 0 : j / chunks;
+            make_digits<D, FB>(a.x, x, t, j - t * chunks);
         }
         __syncthreads();
     }
-    constexpr int FL = 4 / FB;  // flushes of 128 inputs
-    const unsigned char* xr[NT];  // a lane without a token repeats the last one's row: its sums are not stored
-    const int* xq[NT][2];         // the digits' sums of tokens 8 n + 2 q, + 1, and their scales
-    const float* xs[NT][2];
+    constexpr int FL = 4 / FB, R = D == 3 ? 16 : 8;  // flushes of 128 inputs, bytes of a record
+    // a lane without a token repeats the last one's row: its sums are not stored
+    const unsigned char *xr[NT], *xq[NT];
+    const size_t step = even(T) * R;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        xr[n] = x.d + (size_t)min(8 * n + g, T - 1) * x.row + 16 * q;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const size_t t = min(8 * n + 2 * q + e, T - 1);
-            xq[n][e] = x.sums + t * chunks * FL * D;
-            xs[n][e] = D == 3 ? x.scales + t * chunks : a.x_scales + t * a.x_pitch;
-        }
+        xr[n] = x.d + (size_t)min(8 * n + g, T - 1) * x.row + 16 * q + c0 * kChunk;
+        xq[n] = x.records + min(8 * n + 2 * q, (int)even(T) - 2) * R + c0 * FL * step;
     }
 
     const unsigned char* st = ring;
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        const int tr = tile * per + warp / a.ks;
+        const int tr = tile * per + (warp >> a.ks);
         const bool has = tr < rows;
         float acc[MT][NT][4];
 #pragma unroll
@@ -311,22 +326,36 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
                                      : 0x08080808u;
             }
             st = st == ring + (S::kStages - 1) * S::kBytes ? ring : st + S::kBytes;
+            const size_t at = (size_t)(c - c0);
+            // 8 bytes for each of two blocks of 32 inputs
+            uint4 xf[NT][D];
 #pragma unroll
             for (int f = 0; f < FL; ++f) {
                 const int blk = f * FB * PC / 4;  // scale block of the chunk
                 int d[MT][NT][D][4];
+                float xs[NT][2];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const uint32_t z2 = zz[m][blk / 2] >> (16 * (blk & 1));
-                    const int z0 = -(int)(z2 & 0xffu), z1 = -(int)((z2 >> 8) & 0xffu);
+                for (int n = 0; n < NT; ++n) {
+                    int sums[2][D];  // of the digits of tokens 8 n + 2 q, + 1
+                    const int4 r = *reinterpret_cast<const int4*>(xq[n] + (at * FL + f) * step);
+                    if constexpr (D == 3) {
+                        const int4 r1 = *reinterpret_cast<const int4*>(xq[n] + (at * FL + f) * step + 16);
+                        sums[0][0] = r.x, sums[0][1] = r.y, sums[0][D - 1] = r.z, xs[n][0] = __int_as_float(r.w);
+                        sums[1][0] = r1.x, sums[1][1] = r1.y, sums[1][D - 1] = r1.z, xs[n][1] = __int_as_float(r1.w);
+                    } else {
+                        sums[0][0] = r.x, xs[n][0] = __int_as_float(r.y);
+                        sums[1][0] = r.z, xs[n][1] = __int_as_float(r.w);
+                    }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int m = 0; m < MT; ++m) {
+                        const uint32_t z2 = zz[m][blk / 2] >> (16 * (blk & 1));
+                        const int z0 = -(int)(z2 & 0xffu), z1 = -(int)((z2 >> 8) & 0xffu);
 #pragma unroll
                         for (int i = 0; i < D; ++i) {
-                            const int q0 = xq[n][0][(c * FL + f) * D + i], q1 = xq[n][1][(c * FL + f) * D + i];
-                            d[m][n][i][0] = z0 * q0 + kMagicBits, d[m][n][i][1] = z0 * q1 + kMagicBits;
-                            d[m][n][i][2] = z1 * q0 + kMagicBits, d[m][n][i][3] = z1 * q1 + kMagicBits;
+                            d[m][n][i][0] = z0 * sums[0][i] + kMagicBits, d[m][n][i][1] = z0 * sums[1][i] + kMagicBits;
+                            d[m][n][i][2] = z1 * sums[0][i] + kMagicBits, d[m][n][i][3] = z1 * sums[1][i] + kMagicBits;
                         }
+                    }
                 }
 #pragma unroll
                 for (int b = f * FB; b < (f + 1) * FB; ++b) {
@@ -342,36 +371,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < D; ++i) {
-                            const uint2 xf = *reinterpret_cast<const uint2*>(xr[n] + i * x.plane + c * kChunk + (b >> 1) * 64 + (b & 1) * 8);
+                            if (b % 2 == 0)
+                                xf[n][i] = *reinterpret_cast<const uint4*>(xr[n] + i * x.plane + at * kChunk + (b >> 1) * 64);
 #pragma unroll
-                            for (int m = 0; m < MT; ++m) mma_u8s8(d[m][n][i], fr[m], xf.x, xf.y);
+                            for (int m = 0; m < MT; ++m)
+                                mma_u8s8(d[m][n][i], fr[m], b % 2 ? xf[n][i].z : xf[n][i].x, b % 2 ? xf[n][i].w : xf[n][i].y);
                         }
                 }
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float x0 = 1.f, x1 = 1.f;
-                    if constexpr (XS) {
-                        // padded inputs: the weights' scale is 0
-                        const int at = D == 3 ? c : min((c * kChunk + 32 * FB * f) >> a.x_shift, a.x_pitch - 1);
-                        x0 = xs[n][0][at], x1 = xs[n][1][at];
-                    }
+                for (int m = 0; m < MT; ++m) {
+                    const float s0 = scale_of(sc[m][blk] & 0xffffu, a.w.scale_bf16), s1 = scale_of(sc[m][blk] >> 16, a.w.scale_bf16);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const float s0 = scale_of(sc[m][blk] & 0xffffu, a.w.scale_bf16), s1 = scale_of(sc[m][blk] >> 16, a.w.scale_bf16);
-                        float v[4];
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            v[e] = __int_as_float(d[m][n][0][e]) - kMagic;
+                            float v = __int_as_float(d[m][n][0][e]) - kMagic;
 #pragma unroll
-                            for (int i = 1; i < D; ++i) v[e] = fmaf(v[e], 256.f, __int_as_float(d[m][n][i][e]) - kMagic);
-                            if constexpr (XS) v[e] *= e & 1 ? x1 : x0;
-                            acc[m][n][e] = fmaf(v[e], e & 2 ? s1 : s0, acc[m][n][e]);
+                            for (int i = 1; i < D; ++i) v = fmaf(v, 256.f, __int_as_float(d[m][n][i][e]) - kMagic);
+                            acc[m][n][e] = fmaf(v * xs[n][e & 1], e & 2 ? s1 : s0, acc[m][n][e]);
                         }
-                    }
                 }
             }
         }
-        if (a.ks > 1) {  // the warps of a row of tiles: their sums in order, by the first of them
+        if (a.ks > 0) {  // the warps of a row of tiles: their sums in order, by the first of them
             float* mine = reinterpret_cast<float*>(s_mem) + a.sums_at + (size_t)warp * 32 * 4 * NT * MT;
             if (sub) {
 #pragma unroll
@@ -379,7 +401,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
             }
             __syncthreads();
             if (!sub) {
-                for (int j = 1; j < a.ks; ++j)
+                for (int j = 1; j < 1 << a.ks; ++j)
 #pragma unroll
                     for (int i = 0; i < 4 * NT * MT; ++i)
                         acc[i / (4 * NT)][i / 4 % NT][i % 4] += mine[(size_t)j * 32 * 4 * NT * MT + i * 32 + lane];
@@ -393,12 +415,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
                 for (int e = 0; e < 4; ++e) {
                     const size_t t = 8 * n + 2 * q + (e & 1);
                     if (t >= a.x.tokens) continue;
-                    const float factor = XS ? 1.f : a.x_scales[t];
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         const size_t r = ((size_t)tr * MT + m) * 16 + g + 8 * (e >> 1);
                         if (r >= a.w.n_out) continue;
-                        const float v = XS ? acc[m][n][e] : acc[m][n][e] * factor;
+                        const float v = acc[m][n][e];
                         if (a.y_bf16)
                             static_cast<__nv_bfloat16*>(a.y)[t * a.w.n_out + r] = __float2bfloat16_rn(v);
                         else
@@ -410,42 +431,39 @@ __global__ void __launch_bounds__(kWarps * 32, 2) w4_stream_kernel(StreamArgs a)
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Shared memory for the digits, beside the ring: two CTAs an SM.
-constexpr size_t kDigitSmem = 48 * 1024;
+// Shared memory for the digits, beside the ring.
+constexpr size_t kDigitSmem = 60 * 1024;
 
 int flush_blocks(const W4View& w, const W4X& x) {
     const int fb = 4 / w.per_chunk;
-    return x.group ? std::min(fb, x.group / 32) : fb;
+    return x.group && x.group / 32 < fb ? 1 : fb;  // groups of activations smaller than the weights': every 32 inputs
 }
 int digits_of(const W4X& x) { return x.kind == kW4XInt8 ? 1 : 3; }
 
-template <int MT, int NT, int D, int PC, int FB, bool XS>
+template <int MT, int NT, int D, int PC, int FB, bool WS>
 cudaError_t run_stream(StreamArgs& a, int num_sms, cudaStream_t s) {
-    auto kernel = w4_stream_kernel<MT, NT, D, PC, FB, XS>;
-    const size_t ring = (size_t)kWarps * Stage4<MT, PC>::kStages * Stage4<MT, PC>::kBytes;
-    const size_t sums = kWarps * 32 * 4 * NT * MT * sizeof(float);
-    const size_t own = a.digits ? 0 : (digit_bytes(D, a.x.tokens, a.w.chunks, FB) + 15) & ~size_t(15);
-    const int resident = ring + own + sums <= 113 * 1024 ? 2 : 1;
+    auto kernel = w4_stream_kernel<MT, NT, D, PC, FB, WS>;
+    constexpr size_t ring = (size_t)kWarps * Stage4<MT, PC>::kStages * Stage4<MT, PC>::kBytes;
+    constexpr size_t sums = kWarps * 32 * 4 * NT * MT * sizeof(float);
+    static_assert(ring + kDigitSmem + sums <= 227 * 1024, "shared memory");
+    const size_t own = WS ? 0 : (digit_bytes(D, a.x.tokens, a.w.chunks, FB) + 15) & ~size_t(15);
     // Warps that share a row of tiles: the split with the shortest chain of tiles for a warp, where a round
     // costs about as much as 3 tiles (its first loads, its sums joined).
-    const size_t rows = a.w.tile_rows / MT, ctas = (size_t)num_sms * resident;
-    int ks = 1;
+    const size_t rows = a.w.tile_rows / MT;
     size_t best = ~size_t(0);
-    for (int k = 1; k <= kWarps && (size_t)k <= a.w.chunks; k *= 2) {
-        const size_t tiles = (rows + kWarps / k - 1) / (kWarps / k);
-        const size_t cost = (tiles + ctas - 1) / ctas * ((a.w.chunks + k - 1) / k + 3);
-        if (cost < best) best = cost, ks = k;
+    for (int k = 0; 1 << k <= kWarps && (size_t)1 << k <= a.w.chunks; ++k) {
+        const size_t tiles = (rows + (kWarps >> k) - 1) / (kWarps >> k);
+        const size_t cost = (tiles + num_sms - 1) / num_sms * ((a.w.chunks + (1 << k) - 1) / (1 << k) + 3);
+        if (cost < best) best = cost, a.ks = k, a.tiles = (int)tiles;
     }
-    a.ks = ks;
-    a.tiles = (int)((rows + kWarps / ks - 1) / (kWarps / ks));
     a.digits_at = (int)ring;
     a.sums_at = (int)((ring + own) / sizeof(float));
-    const size_t smem = ring + own + (ks > 1 ? sums : 0);
+    const size_t smem = ring + own + (a.ks > 0 ? sums : 0);
     static SmemOnce once;  // the most this kernel is ever given
-    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), (int)(ring + kDigitSmem + 16 + sums));
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), (int)(ring + kDigitSmem + sums));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)std::min(a.tiles, num_sms * resident));
+    cfg.gridDim = dim3((unsigned)std::min(a.tiles, num_sms));
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -453,28 +471,25 @@ cudaError_t run_stream(StreamArgs& a, int num_sms, cudaStream_t s) {
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
-    cfg.numAttrs = a.digits ? 1 : 0;
+    cfg.numAttrs = WS ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
-template <int MT, int NT, int D, bool XS>
+template <int MT, int NT, int D, bool WS>
 cudaError_t run_pc(StreamArgs& a, int num_sms, cudaStream_t s) {
-    const int pc = a.w.per_chunk, fb = flush_blocks(a.w, a.x);
-    if constexpr (D == 1 && XS) {  // groups of activations smaller than the weights'
-        if (fb < 4 / pc)
-            return pc == 2   ? run_stream<MT, NT, D, 2, 1, XS>(a, num_sms, s)
-                   : fb == 2 ? run_stream<MT, NT, D, 1, 2, XS>(a, num_sms, s)
-                             : run_stream<MT, NT, D, 1, 1, XS>(a, num_sms, s);
-    }
-    return pc == 1   ? run_stream<MT, NT, D, 1, 4, XS>(a, num_sms, s)
-           : pc == 2 ? run_stream<MT, NT, D, 2, 2, XS>(a, num_sms, s)
-                     : run_stream<MT, NT, D, 4, 1, XS>(a, num_sms, s);
+    const int pc = a.w.per_chunk;
+    if constexpr (D == 1)
+        if (pc < 4 && flush_blocks(a.w, a.x) == 1)
+            return pc == 1 ? run_stream<MT, NT, D, 1, 1, WS>(a, num_sms, s) : run_stream<MT, NT, D, 2, 1, WS>(a, num_sms, s);
+    return pc == 1   ? run_stream<MT, NT, D, 1, 4, WS>(a, num_sms, s)
+           : pc == 2 ? run_stream<MT, NT, D, 2, 2, WS>(a, num_sms, s)
+                     : run_stream<MT, NT, D, 4, 1, WS>(a, num_sms, s);
 }
-template <int D, bool XS>
+template <int D, bool WS>
 cudaError_t run_nt(StreamArgs& a, int num_sms, cudaStream_t s) {
     // Two row tiles a warp share the activations' fragments and the loop's overhead; one tile a warp where
-    // that would leave SMs without a full CTA, and where 16 tokens' accumulators fill the registers.
-    if (a.x.tokens > 8) return D == 1 ? run_pc<2, 2, D, XS>(a, num_sms, s) : run_pc<1, 2, D, XS>(a, num_sms, s);
-    return a.w.tile_rows < (size_t)num_sms * 2 * kWarps ? run_pc<1, 1, D, XS>(a, num_sms, s) : run_pc<2, 1, D, XS>(a, num_sms, s);
+    // that would leave warps without one, and where 16 tokens' three digits fill the registers.
+    if (a.x.tokens > 8) return D == 1 ? run_pc<2, 2, 1, WS>(a, num_sms, s) : run_pc<1, 2, 3, WS>(a, num_sms, s);
+    return a.w.tile_rows < (size_t)num_sms * kWarps ? run_pc<1, 1, D, WS>(a, num_sms, s) : run_pc<2, 1, D, WS>(a, num_sms, s);
 }
 
 template <int D>
@@ -508,16 +523,13 @@ cudaError_t launch_w4_stream(const W4View& w, const W4X& x, void* y, int y_bf16,
     if (x.tokens > kTokens) return cudaErrorInvalidValue;
     StreamArgs a{};
     a.w = w, a.x = x, a.y = y, a.y_bf16 = y_bf16;
-    a.x_scales = x.scales, a.x_pitch = (int)x.n_groups, a.x_shift = x.group_shift;
-    if (w4_stream_workspace(w, x)) {
-        a.digits = static_cast<unsigned char*>(workspace);
-        const cudaError_t e = digits_of(x) == 3 ? run_digits<3>(x, (int)w.chunks, flush_blocks(w, x), a.digits, s)
-                                                : run_digits<1>(x, (int)w.chunks, flush_blocks(w, x), a.digits, s);
-        if (e != cudaSuccess) return e;
-    }
-    return digits_of(x) == 3 ? run_nt<3, true>(a, num_sms, s)
-           : x.group > 0     ? run_nt<1, true>(a, num_sms, s)
-                             : run_nt<1, false>(a, num_sms, s);
+    const bool three = digits_of(x) == 3;
+    if (w4_stream_workspace(w, x) == 0) return three ? run_nt<3, false>(a, num_sms, s) : run_nt<1, false>(a, num_sms, s);
+    a.digits = static_cast<unsigned char*>(workspace);
+    const int fb = flush_blocks(w, x), chunks = (int)w.chunks;
+    const cudaError_t e = three ? run_digits<3>(x, chunks, fb, a.digits, s) : run_digits<1>(x, chunks, fb, a.digits, s);
+    if (e != cudaSuccess) return e;
+    return three ? run_nt<3, true>(a, num_sms, s) : run_nt<1, true>(a, num_sms, s);
 }
 
 }  // namespace bebelm
