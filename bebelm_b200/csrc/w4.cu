@@ -91,38 +91,51 @@ __device__ __forceinline__ bool x_pairs(const W4X& x) {
     return x.stride % 2 == 0 && reinterpret_cast<uintptr_t>(x.x) % to == 0;
 }
 
-// 128 inputs of a token by half a warp: lane (b, q) the 8 of block b that lane q of an MMA gets
-template <int D, int FB>
-__device__ __forceinline__ void make_digits(const W4X& x, const Digits& o, int t, int c) {
-    const int l = threadIdx.x & 15, b = l >> 2, q = l & 3;
-    const int k = c * kChunk + 32 * b + 2 * q;
+// 128 inputs of a token by half a warp: lane (b, q) the 8 of block b that lane q of an MMA gets, inputs 0, 16, 1, 17, 8,
+// 24, 9, 25 from 32 b + 2 q. First the loads (of several chunks at a time), then the rest.
+template <int D>
+struct Eight {
+    float v[D == 1 ? 1 : 8];
+    uint32_t w[2];  // D = 1: the bytes
+    float scale;
+};
+template <int D>
+__device__ __forceinline__ void load_eight(Eight<D>& r, const W4X& x, bool pairs, int t, int c) {
+    const int l = threadIdx.x & 15, k = c * kChunk + 32 * (l >> 2) + 2 * (l & 3);
     const bool in = (size_t)k < x.n_in;  // n_in is a multiple of 32
     const size_t base = (size_t)t * x.stride + k;
-    uint32_t w[D][2];  // bytes: inputs 0, 16, 1, 17 and 8, 24, 9, 25 from k
-    int sum[D];
-    float scale;
     if constexpr (D == 1) {
         constexpr int kAt[8] = {0, 16, 1, 17, 8, 24, 9, 25};
-        w[0][0] = w[0][1] = 0;
+        r.w[0] = r.w[1] = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t v = in ? static_cast<const unsigned char*>(x.x)[base + kAt[i]] : 0u;
-            w[0][i >> 2] |= v << (8 * (i & 3));
+            r.w[i >> 2] |= v << (8 * (i & 3));
         }
         // padded inputs: any scale
         const int at = x.group ? min(k >> x.group_shift, (int)x.n_groups - 1) : 0;
-        scale = x.scales[(size_t)t * x.n_groups + at];
-        sum[0] = __dp4a((int)w[0][0], 0x01010101, __dp4a((int)w[0][1], 0x01010101, 0));
+        r.scale = x.scales[(size_t)t * x.n_groups + at];
     } else {
-        float v[8];
-        const bool pairs = x_pairs(x);
         constexpr int kAt[4] = {0, 16, 8, 24};
-        uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 u = in ? x_pair(x, base + kAt[i], pairs) : make_float2(0.f, 0.f);
-            v[4 * (i >> 1) + (i & 1)] = u.x, v[4 * (i >> 1) + (i & 1) + 2] = u.y;
+            r.v[4 * (i >> 1) + (i & 1)] = u.x, r.v[4 * (i >> 1) + (i & 1) + 2] = u.y;
         }
+    }
+}
+template <int D, int FB>
+__device__ __forceinline__ void make_digits(const Eight<D>& in, const W4X& x, const Digits& o, int t, int c) {
+    const int l = threadIdx.x & 15, b = l >> 2, q = l & 3;
+    uint32_t w[D][2];
+    int sum[D];
+    float scale;
+    if constexpr (D == 1) {
+        w[0][0] = in.w[0], w[0][1] = in.w[1], scale = in.scale;
+        sum[0] = __dp4a((int)w[0][0], 0x01010101, __dp4a((int)w[0][1], 0x01010101, 0));
+    } else {
+        const float* v = in.v;
+        uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);  // an infinity or a NaN is the largest
 #pragma unroll
@@ -169,9 +182,12 @@ __global__ void __launch_bounds__(256) w4_digits_kernel(W4X x, int chunks, unsig
     const Digits o = digits_at(out, D, x.tokens, chunks);
     // half a warp per 128 inputs of a token; whole warps stay in step
     const int n = (int)x.tokens * chunks;
+    const bool pairs = x_pairs(x);
     for (int i = (blockIdx.x * 256 + threadIdx.x) >> 4; (i & ~1) < n; i += gridDim.x * 16) {
         const int j = min(i, n - 1);
-        make_digits<D, FB>(x, o, j / chunks, j % chunks);
+        Eight<D> e;
+        load_eight(e, x, pairs, j / chunks, j % chunks);
+        make_digits<D, FB>(e, x, o, j / chunks, j % chunks);
     }
 }
 
@@ -284,10 +300,20 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a)
     const Digits x = digits_at(WS ? a.digits : s_mem + a.digits_at, D, T, chunks);
     if constexpr (!WS) {
         const int n = T * chunks;
-#pragma unroll 2
-        for (int i = threadIdx.x >> 4; (i & ~1) < n; i += kWarps * 2) {
-            const int j = min(i, n - 1), t = T == 1 ? 0 : j / chunks;
-            make_digits<D, FB>(a.x, x, t, j - t * chunks);
+        const bool pairs = x_pairs(a.x);
+        constexpr int kU = 4;  // chunks of a half warp whose loads are under way together
+        for (int i = threadIdx.x >> 4; (i & ~1) < n; i += kWarps * 2 * kU) {
+            Eight<D> e[kU];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int j = min(i + u * kWarps * 2, n - 1), t = T == 1 ? 0 : j / chunks;
+                if (((i + u * kWarps * 2) & ~1) < n) load_eight(e[u], a.x, pairs, t, j - t * chunks);
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int j = min(i + u * kWarps * 2, n - 1), t = T == 1 ? 0 : j / chunks;
+                if (((i + u * kWarps * 2) & ~1) < n) make_digits<D, FB>(e[u], a.x, x, t, j - t * chunks);
+            }
         }
         __syncthreads();
     }
@@ -487,9 +513,9 @@ cudaError_t run_pc(StreamArgs& a, int num_sms, cudaStream_t s) {
 template <int D, bool WS>
 cudaError_t run_nt(StreamArgs& a, int num_sms, cudaStream_t s) {
     // Two row tiles a warp share the activations' fragments and the loop's overhead; one tile a warp where
-    // that would leave warps without one, and where 16 tokens' three digits fill the registers.
+    // that would leave a warp fewer than 4 pairs, and where 16 tokens' three digits fill the registers.
     if (a.x.tokens > 8) return D == 1 ? run_pc<2, 2, 1, WS>(a, num_sms, s) : run_pc<1, 2, 3, WS>(a, num_sms, s);
-    return a.w.tile_rows < (size_t)num_sms * kWarps ? run_pc<1, 1, D, WS>(a, num_sms, s) : run_pc<2, 1, D, WS>(a, num_sms, s);
+    return a.w.tile_rows * a.w.chunks < (size_t)num_sms * kWarps * 8 ? run_pc<1, 1, D, WS>(a, num_sms, s) : run_pc<2, 1, D, WS>(a, num_sms, s);
 }
 
 template <int D>
