@@ -15,6 +15,7 @@
 #include <thread>
 #include <unordered_map>
 #include <initializer_list>
+#include <memory>
 #include <vector>
 
 #include <unistd.h>
@@ -2636,7 +2637,7 @@ int bebelm_add_rmsnorm(const void* x, size_t x_stride, const void* residual, siz
     a.bf16 = dtype == BEBELM_BF16;
     a.out = y_dtype == BEBELM_F32 ? kNormOutF32 : y_dtype == BEBELM_BF16 ? kNormOutBf16 : kNormOutInt8;
     if (mem == BEBELM_MEM_DEVICE) {
-        CUDA_TRY(launch_add_rmsnorm(a, s));
+        CUDA_TRY(launch_add_rmsnorm(a, num_sms_of(dev), s));
         return 0;
     }
     std::lock_guard<std::mutex> lk(g_scratch_mu);
@@ -2654,12 +2655,13 @@ int bebelm_add_rmsnorm(const void* x, size_t x_stride, const void* residual, siz
     a.y = d;
     a.sum_out = sum_out ? d + pad256(yb) : nullptr;
     a.y_scales = reinterpret_cast<float*>(d + pad256(yb) + pad256(hb));
-    CUDA_TRY(launch_add_rmsnorm(a, s));
-    std::vector<char> back(out_bytes);
-    TRY(stage_out(P, o, back.data(), out_bytes, s));
-    std::memcpy(y, back.data(), yb);
-    if (hb) std::memcpy(sum_out, back.data() + pad256(yb), hb);
-    if (sb) std::memcpy(y_scales, back.data() + pad256(yb) + pad256(hb), sb);
+    CUDA_TRY(launch_add_rmsnorm(a, num_sms_of(dev), s));
+    const std::unique_ptr<char[]> back(new (std::nothrow) char[out_bytes]);
+    if (!back) return fail(BEBELM_ERR_OOM, "out of host memory");
+    TRY(stage_out(P, o, back.get(), out_bytes, s));
+    std::memcpy(y, back.get(), yb);
+    if (hb) std::memcpy(sum_out, back.get() + pad256(yb), hb);
+    if (sb) std::memcpy(y_scales, back.get() + pad256(yb) + pad256(hb), sb);
     return 0;
 }
 
@@ -2942,10 +2944,12 @@ int bebelm_verify_drafts(const float* target, size_t target_stride, const float*
     a.accepted = reinterpret_cast<int*>(static_cast<char*>(o) + pad256(ob));
     a.workspace = P->q8.p;
     CUDA_TRY(launch_verify(a, sms, s));
-    std::vector<char> back(pad256(ob) + 4 * n_seqs);
-    TRY(stage_out(P, o, back.data(), back.size(), s));
-    std::memcpy(out_tokens, back.data(), ob);
-    std::memcpy(accepted, back.data() + pad256(ob), 4 * n_seqs);
+    const size_t bb = pad256(ob) + 4 * n_seqs;
+    const std::unique_ptr<char[]> back(new (std::nothrow) char[bb]);
+    if (!back) return fail(BEBELM_ERR_OOM, "out of host memory");
+    TRY(stage_out(P, o, back.get(), bb, s));
+    std::memcpy(out_tokens, back.get(), ob);
+    std::memcpy(accepted, back.get() + pad256(ob), 4 * n_seqs);
     return 0;
 }
 

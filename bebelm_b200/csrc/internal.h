@@ -337,7 +337,7 @@ struct AddNormArgs {
     float eps;
     int bf16, out;
 };
-cudaError_t launch_add_rmsnorm(const AddNormArgs& a, cudaStream_t s);
+cudaError_t launch_add_rmsnorm(const AddNormArgs& a, int num_sms, cudaStream_t s);
 
 // A kernel's dynamic shared memory limit, set once per device (the call costs about a microsecond). Two
 // threads may both set it, to the same value.

@@ -73,6 +73,21 @@ def test_float_outputs(rows, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n", [(700, 2048), (610, 2049), (1200, 1032), (80, 16392), (170, 8192), (1300, 1024)])
+def test_rows_that_fill_the_device(rows, n, dtype):
+    x, r, gain = inputs(rows, n, dtype, rows + n)
+    for od in (bb.F32, bb.BF16):
+        check(x, r, gain, *bb.add_rmsnorm(x, gain, r, out_dtype=od))
+    for group in (0, 64):
+        if group and n % group:
+            continue
+        q, sc, h = bb.add_rmsnorm(x, gain, r, out_dtype=bb.INT8, group=group)
+        want, want_sc = codes_of(steps(h.float().cpu().numpy(), gain.cpu().numpy()), group)
+        np.testing.assert_array_equal(q.cpu().numpy(), want)
+        np.testing.assert_array_equal(sc.cpu().numpy().reshape(want_sc.shape), want_sc)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("group", [0, 32, 64, 128, 256])
 @pytest.mark.parametrize("rows,n", [(1, 256), (1, 2048), (9, 512), (5, 1280), (3, 8192), (2, 8448), (1, 32768), (130, 768)])
 def test_codes_are_the_definitions(rows, n, group, dtype):
