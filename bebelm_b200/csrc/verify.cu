@@ -178,17 +178,20 @@ __device__ __forceinline__ double exp2_neg(double y) { return y < -1000.0 ? 0.0 
 
 // the slices of one row joined by a warp (every lane gets the answer); scale = log2(e) / temperature
 __device__ __forceinline__ RowPart join_row(const RowPart* parts, int slices, double scale, bool greedy) {
+    static_assert(kMaxSlices <= 64, "a lane holds two slices");
     const int lane = threadIdx.x & 31;
-    RowPart r{-CUDART_INF_F, 0xffffffffu, 0.0};
-    for (int i = lane; i < slices; i += 32) r.m = fmaxf(r.m, parts[i].m);
+    RowPart p[2], r{-CUDART_INF_F, 0xffffffffu, 0.0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) p[i] = lane + 32 * i < slices ? parts[lane + 32 * i] : r;
+    r.m = fmaxf(p[0].m, p[1].m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) r.m = fmaxf(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
-    for (int i = lane; i < slices; i += 32) {
-        const RowPart p = parts[i];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
         if (greedy) {
-            if (p.m == r.m) r.i = min(r.i, p.i);
-        } else if (p.s > 0.0) {
-            r.s += p.s * exp2_neg(((double)p.m - (double)r.m) * scale);
+            if (p[i].m == r.m) r.i = min(r.i, p[i].i);
+        } else if (p[i].s > 0.0) {
+            r.s += p[i].s * exp2_neg(((double)p[i].m - (double)r.m) * scale);
         }
     }
     if (greedy) {
@@ -247,9 +250,12 @@ struct Row {
         return l > lim ? w : 0.0;
     }
 };
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // 4 entries from j (a multiple of 4); those at and past `end` count as nothing
 template <bool VEC, bool PROBS>
-__device__ __forceinline__ void entries4(const Row<PROBS>& r, size_t j, size_t end, float* v) {
+__device__ __forceinline__ void entries4(const Row<PROBS>& r, unsigned j, unsigned end, float* v) {
     if (VEC && j + 4 <= end) {
         const float4 t = __ldg(reinterpret_cast<const float4*>(r.p + j));
         v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
@@ -259,31 +265,58 @@ __device__ __forceinline__ void entries4(const Row<PROBS>& r, size_t j, size_t e
     }
 }
 
-// PT threads; 64 registers each, so that an SM holds 1024 of them however they are split
+__device__ __forceinline__ double warp_total(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ double warp_running(double v) {  // lane i: the sum of lanes 0 .. i
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += u;
+    }
+    return v;
+}
+
+// PT threads; 64 registers each, so that an SM holds 1024 of them however they are split.
+//
+// The part of a CTA is cut into blocks, a block into one cell of neighbouring entries a warp; the pass leaves every
+// cell's sums, so the border is found by going from the CTA to the block to the cell to the entry, and only the last
+// step computes weights again, 128 of them by one warp. What has one answer a CTA (the rows' factors, the joining of
+// the CTAs' sums, the search) is done by one warp: with f64 divisions and logarithms in all 1024 threads those parts
+// took 15000 of 37000 cycles of a sequence.
 template <int PT, bool VEC, bool PROBS>
 __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a, const RowPart* parts, int slices) {
     cg::cluster_group cl = cg::this_cluster();
+    cluster_arrive();  // the others have started before their memory is written
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), b = blockIdx.x / ctas;
-    constexpr int kBlocks = 64;  // a part's steps whose sums are kept, so that the border's block is gone through alone
-    __shared__ double s_part[PT / 32][4], s_sum[2][4], s_all[16][4], s_block[kBlocks][PT / 32][2];
-    __shared__ double s_prob[2][33], s_m[2][33], s_s[2][33];  // p_i(x_i), q_i(x_i); the rows' maxima and sums
-    const int n = drafts_of(a, b), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = PT / 32;
+    constexpr int kBlocks = 64, kMaxCtas = 16, kWarps = PT / 32;
+    constexpr unsigned kStep = 4 * PT;
+    __shared__ double s_part[kWarps][4], s_all[2][kMaxCtas][4], s_cell[kBlocks][kWarps][2], s_block[kBlocks];
+    __shared__ double s_prob[2][33];  // p_i(x_i), q_i(x_i)
+    __shared__ Row<PROBS> s_row[2][33];
+    __shared__ double s_before, s_border, s_fp, s_fq;
+    __shared__ int s_owner;
+    const int n = drafts_of(a, b), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int* tok = a.tokens + (size_t)b * a.drafts;
     const double scale = 1.4426950408889634074 / (double)a.temperature;
     const RowPart* tp = parts + (size_t)b * (a.drafts + 1) * slices;
     const RowPart* dp = parts + ((size_t)a.seqs * (a.drafts + 1) + (size_t)b * a.drafts) * slices;
     const float* trow = a.target + (size_t)b * (a.drafts + 1) * a.target_stride;
     const float* drow = a.draft ? a.draft + (size_t)b * a.drafts * a.draft_stride : nullptr;
+    const float u_sample = a.u_sample[b];
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // ---- the decisions, in groups of 32 drafts (every CTA makes them for itself) ----
     int n_acc = 0, base = 0;
     for (;;) {
         const int cnt = min(32, n - base);
-        // p and q of each draft, and the maximum and sum of the row behind the group: a warp each, or a
+        const double u = lane < cnt ? (double)a.u[(size_t)b * a.drafts + base + lane] : 0.0;
+        // p and q of each draft, and the factors of its rows and of the row behind the group: a warp each, or a
         // thread each where rows were cut into few slices
         const bool alone = slices <= 4;
-        const int per = alone ? PT : warps;
+        const int per = alone ? PT : kWarps;
         for (int k = alone ? (int)threadIdx.x : warp; k <= 2 * cnt; k += per) {
             const int at = k >> 1, i = base + at, side = k & 1, x = at < cnt ? tok[i] : -1;
             double v = side ? 1.0 : 0.0;
@@ -297,13 +330,13 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
                     const RowPart* rp = (side ? dp : tp) + (size_t)i * slices;
                     const RowPart r = alone ? join_row_alone(rp, slices, scale) : join_row(rp, slices, scale, false);
                     if (in) v = r.s > 0.0 ? exp2_neg(((double)clean(l) - (double)r.m) * scale) / r.s : 0.0;
-                    if (alone || lane == 0) s_m[side][at] = r.m, s_s[side][at] = r.s;
+                    if (alone || lane == 0) s_row[side][at].logits(r.m, r.s, scale);
                 }
             }
             if (alone || lane == 0) s_prob[side][at] = v;
         }
         __syncthreads();
-        const bool yes = lane < cnt && (double)a.u[(size_t)b * a.drafts + base + lane] * s_prob[1][lane] < s_prob[0][lane];
+        const bool yes = lane < cnt && u * s_prob[1][lane] < s_prob[0][lane];
         const int run = __ffs((int)~__ballot_sync(0xffffffffu, yes)) - 1;  // drafts accepted; -1: all 32
         const int got = run < 0 ? 32 : run;
         n_acc = base + got;
@@ -316,15 +349,16 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     const bool refused = n_acc < n;
     const bool with_q = refused && drow;
     const int skip = refused && !drow ? tok[n_acc] : -1;  // a certain draft takes its own place away
-    Row<PROBS> P{trow + (size_t)n_acc * a.target_stride, 0.0, 0.0, 0.f};
-    Row<PROBS> Q{with_q ? drow + (size_t)n_acc * a.draft_stride : P.p, 0.0, 0.0, 0.f};
+    Row<PROBS> P{}, Q{};
     if constexpr (!PROBS) {  // normalised by the sums of the first pass
-        P.logits(s_m[0][n_acc - base], s_s[0][n_acc - base], scale);
-        if (with_q) Q.logits(s_m[1][n_acc - base], s_s[1][n_acc - base], scale);
+        P = s_row[0][n_acc - base];
+        if (with_q) Q = s_row[1][n_acc - base];
     }
-    // this CTA's part of the row, whole groups of 4; a thread takes 4 and the next 4 after all others'
-    const size_t quads = (a.vocab + 3) / 4, j0 = 4 * (quads * me / ctas), j1 = min(a.vocab, 4 * (quads * (me + 1) / ctas));
-    constexpr size_t kStep = 4 * PT;
+    P.p = trow + (size_t)n_acc * a.target_stride;
+    Q.p = with_q ? drow + (size_t)n_acc * a.draft_stride : P.p;
+    // this CTA's part of the row, whole groups of 4
+    const size_t quads = (a.vocab + 3) / 4;
+    const unsigned j0 = (unsigned)(4 * (quads * me / ctas)), j1 = (unsigned)min(a.vocab, 4 * (quads * (me + 1) / ctas));
 
     // The row is gone through once for all sums. p and q are normalised by the first pass's f32-grade sums, which
     // decides p > q as well as exact ones (it differs only where p - q is 1e-7 of p, and weighs as little); with the
@@ -332,12 +366,12 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     // Probabilities in hand are differences at once: A.
     const bool ratio = with_q && !PROBS;
     // of the entries j .. j + 3: their shares of Sp, Sq, A, B
-    auto add4 = [&](auto use_q, size_t j, bool plain, double* sums) {
+    auto add4 = [&](auto use_q, unsigned j, bool plain, double* sums) {
         constexpr bool kQ = decltype(use_q)::value;
         float x[4], y[4];
         entries4<VEC>(P, j, j1, x);
         if constexpr (kQ) entries4<VEC>(Q, j, j1, y);
-        const int sk = !plain && skip >= 0 && (size_t)skip - j < 4 ? skip - (int)j : -1;
+        const int sk = !plain && skip >= 0 && (unsigned)skip - j < 4 ? skip - (int)j : -1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const double p = P.weigh(x[i]);
@@ -354,152 +388,146 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
             }
         }
     };
-    // their weights, normalised by fp = 1 / Sp and fq = 1 / Sq
-    auto weights4 = [&](size_t j, bool plain, double fp, double fq, double* w) {
-        float x[4], y[4];
-        const bool q = with_q && !plain;
-        entries4<VEC>(P, j, j1, x);
-        if (q) entries4<VEC>(Q, j, j1, y);
-        const int sk = !plain && skip >= 0 && (size_t)skip - j < 4 ? skip - (int)j : -1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = P.weigh(x[i]);
-            if (q) {
-                const double v = Q.weigh(y[i]);
-                w[i] = w[i] > v ? fmax(fma(w[i], fp, -(v * fq)), 0.0) : 0.0;
-            }
-            if (i == sk) w[i] = 0.0;
-        }
-    };
     const int steps = (int)((j1 - j0 + kStep - 1) / kStep);
     int shift = 0;  // steps of a block
     while (steps >> shift >= kBlocks) ++shift;
+    const int blocks = (steps + (1 << shift) - 1) >> shift;
+    const unsigned cell = 128u << shift, block_entries = cell * kWarps;
     bool plain = !refused;
-    double before = 0.0, border, fp = 1.0, fq = 1.0;
-    int owner;
+    cluster_wait();
     for (int slot = 0;; ++slot) {  // a second time only where p - q is zero everywhere
-        double sums[4] = {0.0, 0.0, 0.0, 0.0}, seen[2] = {0.0, 0.0};
+        double sums[4] = {0.0, 0.0, 0.0, 0.0}, all_a = 0.0, all_b = 0.0;
         auto go = [&](auto use_q) {
-            for (int t = 0; t < steps; ++t) {
-                const size_t j = j0 + t * kStep + 4 * threadIdx.x;
-                if (j < j1) add4(use_q, j, plain, sums);
-                if ((t + 1) >> shift == t >> shift && t + 1 < steps) continue;
-                double u = sums[2] - seen[0], v = sums[3] - seen[1];  // the block's end
-                seen[0] = sums[2], seen[1] = sums[3];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    u += __shfl_xor_sync(0xffffffffu, u, o);
-                    if (use_q.value && !PROBS) v += __shfl_xor_sync(0xffffffffu, v, o);
-                }
-                if (lane == 0) s_block[t >> shift][warp][0] = u, s_block[t >> shift][warp][1] = v;
+            constexpr bool kRatio = decltype(use_q)::value && !PROBS;
+            for (int t = 0; t < blocks; ++t) {
+                const unsigned c0 = j0 + t * block_entries + warp * cell + 4 * lane;
+                for (int r = 0; r < 1 << shift; ++r)
+                    if (c0 + 128 * r < j1) add4(use_q, c0 + 128 * r, plain, sums);
+                const double u = warp_total(sums[2]);
+                double v = 0.0;
+                if constexpr (kRatio) v = warp_total(sums[3]);
+                sums[2] = sums[3] = 0.0;
+                all_a += u, all_b += v;
+                if (lane == 0) s_cell[t][warp][0] = u, s_cell[t][warp][1] = v;
             }
+            if constexpr (kRatio) sums[0] = warp_total(sums[0]), sums[1] = warp_total(sums[1]);
         };
         if (with_q && !plain)
             go(std::true_type{});
         else
             go(std::false_type{});
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            double v = sums[k];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) s_part[warp][k] = v;
-        }
+        if (lane == 0) s_part[warp][0] = sums[0], s_part[warp][1] = sums[1], s_part[warp][2] = all_a, s_part[warp][3] = all_b;
         __syncthreads();
-        if (threadIdx.x < 4) {
-            double v = 0.0;
-            for (int w = 0; w < warps; ++w) v += s_part[w][threadIdx.x];
-            s_sum[slot][threadIdx.x] = v;
+        if (warp < 4) {  // a warp per sum, into every CTA's memory
+            const double v = warp_total(lane < kWarps ? s_part[lane][warp] : 0.0);
+            if (lane < ctas) *cl.map_shared_rank(&s_all[slot][me][warp], lane) = v;
         }
         cl.sync();
-        // a warp per sum reads the other CTAs' (every warp reading them took 8000 cycles)
-        if (warp < 4 && lane < ctas) s_all[lane][warp] = *cl.map_shared_rank(&s_sum[slot][warp], lane);
+        if (warp == 0) {
+            const bool in = lane < ctas;
+            const double* c = s_all[slot][in ? lane : 0];
+            double fp = 1.0, fq = 1.0, own = in ? c[2] : 0.0;
+            if (ratio && !plain) {
+                const double sp = warp_total(in ? c[0] : 0.0), sq = warp_total(in ? c[1] : 0.0);
+                fp = sp > 0.0 ? 1.0 / sp : 0.0, fq = sq > 0.0 ? 1.0 / sq : 0.0;
+                own = in ? fmax(fma(c[2], fp, -(c[3] * fq)), 0.0) : 0.0;
+            }
+            const double run = warp_running(own), total = __shfl_sync(0xffffffffu, run, 31);
+            // The first CTA whose sum passes the border, or, if rounding leaves none, the last with any weight.
+            const double border = (double)u_sample * total;
+            const unsigned any = __ballot_sync(0xffffffffu, own > 0.0), over = __ballot_sync(0xffffffffu, own > 0.0 && run > border);
+            const double before = __shfl_up_sync(0xffffffffu, run, 1);
+            if (lane == me) s_before = me ? before : 0.0;
+            if (lane == 0) {
+                s_border = border, s_fp = fp, s_fq = fq;
+                s_owner = over ? __ffs((int)over) - 1 : any ? 31 - __clz((int)any) : -1;
+            }
+        }
         __syncthreads();
-        if (ratio && !plain) {
-            double sp = 0.0, sq = 0.0;
-            for (int c = 0; c < ctas; ++c) sp += s_all[c][0], sq += s_all[c][1];
-            fp = sp > 0.0 ? 1.0 / sp : 0.0, fq = sq > 0.0 ? 1.0 / sq : 0.0;
-        } else {
-            fp = fq = 1.0;
-        }
-        const double own = lane >= ctas ? 0.0 : ratio && !plain ? fmax(fma(s_all[lane][2], fp, -(s_all[lane][3] * fq)), 0.0) : s_all[lane][2];
-        double run = own;
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            const double u = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += u;
-        }
-        const double total = __shfl_sync(0xffffffffu, run, 15);
-        if (!(total > 0.0) && !plain) {
-            plain = true;
-            continue;
-        }
-        // The first CTA whose sum passes the border, or, if rounding leaves none, the last with any weight.
-        border = (double)a.u_sample[b] * total;
-        const unsigned any = __ballot_sync(0xffffffffu, own > 0.0), over = __ballot_sync(0xffffffffu, own > 0.0 && run > border);
-        owner = over ? __ffs((int)over) - 1 : any ? 31 - __clz((int)any) : -1;
-        if (me) before = __shfl_sync(0xffffffffu, run, me - 1);
-        break;
+        if (s_owner >= 0 || plain) break;
+        plain = true;
+        __syncthreads();
     }
-    cl.sync();  // nobody reads another CTA's memory after this
-    if (owner < 0) {  // a row without any weight
+    if (s_owner < 0) {  // a row without any weight
         if (me == 0 && warp == 0) write_out(a, b, n_acc, 0);
         return;
     }
-    if (me != owner) return;
-    // The first block whose running sum passes the border; from it on, steps of 4 values a thread in order: the
-    // step, the thread, the value.
-    const int blocks = (steps + (1 << shift) - 1) >> shift;
-    double run = before;
-    int block = 0;
-    for (; block + 1 < blocks; ++block) {
-        double u = 0.0, v = 0.0;
-        for (int w = 0; w < warps; ++w) u += s_block[block][w][0], v += s_block[block][w][1];
-        const double w = ratio && !plain ? fmax(fma(u, fp, -(v * fq)), 0.0) : u;
-        if (w > 0.0 && run + w > border) break;
-        run += w;
+    if (me != s_owner) return;
+    const double border = s_border, fp = s_fp, fq = s_fq;
+    const bool diff = ratio && !plain;
+    auto weight = [&](double u, double v) { return diff ? fmax(fma(u, fp, -(v * fq)), 0.0) : u; };
+    // every cell's weight and the weights of the blocks
+    for (int t = warp; t < blocks; t += kWarps) {
+        const double w = lane < kWarps ? weight(s_cell[t][lane][0], s_cell[t][lane][1]) : 0.0;
+        if (lane < kWarps) s_cell[t][lane][0] = w;
+        const double sum = warp_total(w);
+        if (lane == 0) s_block[t] = sum;
     }
-    __shared__ double s_scan[PT / 32];
-    __shared__ int s_place, s_last;
-    if (threadIdx.x == 0) s_place = INT_MAX, s_last = -1;
     __syncthreads();
-    for (size_t t0 = j0 + ((size_t)block << shift) * kStep; t0 < j1; t0 += kStep) {
-        const size_t f = t0 + 4 * threadIdx.x;
+    if (warp) return;
+    // Of 32 weights in order behind `run`: the first whose running sum passes the border, if there is none the last
+    // with any weight, -1 if there is none either; `run` becomes the sum before it (or of all).
+    auto find = [&](double w, double& run, bool& passed) {
+        const double inc = run + warp_running(w);
+        const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && inc > border), any = __ballot_sync(0xffffffffu, w > 0.0);
+        passed = over != 0;
+        const int at = over ? __ffs((int)over) - 1 : any ? 31 - __clz((int)any) : -1;
+        const double prev = __shfl_up_sync(0xffffffffu, inc, 1);
+        run = over ? (at ? __shfl_sync(0xffffffffu, prev, at) : run) : __shfl_sync(0xffffffffu, inc, 31);
+        return at;
+    };
+    double run = s_before, behind = 0.0;
+    bool passed = false;
+    int block = 0;
+    for (int t = 0; t < blocks && !passed; t += 32) {
+        const double w = t + lane < blocks ? s_block[t + lane] : 0.0, start = run;
+        const int at = find(w, run, passed);
+        if (at >= 0) block = t + at, behind = passed ? run : start + (at ? __shfl_sync(0xffffffffu, warp_running(w), at - 1) : 0.0);
+    }
+    run = behind;
+    const double cw = lane < kWarps ? s_cell[block][lane][0] : 0.0;
+    const double start = run;
+    const int cat = max(find(cw, run, passed), 0);
+    if (!passed) run = start + (cat ? __shfl_sync(0xffffffffu, warp_running(cw), cat - 1) : 0.0);
+    // the cell's entries, 4 a lane in order
+    const unsigned c0 = j0 + block * block_entries + cat * cell, c1 = min(j1, c0 + cell);
+    int place = -1, last = 0;
+    for (unsigned t0 = c0; t0 < c1 && place < 0; t0 += 128) {
+        const unsigned j = t0 + 4 * lane;
         double v[4] = {0.0, 0.0, 0.0, 0.0};
-        if (f < j1) weights4(f, plain, fp, fq, v);
-        int lastw = -1;
+        int mine = -1, lastw = -1;
+        if (j < c1) {
+            float x[4], y[4];
+            entries4<VEC>(P, j, j1, x);
+            if (with_q && !plain) entries4<VEC>(Q, j, j1, y);
+            const int sk = !plain && skip >= 0 && (unsigned)skip - j < 4 ? skip - (int)j : -1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (v[i] > 0.0) lastw = (int)(f + i);
-        const double sum = (v[0] + v[1]) + (v[2] + v[3]);
-        double inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
-        }
-        if (lane == 31) s_scan[warp] = inc;
-        __syncthreads();
-        double at = run, all = 0.0;
-        for (int w = 0; w < PT / 32; ++w) {
-            if (w < warp) at += s_scan[w];
-            all += s_scan[w];
-        }
-        at += inc - sum;
-        for (int i = 0; i < 4; ++i) {
-            at += v[i];
-            if (v[i] > 0.0 && at > border) {
-                atomicMin(&s_place, (int)(f + i));
-                break;
+            for (int i = 0; i < 4; ++i) {
+                v[i] = P.weigh(x[i]);
+                if (with_q && !plain) {
+                    const double q = Q.weigh(y[i]);
+                    if (v[i] > q) lastw = (int)(j + i);
+                    v[i] = v[i] > q ? fmax(fma(v[i], fp, -(q * fq)), 0.0) : 0.0;
+                } else if (i == sk) {
+                    v[i] = 0.0;
+                } else if (v[i] > 0.0) {
+                    lastw = (int)(j + i);
+                }
             }
         }
-        if (lastw >= 0) atomicMax(&s_last, lastw);
-        __syncthreads();
-        if (s_place != INT_MAX) break;
-        run += all;
-        __syncthreads();
+        const double sum = (v[0] + v[1]) + (v[2] + v[3]), inc = warp_running(sum);
+        double at = run + (inc - sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            at += v[i];
+            if (v[i] > 0.0 && at > border && mine < 0) mine = (int)(j + i);
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, mine >= 0);
+        if (hit) place = __shfl_sync(0xffffffffu, mine, __ffs((int)hit) - 1);
+        last = max(last, __reduce_max_sync(0xffffffffu, lastw));
+        run += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (warp == 0) write_out(a, b, n_acc, s_place != INT_MAX ? s_place : max(s_last, 0));
+    write_out(a, b, n_acc, place >= 0 ? place : last);
 }
 
 // CTAs a sequence: parts of 4096 entries at least, up to the portable cluster of 8
