@@ -26,7 +26,9 @@
 //                over in two buffers of up to 128 columns: of few tokens' groups several at once, since a handing
 //                over costs each side some 300 cycles.
 // Bound: the tensor pipe for many tokens (a group of 128: 8 MMAs of N / 2 cycles each against ~N cycles of TMEM reads
-// and N / 2 FMAs a thread). All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
+// and N / 2 FMAs a thread). Measured: 2048 bf16 tokens x 8192 x 2048, groups of 128, 87.6 us: 784 TFLOP/s, 47 % of a
+// library product's rate of 16-bit weights; 777 f32 tokens x 2048 x 2048, groups of 64, 24.5 us (two terms: 532 TFLOP/s
+// of MMAs, a tile a CTA); 24 f32 tokens x 5003 x 2080, groups of 32, 16.3 us, a chain of 17 stages. All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
 // MMAs in flight, reports kErrWaitTimeout and stores nothing.
 #include <cuda.h>
 #include <cudaTypedefs.h>

@@ -8,6 +8,11 @@ one f32 step (2^-23) of the sum of absolute terms A_g of the group; with s steps
 bf16 term of an activation, 3 terms for f32) and 17 additions a step that is 17 s 2^-23 A_g. The groups
 are then scaled and added in f32: one rounding each for the scale product, the activations' scale and the
 addition, (groups + 2) 2^-24 A. A bf16 output adds half a step, 2^-8 of the value.
+
+Up to 16 tokens the activations are whole numbers instead, kept to 2^-23 of the largest M of 128: 2^-23 M Σ|w|, and
+their sums are exact. For these normal activations M < 5.5 against a mean of 0.8, so that is about 7 2^-23 A,
+within the 17 s above. More than 16 f32 tokens are two f16 terms, within 2^-24 of each activation: 2^-24 A more
+than the bf16 terms' 0, again within it.
 """
 import numpy as np
 import pytest
