@@ -55,7 +55,7 @@ struct TcArgs {
     const float* col_scale;   // [tokens]: one factor a token, or null
     const float* x_scales;    // [n_groups][tokens padded to 128]: a factor per group of inputs, or null
     size_t x_pitch, x_groups;
-    int x_group;              // inputs of a group
+    int x_group, x_shift;     // inputs of a group, and their log2 (7 where a group holds 128 or more)
     int y_bf16, tiles, plane_rows;  // plane_rows: rows of B between the terms
     int* err;
 };
@@ -452,7 +452,6 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         const uint32_t t_d = tmem + ((uint32_t)(32 * (w & 3)) << 16) + part * C;
         // this row's scales in a stage: [tile][row % 8][block][row / 8]
         const int sc_at = (((row >> 4) * 8 + (row & 7)) * pc * 2 + ((row >> 3) & 1)) * 2;
-        const int xs_step = a.x_scales && a.x_group < kK ? N * 4 * 32 * FB / a.x_group : 0;  // bytes a sum
         bool ok = true;
         int st = 0, db = 0;
         unsigned d_ph = 0, s_ph = 0;
@@ -473,7 +472,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
                     for (int f = 0; f < U; ++f) {
                         const int sum = h * U + f;
                         const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (sum * FB * pc / 4) * 4), a.w.scale_bf16);
-                        const unsigned char* xs = base + L::kXs + part * C * 4 + sum * xs_step;
+                        const unsigned char* xs = base + L::kXs + part * C * 4 + (sum * FB * 32 >> a.x_shift) * (N * 4);
                         constexpr int B = C < 16 ? C : 16;  // columns in registers at a time
 #pragma unroll
                         for (int j = 0; j < C; j += B) {
@@ -677,6 +676,7 @@ cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, voi
         a.x_pitch = pad(x.tokens, 128);
         a.x_scales = x.group ? xs : nullptr;
         a.x_group = x.group;
+        a.x_shift = x.group ? std::min(x.group_shift, 7) : 7;
         a.x_groups = x.n_groups;
         a.col_scale = x.kind == kW4XF32 ? col : x.kind == kW4XInt8 && !x.group ? x.scales : nullptr;
         w4_terms_kernel<<<(unsigned)std::min<size_t>(x.tokens, 1 << 20), 256, 0, s>>>(x, kp, t, col, x.group ? xs : nullptr, a.x_pitch);

@@ -112,6 +112,10 @@ CASES = [
     (200, 2048, 2048, 64, "f32", 0, True, torch.bfloat16, bb.F32),
     (257, 512, 640, 128, "int8", 32, True, torch.float16, bb.BF16),
     (513, 1280, 1000, 128, "bf16", 0, True, torch.float16, bb.F32),
+    # activations' groups of 64 over weights' groups of 32
+    (6, 256, 70, 32, "int8", 64, True, torch.float16, bb.F32),
+    (17, 256, 70, 32, "int8", 64, True, torch.float16, bb.F32),
+    (90, 192, 257, 32, "int8", 64, False, torch.float16, bb.F32),
 ]
 IDS = ["-".join(str(v).replace("torch.", "") for v in c) for c in CASES]
 
