@@ -2719,14 +2719,21 @@ int w4_fill(bebelm_w4* W, const uint8_t* codes, const void* scales, const uint8_
     return 0;
 }
 
-// Few tokens are bound by the weights' bytes, many by the products: the streaming kernel up to 16
-// tokens, the tensor cores' tiles above.
-constexpr size_t kW4StreamTokens = 16;
+// Few tokens are bound by the weights' bytes, many by the products: the streaming kernel up to 8 tokens, the tensor
+// cores' tiles above 16. Between them int8 activations stream (tiles of 128000 x 2048: 51 us, stream 33), f32
+// and bf16 ones, whose 9 to 16 tokens cost twice the products of 8, only through small layers; a group of 32 ends
+// with every MMA there and counts twice. (16 tokens, stream and tiles: 2048 x 2048 6.6 and 9.6 us, 8192 x 8192
+// 27.0 and 20.7, 4096 x 4096 10.3 and 9.9; in groups of 32 2048 x 2048 8.2 and 10.1, 8192 x 2048 17.4 and 11.3.)
+constexpr size_t kW4StreamTokens = 16, kW4StreamTiles = 1024;
+bool w4_streams(const W4View& w, const W4X& x) {
+    if (x.tokens <= kW4StreamTokens / 2 || x.tokens > kW4StreamTokens) return x.tokens <= kW4StreamTokens;
+    return x.kind == kW4XInt8 || w.tile_rows / 8 * w.chunks * (w.per_chunk == 4 ? 2 : 1) <= kW4StreamTiles;
+}
 size_t w4_scratch(const W4View& w, const W4X& x) {
-    return x.tokens <= kW4StreamTokens ? w4_stream_workspace(w, x) : w4_tc_workspace(w, x);
+    return w4_streams(w, x) ? w4_stream_workspace(w, x) : w4_tc_workspace(w, x);
 }
 cudaError_t w4_run(const bebelm_w4* W, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms, cudaStream_t s) {
-    if (x.tokens <= kW4StreamTokens) return launch_w4_stream(W->v, x, y, y_bf16, workspace, num_sms, s);
+    if (w4_streams(W->v, x)) return launch_w4_stream(W->v, x, y, y_bf16, workspace, num_sms, s);
     return launch_w4_tc(W->v, x, y, y_bf16, workspace, num_sms, W->err.d, s);
 }
 

@@ -25,15 +25,18 @@
 //   warps 12-    read each group's sums, scale and add them; a thread has a row and 32 tokens (16 of 32). Sums go
 //                over in two buffers of up to 128 columns: of few tokens' groups several at once, since a handing
 //                over costs each side some 300 cycles.
+// Where there are tiles for half of the SMs or less, a cluster's CTAs share a tile's inputs: each leaves its sums in
+// its shared memory (where the activations' ring was) and adds up a share of the tokens, the parts in order.
 // Bound: the tensor pipe for many tokens (a group of 128: 8 MMAs of N / 2 cycles each against ~N cycles of TMEM reads
 // and N / 2 FMAs a thread). Measured: 2048 bf16 tokens x 8192 x 2048, groups of 128, 87.6 us: 784 TFLOP/s, 47 % of a
 // library product's rate of 16-bit weights; 777 f32 tokens x 2048 x 2048, groups of 64, 24.5 us (two terms: 532 TFLOP/s
-// of MMAs, a tile a CTA); 24 f32 tokens x 5003 x 2080, groups of 32, 16.3 us, a chain of 17 stages. All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
+// of MMAs, a tile a CTA); 24 f32 tokens x 5003 x 2080, groups of 32, 12.4 us, three CTAs a tile. All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
 // MMAs in flight, reports kErrWaitTimeout and stores nothing.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "internal.h"
@@ -57,6 +60,7 @@ struct TcArgs {
     size_t x_pitch, x_groups;
     int x_group, x_shift;     // inputs of a group, and their log2 (7 where a group holds 128 or more)
     int y_bf16, tiles, plane_rows;  // plane_rows: rows of B between the terms
+    int split;                // CTAs of a cluster that share a tile's inputs; 1: a CTA takes tiles of its own
     int* err;
 };
 
@@ -210,6 +214,27 @@ __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
     return __half2float(__half(r));
 }
 
+__device__ __forceinline__ void store(const TcArgs& a, size_t t, size_t r, float v) {
+    if (a.col_scale) v *= __ldg(a.col_scale + t);
+    if (a.y_bf16)
+        static_cast<__nv_bfloat16*>(a.y)[t * a.w.n_out + r] = __float2bfloat16_rn(v);
+    else
+        static_cast<float*>(a.y)[t * a.w.n_out + r] = v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a word of CTA `rank`'s shared memory, at this CTA's address of it
+__device__ __forceinline__ int ld_cluster(uint32_t addr, int rank) {
+    int v;
+    asm volatile(
+        "{\n\t.reg .u32 p;\n\tmapa.shared::cluster.u32 p, %1, %2;\n\tld.shared::cluster.s32 %0, [p];\n\t}"
+        : "=r"(v)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
+
 template <int N, int TERMS, bool BF16>
 struct Lay {
     static constexpr int kEpiWarps = N == 128 ? 16 : 8, kThreads = 32 * (kFixedWarps + kEpiWarps);
@@ -222,11 +247,11 @@ struct Lay {
     static constexpr int kSB = (kRings - kOffB) / kB < 12 ? (kRings - kOffB) / kB : 12;
     static constexpr int kSmem = kOffB + kSB * kB + 1024;
     static constexpr int kBars = 2 * (kSB + kSW + kSS) + 14;
-    static_assert(kSB >= 4, "ring");
+    static_assert(kSB >= 4, "ring");  // 4 stages also hold a part's sums, N x 128 floats
 };
 
-// FB: blocks of 32 inputs whose sum is scaled together
-template <int N, int TERMS, bool BF16, int FB>
+// FB: blocks of 32 inputs whose sum is scaled together. SPLIT: the CTAs of a cluster share a tile's inputs.
+template <int N, int TERMS, bool BF16, int FB, bool SPLIT>
 __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, TcArgs a) {
     using L = Lay<N, TERMS, BF16>;
     constexpr int SB = L::kSB, SW = L::kSW, SS = L::kSS;  // ring stages
@@ -240,6 +265,11 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int chunks = (int)a.w.chunks, pc = a.w.per_chunk, row_blocks = (int)(a.w.tile_rows / 8);
+    // this CTA's tiles, and its part [c_lo, c_hi) of their chunks of 128 inputs
+    const int split = SPLIT ? a.split : 1, rank = SPLIT ? (int)blockIdx.x % split : 0;
+    const int tile0 = SPLIT ? (int)blockIdx.x / split : (int)blockIdx.x, tile_step = SPLIT ? a.tiles : (int)gridDim.x;
+    const int c_lo = SPLIT ? chunks * rank / split : 0, c_hi = SPLIT ? chunks * (rank + 1) / split : chunks;
+    const int n_chunks = (a.tiles - tile0 + tile_step - 1) / tile_step * (c_hi - c_lo);
     const uint32_t bars = smem_u32(s_bar);
     auto b_full = [&](int i) { return bars + 8 * i; };
     auto b_empty = [&](int i) { return bars + 8 * (SB + i); };
@@ -302,9 +332,9 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
     };
     if (warp == 0) {
         Fill r;
-        for (int tile = blockIdx.x, ok = 1; ok && tile < a.tiles; tile += gridDim.x) {
+        for (int tile = tile0, ok = 1; ok && tile < a.tiles; tile += tile_step) {
             const int t0 = tile / row_blocks * N;
-            for (int i = 0; i < 2 * chunks; ++i) {
+            for (int i = 2 * c_lo; i < 2 * c_hi; ++i) {
                 ok = fill(r, SB, b_full(0), b_empty(0), L::kB);
                 if (!ok) break;
 #pragma unroll
@@ -318,9 +348,9 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         const uint32_t zb = a.w.zeros ? 64u * (pc == 4 ? 8 : 4) : 0u, scb = 256u * (uint32_t)pc;
         const int xs_rows = a.x_scales ? (a.x_group < kK ? kK / a.x_group : 1) : 0;  // groups that meet 128 inputs
         Fill r, q;
-        for (int tile = blockIdx.x, ok = 1; ok && tile < a.tiles; tile += gridDim.x) {
+        for (int tile = tile0, ok = 1; ok && tile < a.tiles; tile += tile_step) {
             const int rb = tile % row_blocks, t0 = tile / row_blocks * N;
-            for (int c = 0; c < chunks; ++c) {
+            for (int c = c_lo; c < c_hi; ++c) {
                 const size_t at = (size_t)rb * chunks + c;
                 ok = fill(r, SW, w_full(0), w_empty(0), 8192u + zb);
                 if (!ok) break;
@@ -346,13 +376,13 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         // 900 cycles, more than 128 tokens' MMAs do: where a chunk is one handing over, two warps take
         // turns, each with an accumulator and two A buffers of its own.
         constexpr uint32_t idesc = instr_desc(N, BF16);
-        const int first = warp == 3, total = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * chunks;
+        const int first = warp == 3;
         const uint64_t b0 = smem_desc(sb + L::kOffB);
         int st = 2 * first;  // ring stage
         uint32_t ab = first, db = first;
         unsigned b_ph = 0, a_ph = 0, d_ph = 1;  // d_ph: of the accumulators' last reads; the first round passes
         bool ok = true;
-        for (int c = first; ok && c < total; c += kIssuers) {
+        for (int c = first; ok && c < n_chunks; c += kIssuers) {
             ok = mbar_wait_warp(a_full(0) + 8 * ab, a_ph);
             if (!ok) break;
             const uint32_t ta = tmem + kColA + 64 * ab;
@@ -404,11 +434,10 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         mbar_wait_warp(drained + 8 * first, 0);
     } else if (warp >= kConvert0 && warp < kEpi0) {
         const int w = warp & 3, g = lane >> 2, rec = pc == 4 ? 8 : 4, set = (warp - kConvert0) >> 2;
-        const int total = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * chunks;
         bool ok = true;
         int st = set, ab = set;
         unsigned w_ph = 0, a_ph = 1;  // the first round of A buffers passes
-        for (int c = set; c < total; c += 2) {
+        for (int c = set; c < n_chunks; c += 2) {
             ok = mbar_wait_warp(w_full(st), w_ph) && mbar_wait_warp(a_empty(ab), a_ph);
             if (!ok) break;
             tc_after();
@@ -455,12 +484,12 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         bool ok = true;
         int st = 0, db = 0;
         unsigned d_ph = 0, s_ph = 0;
-        for (int tile = blockIdx.x; ok && tile < a.tiles; tile += gridDim.x) {
+        for (int tile = tile0; ok && tile < a.tiles; tile += tile_step) {
             const int rb = tile % row_blocks, t0 = tile / row_blocks * N;
             float acc[C];
 #pragma unroll
             for (int i = 0; i < C; ++i) acc[i] = 0.f;
-            for (int c = 0; ok && c < chunks; ++c) {
+            for (int c = c_lo; ok && c < c_hi; ++c) {
                 const unsigned char* base = sm + L::kOffS + st * L::kS;
                 ok = mbar_wait_warp(s_full(st), s_ph);
 #pragma unroll
@@ -507,16 +536,15 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
                 if (++st == SS) st = 0, s_ph ^= 1;
             }
             const size_t r = (size_t)rb * kM + row;
-            if (ok && r < a.w.n_out) {
+            if constexpr (SPLIT) {  // every MMA of this CTA is done: its activations' ring holds the part's sums
+#pragma unroll
+                for (int i = 0; i < C; ++i) reinterpret_cast<float*>(sm + L::kOffB)[(part * C + i) * kM + row] = acc[i];
+            } else if (ok && r < a.w.n_out) {
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const size_t t = (size_t)t0 + part * C + i;
                     if (t >= a.tokens) break;
-                    const float v = a.col_scale ? acc[i] * __ldg(a.col_scale + t) : acc[i];
-                    if (a.y_bf16)
-                        static_cast<__nv_bfloat16*>(a.y)[t * a.w.n_out + r] = __float2bfloat16_rn(v);
-                    else
-                        static_cast<float*>(a.y)[t * a.w.n_out + r] = v;
+                    store(a, t, r, acc[i]);
                 }
             }
         }
@@ -529,6 +557,20 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
     if (warp == 0) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
+    if constexpr (SPLIT) {  // the parts' sums in order, a share of the tokens by each CTA
+        cluster_sync();
+        int fail = 0;
+        for (int j = 0; j < split; ++j) fail |= ld_cluster(smem_u32(&s_fail), j);
+        const int n_lo = N * rank / split, n_hi = N * (rank + 1) / split, rb = tile0 % row_blocks, t0 = tile0 / row_blocks * N;
+        for (int i = n_lo * kM + tid; !fail && i < n_hi * kM; i += L::kThreads) {
+            const size_t r = (size_t)rb * kM + i % kM, t = (size_t)t0 + i / kM;
+            if (r >= a.w.n_out || t >= a.tokens) continue;
+            float v = 0.f;
+            for (int j = 0; j < split; ++j) v += __int_as_float(ld_cluster(sb + L::kOffB + 4 * i, j));
+            store(a, t, r, v);
+        }
+        cluster_sync();  // nobody leaves while its sums are read
     }
 }
 
@@ -614,25 +656,66 @@ size_t terms_bytes(const W4View& w, const W4X& x) {
     return pad((x.kind == kW4XF32 ? 2 : 1) * x.tokens * w.chunks * kK * 2, 256);
 }
 
+// Clusters of k CTAs of a kernel that run at once on the device.
+template <int N, int TERMS, bool BF16, int FB>
+cudaError_t clusters_that_fit(int k, int num_sms, int* n) {
+    static std::atomic<int> known[9];  // + 1
+    *n = known[k].load(std::memory_order_relaxed) - 1;
+    if (*n >= 0) return cudaSuccess;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(k * num_sms));
+    cfg.blockDim = dim3(Lay<N, TERMS, BF16>::kThreads);
+    cfg.dynamicSmemBytes = Lay<N, TERMS, BF16>::kSmem;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)k;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(n, w4_tc_kernel<N, TERMS, BF16, FB, true>, &cfg);
+    if (e == cudaSuccess) known[k].store(*n + 1, std::memory_order_relaxed);
+    return e;
+}
+
 template <int N, int TERMS, bool BF16, int FB>
 cudaError_t run(const CUtensorMap& tm, TcArgs& a, int num_sms, bool pdl, cudaStream_t s) {
     using L = Lay<N, TERMS, BF16>;
-    auto kernel = w4_tc_kernel<N, TERMS, BF16, FB>;
-    static SmemOnce once;
-    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), L::kSmem);
+    static SmemOnce once, once_split;
+    cudaError_t e = once.set(reinterpret_cast<const void*>(w4_tc_kernel<N, TERMS, BF16, FB, false>), L::kSmem);
+    if (e == cudaSuccess) e = once_split.set(reinterpret_cast<const void*>(w4_tc_kernel<N, TERMS, BF16, FB, true>), L::kSmem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
     a.tiles = (int)(a.w.tile_rows / 8 * ((a.tokens + N - 1) / N));
-    cfg.gridDim = dim3((unsigned)std::min(a.tiles, num_sms));
+    // Tiles for half of the SMs or less: clusters of up to 8 share a tile's inputs, at least two chunks a CTA, if all
+    // of them run at once. (24 f32 tokens, 5003 x 2080: 16.3 us with a CTA a tile, 12.4 us with three; 17 bf16 tokens,
+    // 8192 x 8192: 29.7 and 20.4 us with two.)
+    a.split = 1;
+    for (int k = 8; k > 1 && a.split == 1; --k) {
+        if ((size_t)k * 2 > a.w.chunks || (long long)a.tiles * k > num_sms) continue;
+        int n;
+        e = clusters_that_fit<N, TERMS, BF16, FB>(k, num_sms, &n);
+        if (e != cudaSuccess) return e;
+        if (a.tiles <= n) a.split = k;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.split > 1 ? a.tiles * a.split : std::min(a.tiles, num_sms)));
     cfg.blockDim = dim3(L::kThreads);
     cfg.dynamicSmemBytes = L::kSmem;
     cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, tm, a);
+    cudaLaunchAttribute at[2] = {};
+    if (pdl) {
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    if (a.split > 1) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = (unsigned)a.split;
+        at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    cfg.attrs = at;
+    return a.split > 1 ? cudaLaunchKernelEx(&cfg, w4_tc_kernel<N, TERMS, BF16, FB, true>, tm, a)
+                       : cudaLaunchKernelEx(&cfg, w4_tc_kernel<N, TERMS, BF16, FB, false>, tm, a);
 }
 template <int N, int TERMS, bool BF16>
 cudaError_t run_fb(const CUtensorMap& tm, TcArgs& a, int fb, int num_sms, bool pdl, cudaStream_t s) {

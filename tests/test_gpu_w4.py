@@ -9,9 +9,9 @@ bf16 term of an activation, 3 terms for f32) and 17 additions a step that is 17 
 are then scaled and added in f32: one rounding each for the scale product, the activations' scale and the
 addition, (groups + 2) 2^-24 A. A bf16 output adds half a step, 2^-8 of the value.
 
-Up to 16 tokens the activations are whole numbers instead, kept to 2^-23 of the largest M of 128: 2^-23 M Σ|w|, and
+Up to 8 tokens (16 through small layers) the activations are whole numbers instead, kept to 2^-23 of the largest M of 128: 2^-23 M Σ|w|, and
 their sums are exact. For these normal activations M < 5.5 against a mean of 0.8, so that is about 7 2^-23 A,
-within the 17 s above. More than 16 f32 tokens are two f16 terms, within 2^-24 of each activation: 2^-24 A more
+within the 17 s above. More f32 tokens are two f16 terms, within 2^-24 of each activation: 2^-24 A more
 than the bf16 terms' 0, again within it.
 """
 import numpy as np
@@ -112,10 +112,22 @@ CASES = [
     (200, 2048, 2048, 64, "f32", 0, True, torch.bfloat16, bb.F32),
     (257, 512, 640, 128, "int8", 32, True, torch.float16, bb.BF16),
     (513, 1280, 1000, 128, "bf16", 0, True, torch.float16, bb.F32),
+    # 9 to 16 tokens through layers above and below the size where the kernels change
+    (9, 2048, 8192, 128, "f32", 0, True, torch.float16, bb.F32),
+    (12, 2048, 8193, 128, "f32", 0, False, torch.float16, bb.F32),
+    (16, 2080, 5003, 32, "bf16", 0, True, torch.float16, bb.BF16),
+    (13, 8192, 8192, 64, "f32", 0, True, torch.bfloat16, bb.F32),
     # activations' groups of 64 over weights' groups of 32
     (6, 256, 70, 32, "int8", 64, True, torch.float16, bb.F32),
     (17, 256, 70, 32, "int8", 64, True, torch.float16, bb.F32),
     (90, 192, 257, 32, "int8", 64, False, torch.float16, bb.F32),
+    # few tiles of many inputs: 8, 6, 4, 3 and 2 CTAs share a tile's
+    (24, 4096, 128, 128, "f32", 0, True, torch.float16, bb.F32),
+    (40, 1664, 700, 32, "int8", 64, True, torch.float16, bb.F32),
+    (128, 2048, 2500, 64, "f32", 0, True, torch.float16, bb.BF16),
+    (70, 512, 4300, 128, "bf16", 0, False, torch.float16, bb.F32),
+    (256, 1056, 2048, 32, "bf16", 0, True, torch.bfloat16, bb.F32),
+    (20, 384, 300, 128, "int8", 0, True, torch.float16, bb.F32),
 ]
 IDS = ["-".join(str(v).replace("torch.", "") for v in c) for c in CASES]
 
