@@ -28,7 +28,7 @@
 // Where there are tiles for half of the SMs or less, a cluster's CTAs share a tile's inputs: each leaves its sums in
 // its shared memory (where the activations' ring was) and adds up a share of the tokens, the parts in order.
 // Bound: the tensor pipe for many tokens (a group of 128: 8 MMAs of N / 2 cycles each against ~N cycles of TMEM reads
-// and N / 2 FMAs a thread). Measured: 2048 bf16 tokens x 8192 x 2048, groups of 128, 87.6 us: 784 TFLOP/s, 47 % of a
+// and N / 2 FMAs a thread). Measured: 2048 bf16 tokens x 8192 x 2048, groups of 128, 86.7 us: 793 TFLOP/s, 47 % of a
 // library product's rate of 16-bit weights; 777 f32 tokens x 2048 x 2048, groups of 64, 24.5 us (two terms: 532 TFLOP/s
 // of MMAs, a tile a CTA); 24 f32 tokens x 5003 x 2080, groups of 32, 12.4 us, three CTAs a tile. All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
 // MMAs in flight, reports kErrWaitTimeout and stores nothing.
@@ -213,6 +213,22 @@ __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
     r.x = (unsigned short)h;
     return __half2float(__half(r));
 }
+
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t x, uint64_t y) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(y));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(i ? v >> 32 : v)); }
 
 __device__ __forceinline__ void store(const TcArgs& a, size_t t, size_t r, float v) {
     if (a.col_scale) v *= __ldg(a.col_scale + t);
@@ -486,9 +502,9 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         unsigned d_ph = 0, s_ph = 0;
         for (int tile = tile0; ok && tile < a.tiles; tile += tile_step) {
             const int rb = tile % row_blocks, t0 = tile / row_blocks * N;
-            float acc[C];
+            uint64_t acc[C / 2];  // pairs of neighbouring tokens
 #pragma unroll
-            for (int i = 0; i < C; ++i) acc[i] = 0.f;
+            for (int i = 0; i < C / 2; ++i) acc[i] = 0;
             for (int c = c_lo; ok && c < c_hi; ++c) {
                 const unsigned char* base = sm + L::kOffS + st * L::kS;
                 ok = mbar_wait_warp(s_full(st), s_ph);
@@ -500,7 +516,8 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
 #pragma unroll
                     for (int f = 0; f < U; ++f) {
                         const int sum = h * U + f;
-                        const float s = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (sum * FB * pc / 4) * 4), a.w.scale_bf16);
+                        const float s1 = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (sum * FB * pc / 4) * 4), a.w.scale_bf16);
+                        const uint64_t s = pack2(__float_as_uint(s1), __float_as_uint(s1));
                         const unsigned char* xs = base + L::kXs + part * C * 4 + (sum * FB * 32 >> a.x_shift) * (N * 4);
                         constexpr int B = C < 16 ? C : 16;  // columns in registers at a time
 #pragma unroll
@@ -516,15 +533,13 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
                             if (a.x_scales) {
 #pragma unroll
                                 for (int i = 0; i < B; i += 4) {
-                                    const float4 x4 = *reinterpret_cast<const float4*>(xs + (j + i) * 4);
-                                    acc[j + i] = fmaf(__uint_as_float(d[i]) * x4.x, s, acc[j + i]);
-                                    acc[j + i + 1] = fmaf(__uint_as_float(d[i + 1]) * x4.y, s, acc[j + i + 1]);
-                                    acc[j + i + 2] = fmaf(__uint_as_float(d[i + 2]) * x4.z, s, acc[j + i + 2]);
-                                    acc[j + i + 3] = fmaf(__uint_as_float(d[i + 3]) * x4.w, s, acc[j + i + 3]);
+                                    const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(xs + (j + i) * 4);
+                                    fma2(acc[(j + i) / 2], mul2(pack2(d[i], d[i + 1]), x4.x), s);
+                                    fma2(acc[(j + i) / 2 + 1], mul2(pack2(d[i + 2], d[i + 3]), x4.y), s);
                                 }
                             } else {
 #pragma unroll
-                                for (int i = 0; i < B; ++i) acc[j + i] = fmaf(__uint_as_float(d[i]), s, acc[j + i]);
+                                for (int i = 0; i < B; i += 2) fma2(acc[(j + i) / 2], pack2(d[i], d[i + 1]), s);
                             }
                         }
                     }
@@ -538,13 +553,13 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
             const size_t r = (size_t)rb * kM + row;
             if constexpr (SPLIT) {  // every MMA of this CTA is done: its activations' ring holds the part's sums
 #pragma unroll
-                for (int i = 0; i < C; ++i) reinterpret_cast<float*>(sm + L::kOffB)[(part * C + i) * kM + row] = acc[i];
+                for (int i = 0; i < C; ++i) reinterpret_cast<float*>(sm + L::kOffB)[(part * C + i) * kM + row] = half_of(acc[i / 2], i & 1);
             } else if (ok && r < a.w.n_out) {
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const size_t t = (size_t)t0 + part * C + i;
                     if (t >= a.tokens) break;
-                    store(a, t, r, acc[i]);
+                    store(a, t, r, half_of(acc[i / 2], i & 1));
                 }
             }
         }
