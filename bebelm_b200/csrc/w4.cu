@@ -18,8 +18,8 @@
 // Bound: a weight is read once, for at most 16 tokens, so HBM. On the way a weight costs 3/8 of a logic operation (two
 // masks and a shift for a word of 8 codes); unpacked to 16-bit floats it cost 11/8 and the logic unit bound the
 // kernel. Measured (with 16-bit floats): 128000 x 2048, 5 int8 tokens 27.7 us (44), 138 MB at 5.0 TB/s, 76 % of a
-// copy's rate; 8192 x 8192, one bf16 token 12.1 us (16), 35 MB at 2.9 TB/s: launch, digits and the first loads take
-// 5 us of it; 2048 x 2048, one f32 token 4.3 us, all latency.
+// copy's rate; 8192 x 8192, one bf16 token 12.1 us (16), 35 MB at 2.9 TB/s: every CTA makes the digits first, with the
+// ring's first weights in flight; 2048 x 2048, one f32 token 4.2 us, all latency.
 //
 // Layout: rows padded to 128, inputs to 128 (scale 0). A tile of 16 rows x 128 inputs is 1024 bytes,
 // [row / 8][row % 8][q = 0..3][b = 0..3] words of 8 codes; the 8 tiles of 128 rows lie together, then the next 128
@@ -514,8 +514,8 @@ cudaError_t run_pc(StreamArgs& a, int num_sms, cudaStream_t s) {
 }
 template <int D, bool WS>
 cudaError_t run_nt(StreamArgs& a, int num_sms, cudaStream_t s) {
-    // Two row tiles a warp share the activations' fragments and the loop's overhead (128000 x 2048, 5 tokens: 31 ->
-    // 27.7 us); one tile a warp where that would leave a warp fewer than 4 pairs (2048 x 2048: 4.9 -> 4.3 us), and
+    // Two row tiles a warp share the activations' fragments and the loop's overhead (128000 x 2048, 5 tokens: 28.8 ->
+    // 27.8 us, 8192 x 8192 12.8 -> 12.2); one tile a warp where that would leave a warp fewer than 4 pairs (2048 x 2048: 5.3 -> 4.2), and
     // where 16 tokens' three digits fill the registers.
     if (a.x.tokens > 8) return D == 1 ? run_pc<2, 2, 1, WS>(a, num_sms, s) : run_pc<1, 2, 3, WS>(a, num_sms, s);
     return a.w.tile_rows * a.w.chunks < (size_t)num_sms * kWarps * 8 ? run_pc<1, 1, D, WS>(a, num_sms, s) : run_pc<2, 1, D, WS>(a, num_sms, s);

@@ -30,8 +30,9 @@
 // Bound: the tensor pipe for many tokens (a group of 128: 8 MMAs of N / 2 cycles each against ~N cycles of TMEM reads
 // and N / 2 FMAs a thread). Measured: 2048 bf16 tokens x 8192 x 2048, groups of 128, 86.7 us: 793 TFLOP/s, 47 % of a
 // library product's rate of 16-bit weights; 777 f32 tokens x 2048 x 2048, groups of 64, 24.5 us (two terms: 532 TFLOP/s
-// of MMAs, a tile a CTA); 24 f32 tokens x 5003 x 2080, groups of 32, 12.4 us, three CTAs a tile. All waits are bounded; after one gives up the CTA waits (bounded) for its copies and
-// MMAs in flight, reports kErrWaitTimeout and stores nothing.
+// of MMAs, a tile a CTA); 24 f32 tokens x 5003 x 2080, groups of 32, 11.3 us, three CTAs a tile.
+// All waits are bounded; after one gives up the CTA waits (bounded) for its copies and MMAs in flight, reports
+// kErrWaitTimeout and stores nothing.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -600,8 +601,23 @@ __global__ void __launch_bounds__(256) w4_terms_kernel(W4X x, size_t kp, uint16_
         uint16_t* o = out + t * kp;
         if (x.kind == kW4XF32) {
             const float* p = static_cast<const float*>(x.x) + t * x.stride;
+            const bool pairs = (reinterpret_cast<uintptr_t>(p) & 7) == 0;
+            auto pair = [&](size_t k) {
+                if (k >= x.n_in) return make_float2(0.f, 0.f);
+                return pairs ? *reinterpret_cast<const float2*>(p + k) : make_float2(p[k], p[k + 1]);
+            };
+            constexpr int kKeep = 8;  // pairs a thread keeps between the maximum and the terms: rows of 4096
+            float2 keep[kKeep];
             float m = 0.f;
-            for (size_t k = threadIdx.x; k < x.n_in; k += 256) m = fmaxf(m, fabsf(p[k]));
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i) {
+                keep[i] = pair(2 * threadIdx.x + 512 * i);
+                m = fmaxf(m, fmaxf(fabsf(keep[i].x), fabsf(keep[i].y)));
+            }
+            for (size_t k = 2 * threadIdx.x + 512 * kKeep; k < x.n_in; k += 512) {
+                const float2 v = pair(k);
+                m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y)));
+            }
 #pragma unroll
             for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
             __syncthreads();
@@ -615,21 +631,23 @@ __global__ void __launch_bounds__(256) w4_terms_kernel(W4X x, size_t kp, uint16_
             const int e = m > 0.f && em < 255 ? 14 - (max(em, 1) - 127) : 0, e1 = e / 2, e2 = e - e1;
             const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23), f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
             if (threadIdx.x == 0) col_scale[t] = ldexpf(1.f, -e);
-            for (size_t k = 2 * threadIdx.x; k < kp; k += 512) {
+            auto write = [&](size_t k, float2 u) {
                 uint32_t hi = 0, lo = 0;
-                if (k < x.n_in) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float v = p[k + j] * f1 * f2;
-                        const __half a = __float2half_rn(v);
-                        const float rest = v - __half2float(a);
-                        const __half b = __float2half_rn(fabsf(rest) <= 65504.f ? rest : 0.f);  // v not finite: no second term
-                        hi |= (uint32_t)__half_as_ushort(a) << (16 * j), lo |= (uint32_t)__half_as_ushort(b) << (16 * j);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    const float v = (j ? u.y : u.x) * f1 * f2;
+                    const __half a = __float2half_rn(v);
+                    const float rest = v - __half2float(a);
+                    const __half b = __float2half_rn(fabsf(rest) <= 65504.f ? rest : 0.f);  // v not finite: no second term
+                    hi |= (uint32_t)__half_as_ushort(a) << (16 * j), lo |= (uint32_t)__half_as_ushort(b) << (16 * j);
                 }
                 *reinterpret_cast<uint32_t*>(o + k) = hi;
                 *reinterpret_cast<uint32_t*>(o + plane + k) = lo;
-            }
+            };
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i)
+                if (const size_t k = 2 * threadIdx.x + 512 * i; k < kp) write(k, keep[i]);
+            for (size_t k = 2 * threadIdx.x + 512 * kKeep; k < kp; k += 512) write(k, pair(k));
         } else {
             for (size_t k = 2 * threadIdx.x; k < kp; k += 512) {
                 uint32_t v = 0;
