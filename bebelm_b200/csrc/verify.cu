@@ -242,11 +242,17 @@ struct Row {
     double c, k;
     float lim;  // logits at and below it weigh nothing (2^-1000), NaN neither
     // maximum m and sum s of exp((l - m) / temperature), scale = log2(e) / temperature
-    __device__ __forceinline__ void logits(double m, double s, double scale) {
-        const bool any = s > 0.0;  // else nothing is above -inf
-        c = any ? scale : 0.0;
-        k = any ? -(m * scale) - log2(s) : 0.0;
-        lim = any ? (float)((-1000.0 - k) / scale) : CUDART_INF_F;
+    __device__ __forceinline__ void logits(float m, double s, double scale) {
+        const double mc = (double)m * scale;
+        if (!(s > 0.0)) {  // nothing is above -inf
+            c = k = 0.0, lim = CUDART_INF_F;
+        } else if (fabs(mc) >= 1073741824.0) {
+            // A step of f32 at m weighs 2^-64 or less: what is not m is nothing (and c m has no bits left for the rest)
+            c = 0.0, k = -log2(s), lim = nextafterf(m, -CUDART_INF_F);
+        } else {
+            c = scale, k = -mc - log2(s), lim = (float)((-1000.0 - k) / scale);
+            if (fma((double)lim, c, k) >= -1000.0) lim = nextafterf(lim, -CUDART_INF_F);  // rounded up: the last value below
+        }
     }
     __device__ __forceinline__ double weigh(float l) const {
         if constexpr (PROBS) return clean_p(l);

@@ -247,3 +247,19 @@ def test_samples_follow_the_target():
     o, _ = run(t, tok, rng.random((n, 1)).astype(np.float32), rng.random(n).astype(np.float32), dr)
     freq = np.bincount(o[:, 0], minlength=v) / n
     assert (np.abs(freq - p) <= 5 * np.sqrt(p * (1 - p) / n)).all()
+
+
+@pytest.mark.parametrize("draft_rows", [True, False])
+@pytest.mark.parametrize("base,step,temp", [(1000.0, 1e-3, 1e-6), (20.0, 1e-5, 1e-6), (1e12, 65536.0, 1.0), (-3e38, 1e32, 1.0), (3e38, 2e31, 1e6),
+                                            (0.0, 1e5, 300.0)])
+def test_logits_whose_neighbours_are_far_apart(base, step, temp, draft_rows):
+    """Rows where a step of f32 at the largest logit is not small against the temperature: what counts
+    still reaches down to the smallest weights, and the largest always counts."""
+    b, d, v = 12, 3, 9001
+    rng = np.random.default_rng(7)
+    target = (base + step * rng.integers(-30, 1, (b, d + 1, v))).astype(np.float32)
+    draft = (base + step * rng.integers(-30, 1, (b, d, v))).astype(np.float32)
+    tokens = np.array([[rng.choice(np.nonzero(draft[s, i] == draft[s, i].max())[0]) for i in range(d)] for s in range(b)], np.int32)
+    u, us = rng.random((b, d)).astype(np.float32), rng.random(b).astype(np.float32)
+    args = (target, tokens, u, us, draft if draft_rows else None)
+    same(run(*args, temperature=temp), reference(*args, temperature=temp))
