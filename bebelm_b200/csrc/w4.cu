@@ -18,8 +18,8 @@
 // Bound: a weight is read once, for at most 16 tokens, so HBM. On the way a weight costs 3/8 of a logic operation (two
 // masks and a shift for a word of 8 codes); unpacked to 16-bit floats it cost 11/8 and the logic unit bound the
 // kernel. Measured (with 16-bit floats): 128000 x 2048, 5 int8 tokens 27.7 us (44), 138 MB at 5.0 TB/s, 76 % of a
-// copy's rate; 8192 x 8192, one bf16 token 12.1 us (16), 35 MB at 2.9 TB/s: every CTA makes the digits first, with the
-// ring's first weights in flight; 2048 x 2048, one f32 token 4.2 us, all latency.
+// copy's rate; 8192 x 8192, one bf16 token 12.5 us (16), 35 MB at 2.8 TB/s: every CTA makes the digits first, with the
+// ring's first weights in flight; 2048 x 2048, one f32 token 4.3 us, all latency.
 //
 // Layout: rows padded to 128, inputs to 128 (scale 0). A tile of 16 rows x 128 inputs is 1024 bytes,
 // [row / 8][row % 8][q = 0..3][b = 0..3] words of 8 codes; the 8 tiles of 128 rows lie together, then the next 128
@@ -127,7 +127,7 @@ __device__ __forceinline__ void load_eight(Eight<D>& r, const W4X& x, bool pairs
     }
 }
 template <int D, int FB>
-__device__ __forceinline__ void make_digits(const Eight<D>& in, const W4X& x, const Digits& o, int t, int c) {
+__device__ __forceinline__ void make_digits(Eight<D>& in, const W4X& x, const Digits& o, int t, int c) {
     const int l = threadIdx.x & 15, b = l >> 2, q = l & 3;
     uint32_t w[D][2];
     int sum[D];
@@ -136,17 +136,26 @@ __device__ __forceinline__ void make_digits(const Eight<D>& in, const W4X& x, co
         w[0][0] = in.w[0], w[0][1] = in.w[1], scale = in.scale;
         sum[0] = __dp4a((int)w[0][0], 0x01010101, __dp4a((int)w[0][1], 0x01010101, 0));
     } else {
-        const float* v = in.v;
+        float* v = in.v;
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);  // an infinity or a NaN is the largest
 #pragma unroll
         for (int s = 8; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
         const bool odd = m > 0x7f7fffffu;
-        // 2^e: the largest to 2^22 .. 2^23, or half of that where its digits would not fit; e <= 122
-        int e = odd ? 0 : 22 - max((int)(m >> 23) - 127, -100);
-        if (__uint_as_float(m) * __uint_as_float((uint32_t)(127 + e) << 23) > 8355711.f) --e;  // 127 (65536 + 256 + 1)
-        const float f = __uint_as_float((uint32_t)(127 + e) << 23);
+        // 2^e: the largest to 2^22 .. 2^23, or half of that where its digits would not fit; -105 <= e <= 149 (2^-149 is the
+        // step of f32's smallest values, which are whole there), in two factors where 2^e would be too large
+        auto pow2 = [](int i) { return __uint_as_float((uint32_t)(127 + i) << 23); };
+        int e = odd ? 0 : 22 - ((int)(m >> 23) - 127);
+        const bool tiny = e > 122;
+        float most = __uint_as_float(m);
+        if (tiny) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= pow2(27);
+            most *= pow2(27), e -= 27;
+        }
+        if (most * pow2(e) > 8355711.f) --e;  // 127 (65536 + 256 + 1)
+        const float f = pow2(e);
         // X + 0x808080 has the digits + 128 as its bytes
         uint32_t u[8];
 #pragma unroll
@@ -161,7 +170,7 @@ __device__ __forceinline__ void make_digits(const Eight<D>& in, const W4X& x, co
         }
 #pragma unroll
         for (int d = 0; d < D; ++d) sum[d] = __dp4a((int)w[d][0], 0x01010101, __dp4a((int)w[d][1], 0x01010101, 0));
-        scale = odd ? CUDART_NAN_F : __uint_as_float((uint32_t)(127 - e) << 23);
+        scale = odd ? CUDART_NAN_F : tiny ? pow2(-e) * pow2(-27) : pow2(-e);
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) {

@@ -177,6 +177,19 @@ def test_strided_and_unaligned_rows(kind, t):
     assert torch.equal(w.matmul(wide[:, :416], xs), w.matmul(wide[:, :416].contiguous(), xs))
 
 
+@pytest.mark.parametrize("t", [1, 7, 13, 40])
+@pytest.mark.parametrize("unit", [-147, -130, -100, 90])
+def test_the_smallest_and_large_activations(t, unit):
+    """Whole multiples of 2^unit with scales 1 and 1/2, zero points: every sum is a whole multiple of 2^(unit - 1)
+    below 2^24 of them, so outputs are exact down to f32's last denormal step, 2^-149."""
+    codes, sc, z = weights(300, 256, 64, 9, exact=True)
+    sc = sc.clamp(min=0.5)
+    x, _ = activations(t, 256, "f32", 0, 4, exact=True)
+    x = torch.ldexp(x, torch.tensor(unit, device="cuda")) if unit > -127 else torch.ldexp(torch.ldexp(x, torch.tensor(unit + 64, device="cuda")), torch.tensor(-64, device="cuda"))
+    w = bb.W4Weights(codes, sc, z, group=64)
+    assert torch.equal(w.matmul(x).double(), x.double() @ dense(codes, sc, z, 64).t())
+
+
 @pytest.mark.parametrize("t", [3, 70])
 def test_infinities_and_nan_stay_in_their_token(t):
     codes, sc, z = weights(64, 256, 64, 2)
