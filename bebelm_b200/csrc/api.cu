@@ -2770,6 +2770,16 @@ int w4_x(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, const 
     return 0;
 }
 
+// What decides a verification's slices and so its workspace, for the query and the call alike: draft rows are not
+// read at temperature 0 and where there are no drafts.
+VerifyArgs verify_shape(size_t n_seqs, size_t n_drafts, size_t vocab, const float* draft, int probs, float temperature) {
+    VerifyArgs a{};
+    a.seqs = (int)n_seqs, a.drafts = (int)n_drafts, a.vocab = vocab;
+    a.draft = temperature == 0.f || n_drafts == 0 ? nullptr : draft;
+    a.probs = probs ? 1 : 0, a.temperature = temperature;
+    return a;
+}
+
 }  // namespace
 
 extern "C" {
@@ -2877,10 +2887,8 @@ int bebelm_verify_workspace(size_t n_seqs, size_t n_drafts, size_t vocab, int dr
                     n_seqs, n_drafts, vocab);
     int dev;
     TRY(current_device_cached(&dev));
-    VerifyArgs a{};
-    a.seqs = (int)n_seqs, a.drafts = (int)n_drafts, a.vocab = vocab, a.probs = probs, a.temperature = temperature;
     static const float some = 0.f;
-    a.draft = draft_rows ? &some : nullptr;
+    const VerifyArgs a = verify_shape(n_seqs, n_drafts, vocab, draft_rows ? &some : nullptr, probs, temperature);
     *bytes = n_seqs ? verify_workspace(a, num_sms_of(dev)) : 0;
     return 0;
 }
@@ -2919,12 +2927,9 @@ int bebelm_verify_drafts(const float* target, size_t target_stride, const float*
     TRY(current_device_cached(&dev));
     cudaStream_t s = as_stream(stream);
     const int sms = num_sms_of(dev);
-    VerifyArgs a{};
-    a.target = target, a.draft = greedy || !n_drafts ? nullptr : draft;
-    a.target_stride = target_stride, a.draft_stride = draft_stride, a.vocab = vocab;
-    a.seqs = (int)n_seqs, a.drafts = (int)n_drafts;
+    VerifyArgs a = verify_shape(n_seqs, n_drafts, vocab, draft, probs, temperature);
+    a.target = target, a.target_stride = target_stride, a.draft_stride = draft_stride;
     a.tokens = tokens, a.n_drafts = n_per_seq, a.u = u, a.u_sample = u_sample;
-    a.probs = probs ? 1 : 0, a.temperature = temperature;
     a.out = out_tokens, a.accepted = accepted, a.workspace = workspace;
     const size_t need = verify_workspace(a, sms);
     if (mem == BEBELM_MEM_DEVICE) {

@@ -4,6 +4,8 @@ Outputs are whole numbers and must be equal. A border case (a random number with
 border between two tokens) would need a coincidence of 1e-10 in these seeded inputs for the
 drawn token, and of 1e-6 for an acceptance.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -263,3 +265,27 @@ def test_logits_whose_neighbours_are_far_apart(base, step, temp, draft_rows):
     u, us = rng.random((b, d)).astype(np.float32), rng.random(b).astype(np.float32)
     args = (target, tokens, u, us, draft if draft_rows else None)
     same(run(*args, temperature=temp), reference(*args, temperature=temp))
+
+
+@pytest.mark.parametrize("temp", [0.0, 1.0])
+@pytest.mark.parametrize("draft_rows", [0, 1])
+def test_the_queried_workspace_is_enough(draft_rows, temp):
+    """C callers: a call with exactly the bytes that bebelm_verify_workspace gives for the same arguments, draft rows at
+    temperature 0 (where they are not read) and without drafts included. All shapes share buffers of the largest one."""
+    L = bb.load_library()
+    vocab, n = 8192, C.c_size_t()
+    rows = torch.randn(128 * 13, vocab, device="cuda")
+    ints, floats = torch.zeros(128 * 13, dtype=torch.int32, device="cuda"), torch.rand(128 * 13, device="cuda")
+    out, acc = torch.empty(128 * 13, dtype=torch.int32, device="cuda"), torch.empty(128, dtype=torch.int32, device="cuda")
+    ws = torch.empty(8 << 20, dtype=torch.uint8, device="cuda")
+    bad = []
+    for b in list(range(1, 60)) + [64, 70, 99, 128]:
+        for d in (0, 1, 4, 9, 12):
+            assert L.bebelm_verify_workspace(b, d, vocab, draft_rows, 0, temp, C.byref(n)) == bb.OK and n.value <= ws.numel()
+            rc = L.bebelm_verify_drafts(rows.data_ptr(), vocab, rows.data_ptr() if draft_rows else None, vocab, b, d, vocab, 0, temp,
+                                        ints.data_ptr(), None, floats.data_ptr(), floats.data_ptr(), out.data_ptr(), acc.data_ptr(),
+                                        ws.data_ptr() if n.value else None, n.value, bb.MEM_DEVICE, None)
+            if rc != bb.OK:
+                bad.append((b, d, bb.last_error()))
+    torch.cuda.synchronize()
+    assert not bad, (len(bad), bad[:3])
