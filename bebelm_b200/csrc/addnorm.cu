@@ -88,11 +88,8 @@ __device__ __forceinline__ double warp_sum(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
+// |v| as a whole number: in the order of the values, an infinity above them and a NaN above that
+__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // One row per blockDim.x threads (a warp when blockDim.y > 1 rows share the CTA); thread x holds
 // the NV runs of 8 values that start at 8 (x + i blockDim.x).
@@ -102,7 +99,7 @@ __device__ __forceinline__ float warp_max(float v) {
 template <class T, class O, int NV, bool VEC>
 __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 && NV == 2 ? 2 : 0) add_rmsnorm_kernel(AddNormArgs a) {
     __shared__ double s_part[32];
-    __shared__ float s_max[32];
+    __shared__ unsigned s_max[32];
     const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;  // only whole warps leave, and only where no barrier follows
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -145,7 +142,7 @@ __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 &
     }
     const float mean = __double2float_rn(ss / (double)a.n);
     const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, a.eps)));
-    float amax = 0.f;
+    unsigned most = 0;  // of the magnitudes, as a NaN has to be seen
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const size_t e = 8 * ((size_t)threadIdx.x + (size_t)i * blockDim.x);
@@ -164,29 +161,32 @@ __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 &
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[i][j]));
-            amax = warp_max(amax);
+                for (int j = 0; j < 8; ++j) most = max(most, magnitude(v[i][j]));
+            most = __reduce_max_sync(0xffffffffu, most);
             if (warps > 1) {
-                if (lane == 0) s_max[warp] = amax;
+                if (lane == 0) s_max[warp] = most;
                 __syncthreads();
-                amax = warp_max(lane < warps ? s_max[lane] : 0.f);
+                most = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[lane] : 0u);
             }
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const size_t e = 8 * ((size_t)threadIdx.x + (size_t)i * blockDim.x);
             if (a.group) {  // a group is group / 8 neighbouring lanes
-                amax = 0.f;
+                most = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[i][j]));
-                for (unsigned o = 1; o < a.group / 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                for (int j = 0; j < 8; ++j) most = max(most, magnitude(v[i][j]));
+                for (unsigned o = 1; o < a.group / 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
             }
             if (e >= a.n) continue;
+            // a group that is not finite: codes 0 and a scale of NaN, so that it reads back as NaN
+            const bool finite = most < 0x7f800000u;
+            const float amax = __uint_as_float(finite ? most : 0x7fc00000u);
             const float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.f;
             alignas(8) signed char q[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                q[j] = (signed char)fminf(fmaxf(roundf(__fmul_rn(v[i][j], inv)), -127.f), 127.f);
+                q[j] = finite ? (signed char)fminf(fmaxf(roundf(__fmul_rn(v[i][j], inv)), -127.f), 127.f) : (signed char)0;
             signed char* y = static_cast<signed char*>(a.y) + row * a.n + e;
             if constexpr (VEC) {
                 *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(q);

@@ -392,8 +392,9 @@ BEBELM_API int bebelm_sample_greedy(float* logits, size_t n, const uint32_t* his
  *    (scale = max|t| / 127, codes rounded half away from zero; a group of zeros has scale 0).
  *    y may be x or residual when their type and rows are the same; y and sum_out are distinct.
  * The steps and their f32 roundings are the reference's (each one IEEE operation, the sum of
- * squares in f64), so codes do not depend on the launch. Values are expected finite; a NaN or
- * an infinity stays in its row. Host buffers are contiguous. Device buffers lie on the current device. */
+ * squares in f64), so codes do not depend on the launch. Values are expected finite (and below 1.8e19, where f32 squares
+ * overflow and the row's factor becomes 0); a NaN or an infinity stays in its row, and a group of 8-bit values with one among
+ * its t has scale NaN and codes 0. Host buffers are contiguous. Device buffers lie on the current device. */
 BEBELM_API int bebelm_add_rmsnorm(const void* x, size_t x_stride, const void* residual, size_t residual_stride,
                                   int dtype, size_t rows, size_t n, const float* gain, float eps, void* sum_out,
                                   size_t sum_stride, void* y, int y_dtype, float* y_scales, size_t group, int mem,

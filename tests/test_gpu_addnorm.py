@@ -191,3 +191,47 @@ def test_on_another_stream_and_in_a_graph():
     graph.replay()
     want, wh = bb.add_rmsnorm(x, gain, r)
     assert torch.equal(y, want) and torch.equal(h, wh)
+
+
+def float_row_and_codes(x, gain, group, r=None):
+    """The float output and what the 8-bit one stands for."""
+    y, _ = bb.add_rmsnorm(x, gain, r, out_dtype=bb.F32)
+    q, sc, _ = bb.add_rmsnorm(x, gain, r, out_dtype=bb.INT8, group=group)
+    rows, n = x.shape
+    sc = sc.view(rows, -1)
+    return y, q, sc, (q.view(rows, sc.shape[1], -1).float() * sc[..., None]).view(rows, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,group", [(64, 0), (256, 32), (2048, 256), (2048, 0), (41, 0), (16384, 128)])
+def test_8_bit_rows_that_are_not_finite(n, group, dtype):
+    """A group of 8-bit outputs with a NaN or an infinity among its values reads back as NaN: its scale is NaN, its codes 0.
+    Groups and rows beside it are as they are without it."""
+    x, r, gain = inputs(6, n, dtype, n)
+    clean = bb.add_rmsnorm(x, gain, r, out_dtype=bb.INT8, group=group)
+    x[1, n // 2] = float("nan")
+    x[2, n - 1] = float("inf")
+    x[4, 0], x[4, n // 3] = float("-inf"), float("inf")
+    y, q, sc, back = float_row_and_codes(x, gain, group, r)
+    assert torch.isnan(y[1]).all() and torch.isnan(sc[1]).all()  # one NaN makes the row's sum one
+    for row in (1, 2, 4):
+        broken = (~torch.isfinite(y[row])).view(-1, group or n).any(-1)
+        assert broken.any() and torch.equal(torch.isnan(sc[row]), broken)
+        assert torch.equal(torch.isnan(back[row]), broken.repeat_interleave(group or n))
+        assert (q[row].view(-1, group or n)[broken] == 0).all()
+    for row in (0, 3, 5):
+        assert torch.equal(q[row], clean[0][row]) and torch.equal(sc[row], clean[1][row].view(-1))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("group", [0, 64])
+def test_8_bit_rows_under_a_gain_that_is_not_finite(group, bad):
+    x, r, gain = inputs(3, 512, torch.float32, 3)
+    want = bb.add_rmsnorm(x, gain, r, out_dtype=bb.INT8, group=group)
+    gain[100] = bad
+    _, q, sc, back = float_row_and_codes(x, gain, group, r)
+    g = group or 512
+    hit = torch.arange(512 // g, device="cuda") == 100 // g
+    assert torch.equal(torch.isnan(sc), hit.expand(3, -1)) and torch.isnan(back[:, 100]).all()
+    keep = ~hit.repeat_interleave(g)
+    assert torch.equal(q[:, keep], want[0][:, keep]) and (q[:, ~keep] == 0).all()
