@@ -182,7 +182,12 @@ __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 &
             // a group that is not finite: codes 0 and a scale of NaN, so that it reads back as NaN
             const bool finite = most < 0x7f800000u;
             const float amax = __uint_as_float(finite ? most : 0x7fc00000u);
-            const float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.f;
+            float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.f;
+            if (amax > 0.f && amax < 0x1p-100f) {  // 127 / a leaves f32's range below 3.8e-37: both 2^64 times as large
+                inv = __fdiv_rn(127.0f, amax * 0x1p64f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] *= 0x1p64f;
+            }
             alignas(8) signed char q[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)

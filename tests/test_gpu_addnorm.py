@@ -235,3 +235,23 @@ def test_8_bit_rows_under_a_gain_that_is_not_finite(group, bad):
     assert torch.equal(torch.isnan(sc), hit.expand(3, -1)) and torch.isnan(back[:, 100]).all()
     keep = ~hit.repeat_interleave(g)
     assert torch.equal(q[:, keep], want[0][:, keep]) and (q[:, ~keep] == 0).all()
+
+
+@pytest.mark.parametrize("group", [0, 32])
+@pytest.mark.parametrize("unit", [-149, -140, -126, -122, -120, -100])
+def test_8_bit_rows_of_tiny_values(unit, group):
+    """Below 3.8e-37 the factor 127 / a is above f32's range. The codes are those of the same values 2^64 times as large, where
+    it is in range, and zeros stay zeros. h = 1 and 0 with eps = 0 makes t whole multiples of the gain's 2^unit."""
+    rows, n = 3, 256
+    x = torch.ones(rows, n, device="cuda")
+    x[1] = -1
+    g = torch.Generator(device="cuda").manual_seed(unit & 0xff)
+    gain = torch.randint(-9, 10, (n,), device="cuda", generator=g).double()
+    gain[3::5] = 0
+    small = (gain * 2.0 ** unit).float()
+    q, sc, _ = bb.add_rmsnorm(x, small, eps=0.0, out_dtype=bb.INT8, group=group)
+    want, want_sc, _ = bb.add_rmsnorm(x, gain.float(), eps=0.0, out_dtype=bb.INT8, group=group)
+    assert torch.equal(q, want) and (q[:, 3::5] == 0).all() and want.abs().max() == 127
+    exact = gain.view(-1, group or n).abs().amax(-1) * 2.0 ** unit / 127
+    # a / 127 rounded to f32: half a step, 2^-24 of it or half of the smallest denormal
+    assert ((sc.double() - exact).abs() <= (exact * 2.0 ** -24).clamp(min=2.0 ** -150)).all()
