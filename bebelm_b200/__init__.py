@@ -762,6 +762,9 @@ def attn_decode_batched(caches, layer: int, q, k, v, q_gain, k_gain, pos, theta:
 # ------------------------------------------- operators around the attention --
 # These are called once per layer and token, on small tensors: a call's checks are kept to what an
 # attribute read costs, since the kernels behind them take a few microseconds.
+#
+# ``stream`` (a torch stream or a cudaStream_t; default: torch's current one): the call's work is queued there. What the
+# caller passes has to be ready there and to live until that work is done; what the call allocates belongs to it.
 _TORCH_DTYPES = None  # torch dtype -> F32 / BF16 / INT8 / F16
 
 
@@ -820,19 +823,30 @@ def _stream_on(stream, dev: int) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _empty(shape, dtype, dev: int, stream):
+    """A result tensor of a call on ``stream``. The allocator orders a block's uses by the stream that it was
+    allocated under, so that has to be the stream that writes it: a block of the current stream's may have work
+    pending there. The current stream, where the caller reads it, is recorded as a second user."""
+    torch = _torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    ext = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=dev)
+    current = torch.cuda.current_stream(dev)
+    if ext.cuda_stream == current.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(ext):
+        t = torch.empty(shape, dtype=dtype, device=dev)
+    t.record_stream(current)
+    return t
+
+
 def _workspace(workspace, need: int, dev: int, stream):
     """(tensor, pointer, bytes): the caller's scratch, or one from torch's allocator, which keeps
     it from reuse on other streams until the work of ``stream`` that uses it is done."""
     if not need:
         return None, None, 0
-    torch = _torch
     if workspace is None:
-        if stream is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        else:
-            ext = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=dev)
-            with torch.cuda.stream(ext):
-                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = _empty(need, _torch.uint8, dev, stream)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
@@ -889,14 +903,14 @@ def add_rmsnorm(x, gain, residual=None, eps: float = RMS_EPS, out_dtype: int | N
     if od_torch is None:
         raise ValueError("out_dtype must be F32, BF16 or INT8")
     if out is None:
-        out = torch.empty(x.shape, dtype=od_torch, device=dev)
+        out = _empty(x.shape, od_torch, dev, stream)
     else:
         _check_out(out, rows * n, od_torch, dev, "out")
     sp = None
     if od == INT8:
         ng = n // (group or n or 1)
         if scales is None:
-            scales = torch.empty((rows, ng), dtype=torch.float32, device=dev)
+            scales = _empty((rows, ng), torch.float32, dev, stream)
         else:
             _check_out(scales, rows * ng, torch.float32, dev, "scales")
         sp = scales.data_ptr()
@@ -911,7 +925,7 @@ def add_rmsnorm(x, gain, residual=None, eps: float = RMS_EPS, out_dtype: int | N
             raise ValueError("residual must have the type, shape and device of x")
         rs, rp = _rows_of(residual, "residual")[2], residual.data_ptr()
         if sum_out is None:
-            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            h = _empty(x.shape, x.dtype, dev, stream)
         else:
             if sum_out.dtype is not x.dtype or sum_out.shape != x.shape or sum_out.get_device() != dev:
                 raise ValueError("sum_out must have the type, shape and device of x")
@@ -1005,7 +1019,7 @@ class W4Weights:
             raise ValueError("products are F32 or BF16")
         od_torch = torch.float32 if od == F32 else torch.bfloat16
         if out is None:
-            out = torch.empty((*x.shape[:-1], self.n_out), dtype=od_torch, device=dev)
+            out = _empty((*x.shape[:-1], self.n_out), od_torch, dev, stream)
         else:
             _check_out(out, t * self.n_out, od_torch, dev, "out")
         xp = x.data_ptr()
@@ -1098,11 +1112,11 @@ def verify_drafts(target, tokens, u, u_sample, draft=None, n_drafts=None, temper
         _check_in(u_sample, (b,), f32, dev, "u_sample")
         sp = u_sample.data_ptr()
     if out is None:
-        out = torch.empty((b, d1), dtype=i32, device=dev)
+        out = _empty((b, d1), i32, dev, stream)
     else:
         _check_out(out, b * d1, i32, dev, "out")
     if accepted is None:
-        accepted = torch.empty((b,), dtype=i32, device=dev)
+        accepted = _empty((b,), i32, dev, stream)
     else:
         _check_out(accepted, b, i32, dev, "accepted")
     need = C.c_size_t()

@@ -223,3 +223,72 @@ def test_workspaces_are_checked():
     assert product(ws.data_ptr(), 1 << 19) == bb.OK
     torch.cuda.synchronize()
     assert torch.equal(y, w.matmul(x))
+
+
+def later(stream, ms=60):
+    """Keeps a stream busy for a while (about 2 million cycles a millisecond)."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(2_000_000 * ms)
+
+
+def calls_on(stream):
+    """Each operator on ``stream`` with results of its own: name -> function that gives them."""
+    n = 2 ** 21
+    x, gain = torch.randn(64, n // 64, device="cuda"), torch.ones(n // 64, device="cuda")
+    codes, sc, z = W.weights(n // 64, 256, 64, 3)
+    w, a = bb.W4Weights(codes, sc, z, group=64), torch.randn(64, 256, device="cuda")
+    target, tokens = torch.randn(4096, 1, 64, device="cuda"), torch.zeros(4096, 0, dtype=torch.int32, device="cuda")
+    return {"add_rmsnorm": lambda: bb.add_rmsnorm(x, gain, x, stream=stream),
+            "codes": lambda: bb.add_rmsnorm(x, gain, x, out_dtype=bb.INT8, group=32, stream=stream),
+            "matmul": lambda: (w.matmul(a, stream=stream),),
+            "verify_drafts": lambda: bb.verify_drafts(target, tokens, None, None, temperature=0.0, stream=stream)}
+
+
+@pytest.mark.parametrize("raw", [False, True])
+@pytest.mark.parametrize("name", ["add_rmsnorm", "codes", "matmul", "verify_drafts"])
+def test_results_of_a_call_on_another_stream(name, raw):
+    """Blocks of the allocator's and the streams they are in use on. (1) Blocks that the current stream still works with,
+    freed before the call: a result on another stream gets none of them. (2) Results dropped while their stream still works with
+    them: an allocation of the current stream gets none of them. (3) Results dropped while the current stream still reads them: the next call on
+    the other stream gets none of them."""
+    side, current = torch.cuda.Stream(), torch.cuda.current_stream()
+    call = calls_on(side.cuda_stream if raw else side)[name]
+    torch.cuda.synchronize()
+    got = call()
+    side.synchronize()
+    want = [t.clone() for t in got]
+    del got
+    torch.cuda.synchronize()
+    spans = lambda ts: [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts]
+    apart = lambda places, ts: all(p1 <= q0 or q1 <= p0 for p0, p1 in places for q0, q1 in spans(ts))
+
+    held = [torch.full_like(t, 5) for t in want for _ in range(4)]
+    later(current)
+    copies = [t.clone() for t in held]  # queued behind the wait
+    places = spans(held)
+    del held
+    got = call()
+    assert apart(places, got)
+    torch.cuda.synchronize()
+    assert all((c == 5).all() for c in copies) and all(torch.equal(a, b) for a, b in zip(got, want))
+    del got, copies
+
+    later(side)
+    got = call()
+    places = spans(got)
+    del got
+    fresh = [torch.empty_like(t) for t in want for _ in range(4)]
+    assert apart(places, fresh)
+    torch.cuda.synchronize()
+    del fresh
+
+    got = call()
+    current.wait_stream(side)
+    later(current)
+    read = [t.clone() for t in got]
+    places = spans(got)
+    del got
+    other = call()
+    assert apart(places, other)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(read, want)) and all(torch.equal(a, b) for a, b in zip(other, want))
