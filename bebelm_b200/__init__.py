@@ -236,6 +236,41 @@ def _stream_ptr(stream, mem=MEM_DEVICE):
     return C.c_void_p(int(stream))
 
 
+def _cuda_torch():
+    global _torch
+    if not _torch:
+        import torch
+        _torch = torch
+    return _torch
+
+
+def _torch_stream(stream, dev: int):
+    return stream if hasattr(stream, "cuda_stream") else _torch.cuda.ExternalStream(int(stream), device=dev)
+
+
+def _empty(shape, dtype, dev: int, stream):
+    """A result tensor of a call on ``stream``. The allocator orders a block's uses by the stream that it was
+    allocated under, so that has to be the stream that writes it: a block of the current stream's may have work
+    pending there. The current stream, where the caller reads it, is recorded as a second user."""
+    torch = _torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    ext = _torch_stream(stream, dev)
+    current = torch.cuda.current_stream(dev)
+    if ext.cuda_stream == current.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(ext):
+        t = torch.empty(shape, dtype=dtype, device=dev)
+    t.record_stream(current)
+    return t
+
+
+def _empty_like_on(like, shape, stream, dtype=None):
+    """:func:`_empty` on the device of a tensor, in its type unless one is given."""
+    _cuda_torch()
+    return _empty(shape, like.dtype if dtype is None else dtype, like.get_device(), stream)
+
+
 # ------------------------------------------------------------------ drop-ins --
 def attention_decode(q, k, v, n_ctx: int, n_heads: int, n_kv_heads: int, head_dim: int) -> np.ndarray:
     """``attention_decode`` (src/kernels/attention.rs:17-26) on the GPU; host float32 in/out."""
@@ -382,8 +417,8 @@ class Cache:
         (qb, kb, vb, qg, kg), mem = _bufs(q, k, v, q_gain, k_gain)
         n_heads = (qb[2].size if mem == MEM_HOST else qb[2].numel()) // self.head_dim
         if out is None:
-            out = np.zeros(n_heads * self.head_dim, np.float32) if mem == MEM_HOST else qb[2].new_empty(
-                n_heads * self.head_dim, dtype=qb[2].dtype)
+            out = np.zeros(n_heads * self.head_dim, np.float32) if mem == MEM_HOST else _empty_like_on(
+                qb[2], n_heads * self.head_dim, stream)
         ob, _, _ = _buf(out)
         _check(load_library().bebelm_attn_step(self._h, layer, n_heads, qb[0], kb[0], vb[0], qg[0], kg[0], theta, eps,
                                                pos, ob, mem, _stream_ptr(stream, mem)))
@@ -398,7 +433,7 @@ class Cache:
         n_heads = (qb[2].size if mem == MEM_HOST else qb[2].numel()) // self.head_dim
         n_out = group.world * n_heads * self.head_dim
         if out is None:
-            out = np.zeros(n_out, np.float32) if mem == MEM_HOST else qb[2].new_empty(n_out, dtype=qb[2].dtype)
+            out = np.zeros(n_out, np.float32) if mem == MEM_HOST else _empty_like_on(qb[2], n_out, stream)
         ob, _, _ = _buf(out)
         _check(load_library().bebelm_attn_step_allgather(self._h, group._h, layer, n_heads, qb[0], kb[0], vb[0], qg[0],
                                                          kg[0], theta, eps, pos, ob, mem, _stream_ptr(stream, mem)))
@@ -417,7 +452,7 @@ class Cache:
         t = q.numel() // (world * n_heads * self.head_dim)
         in_dtype = BF16 if q.dtype == torch.bfloat16 else F32_TENSOR
         if out is None:
-            out = torch.empty((t, world * n_heads * self.head_dim), dtype=torch.float32, device=q.device)
+            out = _empty_like_on(q, (t, world * n_heads * self.head_dim), stream, torch.float32)
         _check(load_library().bebelm_attn_prefill_allgather(
             self._h, group._h, layer, n_heads, q.data_ptr(), k.data_ptr(), v.data_ptr(), in_dtype, t, pos0,
             q_gain.data_ptr(), k_gain.data_ptr(), theta, eps, out.data_ptr(), _stream_ptr(stream)))
@@ -436,8 +471,8 @@ class Cache:
         (qb,), mem = _bufs(q)
         n_heads = (qb[2].size if mem == MEM_HOST else qb[2].numel()) // self.head_dim
         if out is None:
-            out = np.zeros(n_heads * self.head_dim, np.float32) if mem == MEM_HOST else qb[2].new_empty(
-                n_heads * self.head_dim)
+            out = np.zeros(n_heads * self.head_dim, np.float32) if mem == MEM_HOST else _empty_like_on(
+                qb[2], n_heads * self.head_dim, stream)
         ob, _, _ = _buf(out)
         _check(load_library().bebelm_attn_decode_cached(self._h, layer, n_heads, qb[0], ob, mem, _stream_ptr(stream, mem)))
         return out
@@ -454,7 +489,7 @@ class Cache:
             in_dtype = BF16 if q.dtype == torch.bfloat16 else (F32_TENSOR if tensor_cores else F32)
             t = q.numel() // (n_heads * self.head_dim)
             if out is None:
-                out = torch.empty((t, n_heads * self.head_dim), dtype=torch.float32, device=q.device)
+                out = _empty_like_on(q, (t, n_heads * self.head_dim), stream, torch.float32)
             ptrs = [C.c_void_p(x.data_ptr()) for x in (q, k, v, q_gain, k_gain, out)]
             mem = MEM_DEVICE
             keep = (q, k, v, q_gain, k_gain, out)
@@ -514,7 +549,7 @@ def matmul(dtype: int, w, n_in: int, n_out: int, x, n_tokens: int = 1, out=None,
     if wm != xm:
         raise ValueError("weights and activations must both be host or both be device buffers")
     if out is None:
-        out = np.zeros((n_tokens, n_out), np.float32) if xm == MEM_HOST else xk.new_empty((n_tokens, n_out))
+        out = np.zeros((n_tokens, n_out), np.float32) if xm == MEM_HOST else _empty_like_on(xk, (n_tokens, n_out), stream)
     ob, _, _ = _buf(out)
     _check(load_library().bebelm_matmul(dtype, wp, n_in, n_out, xb, n_tokens, ob, xm, _stream_ptr(stream, xm)))
     return out.reshape(-1) if n_tokens == 1 and out.ndim > 1 and xm == MEM_HOST else out
@@ -586,8 +621,8 @@ class Head:
             tk = np.zeros(1, np.uint32) if token else None
         else:
             import torch
-            lg = hb[2].new_empty(self.vocab) if logits else None
-            tk = hb[2].new_zeros(1, dtype=torch.int32) if token else None
+            lg = _empty_like_on(hb[2], self.vocab, stream) if logits else None
+            tk = _empty_like_on(hb[2], 1, stream, torch.int32) if token else None
         lp = _buf(lg)[0] if lg is not None else None
         tp = None if tk is None else (tk.ctypes.data if mem == MEM_HOST else tk.data_ptr())
         _check(load_library().bebelm_head_logits(self._h, hb[0], eps, lp, tp, mem, _stream_ptr(stream, mem)))
@@ -619,10 +654,12 @@ def sample_greedy(logits, history=(), repeat_penalty: float = 1.0, stream=None):
         _check(load_library().bebelm_sample_greedy(lb[0], n, hist.ctypes.data if hist.size else None, hist.size,
                                                    repeat_penalty, tok.ctypes.data, mem, None))
         return int(tok[0])
-    import torch
+    torch = _cuda_torch()
     hist = history if hasattr(history, "data_ptr") else torch.tensor(list(history), dtype=torch.int32,
                                                                       device=lb[2].device)
-    tok = torch.zeros(1, dtype=torch.int32, device=lb[2].device)
+    if hist is not history and stream is not None:  # made under the current stream, read on the given one
+        hist.record_stream(_torch_stream(stream, hist.get_device()))
+    tok = _empty_like_on(lb[2], 1, stream, torch.int32)
     _check(load_library().bebelm_sample_greedy(lb[0], n, hist.data_ptr() if hist.numel() else None, hist.numel(),
                                                repeat_penalty, tok.data_ptr(), mem, _stream_ptr(stream, mem)))
     return tok
@@ -633,7 +670,7 @@ def attn_layer_step(cache: "Cache", layer: int, weights: AttnWeights, x, pos: in
     """``attn_step`` (src/model.rs:430-455) whole: x [hidden] -> out [hidden]."""
     (xb,), mem = _bufs(x)
     if out is None:
-        out = np.zeros(weights.hidden, np.float32) if mem == MEM_HOST else xb[2].new_empty(weights.hidden)
+        out = np.zeros(weights.hidden, np.float32) if mem == MEM_HOST else _empty_like_on(xb[2], weights.hidden, stream)
     ob, _, _ = _buf(out)
     _check(load_library().bebelm_attn_layer_step(cache._h, layer, weights._h, xb[0], pos, theta, eps, ob, mem,
                                                  _stream_ptr(stream, mem)))
@@ -647,7 +684,7 @@ def attn_layer_batch(cache: "Cache", layer: int, weights: AttnWeights, x, pos0: 
     n = xb[2].size if mem == MEM_HOST else xb[2].numel()
     t = n // weights.hidden
     if out is None:
-        out = np.zeros((t, weights.hidden), np.float32) if mem == MEM_HOST else xb[2].new_empty((t, weights.hidden))
+        out = np.zeros((t, weights.hidden), np.float32) if mem == MEM_HOST else _empty_like_on(xb[2], (t, weights.hidden), stream)
     ob, _, _ = _buf(out)
     _check(load_library().bebelm_attn_layer_batch(cache._h, layer, weights._h, xb[0], t, pos0, 1 if tensor_cores else 0,
                                                   theta, eps, ob, mem, _stream_ptr(stream, mem)))
@@ -751,7 +788,7 @@ def attn_decode_batched(caches, layer: int, q, k, v, q_gain, k_gain, pos, theta:
     numel = qb[2].size if mem == MEM_HOST else qb[2].numel()
     n_heads = numel // (n * caches[0].head_dim)
     if out is None:
-        out = np.zeros((n, n_heads * 64), np.float32) if mem == MEM_HOST else qb[2].new_empty((n, n_heads * 64))
+        out = np.zeros((n, n_heads * 64), np.float32) if mem == MEM_HOST else _empty_like_on(qb[2], (n, n_heads * 64), stream)
     ob, _, _ = _buf(out)
     posa = (C.c_size_t * n)(*[int(p) for p in pos])
     _check(load_library().bebelm_attn_decode_batched(arr, n, layer, n_heads, qb[0], kb[0], vb[0], qg[0], kg[0], theta,
@@ -768,19 +805,13 @@ def attn_decode_batched(caches, layer: int, q, k, v, q_gain, k_gain, pos, theta:
 _TORCH_DTYPES = None  # torch dtype -> F32 / BF16 / INT8 / F16
 
 
-def _cuda_torch():
-    global _torch, _TORCH_DTYPES
-    if _TORCH_DTYPES is None:
-        import torch
-        _torch = torch
-        _TORCH_DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: INT8, torch.float16: F16}
-    return _torch
-
-
 def _dtype_of(t, what: str) -> int:
     """F32 / BF16 / INT8 / F16 of a tensor or array."""
     if _is_torch(t):
-        _cuda_torch()
+        global _TORCH_DTYPES
+        if _TORCH_DTYPES is None:
+            torch = _cuda_torch()
+            _TORCH_DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: INT8, torch.float16: F16}
         dt = _TORCH_DTYPES.get(t.dtype)
     else:
         dt = {"float32": F32, "int8": INT8, "float16": F16}.get(str(t.dtype))
@@ -821,23 +852,6 @@ def _stream_on(stream, dev: int) -> int:
     if stream is None:
         return _torch._C._cuda_getCurrentRawStream(dev)
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-
-
-def _empty(shape, dtype, dev: int, stream):
-    """A result tensor of a call on ``stream``. The allocator orders a block's uses by the stream that it was
-    allocated under, so that has to be the stream that writes it: a block of the current stream's may have work
-    pending there. The current stream, where the caller reads it, is recorded as a second user."""
-    torch = _torch
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    ext = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=dev)
-    current = torch.cuda.current_stream(dev)
-    if ext.cuda_stream == current.cuda_stream:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    with torch.cuda.stream(ext):
-        t = torch.empty(shape, dtype=dtype, device=dev)
-    t.record_stream(current)
-    return t
 
 
 def _workspace(workspace, need: int, dev: int, stream):

@@ -244,15 +244,12 @@ def calls_on(stream):
             "verify_drafts": lambda: bb.verify_drafts(target, tokens, None, None, temperature=0.0, stream=stream)}
 
 
-@pytest.mark.parametrize("raw", [False, True])
-@pytest.mark.parametrize("name", ["add_rmsnorm", "codes", "matmul", "verify_drafts"])
-def test_results_of_a_call_on_another_stream(name, raw):
+def results_belong_to(side, call):
     """Blocks of the allocator's and the streams they are in use on. (1) Blocks that the current stream still works with,
     freed before the call: a result on another stream gets none of them. (2) Results dropped while their stream still works with
-    them: an allocation of the current stream gets none of them. (3) Results dropped while the current stream still reads them: the next call on
-    the other stream gets none of them."""
-    side, current = torch.cuda.Stream(), torch.cuda.current_stream()
-    call = calls_on(side.cuda_stream if raw else side)[name]
+    them: an allocation of the current stream gets none of them. (3) Results dropped while the current stream still reads them: the
+    next call on the other stream gets none of them."""
+    current = torch.cuda.current_stream()
     torch.cuda.synchronize()
     got = call()
     side.synchronize()
@@ -289,6 +286,51 @@ def test_results_of_a_call_on_another_stream(name, raw):
     places = spans(got)
     del got
     other = call()
-    assert apart(places, other)
+    assert apart(places, other) and not current.query()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(read, want)) and all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+@pytest.mark.parametrize("raw", [False, True])
+@pytest.mark.parametrize("name", ["add_rmsnorm", "codes", "matmul", "verify_drafts"])
+def test_results_of_a_call_on_another_stream(name, raw):
+    side = torch.cuda.Stream()
+    results_belong_to(side, calls_on(side.cuda_stream if raw else side)[name])
+
+
+@pytest.mark.parametrize("name", ["attn_prefill", "matmul", "logits", "sample_greedy", "attn_layer_batch"])
+def test_results_of_the_other_calls_on_another_stream(name):
+    """The same for the attention, the K-quant products, the head and the sampler."""
+    side = torch.cuda.Stream()
+    t, n_out = 300, 4096
+    rng = np.random.default_rng(3)
+    packed = lambda rows, n: (0.05 * rng.standard_normal((rows, n))).astype(np.float16).reshape(-1).view(np.uint8)
+    ones = torch.ones(64, device="cuda")
+    if name == "attn_prefill":
+        q, k, v = (torch.randn(t, n, device="cuda") for n in (HIDDEN, KVD, KVD))
+        caches = iter([bb.Cache(n_layers=1, n_kv_heads=KV, max_context=512) for _ in range(5)])  # (to clear one waits for the device)
+        kept = []
+
+        def call():
+            kept.append(next(caches))
+            return (kept[-1].attn_prefill(0, q, k, v, ones, ones, 0, n_heads=HEADS, stream=side),)
+    elif name == "matmul":
+        w, x = torch.from_numpy(packed(n_out, HIDDEN)).cuda(), torch.randn(t, HIDDEN, device="cuda")
+        call = lambda: (bb.matmul(bb.GGML_F16, w, HIDDEN, n_out, x, t, stream=side),)
+    elif name == "logits":
+        head, h = bb.Head(bb.GGML_F16, packed(60000, HIDDEN), HIDDEN, 60000, np.ones(HIDDEN, np.float32)), torch.randn(HIDDEN, device="cuda")
+        call = lambda: head.logits(h, stream=side)
+    elif name == "sample_greedy":
+        logits, history = torch.randn(60000, device="cuda"), torch.tensor([5, 7], dtype=torch.int32, device="cuda")
+        call = lambda: (bb.sample_greedy(logits, history, 1.0, stream=side),)
+    else:
+        gain = np.ones(64, np.float32)
+        weights = bb.AttnWeights((bb.GGML_F16, packed(HIDDEN, HIDDEN)), (bb.GGML_F16, packed(KVD, HIDDEN)), (bb.GGML_F16, packed(KVD, HIDDEN)),
+                                 (bb.GGML_F16, packed(HIDDEN, HIDDEN)), gain, gain, n_heads=HEADS, n_kv_heads=KV, hidden=HIDDEN)
+        x, kept = torch.randn(t, HIDDEN, device="cuda"), []
+        caches = iter([bb.Cache(n_layers=1, n_kv_heads=KV, max_context=512) for _ in range(5)])
+
+        def call():
+            kept.append(next(caches))
+            return (bb.attn_layer_batch(kept[-1], 0, weights, x, 0, stream=side),)
+    results_belong_to(side, call)
