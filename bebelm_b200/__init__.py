@@ -54,6 +54,7 @@ EXPORTS = [
     "bebelm_gguf_array_len", "bebelm_gguf_get_str_at", "bebelm_gguf_validate", "bebelm_attn_weights_from_gguf",
     "bebelm_head_from_gguf", "bebelm_step_plan_launch_allgather", "bebelm_attn_prefill_allgather",
     "bebelm_add_rmsnorm", "bebelm_w4_create", "bebelm_w4_destroy", "bebelm_w4_workspace", "bebelm_w4_matmul",
+    "bebelm_w4_check",
     "bebelm_verify_workspace", "bebelm_verify_drafts",
 ]
 GGML_F32, GGML_F16, GGML_Q4_K, GGML_Q6_K = 0, 1, 12, 14
@@ -159,6 +160,7 @@ def load_library(path: str = LIB_PATH):
         "bebelm_w4_destroy": ([vp], i),
         "bebelm_w4_workspace": ([vp, vp, i, sz, sz, sz, C.POINTER(sz)], i),
         "bebelm_w4_matmul": ([vp, vp, i, sz, vp, sz, sz, vp, i, vp, sz, i, vp], i),
+        "bebelm_w4_check": ([vp, vp], i),
         "bebelm_verify_workspace": ([sz, sz, sz, i, i, f, C.POINTER(sz)], i),
         "bebelm_verify_drafts": ([vp, sz, vp, sz, sz, sz, sz, i, f, vp, vp, vp, vp, vp, vp, vp, sz, i, vp], i),
     }
@@ -1042,6 +1044,12 @@ class W4Weights:
         ws, wp, wb = _workspace(workspace, need.value, dev, stream)
         _check(L.bebelm_w4_matmul(self._h, xp, dt, xs, sp, xg, t, out.data_ptr(), od, wp, wb, MEM_DEVICE, _stream_on(stream, dev)))
         return out
+
+    def check(self, stream=None) -> None:
+        """Synchronises the stream and raises if a bounded device-side wait of a product gave up since the last report
+        (its outputs are invalid then): after a graph's replays, or the last product of a run."""
+        _cuda_torch()
+        _check(load_library().bebelm_w4_check(self._h, _stream_on(stream, self.device)))
 
     def _x_group(self, n_groups: int) -> int:
         if n_groups <= 1:

@@ -2671,12 +2671,16 @@ struct bebelm_w4 {
     int device = 0;
     W4View v{};
     DevBuf codes, scales, zeros;
-    ErrWord err;  // a bounded wait of the many-token kernel that gave up
+    // A bounded wait of the many-token kernel that gave up: in a device-memory call (reported by the next product or
+    // bebelm_w4_check), and in a host-memory call, which has a word of its own (one such call runs at a time), so that
+    // no other thread's call can take its report.
+    ErrWord err, host_err;
     void release() {
         codes.release();
         scales.release();
         zeros.release();
         err.release();
+        host_err.release();
     }
 };
 
@@ -2696,6 +2700,7 @@ int w4_fill(bebelm_w4* W, const uint8_t* codes, const void* scales, const uint8_
     TRY(W->scales.ensure(ns * 2));
     if (zeros) TRY(W->zeros.ensure(tiles * 8 * (v.per_chunk == 4 ? 8 : 4)));
     TRY(W->err.ensure());
+    TRY(W->host_err.ensure());
     TRY(tmp.ensure(256 + (host ? pad256(cb) + pad256(2 * ng) + pad256(ng) : 0)));
     CUDA_TRY(cudaMemset(tmp.p, 0, 256));
     const void *dc = codes, *ds = scales, *dz = zeros;
@@ -2732,16 +2737,20 @@ bool w4_streams(const W4View& w, const W4X& x) {
 size_t w4_scratch(const W4View& w, const W4X& x) {
     return w4_streams(w, x) ? w4_stream_workspace(w, x) : w4_tc_workspace(w, x);
 }
-cudaError_t w4_run(const bebelm_w4* W, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms, cudaStream_t s) {
+cudaError_t w4_run(const bebelm_w4* W, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms, const ErrWord& err,
+                   cudaStream_t s) {
     if (w4_streams(W->v, x)) return launch_w4_stream(W->v, x, y, y_bf16, workspace, num_sms, s);
-    return launch_w4_tc(W->v, x, y, y_bf16, workspace, num_sms, W->err.d, s);
+    const bool expire = g_expire_waits > 0;  // test hook (bebelm_debug_expire_next_wait)
+    if (expire) --g_expire_waits;
+    return launch_w4_tc(W->v, x, y, y_bf16, workspace, num_sms, err.d, expire, s);
 }
 
-int w4_timeout(const bebelm_w4* W) {
-    const int e = W->err.read();
+// A report is taken by one caller only.
+int w4_timeout(const ErrWord& err) {
+    if (!err.read()) return 0;
+    const int e = __atomic_exchange_n(err.h, 0, __ATOMIC_ACQ_REL);
     if (!e) return 0;
-    *reinterpret_cast<volatile int*>(W->err.h) = 0;
-    return fail(BEBELM_ERR_TIMEOUT, "a device-side wait of a 4-bit product timed out (code %d)", e);
+    return fail(BEBELM_ERR_TIMEOUT, "a device-side wait of a 4-bit product timed out (code %d); outputs are invalid", e);
 }
 
 int w4_x(const bebelm_w4* W, const void* x, int x_dtype, size_t x_stride, const float* x_scales, size_t x_group,
@@ -2854,13 +2863,13 @@ int bebelm_w4_matmul(const bebelm_w4* W, const void* x, int x_dtype, size_t x_st
     DeviceGuard g(W->device);
     cudaStream_t s = as_stream(stream);
     const int sms = num_sms_of(W->device);
-    TRY(w4_timeout(W));  // of an earlier device-memory call
+    TRY(w4_timeout(W->err));  // of an earlier device-memory call
     if (mem == BEBELM_MEM_DEVICE) {
         const size_t need = w4_scratch(v, xv);
         if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
             return fail(BEBELM_ERR_INVALID, "the product needs %zu bytes of workspace, 256-byte aligned (got %zu)", need,
                         workspace ? workspace_bytes : 0);
-        CUDA_TRY(w4_run(W, xv, y, y_dtype == BEBELM_BF16, workspace, sms, s));
+        CUDA_TRY(w4_run(W, xv, y, y_dtype == BEBELM_BF16, workspace, sms, W->err, s));
         return 0;
     }
     std::lock_guard<std::mutex> lk(g_scratch_mu);
@@ -2874,9 +2883,16 @@ int bebelm_w4_matmul(const bebelm_w4* W, const void* x, int x_dtype, size_t x_st
     xv.scales = static_cast<const float*>(dsc);
     xv.stride = v.n_in;
     TRY(P->q8.ensure(std::max<size_t>(w4_scratch(v, xv), 256), false, s));
-    CUDA_TRY(w4_run(W, xv, o, y_dtype == BEBELM_BF16, P->q8.p, sms, s));
+    CUDA_TRY(w4_run(W, xv, o, y_dtype == BEBELM_BF16, P->q8.p, sms, W->host_err, s));
     TRY(stage_out(P, o, y, yb, s));
-    return w4_timeout(W);
+    return w4_timeout(W->host_err);
+}
+
+int bebelm_w4_check(const bebelm_w4* W, void* stream) {
+    if (!W) return fail(BEBELM_ERR_INVALID, "null weights");
+    DeviceGuard g(W->device);
+    CUDA_TRY(cudaStreamSynchronize(as_stream(stream)));
+    return w4_timeout(W->err);
 }
 
 int bebelm_verify_workspace(size_t n_seqs, size_t n_drafts, size_t vocab, int draft_rows, int probs, float temperature,

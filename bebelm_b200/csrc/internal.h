@@ -382,9 +382,9 @@ size_t w4_tc_workspace(const W4View& w, const W4X& x);
 cudaError_t launch_w4_stream(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms,
                              cudaStream_t s);
 // cudaErrorNotSupported (nothing launched) where the activations cannot be described to TMA. A bounded wait
-// that gives up stores kErrWaitTimeout to *err.
+// that gives up stores kErrWaitTimeout to *err; `expire` makes one give up (a test hook).
 cudaError_t launch_w4_tc(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms, int* err,
-                         cudaStream_t s);
+                         bool expire, cudaStream_t s);
 
 // ---- drafted tokens against the target's rows (verify.cu) ----
 struct VerifyArgs {

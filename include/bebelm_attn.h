@@ -217,7 +217,8 @@ BEBELM_API int bebelm_kv_check(const bebelm_kv* kv, void* stream);
  * the first CTA first waits, with a short limit, on a barrier nothing completes,
  * records BEBELM_ERR_TIMEOUT in the pool's error word and leaves once its own
  * copies have landed. No GPU fault is involved. Lets a test check that a wait
- * that gives up is reported and that the next call is correct again. */
+ * that gives up is reported and that the next call is correct again. The same
+ * for a launch of the many-token 4-bit product (reported by bebelm_w4_check). */
 BEBELM_API int bebelm_debug_expire_next_wait(int n_launches);
 
 /* ---------------------------------------------- quantized weights (GGML) --- */
@@ -424,11 +425,16 @@ BEBELM_API int bebelm_w4_workspace(const bebelm_w4* w, const void* x, int x_dtyp
  * A group is summed before its scale is applied, so the sum of |code - zero| |x| over a group has to
  * stay below 3.4e38. Infinities and NaN stay in their token's row. Device memory: `workspace` (256-byte aligned, of
  * bebelm_w4_workspace bytes) is used until the call's work is done; calls that may overlap need one
- * each. A bounded wait that gives up leaves its tile unwritten; the handle's next product reports it
- * (BEBELM_ERR_TIMEOUT). Host memory: none. */
+ * each. A bounded wait that gives up leaves its tile unwritten (BEBELM_ERR_TIMEOUT): host-memory calls report it themselves,
+ * for device memory, a captured graph's replays among it, bebelm_w4_check or the handle's next product does, once.
+ * Host memory: no workspace. */
 BEBELM_API int bebelm_w4_matmul(const bebelm_w4* w, const void* x, int x_dtype, size_t x_stride, const float* x_scales,
                                 size_t x_group, size_t n_tokens, void* y, int y_dtype, void* workspace,
                                 size_t workspace_bytes, int mem, void* stream);
+
+/* Synchronises the stream and reports whether a product of the handle timed out since the last report: call it on the
+ * stream of the products (after a graph's replays, or a run's last product) before their outputs are relied on. */
+BEBELM_API int bebelm_w4_check(const bebelm_w4* w, void* stream);
 
 /* ------------------------------------------ drafted tokens, verified ---
  * No counterpart in the reference. Tokens that a smaller model (or a lookup) drafted, checked

@@ -252,3 +252,55 @@ def test_two_streams_and_a_graph(kind, t):
     static.copy_(b)
     graph.replay()
     assert torch.equal(out, wb)
+
+
+@pytest.mark.parametrize("t,n_in,n_out", [(40, 1024, 300), (24, 256, 200 * 128), (200, 2048, 2048)])
+def test_a_wait_that_gives_up_is_reported(t, n_in, n_out):
+    """A bounded wait of the many-token kernel runs out (forced: the first CTA waits, with a short limit, on a barrier nothing
+    completes; no fault). Its tile stays unwritten, check() reports it once, the next product is right; a host-memory
+    call reports it itself; every replay of a graph that was captured with it is reported."""
+    L = bb.load_library()
+    codes, sc, z = weights(n_out, n_in, 64, 3)
+    w = bb.W4Weights(codes, sc, z, group=64)
+    x, _ = activations(t, n_in, "f32", 0, 4)
+    want = w.matmul(x)
+    w.check()
+    try:
+        out = torch.full_like(want, 7)
+        assert L.bebelm_debug_expire_next_wait(1) == bb.OK
+        w.matmul(x, out=out)
+        with pytest.raises(bb.BebelmError) as e:
+            w.check()
+        assert e.value.code == bb.ERR_TIMEOUT
+        tile = 32 if t <= 32 else 64 if t <= 64 else 128  # tokens
+        assert (out[:tile, :128] == 7).all()  # the first CTA's tile of 128 rows (its first)
+        wrong = (out != want).view(-1).nonzero().numel()
+        assert wrong <= t * n_out // 2
+        w.check()  # once
+        assert torch.equal(w.matmul(x), want)
+
+        xh = x.cpu().numpy()
+        assert L.bebelm_debug_expire_next_wait(1) == bb.OK
+        with pytest.raises(bb.BebelmError) as e:
+            w.matmul(xh)
+        assert e.value.code == bb.ERR_TIMEOUT
+        np.testing.assert_array_equal(w.matmul(xh), want.cpu().numpy())
+        w.check()
+
+        graph = torch.cuda.CUDAGraph()
+        assert L.bebelm_debug_expire_next_wait(1) == bb.OK
+        with torch.cuda.graph(graph):
+            w.matmul(x, out=out)
+        for _ in range(2):
+            graph.replay()
+            with pytest.raises(bb.BebelmError):
+                w.check()
+        # without a check the handle's next product reports it, before its own work
+        graph.replay()
+        torch.cuda.synchronize()
+        with pytest.raises(bb.BebelmError):
+            w.matmul(x)
+        assert torch.equal(w.matmul(x), want)
+    finally:
+        assert L.bebelm_debug_expire_next_wait(0) == bb.OK
+    w.check()

@@ -92,3 +92,7 @@ def test_python_shapes_are_checked():
         bb.W4Weights(np.zeros((4, 64), np.int32), np.zeros((4, 4), np.float16), group=32)
     with pytest.raises(ValueError):
         bb.verify_drafts(np.zeros((2, 3, 5), np.float32), np.zeros((2, 3), np.int32), None, None)
+
+
+def test_w4_check_needs_a_handle():
+    assert bb.load_library().bebelm_w4_check(None, None) == bb.ERR_INVALID and bb.last_error()
