@@ -88,8 +88,17 @@ __device__ __forceinline__ double warp_sum(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// |v| as a whole number: in the order of the values, an infinity above them and a NaN above that
-__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// the larger one; NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
 
 // One row per blockDim.x threads (a warp when blockDim.y > 1 rows share the CTA); thread x holds
 // the NV runs of 8 values that start at 8 (x + i blockDim.x).
@@ -99,7 +108,7 @@ __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(
 template <class T, class O, int NV, bool VEC>
 __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 && NV == 2 ? 2 : 0) add_rmsnorm_kernel(AddNormArgs a) {
     __shared__ double s_part[32];
-    __shared__ unsigned s_max[32];
+    __shared__ float s_max[32];
     const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;  // only whole warps leave, and only where no barrier follows
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -142,7 +151,7 @@ __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 &
     }
     const float mean = __double2float_rn(ss / (double)a.n);
     const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, a.eps)));
-    unsigned most = 0;  // of the magnitudes, as a NaN has to be seen
+    float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const size_t e = 8 * ((size_t)threadIdx.x + (size_t)i * blockDim.x);
@@ -161,37 +170,31 @@ __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 &
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) most = max(most, magnitude(v[i][j]));
-            most = __reduce_max_sync(0xffffffffu, most);
+                for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[i][j]));
+            amax = warp_max(amax);
             if (warps > 1) {
-                if (lane == 0) s_max[warp] = most;
+                if (lane == 0) s_max[warp] = amax;
                 __syncthreads();
-                most = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[lane] : 0u);
+                amax = warp_max(lane < warps ? s_max[lane] : 0.f);
             }
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const size_t e = 8 * ((size_t)threadIdx.x + (size_t)i * blockDim.x);
             if (a.group) {  // a group is group / 8 neighbouring lanes
-                most = 0;
+                amax = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) most = max(most, magnitude(v[i][j]));
-                for (unsigned o = 1; o < a.group / 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[i][j]));
+                for (unsigned o = 1; o < a.group / 8; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             }
             if (e >= a.n) continue;
-            // a group that is not finite: codes 0 and a scale of NaN, so that it reads back as NaN
-            const bool finite = most < 0x7f800000u;
-            const float amax = __uint_as_float(finite ? most : 0x7fc00000u);
-            float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.f;
-            if (amax > 0.f && amax < 0x1p-100f) {  // 127 / a leaves f32's range below 3.8e-37: both 2^64 times as large
-                inv = __fdiv_rn(127.0f, amax * 0x1p64f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] *= 0x1p64f;
-            }
+            // 127 / a leaves f32's range below 3.8e-37: there both are formed 2^64 times as large
+            const float up = amax < 0x1p-100f ? 0x1p64f : 1.f;
+            const float inv = amax > 0.f ? __fdiv_rn(127.0f, __fmul_rn(amax, up)) : 0.f;
             alignas(8) signed char q[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                q[j] = finite ? (signed char)fminf(fmaxf(roundf(__fmul_rn(v[i][j], inv)), -127.f), 127.f) : (signed char)0;
+            for (int j = 0; j < 8; ++j)  // |t inv| < 127.5; a NaN (0 times an infinity, or t's) gives 0
+                q[j] = (signed char)__float2int_rz(roundf(__fmul_rn(__fmul_rn(v[i][j], up), inv)));
             signed char* y = static_cast<signed char*>(a.y) + row * a.n + e;
             if constexpr (VEC) {
                 *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(q);
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(1024, VEC && sizeof(T) == 2 && sizeof(O) > 1 &
                     if (e + j < a.n) y[j] = q[j];
             }
             if (a.group ? e % a.group == 0 : e == 0)
-                a.y_scales[a.group ? row * (a.n / a.group) + e / a.group : row] = __fdiv_rn(amax, 127.0f);
+                a.y_scales[a.group ? row * (a.n / a.group) + e / a.group : row] = __fadd_rn(__fdiv_rn(amax, 127.0f), __fsub_rn(amax, amax));  // an infinity: NaN
         }
     }
 }
