@@ -31,8 +31,8 @@
 // and N / 2 FMAs a thread). Measured: 2048 bf16 tokens x 8192 x 2048, groups of 128, 86.7 us: 793 TFLOP/s, 47 % of a
 // library product's rate of 16-bit weights; 777 f32 tokens x 2048 x 2048, groups of 64, 24.5 us (two terms: 532 TFLOP/s
 // of MMAs, a tile a CTA); 24 f32 tokens x 5003 x 2080, groups of 32, 11.3 us, three CTAs a tile.
-// All waits are bounded (4 million polls, some 6 s); after one gives up the CTA's others do too, it waits (bounded) for
-// its copies and MMAs in flight, reports kErrWaitTimeout and stores nothing.
+// All waits are bounded (4 million polls, some 6 s); after one gives up the CTA waits (bounded) for its copies and MMAs
+// in flight, reports kErrWaitTimeout and stores nothing more.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -62,7 +62,7 @@ struct TcArgs {
     int x_group, x_shift;     // inputs of a group, and their log2 (7 where a group holds 128 or more)
     int y_bf16, tiles, plane_rows;  // plane_rows: rows of B between the terms
     int split;                // CTAs of a cluster that share a tile's inputs; 1: a CTA takes tiles of its own
-    int expire;               // test hook: the first CTA's first copy waits, with a short limit, on a barrier nothing completes
+    int expire;               // test hook: the first CTA first waits, with a short limit, on a barrier nothing completes
     int* err;
 };
 
@@ -75,7 +75,7 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {  // 128B swizzle,
 __host__ __device__ constexpr uint32_t instr_desc(int n, bool bf16) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity, const volatile int* failed = nullptr, int limit = kWaitLimit) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity, int limit = kWaitLimit) {
     for (int it = 0; it < limit; ++it) {
         uint32_t ok;
         asm volatile(
@@ -84,24 +84,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity, const v
             : "r"(bar), "r"(parity)
             : "memory");
         if (ok) return true;
-        if (failed && it % 1024 == 1023 && *failed) return false;  // a wait that this one may hang on gave up
     }
     return false;
 }
 // A try_wait takes about 280 cycles even for a phase that is complete, a test_wait 80; but polling with it slows the
 // other warps down. So one test, then try_wait, which sleeps.
-__device__ __forceinline__ bool mbar_ready_or_wait(uint32_t bar, unsigned parity, const volatile int* failed) {
+__device__ __forceinline__ bool mbar_ready_or_wait(uint32_t bar, unsigned parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
-    return ok || mbar_wait(bar, parity, failed);
+    return ok || mbar_wait(bar, parity);
 }
-// by a whole warp; `failed`: the CTA's word that a wait gave up, null where copies or MMAs in flight have to be waited for
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, unsigned parity, const volatile int* failed) {
-    return __all_sync(0xffffffffu, mbar_ready_or_wait(bar, parity, failed));
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, unsigned parity) {
+    return __all_sync(0xffffffffu, mbar_ready_or_wait(bar, parity));
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -332,7 +330,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         unsigned ph = 1;  // the first round passes
     };
     auto fill = [&](Fill& r, int stages, uint32_t full0, uint32_t empty0, uint32_t bytes) -> bool {
-        if (!mbar_wait_warp(empty0 + 8 * r.st, r.ph, &s_fail)) {
+        if (!mbar_wait_warp(empty0 + 8 * r.st, r.ph)) {
             if (lane == 0) s_fail = 1;
             return false;
         }
@@ -347,16 +345,14 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
     auto landed = [&](Fill& r, int stages, uint32_t full0) {
         for (; r.done > 0; --r.done) {
             if (--r.st < 0) r.st = stages - 1, r.ph ^= 1;
-            mbar_wait_warp(full0 + 8 * r.st, r.ph ^ 1, nullptr);
+            mbar_wait_warp(full0 + 8 * r.st, r.ph ^ 1);
         }
     };
     if (warp == 0) {
         Fill r;
         bool ok = true;
-        if (a.expire && blockIdx.x == 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(never, 0, nullptr, kWaitLimit >> 8));
-            if (lane == 0) s_fail = 1;
-        }
+        if (a.expire && blockIdx.x == 0 && !__all_sync(0xffffffffu, mbar_wait(never, 0, kWaitLimit >> 8)) && lane == 0) s_fail = 1;
+        __syncwarp();
         for (int tile = tile0; ok && tile < a.tiles; tile += tile_step) {
             const int t0 = tile / row_blocks * N;
             for (int i = 2 * c_lo; i < 2 * c_hi; ++i) {
@@ -408,7 +404,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         unsigned b_ph = 0, a_ph = 0, d_ph = 1;  // d_ph: of the accumulators' last reads; the first round passes
         bool ok = true;
         for (int c = first; ok && c < n_chunks; c += kIssuers) {
-            ok = mbar_wait_warp(a_full(0) + 8 * ab, a_ph, &s_fail);
+            ok = mbar_wait_warp(a_full(0) + 8 * ab, a_ph);
             if (!ok) break;
             const uint32_t ta = tmem + kColA + 64 * ab;
             uint64_t bd = 0;
@@ -418,11 +414,11 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
                 // The accumulator first: once it is free, every chunk before the last two is done, so the
                 // stage's phase before the one waited for is over whichever warp used it.
                 if (i % kUnit == 0) {
-                    ok = mbar_wait_warp(d_empty(0) + 8 * db, d_ph, &s_fail);
+                    ok = mbar_wait_warp(d_empty(0) + 8 * db, d_ph);
                     if (!ok) break;
                 }
                 if (i % 4 == 0) {
-                    ok = mbar_wait_warp(b_full(0) + 8 * st, b_ph, &s_fail);
+                    ok = mbar_wait_warp(b_full(0) + 8 * st, b_ph);
                     if (!ok) break;
                     bd = b0 + (uint64_t)(st * (L::kB >> 4));
                 }
@@ -456,14 +452,14 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
         }
         if (!ok && lane == 0) s_fail = 1;
         commit(drained + 8 * first);  // every MMA of this warp done, also after a failed wait
-        mbar_wait_warp(drained + 8 * first, 0, nullptr);
+        mbar_wait_warp(drained + 8 * first, 0);
     } else if (warp >= kConvert0 && warp < kEpi0) {
         const int w = warp & 3, g = lane >> 2, rec = pc == 4 ? 8 : 4, set = (warp - kConvert0) >> 2;
         bool ok = true;
         int st = set, ab = set;
         unsigned w_ph = 0, a_ph = 1;  // the first round of A buffers passes
         for (int c = set; c < n_chunks; c += 2) {
-            ok = mbar_wait_warp(w_full(st), w_ph, &s_fail) && mbar_wait_warp(a_empty(ab), a_ph, &s_fail);
+            ok = mbar_wait_warp(w_full(st), w_ph) && mbar_wait_warp(a_empty(ab), a_ph);
             if (!ok) break;
             tc_after();
             const unsigned char* base = sm + L::kOffW + st * L::kW;
@@ -516,10 +512,10 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
             for (int i = 0; i < C / 2; ++i) acc[i] = 0;
             for (int c = c_lo; ok && c < c_hi; ++c) {
                 const unsigned char* base = sm + L::kOffS + st * L::kS;
-                ok = mbar_wait_warp(s_full(st), s_ph, &s_fail);
+                ok = mbar_wait_warp(s_full(st), s_ph);
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    ok = ok && mbar_wait_warp(d_full(db), d_ph, &s_fail);
+                    ok = ok && mbar_wait_warp(d_full(db), d_ph);
                     if (!ok) break;
                     tc_after();
 #pragma unroll
@@ -563,7 +559,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
             if constexpr (SPLIT) {  // every MMA of this CTA is done: its activations' ring holds the part's sums
 #pragma unroll
                 for (int i = 0; i < C; ++i) reinterpret_cast<float*>(sm + L::kOffB)[(part * C + i) * kM + row] = half_of(acc[i / 2], i & 1);
-            } else if (ok && r < a.w.n_out) {
+            } else if (ok && r < a.w.n_out && !*reinterpret_cast<volatile int*>(&s_fail)) {
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const size_t t = (size_t)t0 + part * C + i;
