@@ -17,6 +17,7 @@ library is missing or no sm_100 device is visible, calls raise.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 
 import numpy as np
@@ -1001,8 +1002,12 @@ class W4Weights:
             t = x.size // self.n_in
             sc, xg = None, 0
             if x.dtype == np.int8:
-                sc = np.ascontiguousarray(x_scales, np.float32).reshape(t, -1)
-                xg = self._x_group(sc.shape[1] if t else 1)
+                if x_scales is None:
+                    raise ValueError("int8 activations need x_scales [n_tokens, n_in / x_group]")
+                sc = np.ascontiguousarray(x_scales, np.float32)
+                xg = self._x_group(sc.shape, x.shape[:-1])
+            elif x_scales is not None:
+                raise ValueError("x_scales are for int8 activations")
             if out_dtype not in (None, F32) or out is not None or workspace is not None:
                 raise ValueError("host products are float32, without buffers")
             y = np.empty((t, self.n_out), np.float32)
@@ -1020,11 +1025,9 @@ class W4Weights:
             raise ValueError(f"x has {n} columns, the weights {self.n_in}")
         sp, xg = None, 0
         if dt == INT8:
-            ns = x_scales.numel() if x_scales is not None else -1
-            if ns < t or x_scales.dtype is not torch.float32 or not x_scales.is_contiguous() or x_scales.get_device() != dev or (
-                    t and ns % t):
+            if x_scales is None or x_scales.dtype is not torch.float32 or not x_scales.is_contiguous() or x_scales.get_device() != dev:
                 raise ValueError("int8 activations need contiguous float32 x_scales [n_tokens, n_in / x_group]")
-            xg = self._x_group(ns // t if t else 1)
+            xg = self._x_group(x_scales.shape, x.shape[:-1])
             sp = x_scales.data_ptr()
         elif x_scales is not None:
             raise ValueError("x_scales are for int8 activations")
@@ -1051,12 +1054,17 @@ class W4Weights:
         _cuda_torch()
         _check(load_library().bebelm_w4_check(self._h, _stream_on(stream, self.device)))
 
-    def _x_group(self, n_groups: int) -> int:
-        if n_groups <= 1:
+    def _x_group(self, shape, lead) -> int:
+        """The inputs of a scale, 0 for all of a token's, from the shape of x_scales: x's leading dimensions or their product,
+        then the groups (left out where a token has one scale)."""
+        shape, lead = tuple(shape), tuple(lead)
+        tokens = (math.prod(lead),)
+        if shape in (lead, tokens):
             return 0
-        if self.n_in % n_groups:
-            raise ValueError(f"{n_groups} scales a token do not divide {self.n_in} inputs")
-        return self.n_in // n_groups
+        n = shape[-1] if shape[:-1] in (lead, tokens) else 0
+        if n < 1 or self.n_in % n:
+            raise ValueError(f"x_scales {list(shape)} are not [n_tokens, n_in / x_group] for x {[*lead, self.n_in]}")
+        return self.n_in // n if n > 1 else 0
 
     def close(self):
         if self._h:

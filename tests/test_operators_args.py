@@ -96,3 +96,36 @@ def test_python_shapes_are_checked():
 
 def test_w4_check_needs_a_handle():
     assert bb.load_library().bebelm_w4_check(None, None) == bb.ERR_INVALID and bb.last_error()
+
+
+def no_weights(n_in=512, n_out=4):
+    """W4Weights without a handle: what is checked before the library is called."""
+    w = object.__new__(bb.W4Weights)
+    w.n_in, w.n_out, w.group, w.device, w._h = n_in, n_out, 64, 0, C.c_void_p()
+    return w
+
+
+@pytest.mark.parametrize("shape,lead,group", [
+    ((3, 4), (3,), 128), ((3, 1), (3,), 0), ((3,), (3,), 0), ((4,), (), 128), ((1, 4), (), 128), ((), (), 0), ((1,), (), 0),
+    ((2, 3, 4), (2, 3), 128), ((6, 4), (2, 3), 128), ((2, 3), (2, 3), 0), ((6,), (2, 3), 0), ((0, 4), (0,), 128), ((4, 4), (4,), 128),
+    ((4, 3), (3,), None), ((12,), (3,), None), ((1, 3, 4), (3,), None), ((3, 2, 2), (3,), None), ((3, 0), (3,), None), ((3, 5), (3,), None),
+    ((4, 1), (3,), None), ((8,), (4,), None), ((3, 2, 4), (2, 3), None), ((4, 2, 3), (2, 3), None),
+])
+def test_the_shape_of_x_scales(shape, lead, group):
+    w = no_weights()
+    if group is not None:
+        assert w._x_group(shape, lead) == group
+        return
+    with pytest.raises(ValueError):
+        w._x_group(shape, lead)
+
+
+def test_w4_host_activations_are_checked():
+    """int8 activations without scales (one token too, which was taken as a token with a scale of NaN), scales of other shapes,
+    and scales beside float activations."""
+    w = no_weights()
+    q, x = np.ones((3, 512), np.int8), np.ones((3, 512), np.float32)
+    for args in ((q[:1], None), (q[0], None), (q, None), (q, np.ones((4, 3), np.float32)), (q, np.ones((3, 5), np.float32)),
+                 (x, np.ones((3, 4), np.float32)), (x[0], np.ones(4, np.float32))):
+        with pytest.raises(ValueError):
+            w.matmul(*args)
