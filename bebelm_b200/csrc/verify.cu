@@ -29,6 +29,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -559,15 +560,37 @@ int pick_ctas(const VerifyArgs& a) {
     return ctas;
 }
 
+// Whether a device runs clusters of 16 CTAs of a kernel, which have to be asked for; asked once a device. Where the
+// answer is an error it is no.
+bool clusters_of_16(const void* kernel, int threads, std::atomic<int>* known) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    int k = known[dev].load(std::memory_order_acquire);
+    if (k) return k > 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3((unsigned)threads);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 16;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const bool yes = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                     cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+    if (!yes) cudaGetLastError();
+    known[dev].store(yes ? 2 : 1, std::memory_order_release);
+    return yes;
+}
+
 template <int PT, bool VEC, bool PROBS>
 cudaError_t launch_pick(const VerifyArgs& a, const RowPart* parts, int slices, int num_sms, cudaStream_t s) {
     auto kernel = verify_pick_kernel<PT, VEC, PROBS>;
     int ctas = pick_ctas(a);
-    if (PT == 1024 && a.vocab >= 65536 && a.seqs * 16 <= num_sms) {  // 16 have to be asked for
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
+    static std::atomic<int> known[64];
+    if (PT == 1024 && a.vocab >= 65536 && a.seqs * 16 <= num_sms && clusters_of_16(reinterpret_cast<const void*>(kernel), PT, known))
         ctas = 16;
-    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.seqs * ctas));
     cfg.blockDim = dim3(PT);
