@@ -9,8 +9,13 @@
 // The inner sum runs on the tensor cores in whole numbers (m16n8k32, u8 x s8 -> s32), exactly. int8 activations are
 // one such product. bf16 and f32 activations are made whole per token and 128 inputs: X = round(x · 2^e), e chosen
 // so that the largest |X| is in (2^21.99, 2^22.99), and X = 65536 d1 + 256 d2 + d3 with d in [-128, 127]: three
-// products. That keeps an activation to 2^-23 of the largest of its 128 (half a step of X; a sum's error is that
-// of f32 sums), and bf16 ones down to 2^-16 of the largest exactly. A chunk with an infinity or a NaN is a NaN.
+// products. That keeps an activation to 2^-23 of the largest of its 128 (half a step of X). Where the largest is at most
+// 8 times the mean magnitude (6 standard deviations of normal values) that is 2^-20 of the mean, and a sum's error is that of f32
+// sums. Where it is more, a few far larger activations would leave the rest few bits that the weights may yet see alone: there
+// what rounding left is kept too, in units of 2^-15, as two more digits and products: 2^-38 of the largest. They cost 33 to
+// 50 % of a call's time (2048 x 2048 4.4 -> 6.6 us, 8192 x 8192 12.3 -> 16.7 us, 128000 x 2048 32.4 -> 40.6 us, each with
+// two such activations a token), and run in a loop of their own, since in one loop they took 1 us of the others' time. A chunk
+// with an infinity or a NaN is a NaN.
 // z is taken off as z · Σ X, also whole: the accumulators start at -z Σ d, plus the bits of 1.5 · 2^23, so that they
 // are read as floats without a conversion (|Σ (c - z) d| <= 127 · 128 · 128 < 2^22). A flush per group makes a float of
 // the digits and applies the scales in f32.
@@ -18,8 +23,8 @@
 // Bound: a weight is read once, for at most 16 tokens, so HBM. On the way a weight costs 3/8 of a logic operation (two
 // masks and a shift for a word of 8 codes); unpacked to 16-bit floats it cost 11/8 and the logic unit bound the
 // kernel. Measured (with 16-bit floats): 128000 x 2048, 5 int8 tokens 27.7 us (44), 138 MB at 5.0 TB/s, 76 % of a
-// copy's rate; 8192 x 8192, one bf16 token 12.5 us (16), 35 MB at 2.8 TB/s: every CTA makes the digits first, with the
-// ring's first weights in flight; 2048 x 2048, one f32 token 4.3 us, all latency.
+// copy's rate; 8192 x 8192, one bf16 token 12.4 us (16), 35 MB at 2.8 TB/s: every CTA makes the digits first, with the
+// ring's first weights in flight; 2048 x 2048, one f32 token 4.4 us, all latency.
 //
 // Layout: rows padded to 128, inputs to 128 (scale 0). A tile of 16 rows x 128 inputs is 1024 bytes,
 // [row / 8][row % 8][q = 0..3][b = 0..3] words of 8 codes; the 8 tiles of 128 rows lie together, then the next 128
@@ -33,6 +38,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "internal.h"
 
@@ -59,22 +65,26 @@ __device__ __forceinline__ float scale_of(uint32_t h, int bf16) {
     return __half2float(__half(r));
 }
 
-// The activations as digits, in shared memory or (where that is too small) the workspace: D planes of rows of
-// `row` bytes, and a record per flush and token: the digits' sums and the scale, {Σ d, scale} or {Σ d1, Σ d2, Σ d3, scale}.
+// The activations as digits, in shared memory or (where that is too small) the workspace: planes of rows of `row`
+// bytes (1, or 3 and the 2 of the low digits), and a record per flush and token: the digits' sums and the scale,
+// {Σ d, scale} or {Σ d1, Σ d2, Σ d3, scale}, and {Σ d4, Σ d5} apart. A scale below zero stands for its magnitude and
+// says that the token has low digits in these 128 inputs; where it has none they are not written.
 struct Digits {
-    unsigned char* d;
-    unsigned char* records;
+    unsigned char *d, *records, *low;
     size_t row, plane;
 };
+constexpr int kLow = 2;  // low digits
+__host__ __device__ constexpr int planes_of(int D) { return D == 3 ? 3 + kLow : D; }
 __host__ __device__ inline size_t digit_row(size_t chunks) { return chunks * kChunk + 64; }  // 64 modulo 128: no bank twice
 __host__ __device__ inline size_t even(size_t n) { return (n + 1) & ~size_t(1); }
 __host__ __device__ inline size_t digit_bytes(int D, size_t tokens, size_t chunks, int fb) {
-    return D * tokens * digit_row(chunks) + even(tokens) * chunks * (4 / fb) * (D == 3 ? 16 : 8);
+    return planes_of(D) * tokens * digit_row(chunks) + even(tokens) * chunks * (4 / fb) * (D == 3 ? 16 + 4 * kLow : 8);
 }
-__host__ __device__ inline Digits digits_at(unsigned char* p, int D, size_t tokens, size_t chunks) {
+__host__ __device__ inline Digits digits_at(unsigned char* p, int D, size_t tokens, size_t chunks, int fb) {
     Digits o;
     o.row = digit_row(chunks), o.plane = tokens * o.row;
-    o.d = p, o.records = p + D * o.plane;
+    o.d = p, o.records = p + planes_of(D) * o.plane;
+    o.low = o.records + even(tokens) * chunks * (4 / fb) * 16;
     return o;
 }
 
@@ -126,51 +136,72 @@ __device__ __forceinline__ void load_eight(Eight<D>& r, const W4X& x, bool pairs
         }
     }
 }
+__device__ __forceinline__ float pow2(int i) { return __uint_as_float((uint32_t)(127 + i) << 23); }
+// Of 128 inputs with the largest magnitude m (its bits): v -> X = round(v 2^27 2^e) if tiny, else round(v 2^e).
+// 2^e takes the largest to 2^22 .. 2^23, or half of that where its digits would not fit; -105 <= e <= 122 here, up to 149
+// with the 27 (2^-149 is the step of f32's smallest values, which are whole there).
+struct Whole {
+    int e;
+    bool tiny, odd;  // odd: an infinity or a NaN among them
+};
+__device__ __forceinline__ Whole whole_of(uint32_t m) {
+    Whole w;
+    w.odd = m > 0x7f7fffffu;
+    w.e = w.odd ? 0 : 22 - ((int)(m >> 23) - 127);
+    w.tiny = w.e > 122;
+    float most = __uint_as_float(m);
+    if (w.tiny) most *= pow2(27), w.e -= 27;
+    if (most * pow2(w.e) > 8355711.f) --w.e;  // 127 (65536 + 256 + 1)
+    return w;
+}
+// Of four whole numbers, plus 128 each, the digits: byte `at` of each
+__device__ __forceinline__ uint32_t bytes_of(const uint32_t* p, int at) {
+    const uint32_t s = at == 2 ? 0x0062u : 0x5140u, a = __byte_perm(p[0], p[1], s), b = __byte_perm(p[2], p[3], s);
+    return __byte_perm(a, b, at == 1 ? 0x7632 : 0x5410) ^ 0x80808080u;
+}
+
+// Whether the token has low digits among these 128 inputs is the answer (of half a warp).
 template <int D, int FB>
-__device__ __forceinline__ void make_digits(Eight<D>& in, const W4X& x, const Digits& o, int t, int c) {
+__device__ __forceinline__ bool make_digits(Eight<D>& in, const W4X& x, const Digits& o, int t, int c) {
     const int l = threadIdx.x & 15, b = l >> 2, q = l & 3;
     uint32_t w[D][2];
     int sum[D];
     float scale;
+    bool low = false;
     if constexpr (D == 1) {
         w[0][0] = in.w[0], w[0][1] = in.w[1], scale = in.scale;
         sum[0] = __dp4a((int)w[0][0], 0x01010101, __dp4a((int)w[0][1], 0x01010101, 0));
     } else {
         float* v = in.v;
         uint32_t m = 0;
+        float total = 0.f;  // of the magnitudes, over 128
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);  // an infinity or a NaN is the largest
+        for (int i = 0; i < 8; ++i) {
+            m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);  // an infinity or a NaN is the largest
+            total = fmaf(fabsf(v[i]), 1.f / kChunk, total);
+        }
 #pragma unroll
-        for (int s = 8; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
-        const bool odd = m > 0x7f7fffffu;
-        // 2^e: the largest to 2^22 .. 2^23, or half of that where its digits would not fit; -105 <= e <= 149 (2^-149 is the
-        // step of f32's smallest values, which are whole there), in two factors where 2^e would be too large
-        auto pow2 = [](int i) { return __uint_as_float((uint32_t)(127 + i) << 23); };
-        int e = odd ? 0 : 22 - ((int)(m >> 23) - 127);
-        const bool tiny = e > 122;
-        float most = __uint_as_float(m);
+        for (int s = 8; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s)), total += __shfl_xor_sync(0xffffffffu, total, s);
+        const Whole wh = whole_of(m);
+        const bool odd = wh.odd, tiny = wh.tiny;
+        const int e = wh.e;
+        // the largest more than 8 times the mean
+        low = !odd && __uint_as_float(m) * ((float)min(kChunk, (int)(x.n_in - (size_t)c * kChunk)) * (1.f / (8 * kChunk))) > total;
         if (tiny) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] *= pow2(27);
-            most *= pow2(27), e -= 27;
         }
-        if (most * pow2(e) > 8355711.f) --e;  // 127 (65536 + 256 + 1)
         const float f = pow2(e);
         // X + 0x808080 has the digits + 128 as its bytes
         uint32_t u[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = odd ? 0x808080u : (uint32_t)(__float2int_rn(v[i] * f) + 0x808080);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t *p = u + 4 * h, a0 = __byte_perm(p[0], p[1], 0x5140), a1 = __byte_perm(p[2], p[3], 0x5140),
-                           b0 = __byte_perm(p[0], p[1], 0x0062), b1 = __byte_perm(p[2], p[3], 0x0062);
-            w[D - 1][h] = __byte_perm(a0, a1, 0x5410) ^ 0x80808080u;
-            w[D - 2][h] = __byte_perm(a0, a1, 0x7632) ^ 0x80808080u;
-            w[0][h] = __byte_perm(b0, b1, 0x5410) ^ 0x80808080u;
-        }
+        for (int h = 0; h < 2; ++h) w[D - 1][h] = bytes_of(u + 4 * h, 0), w[D - 2][h] = bytes_of(u + 4 * h, 1), w[0][h] = bytes_of(u + 4 * h, 2);
 #pragma unroll
         for (int d = 0; d < D; ++d) sum[d] = __dp4a((int)w[d][0], 0x01010101, __dp4a((int)w[d][1], 0x01010101, 0));
         scale = odd ? CUDART_NAN_F : tiny ? pow2(-e) * pow2(-27) : pow2(-e);
+        if (low) scale = -scale;
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) {
@@ -185,12 +216,49 @@ __device__ __forceinline__ void make_digits(Eight<D>& in, const W4X& x, const Di
         else
             *reinterpret_cast<int2*>(r) = make_int2(sum[0], __float_as_int(scale));
     }
+    return low;
+}
+
+// The low digits of the same 128 inputs, where `mine` says that the token has them: of what rounding to X left, at most 1/2, in
+// units of 2^-15. By a whole warp.
+template <int FB>
+__device__ __forceinline__ void make_low(const Eight<3>& in, const W4X& x, const Digits& o, int t, int c, bool mine) {
+    const int l = threadIdx.x & 15, b = l >> 2, q = l & 3;
+    uint32_t m = 0, u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(in.v[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
+    const Whole wh = whole_of(m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float y = (wh.tiny ? in.v[i] * pow2(27) : in.v[i]) * pow2(wh.e);
+        u[i] = (uint32_t)(mine ? __float2int_rn((y - (float)__float2int_rn(y)) * 32768.f) + 0x8080 : 0x8080);
+    }
+    int sum[kLow];
+#pragma unroll
+    for (int d = 0; d < kLow; ++d) {
+        const uint2 w = make_uint2(bytes_of(u, 1 - d), bytes_of(u + 4, 1 - d));
+        sum[d] = __dp4a((int)w.x, 0x01010101, __dp4a((int)w.y, 0x01010101, 0));
+#pragma unroll
+        for (int s = 1; s < 4 * FB; s <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], s);
+        if (mine) *reinterpret_cast<uint2*>(o.d + (3 + d) * o.plane + t * o.row + c * kChunk + (b >> 1) * 64 + q * 16 + (b & 1) * 8) = w;
+    }
+    if (mine && l % (4 * FB) == 0)
+        *reinterpret_cast<int2*>(o.low + ((size_t)(c * (4 / FB) + b / FB) * even(x.tokens) + t) * 8) = make_int2(sum[0], sum[1]);
+}
+// A record is read with its neighbour's: the one behind an odd number of tokens says that there are no low digits.
+template <int FB>
+__device__ __forceinline__ void end_records(const W4X& x, const Digits& o, int t, int c) {
+    const int l = threadIdx.x & 15;
+    if (x.tokens % 2 && t == (int)x.tokens - 1 && l < 4 / FB)
+        *reinterpret_cast<float*>(o.records + ((size_t)(c * (4 / FB) + l) * even(x.tokens) + t + 1) * 16 + 12) = 0.f;
 }
 
 template <int D, int FB>
 __global__ void __launch_bounds__(256) w4_digits_kernel(W4X x, int chunks, unsigned char* out) {
     asm volatile("griddepcontrol.launch_dependents;");
-    const Digits o = digits_at(out, D, x.tokens, chunks);
+    const Digits o = digits_at(out, D, x.tokens, chunks, FB);
     // half a warp per 128 inputs of a token; whole warps stay in step
     const int n = (int)x.tokens * chunks;
     const bool pairs = x_pairs(x);
@@ -198,7 +266,14 @@ __global__ void __launch_bounds__(256) w4_digits_kernel(W4X x, int chunks, unsig
         const int j = min(i, n - 1);
         Eight<D> e;
         load_eight(e, x, pairs, j / chunks, j % chunks);
-        make_digits<D, FB>(e, x, o, j / chunks, j % chunks);
+        const bool low = make_digits<D, FB>(e, x, o, j / chunks, j % chunks);
+        if constexpr (D == 3) {
+            if (__any_sync(0xffffffffu, low)) {
+                load_eight(e, x, pairs, j / chunks, j % chunks);
+                make_low<FB>(e, x, o, j / chunks, j % chunks, low);
+            }
+            end_records<FB>(x, o, j / chunks, j % chunks);
+        }
     }
 }
 
@@ -261,81 +336,70 @@ struct Stage4 {
     static constexpr int kBytes = kZeroAt + MT * 32 * kZero;
 };
 
-// A warp: MT x 16 rows x NT x 8 tokens over its part of the inputs. D digits an activation; PC scales of a row in
-// 128 inputs; FB: blocks of 32 inputs after which a sum meets its scales; WS: the digits are in the workspace.
-template <int MT, int NT, int D, int PC, int FB, bool WS>
-__global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a) {
+// The producer of a warp's ring: it runs S::kStages - 1 tiles ahead of the sums, a chunk after the other.
+template <int MT, int PC>
+struct Producer {
     using S = Stage4<MT, PC>;
-    extern __shared__ __align__(16) unsigned char s_mem[];
+    int tile, left;
+    const unsigned char *code, *scale, *zero;
+    uint32_t ring, dst;
+
+    // the pointers of the next row of tiles, if there is one
+    __device__ __forceinline__ void start(const StreamArgs& a) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, sub = warp & ((1 << a.ks) - 1);
+        const int chunks = (int)a.w.chunks, c0 = chunks * sub >> a.ks, c1 = chunks * (sub + 1) >> a.ks;
+        const int tr = tile * (kWarps >> a.ks) + (warp >> a.ks);
+        if (tile >= a.tiles || tr >= (int)(a.w.tile_rows / MT)) return;
+        const size_t at = ((size_t)(tr * MT >> 3) * chunks + c0) * 8 + (tr * MT & 7);
+        code = reinterpret_cast<const unsigned char*>(a.w.codes) + at * 1024 + lane * 16;
+        scale = reinterpret_cast<const unsigned char*>(a.w.scales) + (at * 8 + g) * (4 * PC);
+        zero = reinterpret_cast<const unsigned char*>(a.w.zeros) + (at * 8 + g) * S::kZero;
+        left = c1 - c0;
+        tile += gridDim.x;
+    }
+    __device__ __forceinline__ void next(const StreamArgs& a) {
+        const int lane = threadIdx.x & 31;
+        if (left > 0) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                copy_async<16>(dst + m * 1024 + lane * 16, code + m * 1024);
+                copy_async<16>(dst + m * 1024 + 512 + lane * 16, code + m * 1024 + 512);
+                copy_async<4 * PC>(dst + S::kScaleAt + (m * 32 + lane) * 4 * PC, scale + m * (32 * PC));
+                if (a.w.zeros) copy_async<S::kZero>(dst + S::kZeroAt + (m * 32 + lane) * S::kZero, zero + m * (8 * S::kZero));
+            }
+            code += 8192, scale += 256 * PC, zero += 64 * S::kZero;
+            if (--left == 0) start(a);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        dst = dst == ring + (S::kStages - 1) * S::kBytes ? ring : dst + S::kBytes;
+    }
+    __device__ __forceinline__ void fill(const StreamArgs& a, unsigned char* mem) {
+        tile = blockIdx.x, left = 0, code = scale = zero = nullptr;
+        ring = dst = (uint32_t)__cvta_generic_to_shared(mem);
+        start(a);
+        for (int i = 0; i < S::kStages - 1; ++i) next(a);
+    }
+};
+
+// The tiles of a warp: MT x 16 rows x NT x 8 tokens over its part of the inputs. LOW: some token has low digits.
+template <int MT, int NT, int D, int PC, int FB, bool WS, bool LOW>
+__device__ __forceinline__ void stream_tiles(const StreamArgs& a, unsigned char* s_mem, unsigned char* ring, Producer<MT, PC>& p) {
+    using S = Stage4<MT, PC>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int per = kWarps >> a.ks, sub = warp & ((1 << a.ks) - 1);
     const int chunks = (int)a.w.chunks, T = (int)a.x.tokens, rows = (int)(a.w.tile_rows / MT);
     const int c0 = chunks * sub >> a.ks, c1 = chunks * (sub + 1) >> a.ks;
     const bool zeros = a.w.zeros != nullptr;
-    unsigned char* ring = s_mem + warp * S::kStages * S::kBytes;
-
-    // The producer runs S::kStages - 1 tiles ahead of the sums, a chunk after the other.
-    int p_tile = blockIdx.x, p_left = 0;
-    const unsigned char *p_code = nullptr, *p_scale = nullptr, *p_zero = nullptr;
-    auto p_start = [&]() {  // the pointers of the producer's next row of tiles, if there is one
-        const int tr = p_tile * per + (warp >> a.ks);
-        if (p_tile >= a.tiles || tr >= rows) return;
-        const size_t at = ((size_t)(tr * MT >> 3) * chunks + c0) * 8 + (tr * MT & 7);
-        p_code = reinterpret_cast<const unsigned char*>(a.w.codes) + at * 1024 + lane * 16;
-        p_scale = reinterpret_cast<const unsigned char*>(a.w.scales) + (at * 8 + g) * (4 * PC);
-        p_zero = reinterpret_cast<const unsigned char*>(a.w.zeros) + (at * 8 + g) * S::kZero;
-        p_left = c1 - c0;
-        p_tile += gridDim.x;
-    };
-    p_start();
-    const uint32_t ring_u = (uint32_t)__cvta_generic_to_shared(ring);
-    uint32_t p_dst = ring_u;
-    auto produce = [&]() {
-        if (p_left > 0) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                copy_async<16>(p_dst + m * 1024 + lane * 16, p_code + m * 1024);
-                copy_async<16>(p_dst + m * 1024 + 512 + lane * 16, p_code + m * 1024 + 512);
-                copy_async<4 * PC>(p_dst + S::kScaleAt + (m * 32 + lane) * 4 * PC, p_scale + m * (32 * PC));
-                if (zeros) copy_async<S::kZero>(p_dst + S::kZeroAt + (m * 32 + lane) * S::kZero, p_zero + m * (8 * S::kZero));
-            }
-            p_code += 8192, p_scale += 256 * PC, p_zero += 64 * S::kZero;
-            if (--p_left == 0) p_start();
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        p_dst = p_dst == ring_u + (S::kStages - 1) * S::kBytes ? ring_u : p_dst + S::kBytes;
-    };
-    // The weights do not depend on the kernel before, the activations may.
-    for (int i = 0; i < S::kStages - 1; ++i) produce();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Digits x = digits_at(WS ? a.digits : s_mem + a.digits_at, D, T, chunks);
-    if constexpr (!WS) {
-        const int n = T * chunks;
-        const bool pairs = x_pairs(a.x);
-        constexpr int kU = 4;  // chunks of a half warp whose loads are under way together
-        for (int i = threadIdx.x >> 4; (i & ~1) < n; i += kWarps * 2 * kU) {
-            Eight<D> e[kU];
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int j = min(i + u * kWarps * 2, n - 1), t = T == 1 ? 0 : j / chunks;
-                if (((i + u * kWarps * 2) & ~1) < n) load_eight(e[u], a.x, pairs, t, j - t * chunks);
-            }
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int j = min(i + u * kWarps * 2, n - 1), t = T == 1 ? 0 : j / chunks;
-                if (((i + u * kWarps * 2) & ~1) < n) make_digits<D, FB>(e[u], a.x, x, t, j - t * chunks);
-            }
-        }
-        __syncthreads();
-    }
+    const Digits x = digits_at(WS ? a.digits : s_mem + a.digits_at, D, T, chunks, FB);
     constexpr int FL = 4 / FB, R = D == 3 ? 16 : 8;  // flushes of 128 inputs, bytes of a record
     // a lane without a token repeats the last one's row: its sums are not stored
-    const unsigned char *xr[NT], *xq[NT];
+    const unsigned char *xr[NT], *xq[NT], *xl[NT];
     const size_t step = even(T) * R;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         xr[n] = x.d + (size_t)min(8 * n + g, T - 1) * x.row + 16 * q + c0 * kChunk;
         xq[n] = x.records + min(8 * n + 2 * q, (int)even(T) - 2) * R + c0 * FL * step;
+        xl[n] = x.low + min(8 * n + 2 * q, (int)even(T) - 2) * 8 + c0 * FL * (step / 2);
     }
 
     const unsigned char* st = ring;
@@ -347,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a)
         for (int i = 0; i < MT * NT * 4; ++i) acc[i / (4 * NT)][i / 4 % NT][i % 4] = 0.f;
         for (int c = c0; has && c < c1; ++c) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-            produce();  // into the stage of the tile before this one
+            p.next(a);  // into the stage of the tile before this one
             uint4 va[MT], vb[MT];
             uint32_t zz[MT][(PC + 1) / 2], sc[MT][PC];
 #pragma unroll
@@ -371,6 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a)
                 const int blk = f * FB * PC / 4;  // scale block of the chunk
                 int d[MT][NT][D][4];
                 float xs[NT][2];
+                int signs = 0;  // of the scales: below zero where a token has low digits here
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     int sums[2][D];  // of the digits of tokens 8 n + 2 q, + 1
@@ -379,6 +444,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a)
                         const int4 r1 = *reinterpret_cast<const int4*>(xq[n] + (at * FL + f) * step + 16);
                         sums[0][0] = r.x, sums[0][1] = r.y, sums[0][D - 1] = r.z, xs[n][0] = __int_as_float(r.w);
                         sums[1][0] = r1.x, sums[1][1] = r1.y, sums[1][D - 1] = r1.z, xs[n][1] = __int_as_float(r1.w);
+                        signs |= r.w | r1.w;
                     } else {
                         sums[0][0] = r.x, xs[n][0] = __int_as_float(r.y);
                         sums[1][0] = r.z, xs[n][1] = __int_as_float(r.w);
@@ -425,8 +491,53 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a)
                             float v = __int_as_float(d[m][n][0][e]) - kMagic;
 #pragma unroll
                             for (int i = 1; i < D; ++i) v = fmaf(v, 256.f, __int_as_float(d[m][n][i][e]) - kMagic);
-                            acc[m][n][e] = fmaf(v * xs[n][e & 1], e & 2 ? s1 : s0, acc[m][n][e]);
+                            acc[m][n][e] = fmaf(v * (LOW ? fabsf(xs[n][e & 1]) : xs[n][e & 1]), e & 2 ? s1 : s0, acc[m][n][e]);
                         }
+                }
+                if constexpr (LOW) {
+                    if (__any_sync(0xffffffffu, signs < 0)) {  // the same sums of the low digits
+                        int l[MT][NT][kLow][4];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const int4 r = *reinterpret_cast<const int4*>(xl[n] + (at * FL + f) * (step / 2));
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) {
+                                const uint32_t z2 = zz[m][blk / 2] >> (16 * (blk & 1));
+                                const int z0 = -(int)(z2 & 0xffu), z1 = -(int)((z2 >> 8) & 0xffu);
+                                l[m][n][0][0] = z0 * r.x + kMagicBits, l[m][n][0][1] = z0 * r.z + kMagicBits;
+                                l[m][n][0][2] = z1 * r.x + kMagicBits, l[m][n][0][3] = z1 * r.z + kMagicBits;
+                                l[m][n][1][0] = z0 * r.y + kMagicBits, l[m][n][1][1] = z0 * r.w + kMagicBits;
+                                l[m][n][1][2] = z1 * r.y + kMagicBits, l[m][n][1][3] = z1 * r.w + kMagicBits;
+                            }
+                        }
+#pragma unroll
+                        for (int b = f * FB; b < (f + 1) * FB; ++b)
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) {
+                                const uint32_t wa = b == 0 ? va[m].x : b == 1 ? va[m].y : b == 2 ? va[m].z : va[m].w;
+                                const uint32_t wb = b == 0 ? vb[m].x : b == 1 ? vb[m].y : b == 2 ? vb[m].z : vb[m].w;
+                                const uint32_t fr[4] = {wa & 0x0f0f0f0fu, wb & 0x0f0f0f0fu, (wa >> 4) & 0x0f0f0f0fu, (wb >> 4) & 0x0f0f0f0fu};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int i = 0; i < kLow; ++i) {
+                                        const uint2 u = *reinterpret_cast<const uint2*>(xr[n] + (D + i) * x.plane + at * kChunk + (b >> 1) * 64 + (b & 1) * 8);
+                                        mma_u8s8(l[m][n][i], fr, u.x, u.y);
+                                    }
+                            }
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            const float s0 = scale_of(sc[m][blk] & 0xffffu, a.w.scale_bf16), s1 = scale_of(sc[m][blk] >> 16, a.w.scale_bf16);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float v = fmaf(__int_as_float(l[m][n][0][e]) - kMagic, 256.f, __int_as_float(l[m][n][1][e]) - kMagic);
+                                    // a token without low digits has none written: its sums are not used
+                                    if (xs[n][e & 1] < 0.f) acc[m][n][e] = fmaf(v * 0x1p-15f * -xs[n][e & 1], e & 2 ? s1 : s0, acc[m][n][e]);
+                                }
+                        }
+                    }
                 }
             }
         }
@@ -465,11 +576,86 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(StreamArgs a)
                 }
         }
     }
+}
+// Apart from the kernel's own loop, from which these sums would take registers (in one loop 8192 x 8192 took 13.2 us
+// instead of 12.3): called where some token has low digits.
+template <int MT, int NT, int PC, int FB, bool WS>
+__device__ __noinline__ void stream_tiles_low(const StreamArgs* args, unsigned char* s_mem, unsigned char* ring, const Producer<MT, PC>* from) {
+    Producer<MT, PC> p = *from;
+    stream_tiles<MT, NT, 3, PC, FB, WS, true>(*args, s_mem, ring, p);
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Shared memory for the digits, beside the ring.
-constexpr size_t kDigitSmem = 60 * 1024;
+// D digits an activation; PC scales of a row in 128 inputs; FB: blocks of 32 inputs after which a sum meets its scales; WS: the
+// digits are in the workspace.
+template <int MT, int NT, int D, int PC, int FB, bool WS>
+__global__ void __launch_bounds__(kWarps * 32, 1) w4_stream_kernel(const __grid_constant__ StreamArgs a) {
+    using S = Stage4<MT, PC>;
+    extern __shared__ __align__(16) unsigned char s_mem[];
+    const int chunks = (int)a.w.chunks, T = (int)a.x.tokens;
+    unsigned char* ring = s_mem + (threadIdx.x >> 5) * S::kStages * S::kBytes;
+    // The weights do not depend on the kernel before, the activations may.
+    Producer<MT, PC> p;
+    p.fill(a, ring);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Digits x = digits_at(WS ? a.digits : s_mem + a.digits_at, D, T, chunks, FB);
+    int more = 0;  // some token has low digits somewhere
+    if constexpr (WS) {
+        if constexpr (D == 3) {
+            int signs = 0;
+            for (int i = threadIdx.x; i < (int)even(T) * chunks * (4 / FB); i += kWarps * 32)
+                signs |= *reinterpret_cast<const int*>(x.records + (size_t)i * 16 + 12);
+            more = __syncthreads_or(signs < 0);
+        }
+    } else {
+        const int n = T * chunks;
+        const bool pairs = x_pairs(a.x);
+        bool mine = false;
+        constexpr int kU = 4;  // chunks of a half warp whose loads are under way together
+        for (int i = threadIdx.x >> 4; (i & ~1) < n; i += kWarps * 2 * kU) {
+            Eight<D> e[kU];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int j = min(i + u * kWarps * 2, n - 1), t = T == 1 ? 0 : j / chunks;
+                if (((i + u * kWarps * 2) & ~1) < n) load_eight(e[u], a.x, pairs, t, j - t * chunks);
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int j = min(i + u * kWarps * 2, n - 1), t = T == 1 ? 0 : j / chunks;
+                if (((i + u * kWarps * 2) & ~1) < n) mine |= make_digits<D, FB>(e[u], a.x, x, t, j - t * chunks);
+            }
+        }
+        if constexpr (D == 3) {
+            more = __syncthreads_or(mine);
+            if (more) {
+#pragma unroll 1
+                for (int i = threadIdx.x >> 4; (i & ~1) < n; i += kWarps * 2) {
+                    const int j = min(i, n - 1), t = j / chunks, c = j - t * chunks;
+                    Eight<3> e;
+                    load_eight(e, a.x, pairs, t, c);
+                    const bool low = *reinterpret_cast<const float*>(x.records + ((size_t)c * (4 / FB) * even(T) + t) * 16 + 12) < 0.f;
+                    make_low<FB>(e, a.x, x, t, c, low);
+                    end_records<FB>(a.x, x, t, c);
+                }
+                __syncthreads();
+            }
+        } else {
+            __syncthreads();
+        }
+    }
+    if constexpr (D == 3) {
+        if (more) {
+            const Producer<MT, PC> copy = p;
+            stream_tiles_low<MT, NT, PC, FB, WS>(&a, s_mem, ring, &copy);
+            return;
+        }
+    }
+    stream_tiles<MT, NT, D, PC, FB, WS, false>(a, s_mem, ring, p);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Shared memory for the digits, beside the ring (of one row tile a warp, or of two with one tile of tokens).
+constexpr size_t digit_smem(int D) { return (D == 3 ? 78 : 60) * 1024; }
 
 int flush_blocks(const W4View& w, const W4X& x) {
     const int fb = 4 / w.per_chunk;
@@ -482,7 +668,7 @@ cudaError_t run_stream(StreamArgs& a, int num_sms, cudaStream_t s) {
     auto kernel = w4_stream_kernel<MT, NT, D, PC, FB, WS>;
     constexpr size_t ring = (size_t)kWarps * Stage4<MT, PC>::kStages * Stage4<MT, PC>::kBytes;
     constexpr size_t sums = kWarps * 32 * 4 * NT * MT * sizeof(float);
-    static_assert(ring + kDigitSmem + sums <= 227 * 1024, "shared memory");
+    static_assert(ring + digit_smem(D) + sums <= 227 * 1024, "shared memory");
     const size_t own = WS ? 0 : (digit_bytes(D, a.x.tokens, a.w.chunks, FB) + 15) & ~size_t(15);
     // Warps that share a row of tiles: the split with the shortest chain of tiles for a warp, where a round
     // costs about as much as 3 tiles (its first loads, its sums joined).
@@ -497,7 +683,7 @@ cudaError_t run_stream(StreamArgs& a, int num_sms, cudaStream_t s) {
     a.sums_at = (int)((ring + own) / sizeof(float));
     const size_t smem = ring + own + (a.ks > 0 ? sums : 0);
     static SmemOnce once;  // the most this kernel is ever given
-    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), (int)(ring + kDigitSmem + sums));
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), (int)(ring + digit_smem(D) + sums));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)std::min(a.tiles, num_sms));
@@ -553,7 +739,7 @@ cudaError_t launch_w4_pack(const uint8_t* codes, const unsigned short* scales, c
 
 size_t w4_stream_workspace(const W4View& w, const W4X& x) {
     const size_t n = digit_bytes(digits_of(x), x.tokens, w.chunks, flush_blocks(w, x));
-    return n <= kDigitSmem ? 0 : n;
+    return n <= digit_smem(digits_of(x)) ? 0 : n;
 }
 
 cudaError_t launch_w4_stream(const W4View& w, const W4X& x, void* y, int y_bf16, void* workspace, int num_sms,

@@ -419,9 +419,12 @@ BEBELM_API int bebelm_w4_workspace(const bebelm_w4* w, const void* x, int x_dtyp
  * with x_scales [n_tokens][n_in / x_group] (x_group 32, 64, 128 or 256, or 0: one scale a token), as
  * bebelm_add_rmsnorm writes them. y [n_tokens][n_out] in y_dtype (BEBELM_F32 or BEBELM_BF16), not
  * overlapping x. Codes less zero points and int8 activations are taken exactly, sums are f32. Other activations:
- *  - up to 8 tokens: to 2^-23 of the largest of their 128 neighbours (inputs 128 i .. 128 i + 127);
+ *  - up to 8 tokens, by the largest of their 128 neighbours (inputs 128 i .. 128 i + 127): to 2^-23 of it where it is at
+ *    most 8 times their mean magnitude, else to 2^-38 of it;
  *  - more than 16: BEBELM_BF16 exactly, BEBELM_F32 to 2^-24 of each (and 2^-39 of its token's largest);
  *  - 9 to 16: one or the other, by the size of the weights.
+ * A token's result does not depend on what the tokens beside it hold; its last bits may depend on how many they are (up to
+ * 8 they do not).
  * A group is summed before its scale is applied, so the sum of |code - zero| |x| over a group has to
  * stay below 3.4e38. Infinities and NaN stay in their token's row. Device memory: `workspace` (256-byte aligned, of
  * bebelm_w4_workspace bytes) is used until the call's work is done; calls that may overlap need one

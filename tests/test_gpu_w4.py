@@ -304,3 +304,90 @@ def test_a_wait_that_gives_up_is_reported(t, n_in, n_out):
     finally:
         assert L.bebelm_debug_expire_next_wait(0) == bb.OK
     w.check()
+
+
+def dead_inputs(n_in):
+    """Two inputs of every 128 whose codes are their zero points in all rows, so that nothing there may reach an output."""
+    return [c + i for c in range(0, n_in, 128) for i in (5, 17)]
+
+
+def weights_with_dead_inputs(n_out, n_in, group, seed, zeros=True, exact=True, scales=torch.float16):
+    codes, sc, z = weights(n_out, n_in, group, seed, zeros, scales, exact)
+    full = torch.stack((codes & 15, codes >> 4), -1).view(n_out, n_in)
+    for k in dead_inputs(n_in):
+        full[:, k] = 8 if z is None else z[:, k // group]
+    return full[:, 0::2] | full[:, 1::2] << 4, sc, z
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("t", [1, 2, 7, 8, 9, 13, 16, 17, 70])
+@pytest.mark.parametrize("n_in,group", [(416, 32), (448, 64), (512, 128), (768, 256)])
+def test_every_digit_of_every_input(n_in, group, t, kind):
+    """One activation of 19 bits (bf16: 8) at a time, at every input, alone and beside one 2^15 or 2^18 times as large that the weights
+    do not see: products with the 5 bits of a code less its zero point have 24 bits, so outputs are exact. A digit or a term that is lost,
+    misplaced or added under a wrong zero point shows at its input."""
+    n_out = 70
+    codes, sc, z = weights_with_dead_inputs(n_out, n_in, group, 5 + group)
+    w, wd = bb.W4Weights(codes, sc, z, group=group), dense(codes, sc, z, group)
+    dead = set(dead_inputs(n_in))
+    live = [k for k in range(n_in) if k not in dead]
+    g = torch.Generator(device="cuda").manual_seed(t * 1000 + n_in)
+    for far in (None, 15, 18):
+        for at in range(0, len(live), t):
+            k = torch.tensor([live[(at + i) % len(live)] for i in range(t)], device="cuda")
+            bits = 19 if kind == "f32" else 8
+            x = torch.zeros(t, n_in, device="cuda", dtype=torch.float64)
+            v = torch.randint(1 << (bits - 1), 1 << bits, (t,), device="cuda", generator=g) * (1 - 2 * torch.randint(0, 2, (t,), device="cuda", generator=g))
+            rows = torch.arange(t, device="cuda")
+            x[rows, k] = v.double()
+            if far:
+                x[rows, k // 128 * 128 + 5] = 2.0 ** (bits + far)
+            x = x.to(KINDS[kind])
+            y = w.matmul(x, out_dtype=bb.F32).double()
+            want = x.double() @ wd.t()
+            assert torch.equal(y, want), (far, at, float((y - want).abs().max()))
+
+
+@pytest.mark.parametrize("case", [(1, 2048, 300, 128, "f32"), (1, 8192, 300, 128, "bf16"), (4, 2080, 515, 32, "f32"), (7, 1024, 100, 64, "bf16"),
+                                  (8, 2048, 333, 128, "f32"), (8, 8192, 48, 64, "f32"), (12, 1024, 700, 32, "f32"), (16, 640, 400, 640, "bf16"),
+                                  (16, 2048, 8192, 128, "f32"), (24, 2080, 300, 32, "f32"), (130, 512, 260, 128, "f32")],
+                         ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("outlier", [10.0, 1e2, 1e3, 1e4, 1e5])
+def test_activations_beside_far_larger_ones(case, outlier):
+    """A residual stream's: one of 128 activations is far larger than the rest, and the weights (at their zero points there) do not
+    see it, so the rest must come out as precisely as without it. Bound, A = Σ|w||x| over the rest: as digits each activation is kept to
+    2^-23 of the largest M of 128 where M is at most 8 times their mean magnitude, else to 2^-38 M (half steps: the largest is 2^21.99 steps or
+    2^37.99 at least, hence 2^-22.99 and 2^-37.99); in more than 16 tokens f32 to 2^-24 of itself and 2^-39 of its token's largest. A sum's roundings: 3 a
+    scaled sum (one a group, 128 or 32 inputs) and one for each that it is added to; more than 16 tokens 17 per 16 inputs of a group and term."""
+    t, n_in, n_out, group, kind = case
+    codes, sc, z = weights_with_dead_inputs(n_out, n_in, group, 3, exact=False)
+    w, wd = bb.W4Weights(codes, sc, z, group=group), dense(codes, sc, z, group)
+    x, _ = activations(t, n_in, kind, 0, 11)
+    x[:, 5::128] = outlier * (1 + torch.rand_like(x[:, 5::128].float())).to(x.dtype)
+    x[0] = activations(1, n_in, kind, 0, 12)[0]  # a token without them, beside the others
+    x[0, 5::128] = 0
+    y = w.matmul(x, out_dtype=bb.F32).double()
+    xd = x.double()
+    want, a = xd @ wd.t(), xd.abs().clone()
+    a[:, 5::128] = 0
+    wa = wd.abs()
+    flushes = n_in / min(group, 128)
+    steps = 3 * 17 * max(1, group // 16) * 2 if t > 16 else 0
+    tol = (flushes + 8 + steps) * 2.0 ** -24 * (a @ wa.t())
+    if t > 16:
+        err = 2.0 ** -39 * xd.abs().amax(-1, keepdim=True) + 2.0 ** -24 * a if kind == "f32" else torch.zeros_like(a)
+    else:
+        pad = torch.nn.functional.pad(xd.abs(), (0, -n_in % 128)).view(t, -1, 128)
+        counts = torch.full((pad.shape[1],), 128.0, device="cuda", dtype=torch.float64)
+        if n_in % 128:
+            counts[-1] = n_in % 128
+        big = pad.amax(-1)
+        # (next to the border either may hold)
+        err = torch.where(big <= 8.001 * pad.sum(-1) / counts, 2.0 ** -22.99 * big, 2.0 ** -37.99 * big).repeat_interleave(128, 1)[:, :n_in]
+    tol = tol + (err * (a > 0)) @ wa.t()
+    bad = (y - want).abs() > tol
+    assert not bad.any(), (int(bad.sum()), float(((y - want).abs() / tol.clamp(min=1e-300)).max()))
+    # a token's results do not depend on the tokens beside it
+    if t > 1 and t <= 8:
+        assert torch.equal(w.matmul(x[:1], out_dtype=bb.F32).double()[0], y[0])
+        assert torch.equal(w.matmul(x[1:2], out_dtype=bb.F32).double()[0], y[1])
