@@ -157,21 +157,15 @@ __device__ __forceinline__ void tmem_st_tile(uint32_t taddr, const uint32_t* r) 
 // 32 lanes x C columns (16 or 32); tmem_ld_wait() before the registers are used
 template <int C>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
-    if constexpr (C == 8) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                     : "r"(taddr));
-    } else {
 #pragma unroll
-        for (int i = 0; i < C; i += 16)
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-                "%15}, [%16];"
-                : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]),
-                  "=r"(r[i + 7]), "=r"(r[i + 8]), "=r"(r[i + 9]), "=r"(r[i + 10]), "=r"(r[i + 11]), "=r"(r[i + 12]),
-                  "=r"(r[i + 13]), "=r"(r[i + 14]), "=r"(r[i + 15])
-                : "r"(taddr + i));
-    }
+    for (int i = 0; i < C; i += 16)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+            "%15}, [%16];"
+            : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]),
+              "=r"(r[i + 7]), "=r"(r[i + 8]), "=r"(r[i + 9]), "=r"(r[i + 10]), "=r"(r[i + 11]), "=r"(r[i + 12]),
+              "=r"(r[i + 13]), "=r"(r[i + 14]), "=r"(r[i + 15])
+            : "r"(taddr + i));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -524,7 +518,7 @@ __global__ void __launch_bounds__(Lay<N, TERMS, BF16>::kThreads, 1) w4_tc_kernel
                         const float s1 = scale_of(*reinterpret_cast<const unsigned short*>(base + sc_at + (sum * FB * pc / 4) * 4), a.w.scale_bf16);
                         const uint64_t s = pack2(__float_as_uint(s1), __float_as_uint(s1));
                         const unsigned char* xs = base + L::kXs + part * C * 4 + (sum * FB * 32 >> a.x_shift) * (N * 4);
-                        constexpr int B = C < 16 ? C : 16;  // columns in registers at a time
+                        constexpr int B = 16;  // columns in registers at a time
 #pragma unroll
                         for (int j = 0; j < C; j += B) {
                             uint32_t d[B];

@@ -391,3 +391,43 @@ def test_activations_beside_far_larger_ones(case, outlier):
     if t > 1 and t <= 8:
         assert torch.equal(w.matmul(x[:1], out_dtype=bb.F32).double()[0], y[0])
         assert torch.equal(w.matmul(x[1:2], out_dtype=bb.F32).double()[0], y[1])
+
+
+@pytest.mark.parametrize("t", [1, 8, 9, 16, 17, 40, 130])
+@pytest.mark.parametrize("n_in,group", [(32, 32), (64, 64), (64, 32), (128, 128)])
+def test_the_smallest_layers(n_in, group, t):
+    """Fewer inputs than a tile's 64 or 128, one row and three."""
+    for n_out in (1, 3):
+        for kind, xg in (("f32", 0), ("bf16", 0), ("int8", 0), ("int8", 32)):
+            check((t, n_in, n_out, group, kind, xg, True, torch.float16, bb.F32), True)
+
+
+def test_calls_of_one_handle_from_threads():
+    """Products of one handle at once: device memory on a stream a thread, and host memory."""
+    import threading
+    codes, sc, z = weights(300, 512, 64, 3)
+    w = bb.W4Weights(codes, sc, z, group=64)
+    xs = [activations(t, 512, "f32", 0, t)[0] for t in (1, 5, 20, 40)]
+    want = [w.matmul(x) for x in xs]
+    host = [(x.cpu().numpy(), y.cpu().numpy()) for x, y in zip(xs, want)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        for _ in range(20):
+            if i % 2:
+                y = w.matmul(xs[i], stream=stream)
+                stream.synchronize()
+                if not torch.equal(y, want[i]):
+                    bad.append(i)
+            elif not np.array_equal(w.matmul(host[i][0]), host[i][1]):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
+    w.check()
