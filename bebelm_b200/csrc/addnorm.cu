@@ -17,7 +17,7 @@
 // is read once. Rows of up to 1024 values take a warp each (no barrier); longer ones a CTA each with
 // 8 or 16 values a thread, one barrier for the sum and one more for a scale of the whole row. Measured:
 // 8192 bf16 rows of 2048 with their sum 23.4 us (134 MB at 5.7 TB/s, 87 % of a copy's rate); one row
-// of 2048 2.9 us. Streaming cache hints on the loads cost 17 %, a gain read ahead of the sum 15 % (registers).
+// of 2048 to int8 2.8 us, 1037 f32 rows of 2080 5.0 us. Streaming cache hints on the loads cost 17 %, a gain read ahead of the sum 15 % (registers).
 #include <algorithm>
 #include <cstdint>
 

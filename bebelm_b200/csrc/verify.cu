@@ -13,7 +13,8 @@
 // A drawn token is the place where a running sum over the vocabulary passes a border. With V entries a
 // relative error e of the sums moves it with probability about V e: for 1.3e5 entries f32 is not
 // enough (1e-2), so the row a token is drawn from is summed in f64 from f64 exponentials. Whether a
-// draft is accepted is one comparison: its row's sum may have the 1e-7 of f32 exponentials.
+// draft is accepted is one comparison, which goes the other way with the probability of its relative error: its row's sum
+// is of f32 exponentials, up to some hundreds a thread in f32, the rest in f64 (about 1e-6).
 //
 //   verify_rows_kernel   one pass over every row that can matter: per slice the running maximum and the
 //                        sum of exponentials below it (greedy: the maximum and its index). Bound: HBM.
@@ -290,7 +291,8 @@ __device__ __forceinline__ double warp_running(double v) {  // lane i: the sum o
     return v;
 }
 
-// PT threads; 64 registers each, so that an SM holds 1024 of them however they are split.
+// PT threads; 64 registers each, so that an SM holds 1024 of them however they are split (the forms for logits spill 100
+// and 124 bytes, with vector loads and without).
 //
 // The part of a CTA is cut into blocks, a block into one cell of neighbouring entries a warp; the pass leaves every
 // cell's sums, so the border is found by going from the CTA to the block to the cell to the entry, and only the last

@@ -586,6 +586,8 @@ __device__ __noinline__ void stream_tiles_low(const StreamArgs* args, unsigned c
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
+// The forms for 9 to 16 float tokens fill the registers and spill (up to 380 bytes in groups of 32 with digits in the
+// workspace, else up to 70).
 // D digits an activation; PC scales of a row in 128 inputs; FB: blocks of 32 inputs after which a sum meets its scales; WS: the
 // digits are in the workspace.
 template <int MT, int NT, int D, int PC, int FB, bool WS>

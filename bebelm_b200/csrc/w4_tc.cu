@@ -154,7 +154,7 @@ __device__ __forceinline__ void tmem_st_tile(uint32_t taddr, const uint32_t* r) 
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-// 32 lanes x C columns (16 or 32); tmem_ld_wait() before the registers are used
+// 32 lanes x C columns (a multiple of 16); tmem_ld_wait() before the registers are used
 template <int C>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
 #pragma unroll
