@@ -13,8 +13,8 @@
 // A drawn token is the place where a running sum over the vocabulary passes a border. With V entries a
 // relative error e of the sums moves it with probability about V e: for 1.3e5 entries f32 is not
 // enough (1e-2), so the row a token is drawn from is summed in f64 from f64 exponentials. Whether a
-// draft is accepted is one comparison, which goes the other way with the probability of its relative error: its row's sum
-// is of f32 exponentials, up to some hundreds a thread in f32, the rest in f64 (about 1e-6).
+// draft is accepted is one comparison: its rows' sums are of f32 exponentials, a thread's in f32 (about 1e-6), unless u q
+// lies so near p that their error could decide; then both rows are summed in f64 as well.
 //
 //   verify_rows_kernel   one pass over every row that can matter: per slice the running maximum and the
 //                        sum of exponentials below it (greedy: the maximum and its index). Bound: HBM.
@@ -25,7 +25,7 @@
 //
 // Measured (logits in f32 with draft rows, vocabulary 128000): 64 sequences of 8 drafts 132 us, of which the rows' kernel
 // takes 80 (557 MB at 7 TB/s: some of it lies in L2) and the pick 48 (its f64 pass; at the f64 pipe's rate 16); one sequence of
-// 4 drafts 16.4 us, a chain of latencies. 24 sequences of 5 looked-up drafts, probabilities of 32003: 7.0 us.
+// 4 drafts 15.4 us, a chain of latencies. 24 sequences of 5 looked-up drafts, probabilities of 32003: 7.0 us.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -121,10 +121,11 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(VerifyArgs a, 
                 m = mx;
             }
             if (m > -CUDART_INF_F) {
+                float part[kU];
 #pragma unroll
                 for (int u = 0; u < kU; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s += ex2f((v[u][j] - m) * c);
+                    part[u] = (ex2f((v[u][0] - m) * c) + ex2f((v[u][1] - m) * c)) + (ex2f((v[u][2] - m) * c) + ex2f((v[u][3] - m) * c));
+                s += (part[0] + part[1]) + (part[2] + part[3]);
             }
         }
     }
@@ -291,8 +292,59 @@ __device__ __forceinline__ double warp_running(double v) {  // lane i: the sum o
     return v;
 }
 
-// PT threads; 64 registers each, so that an SM holds 1024 of them however they are split (the forms for logits spill 100
-// and 124 bytes, with vector loads and without).
+// How far sums of the rows' kernel may be off, as a part of p (and q, hence twice): 2^-24 each for a thread's additions, 16
+// entries at a time (5 steps with the factor of a new maximum), and 64 steps for the exponentials, whose arguments have three
+// roundings and reach some log2(vocab) where they weigh.
+double near_border(size_t vocab, int slices) {
+    const size_t rounds = (vocab + (size_t)slices * kRowThreads * 16 - 1) / ((size_t)slices * kRowThreads * 16);
+    return (double)(5 * rounds + 64) * 0x1p-23;
+}
+
+// Whether u q(x) < p(x) for draft i and its logits, from sums of both rows in f64 by the whole cluster: p(x) is x's share of
+// them. The rows' factors (the target's, and 33 behind it the draft's) are the first pass's, whose error cancels. part, all:
+// shared memory of two values a warp and a CTA. One draft in some ten thousand comes here, so it is a call with few
+// arguments (64 sequences 132.3 us; in line, or with the rows' pointers as arguments, 133; without it 130.4).
+template <int PT, bool VEC>
+__device__ __noinline__ bool accepted_in_f64(const VerifyArgs* args, const Row<false>* prow, int i, double* part, double* all) {
+    const int b = blockIdx.x / (int)cg::this_cluster().num_blocks();
+    const Row<false>* qrow = prow + 33;
+    const float* p = args->target + ((size_t)b * (args->drafts + 1) + i) * args->target_stride;
+    const float* q = args->draft ? args->draft + ((size_t)b * args->drafts + i) * args->draft_stride : nullptr;
+    const int x = args->tokens[(size_t)b * args->drafts + i];
+    const double u = (double)args->u[(size_t)b * args->drafts + i];
+    cg::cluster_group cl = cg::this_cluster();
+    const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const size_t vocab = args->vocab, quads = (vocab + 3) / 4;
+    const unsigned j0 = (unsigned)(4 * (quads * me / ctas)), j1 = (unsigned)min(vocab, 4 * (quads * (me + 1) / ctas));
+    for (int side = 0; side < 2; ++side) {
+        double sum = 0.0;
+        if (side == 0 || q) {
+            Row<false> r = side ? *qrow : *prow;
+            r.p = side ? q : p;
+            for (unsigned j = j0 + 4 * threadIdx.x; j < j1; j += 4 * PT) {
+                float v[4];
+                entries4<VEC>(r, j, j1, v);
+                sum += (r.weigh(v[0]) + r.weigh(v[1])) + (r.weigh(v[2]) + r.weigh(v[3]));
+            }
+        }
+        sum = warp_total(sum);
+        if (lane == 0) part[2 * warp + side] = sum;
+    }
+    __syncthreads();
+    if (warp < 2) {  // a warp per sum, into every CTA's memory
+        const double v = warp_total(lane < PT / 32 ? part[2 * lane + warp] : 0.0);
+        if (lane < ctas) *cl.map_shared_rank(&all[2 * me + warp], lane) = v;
+    }
+    cl.sync();
+    double sp = 0.0, sq = 0.0;
+    for (int c = 0; c < ctas; ++c) sp += all[2 * c], sq += all[2 * c + 1];
+    const double wp = prow->weigh(__ldg(p + x)) / sp, wq = q ? qrow->weigh(__ldg(q + x)) / sq : 1.0;
+    cl.sync();  // read by all before anything is written there again
+    return u * wq < wp;
+}
+
+// PT threads; 64 registers each, so that an SM holds 1024 of them however they are split (the forms for logits spill
+// some 250 bytes).
 //
 // The part of a CTA is cut into blocks, a block into one cell of neighbouring entries a warp; the pass leaves every
 // cell's sums, so the border is found by going from the CTA to the block to the cell to the entry, and only the last
@@ -300,7 +352,7 @@ __device__ __forceinline__ double warp_running(double v) {  // lane i: the sum o
 // the CTAs' sums, the search) is done by one warp: with f64 divisions and logarithms in all 1024 threads those parts
 // took 15000 of 37000 cycles of a sequence.
 template <int PT, bool VEC, bool PROBS>
-__global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a, const RowPart* parts, int slices) {
+__global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(const __grid_constant__ VerifyArgs a, const RowPart* parts, int slices, double near) {
     cg::cluster_group cl = cg::this_cluster();
     cluster_arrive();  // the others have started before their memory is written
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), b = blockIdx.x / ctas;
@@ -325,6 +377,7 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
 
     // ---- the decisions, in groups of 32 drafts (every CTA makes them for itself) ----
     int n_acc = 0, base = 0;
+    bool others_started = false;
     for (;;) {
         const int cnt = min(32, n - base);
         const double u = lane < cnt ? (double)a.u[(size_t)b * a.drafts + base + lane] : 0.0;
@@ -361,8 +414,20 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
             for (int k = warp; k <= 2 * cnt; k += kWarps) decide(k, std::false_type{});
         }
         __syncthreads();
-        const bool yes = lane < cnt && u * s_prob[1][lane] < s_prob[0][lane];
-        const int run = __ffs((int)~__ballot_sync(0xffffffffu, yes)) - 1;  // drafts accepted; -1: all 32
+        const double uq = lane < cnt ? u * s_prob[1][lane] : 0.0, pr = lane < cnt ? s_prob[0][lane] : 0.0;
+        unsigned yes = __ballot_sync(0xffffffffu, lane < cnt && uq < pr);
+        if constexpr (!PROBS) {
+            // the first refused draft and those before it that are near their border (the same ones in every warp and CTA)
+            unsigned unsure = __ballot_sync(0xffffffffu, pr > 0.0 && fabs(uq - pr) <= near * pr);
+            while (const unsigned left = unsure & (yes ^ (yes + 1))) {
+                const int at = __ffs((int)left) - 1, i = base + at;
+                if (!others_started) cluster_wait(), others_started = true;
+                const bool ok = accepted_in_f64<PT, VEC>(&a, &s_row[0][at], i, &s_part[0][0], &s_all[0][0][0]);
+                yes = ok ? yes | 1u << at : yes & ~(1u << at);
+                unsure &= ~(1u << at);
+            }
+        }
+        const int run = __ffs((int)~yes) - 1;  // drafts accepted; -1: all 32
         const int got = run < 0 ? 32 : run;
         n_acc = base + got;
         if (got < cnt || base + cnt == n) break;
@@ -419,7 +484,7 @@ __global__ void __launch_bounds__(PT, 1024 / PT) verify_pick_kernel(VerifyArgs a
     const int blocks = (steps + (1 << shift) - 1) >> shift;
     const unsigned cell = 128u << shift, block_entries = cell * kWarps;
     bool plain = !refused;
-    cluster_wait();
+    if (!others_started) cluster_wait();
     for (int slot = 0;; ++slot) {  // a second time only where p - q is zero everywhere
         double sums[4] = {0.0, 0.0, 0.0, 0.0}, all_a = 0.0, all_b = 0.0;
         auto go = [&](auto use_q) {
@@ -605,7 +670,7 @@ cudaError_t launch_pick(const VerifyArgs& a, const RowPart* parts, int slices, i
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = PROBS ? 1 : 2;
-    return cudaLaunchKernelEx(&cfg, kernel, a, parts, slices);
+    return cudaLaunchKernelEx(&cfg, kernel, a, parts, slices, near_border(a.vocab, slices));
 }
 
 template <bool PROBS>

@@ -450,8 +450,7 @@ BEBELM_API int bebelm_w4_check(const bebelm_w4* w, void* stream);
  * [n_seqs][n_drafts] and u_sample [n_seqs] uniform random numbers in [0, 1).
  *  - Draft i is accepted iff all before it were and u_i * q_i(token) < p_i(token). A token outside the
  *    vocabulary is refused (host memory: BEBELM_ERR_INVALID), a count outside 0..n_drafts taken as the nearer of them
- *    (host memory: likewise). Here p and q of logits come from f32 exponentials and sums, to about 1e-6; the sums
- *    that a token is drawn from are f64.
+ *    (host memory: likewise).
  *  - The next token: after a refusal at i from max(p_i - q_i, 0) (p_i if that is zero everywhere), after all
  *    drafts from the row behind them: the lowest index whose running sum exceeds u_sample times the total.
  *  - temperature 0: accepted iff equal to the row's first maximum, which is also the next token

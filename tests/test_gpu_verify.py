@@ -289,3 +289,25 @@ def test_the_queried_workspace_is_enough(draft_rows, temp):
                 bad.append((b, d, bb.last_error()))
     torch.cuda.synchronize()
     assert not bad, (len(bad), bad[:3])
+
+
+@pytest.mark.parametrize("temp", [1.0, 0.625, 2.5])
+@pytest.mark.parametrize("draft_rows", [True, False])
+@pytest.mark.parametrize("b,d,v", [(3, 4, 50), (2, 40, 1000), (5, 6, 4099), (40, 3, 9000), (2, 5, 32003), (3, 4, 128000)])
+def test_random_numbers_next_to_the_border(b, d, v, draft_rows, temp):
+    """u is the f32 next below, at or next above p / q of its draft, so u q and p differ by less than two f32 steps (2^-23 of p), and by
+    more than 1e-10 of p (which the inputs' p / q, not themselves f32, are checked for): the decision is that of 64-bit sums."""
+    t, tok, u, us, dr = inputs(b, d, v, temp, v + d, draft_rows=draft_rows)
+    rng = np.random.default_rng(d)
+    for s in range(b):
+        for i in range(d):
+            x = tok[s, i]
+            p, q = softmax64(t[s, i], temp)[x], softmax64(dr[s, i], temp)[x] if draft_rows else 1.0
+            # most drafts on the accepted side, so that later ones are reached
+            at = np.float32(min(p / q, 0.999))
+            side = rng.choice((-2, -1, -1, -1, -1, 0, 1), p=(.2, .2, .2, .15, .15, .05, .05))
+            for _ in range(abs(side)):
+                at = np.nextafter(at, np.float32(0 if side < 0 else 1))
+            u[s, i] = at
+            assert abs(float(at) * q / p - 1) > 1e-10
+    same(run(t, tok, u, us, dr, temperature=temp), reference(t, tok, u, us, dr, temperature=temp))
