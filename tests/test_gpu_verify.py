@@ -311,3 +311,18 @@ def test_random_numbers_next_to_the_border(b, d, v, draft_rows, temp):
             u[s, i] = at
             assert abs(float(at) * q / p - 1) > 1e-10
     same(run(t, tok, u, us, dr, temperature=temp), reference(t, tok, u, us, dr, temperature=temp))
+
+
+@pytest.mark.parametrize("shift", [0.0, 13.7])
+@pytest.mark.parametrize("near", [1e-2, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("b,d,v", [(4, 2, 1000), (6, 2, 9000), (40, 1, 20000), (3, 2, 70001), (2, 1, 128000)])
+def test_drafts_from_rows_almost_the_targets(b, d, v, near, shift):
+    """Draft logits within `near` of the target's, or of those and a constant: p - q is `near` of p, on either side, and its sums have to hold the token's place among v
+    all the same. u next to 1 refuses a draft whose p is below q (its smallest p / q is 1 - near or so)."""
+    t, tok, u, us, dr = inputs(b, d, v, 1.0, 7 * v + b, near=near)
+    dr += np.float32(shift)
+    u[:] = np.nextafter(np.float32(1), np.float32(0))
+    for s in range(b):
+        for i in range(d):  # drafts that are refused, except a few
+            tok[s, i] = int((softmax64(t[s, i], 1.0) / softmax64(dr[s, i], 1.0)).argmin()) if (s + i) % 4 else tok[s, i]
+    same(run(t, tok, u, us, dr), reference(t, tok, u, us, dr))
