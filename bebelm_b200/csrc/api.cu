@@ -300,6 +300,7 @@ struct bebelm_kv_pool {
     int n_seqs = 0;              // live sequences drawing from this pool
     // scratch shared by every call on this pool's sequences (stream-ordered)
     DevBuf io, qn, part, counters, seqdesc, pf, q8, proj, sample;
+    DevBuf host_ws;  // workspaces of host-memory calls (which end before the next one starts): q8 may be in use by work that is only queued
     ErrWord err;
     PinBuf pin;
     cudaEvent_t out_ev[kStageEvents] = {};  // chunks of a large output copied back
@@ -483,6 +484,7 @@ void pool_free(bebelm_kv_pool* P) {
     P->q8.release();
     P->proj.release();
     P->sample.release();
+    P->host_ws.release();
     P->err.release();
     P->pin.release();
     for (cudaEvent_t& e : P->out_ev)
@@ -2882,8 +2884,8 @@ int bebelm_w4_matmul(const bebelm_w4* W, const void* x, int x_dtype, size_t x_st
     xv.x = dx;
     xv.scales = static_cast<const float*>(dsc);
     xv.stride = v.n_in;
-    TRY(P->q8.ensure(std::max<size_t>(w4_scratch(v, xv), 256), false, s));
-    CUDA_TRY(w4_run(W, xv, o, y_dtype == BEBELM_BF16, P->q8.p, sms, W->host_err, s));
+    TRY(P->host_ws.ensure(std::max<size_t>(w4_scratch(v, xv), 256), false, s));
+    CUDA_TRY(w4_run(W, xv, o, y_dtype == BEBELM_BF16, P->host_ws.p, sms, W->host_err, s));
     TRY(stage_out(P, o, y, yb, s));
     return w4_timeout(W->host_err);
 }
@@ -2964,13 +2966,13 @@ int bebelm_verify_drafts(const float* target, size_t target_stride, const float*
                    {tokens, tb, &d2}, {n_per_seq, n_per_seq ? 4 * n_seqs : 0, &d3},
                    {greedy ? nullptr : u, greedy ? 0 : tb, &d4}, {greedy ? nullptr : u_sample, greedy ? 0 : 4 * n_seqs, &d5}};
     TRY(stage_in(P, st, 6, pad256(ob) + 4 * n_seqs, &o, s));
-    TRY(P->q8.ensure(std::max<size_t>(need, 256), false, s));
+    TRY(P->host_ws.ensure(std::max<size_t>(need, 256), false, s));
     a.target = static_cast<const float*>(d0), a.draft = static_cast<const float*>(d1);
     a.tokens = static_cast<const int*>(d2), a.n_drafts = static_cast<const int*>(d3);
     a.u = static_cast<const float*>(d4), a.u_sample = static_cast<const float*>(d5);
     a.out = static_cast<int*>(o);
     a.accepted = reinterpret_cast<int*>(static_cast<char*>(o) + pad256(ob));
-    a.workspace = P->q8.p;
+    a.workspace = P->host_ws.p;
     CUDA_TRY(launch_verify(a, sms, s));
     const size_t bb = pad256(ob) + 4 * n_seqs;
     const std::unique_ptr<char[]> back(new (std::nothrow) char[bb]);

@@ -339,3 +339,28 @@ def test_results_of_the_other_calls_on_another_stream(name):
             kept.append(next(caches))
             return (bb.attn_layer_batch(kept[-1], 0, weights, x, 0, stream=side),)
     results_belong_to(side, call)
+
+
+def test_host_calls_beside_queued_device_products():
+    """Host-memory products and verifications while K-quant products, which quantize into the library's scratch, are queued on
+    another stream: neither disturbs the other."""
+    import test_gpu_quant as Q
+    n_in, n_out, t = 2048, 2048, 64
+    w = torch.from_numpy(Q.random_q4k(n_out, n_in, 3)).cuda()
+    x = torch.randn(t, n_in, device="cuda")
+    want = bb.matmul(bb.GGML_Q4_K, w, n_in, n_out, x, t)
+    codes, sc, z = W.weights(300, 512, 64, 3)
+    w4 = bb.W4Weights(codes, sc, z, group=64)
+    xh = W.activations(40, 512, "f32", 0, 1)[0].cpu().numpy()
+    wanth = w4.matmul(xh)
+    args = V.inputs(3, 4, 9000, 1.0, 2)
+    wantv = bb.verify_drafts(*args[:4], draft=args[4])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        outs = [bb.matmul(bb.GGML_Q4_K, w, n_in, n_out, x, t, stream=side) for _ in range(30)]
+        for _ in range(4):
+            np.testing.assert_array_equal(w4.matmul(xh), wanth)
+            V.same(bb.verify_drafts(*args[:4], draft=args[4]), wantv)
+        side.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
