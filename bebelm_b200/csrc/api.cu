@@ -2886,8 +2886,8 @@ int bebelm_w4_matmul(const bebelm_w4* W, const void* x, int x_dtype, size_t x_st
     xv.stride = v.n_in;
     TRY(P->host_ws.ensure(std::max<size_t>(w4_scratch(v, xv), 256), false, s));
     CUDA_TRY(w4_run(W, xv, o, y_dtype == BEBELM_BF16, P->host_ws.p, sms, W->host_err, s));
-    TRY(stage_out(P, o, y, yb, s));
-    return w4_timeout(W->host_err);
+    const int rc = stage_out(P, o, y, yb, s), late = w4_timeout(W->host_err);
+    return rc ? rc : late;
 }
 
 int bebelm_w4_check(const bebelm_w4* W, void* stream) {
